@@ -71,6 +71,8 @@ SOURCES: Dict[str, List[str]] = {
     "rglru": [],
     "hyper_streams": [],
     "matrix_recurrence": [],
+    "copy_pages": [],
+    "logprobs": [],
 }
 
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .csrc.build import load_library
@@ -22,6 +23,9 @@ _REFUSALS = {
     -3: "unsupported size",
     -4: "misaligned pointer",
     -5: "scratch capacity exceeded",
+    -6: "a page outside its store",
+    -7: "a target named twice, or also a source",
+    -8: "out of host memory",
 }
 
 
@@ -147,6 +151,61 @@ def clear_slot(stores, slot: int) -> None:
         base[i] = store.data_ptr() + slot * size[i]
         entries[i] = store.shape[0]
     _check(load_library("elementwise").tb_clear_slot(_i32(count), base, pitch, size, entries, _stream()), "clear_slot")
+
+
+def copy_pages(moves) -> None:
+    """``store[:, targets[i]] = store[:, sources[i]]`` for every ``(store, sources, targets)`` of ``moves``, all in one launch
+    (more than 3,968 pages or eight stores: several).
+
+    A store is a contiguous tensor ``[entries, pages, ...]`` of any type (cache pages, or state slots); ``sources`` and
+    ``targets`` are host lists or arrays of page indices.  No target may be named twice or be a source of the same store; a
+    call that breaks this, or names a page outside a store, raises :class:`KernelError` and copies nothing.  The indices
+    travel in the launch: nothing has to outlive the call."""
+    global launch_count
+    count = len(moves)
+    base, pitch, size = (_pointer * count)(), (_i64 * count)(), (_i64 * count)()
+    entries, pages, counts = (_i32 * count)(), (_i32 * count)(), (_i32 * count)()
+    sources, targets = (_pointer * count)(), (_pointer * count)()
+    kept = []                                            # the index arrays live until the call returns
+    device = None
+    for i, (store, source, target) in enumerate(moves):
+        _cuda(store)
+        _need(store.dim() >= 2 and store.is_contiguous(), "copy_pages takes contiguous stores [entries, pages, ...]")
+        if device is None:
+            device = store.device
+            _need(device.index == torch.cuda.current_device(), "copy_pages runs on the current device")
+        _need(store.device == device, "copy_pages takes stores of one device")
+        source, target = _host_indices(source), _host_indices(target)
+        _need(source.size == target.size, "copy_pages takes as many targets as sources")
+        for j in range(i):
+            _need(moves[j][0].data_ptr() != store.data_ptr() or not store.numel(), "copy_pages takes a store once a call")
+        kept.append((source, target))
+        shape = store.shape
+        entries[i], pages[i] = shape[0], shape[1]
+        # (from the sizes: a tensor without numbers, or an extent of one, may have any stride)
+        size[i] = store.numel() // (shape[0] * shape[1]) * store.element_size() if store.numel() else 0
+        pitch[i] = size[i] * shape[1]
+        base[i], counts[i] = store.data_ptr(), source.size
+        sources[i], targets[i] = source.ctypes.data, target.ctypes.data
+    launches = _i32(0)
+    status = load_library("copy_pages").tb_copy_pages(_i32(count), base, pitch, size, entries, pages, counts, sources, targets,
+                                                      ctypes.byref(launches), _stream())
+    launch_count -= 1                                    # (_check counts one; a call may launch none or several)
+    _check(status, "copy_pages")
+    launch_count += launches.value
+
+
+def _host_indices(indices) -> np.ndarray:
+    if isinstance(indices, torch.Tensor):
+        _need(not indices.is_cuda, "page indices are host lists or arrays")
+        indices = indices.numpy()
+    array = np.asarray(indices)
+    if array.size == 0:
+        return np.empty(0, dtype=np.int32)
+    _need(array.ndim == 1 and array.dtype.kind in "iu", "page indices are one-dimensional lists of integers")
+    if array.dtype != np.int32:
+        _need(int(array.min()) >= 0 and int(array.max()) < 2 ** 31, "a page outside its store")
+    return np.ascontiguousarray(array, dtype=np.int32)
 
 
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
@@ -290,6 +349,36 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tenso
                          _i32(rows), _i32(logits.shape[1]), _ptr(values), _ptr(indices), _i32(parts), _stream()),
            "sample")
     return out
+
+
+MAX_ALTERNATIVES = 64
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int = 0) -> tuple:
+    """``(logprob [S], entropy [S], alternative log probabilities [S, k], alternative ids [S, k])`` of 32-bit logits ``[S, V]``
+    (rows contiguous, any distance apart), with ``k = alternatives`` up to 64 and ``V``.
+
+    ``logprob[s]`` is that of ``tokens[s]`` (int32; NaN for a token outside the vocabulary); the entropy is in nats; the
+    alternatives are the most probable tokens in order, equal logits by ascending id.  A logit of -inf has probability 0; a
+    NaN or +inf makes its row's numbers NaN."""
+    _cuda(logits, tokens)
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+          "logits must be float32 [S, V] with contiguous rows")
+    rows, vocab = logits.shape
+    _need(tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows,
+          "tokens must be contiguous int32 [S]")
+    _need(logits.device == tokens.device, "token_logprobs takes tensors of one device")
+    _need(0 <= alternatives <= min(MAX_ALTERNATIVES, vocab),
+          f"token_logprobs gives up to {MAX_ALTERNATIVES} alternatives, and no more than the vocabulary has tokens")
+    device = logits.device
+    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    values = torch.empty((rows, alternatives), dtype=torch.float32, device=device)
+    ids = torch.empty((rows, alternatives), dtype=torch.int32, device=device)
+    _check(load_library("logprobs").tb_token_logprobs(_ptr(logits), _i64(logits.stride(0)), _ptr(tokens), _ptr(logprob),
+                                                      _ptr(entropy), _ptr(values), _ptr(ids), _i32(rows), _i32(vocab),
+                                                      _i32(alternatives), _stream()), "token_logprobs")
+    return logprob, entropy, values, ids
 
 
 _sm_counts = {}
