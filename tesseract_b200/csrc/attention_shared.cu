@@ -1,0 +1,666 @@
+// Decoded rows over paged keys and values, where groups of rows have their first keys in common: those are read once for
+// the whole group instead of once a row.
+//
+// Per row b and head h over the keys 0..p_b of the row (p_b: its position; -1: none), c = h / fold the kv head:
+//   s_j = scale * q_bh . k_cj     o = sum_j 2^(s_j log2 e - m) v_cj / sum_j 2^(s_j log2 e - m)      (no key: 0)
+// The keys are cut into the part that the row's group has in common, [0, L), L a multiple of 64, and the part behind,
+// [L, p_b].  A softmax over disjoint parts is put together from their maxima m, sums l and unnormalised sums a of values,
+// all kept in 32 bits:  m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum a_i 2^(m_i - m) / l.  Both parts are cut further
+// into runs of keys, so that few rows fill the chip; every run leaves (m, l, a) per row and head in scratch memory and a second
+// kernel puts them together in the order of the runs (no atomics: the same call gives the same bits).
+//
+// What a block does: one tile of folded rows (the `fold` query heads of a kv head, row after row of the group, or of one row
+// behind the common part) against one run of keys of one kv head.
+//   attend_mma   bfloat16, tiles of 16 folded rows: every warp streams every eighth tile of 16 keys through a cp.async ring of its
+//                own into mma.sync.m16n8k16; scores and sums in 32 bits, the weights rounded to bfloat16 for their product with the
+//                values (as in this package's other attention kernels in bfloat16: relative 2^-9 of each, averaged over the keys).
+//   attend_f32   32-bit, tiles of 8 folded rows, multiply-adds only: a lane scores one key against the tile's rows, then owns a
+//                few columns of the values.
+// Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
+// (numbers of an earlier owner, NaN) reaches nothing.
+#include "common.cuh"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMasked = -1.0e30f;
+constexpr int kBlock = 64;                    // keys that common parts and runs are counted in
+
+struct SharedParams {
+    const void* q;                            // [rows, heads * head_dim], row stride q_stride
+    void* out;
+    const void* cache;                        // [page][K|V][kv head][page_size][head_dim]
+    const int* positions;                     // [rows]
+    const int* table;                         // [rows, table_stride]
+    const int* members;                       // [rows]: the rows group by group
+    const int* group_start;                   // [groups + 1]: where a group's rows begin in `members`
+    const int* prefix;                        // [groups]: keys in common
+    const int* group_of;                      // [rows]
+    float* part_a;                            // [rows][heads][parts][head_dim]
+    float2* part_ml;                          // [rows][heads][parts]
+    int64_t q_stride, out_stride;
+    int table_stride, table_keys;             // keys that a row of the table can name
+    int rows, groups, heads, kv_heads, fold, head_dim;
+    int tiles;                                // tiles of all groups' folded rows
+    int prefix_parts, prefix_run;             // runs of a common part: at most so many, of at least so many blocks of keys each
+    int tail_parts, tail_run;                 // the same behind it
+    Paging paging;
+    float scale_log2;
+};
+
+// One block's work.
+struct Work {
+    int first_member, member_rows;            // the tile's rows: `members[first_member ..]`, or (member_rows 0) the one row `row`
+    int row;                                  // a row whose table names the keys
+    int folded, first_folded;                 // folded rows of the group or row, and the first of the tile
+    int kv_head, begin, end;                  // keys [begin, end)
+    int part;                                 // slot of the partial result
+};
+
+__device__ __forceinline__ int common_keys(const SharedParams& p, int group) {
+    if (p.prefix_parts == 0 || p.group_start[group + 1] - p.group_start[group] < 2) return 0;
+    return min(p.prefix[group], p.table_keys) & ~(kBlock - 1);
+}
+
+// How `blocks` blocks of keys are cut: runs of the same number of blocks, at most `parts`.  Returns the blocks of a run.
+__device__ __forceinline__ int run_blocks(int blocks, int parts, int run) {
+    const int n = min(parts, (blocks + run - 1) / run);
+    return (blocks + n - 1) / n;
+}
+
+// Finds the work of block `index`; false if there is none.  Tiles of common parts first, then the parts behind, row by row.
+template <int TILE>
+__device__ bool find_work(const SharedParams& p, int64_t index, Work& w) {
+    const int64_t of_prefix = (int64_t)p.tiles * p.kv_heads * p.prefix_parts;
+    if (index < of_prefix) {
+        const int part = (int)(index % p.prefix_parts);
+        const int64_t rest = index / p.prefix_parts;
+        w.kv_head = (int)(rest % p.kv_heads);
+        int tile = (int)(rest / p.kv_heads);
+        // which group: a warp counts the tiles of 32 groups at a time
+        const int lane = threadIdx.x & 31;
+        int group = -1;
+        for (int base = 0; base < p.groups; base += 32) {
+            const int g = base + lane;
+            int mine = 0;
+            if (g < p.groups) {
+                const int n = p.group_start[g + 1] - p.group_start[g];
+                if (n > 1) mine = (n * p.fold + TILE - 1) / TILE;
+            }
+            int up_to = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
+                if (lane >= o) up_to += other;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, up_to > tile);
+            if (past) {
+                const int who = __ffs(past) - 1;
+                group = base + who;
+                tile -= __shfl_sync(0xffffffffu, up_to - mine, who);
+                break;
+            }
+            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+        }
+        if (group < 0) return false;
+        const int blocks = common_keys(p, group) / kBlock;
+        if (blocks == 0) return false;
+        const int run = run_blocks(blocks, p.prefix_parts, p.prefix_run);
+        w.begin = part * run * kBlock;
+        w.end = min(blocks, (part + 1) * run) * kBlock;
+        if (w.begin >= w.end) return false;
+        w.first_member = p.group_start[group];
+        w.member_rows = p.group_start[group + 1] - w.first_member;
+        w.row = p.members[w.first_member];
+        w.folded = w.member_rows * p.fold;
+        w.first_folded = tile * TILE;
+        w.part = part;
+        return true;
+    }
+    index -= of_prefix;
+    const int part = (int)(index % p.tail_parts);
+    int64_t rest = index / p.tail_parts;
+    w.kv_head = (int)(rest % p.kv_heads);
+    rest /= p.kv_heads;
+    const int tiles = (p.fold + TILE - 1) / TILE;
+    w.row = (int)(rest / tiles);
+    if (w.row >= p.rows) return false;
+    w.first_folded = (int)(rest % tiles) * TILE;
+    const int first = common_keys(p, p.group_of[w.row]);
+    const int last = min(p.positions[w.row] + 1, p.table_keys);
+    if (last <= first) return false;
+    const int blocks = (last - first + kBlock - 1) / kBlock;
+    const int run = run_blocks(blocks, p.tail_parts, p.tail_run);
+    w.begin = first + part * run * kBlock;
+    w.end = min(last, w.begin + run * kBlock);
+    if (w.begin >= w.end) return false;
+    w.member_rows = 0;
+    w.folded = p.fold;
+    w.part = p.prefix_parts + part;
+    return true;
+}
+
+// Row of the batch and head of folded row `fr`.
+__device__ __forceinline__ void place_of(const SharedParams& p, const Work& w, int fr, int& row, int& head) {
+    const int member = fr / p.fold;
+    row = w.member_rows > 0 ? p.members[w.first_member + member] : w.row;
+    head = w.kv_head * p.fold + (fr - member * p.fold);
+}
+
+__device__ __forceinline__ int64_t slot_of(const SharedParams& p, int row, int head, int part) {
+    return ((int64_t)row * p.heads + head) * (p.prefix_parts + p.tail_parts) + part;
+}
+
+// The warps' results of a tile, (m, l) in `ml` [warps][TILE][2] and sums in `acc` [warps][TILE][PITCH], put together in the
+// order of the warps and left as the run's.  Every warp has written its own (a barrier in front).
+template <int TILE, int PITCH, int WARPS>
+__device__ void leave_run(const SharedParams& p, const Work& w, const float* ml, const float* acc) {
+    const int rows = min(TILE, w.folded - w.first_folded);
+    for (int idx = threadIdx.x; idx < rows * p.head_dim; idx += WARPS * 32) {
+        const int r = idx / p.head_dim, col = idx - r * p.head_dim;
+        float big = kMasked;
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) big = fmaxf(big, ml[(v * TILE + r) * 2]);
+        float a = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) {
+            const float weight = exp2f(ml[(v * TILE + r) * 2] - big);
+            a += weight * acc[(v * TILE + r) * PITCH + col];
+            l += weight * ml[(v * TILE + r) * 2 + 1];
+        }
+        int row, head;
+        place_of(p, w, w.first_folded + r, row, head);
+        const int64_t slot = slot_of(p, row, head, w.part);
+        p.part_a[slot * p.head_dim + col] = a;
+        if (col == 0) p.part_ml[slot] = make_float2(big, l);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ bfloat16, mma.sync
+
+constexpr int kKeys = 16;                     // keys of a warp's tile
+constexpr int kRows = 16;                     // folded rows of a block's tile
+// Warps and ring depth so that two blocks share a multiprocessor up to a padded head size of 128.
+template <int D>
+constexpr int kWarps = D <= 64 ? 8 : D <= 128 ? 6 : 4;
+template <int D>
+constexpr int kStages = D > 64 && D <= 128 ? 2 : 3;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int bytes = valid ? 16 : 0;         // (0: the destination is filled with zeros)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float fast_exp2(float x) {      // 2^x, relative error about 2^-22
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// Byte offset of 16-byte chunk `chunk` of row `row` in a [rows][D] tile, permuted so that the eight rows which an ldmatrix reads lie
+// on different banks.
+template <int D>
+__device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
+    constexpr int CH = D / 8;
+    const int key = CH >= 8 ? (row & 7) : ((row >> 1) & (CH - 1));
+    return (uint32_t)(row * (D * 2) + ((chunk ^ key) << 4));
+}
+
+template <int D>
+__device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* smem) {
+    constexpr int WARPS = kWarps<D>, STAGES = kStages<D>, CH = D / 8, PASSES = kKeys * CH / 32;
+    constexpr uint32_t kTileBytes = kKeys * D * 2, kStageBytes = 2 * kTileBytes;
+    constexpr bool QREG = D <= 128;           // the queries' fragments stay in registers
+    constexpr int PITCH = D + 8;              // floats between rows of the sums that are put together (bank conflicts)
+    static_assert((kKeys * CH) % 32 == 0, "a warp copies whole passes of 32 chunks");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = min(kRows, w.folded - w.first_folded);
+    const uint32_t q_tile = smem_u32(smem);
+    const uint32_t ring = q_tile + kRows * D * 2 + warp * (STAGES * kStageBytes);
+    const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
+    for (int idx = threadIdx.x; idx < kRows * CH; idx += WARPS * 32) {
+        const int r = idx / CH, c = idx % CH;
+        const bool ok = r < rows && c * 8 < p.head_dim;
+        const __nv_bfloat16* src = q;
+        if (ok) {
+            int row, head;
+            place_of(p, w, w.first_folded + r, row, head);
+            src = q + (int64_t)row * p.q_stride + (int64_t)head * p.head_dim + c * 8;
+        }
+        cp_async16(q_tile + tile_offset<D>(r, c), src, ok);
+    }
+    const int* table = p.table + (int64_t)w.row * p.table_stride;
+    const int64_t head_block = (int64_t)p.paging.size * p.head_dim;
+    const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
+    const __nv_bfloat16* base = (const __nv_bfloat16*)p.cache + (int64_t)w.kv_head * head_block;
+    // the pages of a tile's keys are looked up one tile ahead of its copies, which depend on them
+    auto look_up = [&](int key0, int (&pages)[PASSES]) {
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+            const int key = key0 + (pass * 32 + lane) / CH;
+            pages[pass] = key < w.end ? table[p.paging.page_of(key)] : 0;
+        }
+    };
+    auto bring = [&](uint32_t dst, int key0, const int (&pages)[PASSES]) {
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+            const int idx = pass * 32 + lane, r = idx / CH, c = idx % CH, key = key0 + r;
+            const bool ok = key < w.end && c * 8 < p.head_dim;
+            const __nv_bfloat16* src = base;
+            if (ok) src = base + (int64_t)pages[pass] * page_block + (int64_t)p.paging.within(key) * p.head_dim + c * 8;
+            const uint32_t offset = tile_offset<D>(r, c);
+            cp_async16(dst + offset, src, ok);
+            cp_async16(dst + kTileBytes + offset, src + v_offset, ok);
+        }
+    };
+    int next_pages[PASSES];
+    int load_key = w.begin + warp * kKeys;
+    constexpr int STEP = WARPS * kKeys;
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st) {
+        if (load_key < w.end) {
+            look_up(load_key, next_pages);
+            bring(ring + st * kStageBytes, load_key, next_pages);
+        }
+        cp_async_commit();                    // one group a stage, empty or not; the first holds the queries too
+        load_key += STEP;
+    }
+    if (load_key < w.end) look_up(load_key, next_pages);
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();                          // the queries are there
+    uint32_t qf[QREG ? D / 16 : 1][4];
+    if (QREG) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) ldmatrix_x4(qf[ks], q_tile + tile_offset<D>(lane & 15, ks * 2 + (lane >> 4)));
+    }
+    float o[D / 8][4], m[2] = {kMasked, kMasked}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int dt = 0; dt < D / 8; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dt][e] = 0.0f;
+
+    int it = 0;
+    for (int key0 = w.begin + warp * kKeys; key0 < w.end; key0 += STEP, ++it) {
+        if (load_key < w.end) bring(ring + ((it + STAGES - 1) % STAGES) * kStageBytes, load_key, next_pages);
+        cp_async_commit();
+        load_key += STEP;
+        if (load_key < w.end) look_up(load_key, next_pages);
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();
+        const uint32_t k_tile = ring + (it % STAGES) * kStageBytes, v_tile = k_tile + kTileBytes;
+        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t a[4], b[4];
+            if (QREG) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = qf[ks][e];
+            } else {
+                ldmatrix_x4(a, q_tile + tile_offset<D>(lane & 15, ks * 2 + (lane >> 4)));
+            }
+            ldmatrix_x4(b, k_tile + tile_offset<D>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+            mma_bf16(s[0], a, b[0], b[1]);
+            mma_bf16(s[1], a, b[2], b[3]);
+        }
+        // this thread's scores: rows lane / 4 and lane / 4 + 8, keys 2 (lane % 4), + 1, + 8, + 9
+        float high[2] = {kMasked, kMasked};
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool there = key0 + nt * 8 + 2 * (lane & 3) + (e & 1) < w.end;
+                s[nt][e] = there ? s[nt][e] * p.scale_log2 : kMasked;
+                high[e >> 1] = fmaxf(high[e >> 1], s[nt][e]);
+            }
+        float correction[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 1));
+            high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 2));
+            const float m_new = fmaxf(m[i], high[i]);
+            correction[i] = fast_exp2(m[i] - m_new);
+            m[i] = m_new;
+            l[i] *= correction[i];
+        }
+#pragma unroll
+        for (int dt = 0; dt < D / 8; ++dt) {
+            o[dt][0] *= correction[0];
+            o[dt][1] *= correction[0];
+            o[dt][2] *= correction[1];
+            o[dt][3] *= correction[1];
+        }
+        uint32_t weights[4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+            float e4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                e4[e] = s[nt][e] > 0.5f * kMasked ? fast_exp2(s[nt][e] - m[e >> 1]) : 0.0f;
+                if (s[nt][e] != s[nt][e]) e4[e] = s[nt][e];        // a NaN score stays one
+                l[e >> 1] += e4[e];
+            }
+            weights[2 * nt] = pack_bf16(e4[0], e4[1]);
+            weights[2 * nt + 1] = pack_bf16(e4[2], e4[3]);
+        }
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, v_tile + tile_offset<D>((lane & 7) + (((lane >> 3) & 1) << 3), dp * 2 + (lane >> 4)));
+            mma_bf16(o[2 * dp], weights, b[0], b[1]);
+            mma_bf16(o[2 * dp + 1], weights, b[2], b[3]);
+        }
+        __syncwarp();                         // every lane is done with this stage before it is filled again
+    }
+    cp_async_wait<0>();
+    __syncthreads();                          // the rings become the place where the warps' results meet
+    float* ml = reinterpret_cast<float*>(smem);
+    float* acc = ml + WARPS * kRows * 2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int r = (lane >> 2) + i * 8;
+        if ((lane & 3) == 0) {
+            ml[(warp * kRows + r) * 2] = m[i];
+            ml[(warp * kRows + r) * 2 + 1] = l[i];
+        }
+#pragma unroll
+        for (int dt = 0; dt < D / 8; ++dt)
+            *reinterpret_cast<float2*>(acc + (warp * kRows + r) * PITCH + dt * 8 + 2 * (lane & 3)) =
+                make_float2(o[dt][2 * i], o[dt][2 * i + 1]);
+    }
+    __syncthreads();
+    leave_run<kRows, PITCH, WARPS>(p, w, ml, acc);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kWarps<D> * 32) shared_mma_kernel(const SharedParams p) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    pdl_wait();
+    pdl_trigger();
+    Work w;
+    if (find_work<kRows>(p, blockIdx.x, w)) attend_mma<D>(p, w, smem);
+}
+
+template <int D>
+constexpr size_t mma_bytes() {
+    constexpr size_t tiles = (size_t)kRows * D * 2 + (size_t)kWarps<D> * kStages<D> * 2 * kKeys * D * 2;
+    constexpr size_t meet = (size_t)kWarps<D> * kRows * (2 + D + 8) * sizeof(float);
+    return tiles > meet ? tiles : meet;
+}
+
+// ------------------------------------------------------------------------------------------------ 32-bit
+
+constexpr int kF32Rows = 8;                   // folded rows of a tile
+constexpr int kF32Warps = 8;
+constexpr int kF32Keys = 32;                  // keys of a warp's tile: a lane scores one
+
+// D: head size padded to 64, 128 or 256.
+template <int D>
+__device__ void attend_f32(const SharedParams& p, const Work& w, float* smem) {
+    constexpr int COLS = D / 32;              // columns of the values that a lane owns: lane, lane + 32, ...
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = min(kF32Rows, w.folded - w.first_folded);
+    const int dim = p.head_dim;
+    float* queries = smem;                                               // [kF32Rows][D], zeros beyond the rows
+    float* weights = queries + kF32Rows * D + warp * (kF32Keys * kF32Rows);      // [key][row] of this warp
+    const float* q = (const float*)p.q;
+    for (int idx = threadIdx.x; idx < kF32Rows * D; idx += kF32Warps * 32) {
+        const int r = idx / D, col = idx % D;
+        float v = 0.0f;
+        if (r < rows && col < dim) {
+            int row, head;
+            place_of(p, w, w.first_folded + r, row, head);
+            v = q[(int64_t)row * p.q_stride + (int64_t)head * dim + col];
+        }
+        queries[idx] = v;
+    }
+    __syncthreads();
+    const int* table = p.table + (int64_t)w.row * p.table_stride;
+    const int64_t head_block = (int64_t)p.paging.size * dim;
+    const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
+    const float* base = (const float*)p.cache + (int64_t)w.kv_head * head_block;
+    float m[kF32Rows], l[kF32Rows], o[kF32Rows][COLS];
+#pragma unroll
+    for (int r = 0; r < kF32Rows; ++r) {
+        m[r] = kMasked;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) o[r][c] = 0.0f;
+    }
+    for (int key0 = w.begin + warp * kF32Keys; key0 < w.end; key0 += kF32Warps * kF32Keys) {
+        const int key = key0 + lane;
+        const bool there = key < w.end;
+        int64_t at = 0;                       // (a lane without a key reads page 0, which is always there)
+        if (there) at = (int64_t)table[p.paging.page_of(key)] * page_block + (int64_t)p.paging.within(key) * dim;
+        const float* k = base + at;
+        float s[kF32Rows];
+#pragma unroll
+        for (int r = 0; r < kF32Rows; ++r) s[r] = 0.0f;
+#pragma unroll 4
+        for (int d = 0; d < dim; d += 4) {
+            const float4 kv = *reinterpret_cast<const float4*>(k + d);
+#pragma unroll
+            for (int r = 0; r < kF32Rows; ++r) {
+                const float4 qv = *reinterpret_cast<const float4*>(queries + r * D + d);
+                s[r] = fmaf(qv.x, kv.x, s[r]);
+                s[r] = fmaf(qv.y, kv.y, s[r]);
+                s[r] = fmaf(qv.z, kv.z, s[r]);
+                s[r] = fmaf(qv.w, kv.w, s[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kF32Rows; ++r) {
+            const float score = there ? s[r] * p.scale_log2 : kMasked;
+            const float m_new = fmaxf(m[r], warp_max(score));
+            const float correction = exp2f(m[r] - m_new);
+            m[r] = m_new;
+            const float weight = there ? exp2f(score - m_new) : 0.0f;
+            l[r] = l[r] * correction + weight;             // (this lane's keys; the lanes meet at the end)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) o[r][c] *= correction;
+            weights[lane * kF32Rows + r] = weight;
+        }
+        __syncwarp();
+        const int count = min(kF32Keys, w.end - key0);
+#pragma unroll 4
+        for (int j = 0; j < count; ++j) {
+            const float* v = base + v_offset + __shfl_sync(0xffffffffu, at, j);
+            float weight[kF32Rows];
+#pragma unroll
+            for (int r = 0; r < kF32Rows; r += 4)
+                *reinterpret_cast<float4*>(weight + r) = *reinterpret_cast<const float4*>(weights + j * kF32Rows + r);
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+                const float value = c * 32 + lane < dim ? v[c * 32 + lane] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < kF32Rows; ++r) o[r][c] = fmaf(weight[r], value, o[r][c]);
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    float* ml = smem;
+    float* acc = ml + kF32Warps * kF32Rows * 2;
+#pragma unroll
+    for (int r = 0; r < kF32Rows; ++r) {
+        const float sum = warp_sum(l[r]);
+        if (lane == 0) {
+            ml[(warp * kF32Rows + r) * 2] = m[r];
+            ml[(warp * kF32Rows + r) * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[(warp * kF32Rows + r) * D + c * 32 + lane] = o[r][c];
+    }
+    __syncthreads();
+    leave_run<kF32Rows, D, kF32Warps>(p, w, ml, acc);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kF32Warps * 32) shared_f32_kernel(const SharedParams p) {
+    extern __shared__ __align__(128) float f32_smem[];
+    pdl_wait();
+    pdl_trigger();
+    Work w;
+    if (find_work<kF32Rows>(p, blockIdx.x, w)) attend_f32<D>(p, w, f32_smem);
+}
+
+template <int D>
+constexpr size_t f32_bytes() {
+    constexpr size_t tiles = (size_t)kF32Rows * D + (size_t)kF32Warps * kF32Keys * kF32Rows;
+    constexpr size_t meet = (size_t)kF32Warps * kF32Rows * (2 + D);
+    return (tiles > meet ? tiles : meet) * sizeof(float);
+}
+
+// ------------------------------------------------------------------------------------------------ the runs put together
+
+// A warp a (row, head): the weights of its runs 32 at a time, then the columns.
+template <typename T>
+__global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (index >= (int64_t)p.rows * p.heads) return;
+    const int row = (int)(index / p.heads), head = (int)(index % p.heads);
+    // the runs that the row has: the same rule as where they were made
+    const int common = common_keys(p, p.group_of[row]), last = min(p.positions[row] + 1, p.table_keys);
+    int of_prefix = 0, of_tail = 0;
+    if (common > 0) {
+        const int run = run_blocks(common / kBlock, p.prefix_parts, p.prefix_run);
+        of_prefix = (common / kBlock + run - 1) / run;
+    }
+    if (last > common) {
+        const int blocks = (last - common + kBlock - 1) / kBlock, run = run_blocks(blocks, p.tail_parts, p.tail_run);
+        of_tail = (blocks + run - 1) / run;
+    }
+    const int64_t slot = slot_of(p, row, head, 0);
+    const float2* ml = p.part_ml + slot;
+    auto slot_at = [&](int s) { return s < of_prefix ? s : p.prefix_parts + s - of_prefix; };
+    const int parts = of_prefix + of_tail;
+    float big = kMasked;
+    for (int s = lane; s < parts; s += 32) big = fmaxf(big, ml[slot_at(s)].x);
+    big = warp_max(big);
+    float sum = 0.0f;
+    for (int s = 0; s < parts; ++s) {
+        const float2 v = ml[slot_at(s)];
+        sum += exp2f(v.x - big) * v.y;
+    }
+    const float inverse = parts > 0 ? 1.0f / sum : 0.0f;
+    T* out = (T*)p.out + (int64_t)row * p.out_stride + (int64_t)head * p.head_dim;
+    for (int col = lane; col < p.head_dim; col += 32) {
+        float a = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < parts; ++s) a += exp2f(ml[slot_at(s)].x - big) * p.part_a[(slot + slot_at(s)) * p.head_dim + col];
+        Elem<T>::store(out + col, a * inverse);
+    }
+}
+
+template <typename Kernel>
+int launch(Kernel kernel, int64_t blocks, int threads, size_t smem, const SharedParams& p, cudaStream_t stream) {
+    if (blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
+    if (smem > 48 * 1024) {
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return (int)err;
+    }
+    if (cudaError_t err = tb_launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), smem, stream, p)) return (int)err;
+    return tb_launch_status();
+}
+
+}  // namespace
+
+// Folded rows of a tile: what `tiles` counts.
+TB_EXPORT int tb_attention_shared_tile(int dtype) { return dtype == TB_F32 ? kF32Rows : kRows; }
+
+// rows of q and out: [rows, heads * head_dim] with a stride; positions[b]: the last key of row b (-1: none); table: [rows, columns]
+// pages; members, group_start, prefix, group_of: the groups (SharedParams); tiles: the tiles of all groups of two rows or more,
+// ceil(rows of the group * heads / kv_heads / tile) each, no fewer.  prefix[g] is at most positions[b] + 1 for the rows of the group.
+// part_a, part_ml: rows * heads * (prefix_parts + tail_parts) * (head_dim and 2) floats.
+TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* cache,
+                                  const int* positions, const int* table, int table_stride, int table_columns, const int* members,
+                                  const int* group_start, const int* prefix, const int* group_of, int rows, int groups, int heads,
+                                  int kv_heads, int head_dim, int page_size, float scale, int tiles, int prefix_parts,
+                                  int prefix_run, int tail_parts, int tail_run, float* part_a, float* part_ml,
+                                  int64_t part_floats, int dtype, cudaStream_t stream) {
+    if (rows == 0) return 0;
+    if (dtype != TB_F32 && dtype != TB_BF16) return TB_ERR_BAD_DTYPE;
+    if (rows < 0 || groups < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || page_size < 1 || tiles < 0) return TB_ERR_BAD_SIZE;
+    if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0) return TB_ERR_BAD_SIZE;
+    if (prefix_parts < 0 || tail_parts < 1 || prefix_run < 1 || tail_run < 1) return TB_ERR_BAD_SIZE;
+    const int element = dtype == TB_F32 ? 4 : 2;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)part_a) % 16 != 0) return TB_ERR_BAD_ALIGN;
+    if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
+    const int64_t parts = (int64_t)rows * heads * (prefix_parts + tail_parts);
+    if (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim) return -5;
+    SharedParams p;
+    p.q = q;
+    p.out = out;
+    p.cache = cache;
+    p.positions = positions;
+    p.table = table;
+    p.members = members;
+    p.group_start = group_start;
+    p.prefix = prefix;
+    p.group_of = group_of;
+    p.part_a = part_a;
+    p.part_ml = (float2*)part_ml;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.table_stride = table_stride;
+    const int64_t keys = (int64_t)table_columns * page_size;
+    p.table_keys = (int)(keys < 0x7fffff00 ? keys : 0x7fffff00);
+    p.rows = rows;
+    p.groups = groups;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.fold = heads / kv_heads;
+    p.head_dim = head_dim;
+    p.tiles = tiles;
+    p.prefix_parts = prefix_parts;
+    p.prefix_run = prefix_run;
+    p.tail_parts = tail_parts;
+    p.tail_run = tail_run;
+    p.paging = tb_paging(page_size);
+    p.scale_log2 = scale * kLog2e;
+    const int tile = tb_attention_shared_tile(dtype);
+    const int64_t blocks = (int64_t)tiles * kv_heads * prefix_parts +
+                           (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
+    int status;
+    if (dtype == TB_F32) {
+        if (head_dim <= 64) status = launch(shared_f32_kernel<64>, blocks, kF32Warps * 32, f32_bytes<64>(), p, stream);
+        else if (head_dim <= 128) status = launch(shared_f32_kernel<128>, blocks, kF32Warps * 32, f32_bytes<128>(), p, stream);
+        else status = launch(shared_f32_kernel<256>, blocks, kF32Warps * 32, f32_bytes<256>(), p, stream);
+    } else if (head_dim <= 32) {
+        status = launch(shared_mma_kernel<32>, blocks, kWarps<32> * 32, mma_bytes<32>(), p, stream);
+    } else if (head_dim <= 64) {
+        status = launch(shared_mma_kernel<64>, blocks, kWarps<64> * 32, mma_bytes<64>(), p, stream);
+    } else if (head_dim <= 128) {
+        status = launch(shared_mma_kernel<128>, blocks, kWarps<128> * 32, mma_bytes<128>(), p, stream);
+    } else {
+        status = launch(shared_mma_kernel<256>, blocks, kWarps<256> * 32, mma_bytes<256>(), p, stream);
+    }
+    if (status != 0) return status;
+    const int64_t joins = ((int64_t)rows * heads + 3) / 4;
+    return dtype == TB_F32 ? launch(shared_join_kernel<float>, joins, 128, 0, p, stream)
+                           : launch(shared_join_kernel<__nv_bfloat16>, joins, 128, 0, p, stream);
+}

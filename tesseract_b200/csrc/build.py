@@ -73,6 +73,7 @@ SOURCES: Dict[str, List[str]] = {
     "matrix_recurrence": [],
     "copy_pages": [],
     "logprobs": [],
+    "attention_shared": [],
 }
 
 

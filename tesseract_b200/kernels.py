@@ -298,6 +298,42 @@ def attention_rows(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, posi
     return out
 
 
+def attention_shared_tile(dtype: torch.dtype) -> int:
+    """Folded rows (rows of a group times query heads per kv head) that a block of ``attention_shared`` takes."""
+    return {torch.float32: 8, torch.bfloat16: 16}[dtype]
+
+
+def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+                     shared, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, choice
+                     ) -> torch.Tensor:
+    """Paged attention of decoded rows, one a sequence, whose groups have their first keys in common (``shared``: a
+    ``SharedRows``): those are read once a group.  Row ``b`` reads keys 0 to ``positions[b]`` (int32 ``[B]``; -1: none, the row
+    gives zeros) through row ``b`` of ``block_table``, a group's keys in common through its first member's.
+    ``q``/``out``: ``[B, num_heads*head_dim]`` views; ``choice``: ``plan.shared_attention``'s answer for ``shared``."""
+    _cuda(q, out, cache, positions, block_table, shared.members)
+    rows = q.shape[0]
+    _need(q.dtype == out.dtype == cache.dtype, "attention dtypes disagree")
+    _need(q.dim() == 2 and q.shape[1] == num_heads * head_dim and out.shape == q.shape and q.stride(1) == 1
+          and out.stride(1) == 1, "q/out layout")
+    _need(positions.dtype == torch.int32 and block_table.dtype == torch.int32, "positions and block_table must be int32")
+    _need(positions.is_contiguous() and positions.numel() == rows, "one position a row")
+    _need(block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
+          and block_table.shape[0] == rows, "block table: a row a row of q, rows contiguous")
+    _need(cache.is_contiguous() and tuple(cache.shape[1:]) == (2, num_kv_heads, page_size, head_dim), "cache layout")
+    _need(shared.members.numel() == rows == shared.group_of.numel(), "shared: a place for every row")
+    parts = rows * num_heads * (choice.prefix_parts + choice.tail_parts)
+    scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
+    _check(load_library("attention_shared").tb_attention_shared(
+        _ptr(q), _i64(q.stride(0)), _ptr(out), _i64(out.stride(0)), _ptr(cache), _ptr(positions), _ptr(block_table),
+        _i32(block_table.stride(0)), _i32(block_table.shape[1]), _ptr(shared.members), _ptr(shared.group_start),
+        _ptr(shared.prefix), _ptr(shared.group_of), _i32(rows), _i32(shared.prefix.numel()), _i32(num_heads),
+        _i32(num_kv_heads), _i32(head_dim), _i32(page_size), _f32(scale), _i32(choice.tiles), _i32(choice.prefix_parts),
+        _i32(choice.prefix_run), _i32(choice.tail_parts), _i32(choice.tail_run), _ptr(scratch),
+        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(_code(q.dtype)), _stream()),
+        "attention_shared")
+    return out
+
+
 def gemm_f32_nt(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """``out[M,N] = a[M,K] @ w[N,K]^T`` in true 32-bit arithmetic."""
     _cuda(a, w, out)

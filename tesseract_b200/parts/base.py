@@ -284,6 +284,51 @@ class CacheBinding:
     page_size: int = 0
 
 
+SHARED_BLOCK = 64       # keys in common count in whole blocks of this many (attention_shared.cu)
+
+
+@dataclass
+class SharedRows:
+    """Which rows of a decode step have their first keys in common (continuations of one prompt), for one cache group.
+
+    Every row is in exactly one group.  The rows of a group read the same numbers at the first ``prefix`` positions, whichever
+    row's block table they are read through; a row alone in its group has nothing in common with others, whatever its
+    ``prefix``."""
+
+    members: torch.Tensor        # int32 [rows]: the rows, group by group
+    group_start: torch.Tensor    # int32 [groups + 1]: where a group's rows begin in ``members``
+    prefix: torch.Tensor         # int32 [groups]: keys in common, none of them behind the position of a row of the group
+    group_of: torch.Tensor       # int32 [rows]
+    sizes: Tuple[int, ...]       # host copies for decisions: rows of each group,
+    blocks: Tuple[int, ...]      # whole blocks of keys in common (0 for a row alone),
+    longest_tail: int            # and the most keys that a row reads behind them
+
+    @classmethod
+    def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":
+        """``groups``: the rows of each group; ``prefixes``: their keys in common; ``positions``: the position of every row
+        (-1 for a row without keys)."""
+        rows = len(positions)
+        members = [row for group in groups for row in group]
+        if sorted(members) != list(range(rows)):
+            raise ValueError("every row of the step belongs to exactly one group")
+        if len(prefixes) != len(groups) or any(not group for group in groups):
+            raise ValueError("a group has rows and one number of keys in common")
+        group_of, start, blocks, tail = [0] * rows, [0], [], 0
+        for index, (group, prefix) in enumerate(zip(groups, prefixes)):
+            last = min(positions[row] for row in group)
+            if not 0 <= prefix <= last + 1:
+                raise ValueError(f"{prefix} keys in common, but a row of the group reads {last + 1}")
+            start.append(start[-1] + len(group))
+            blocks.append(prefix // SHARED_BLOCK if len(group) > 1 else 0)
+            for row in group:
+                group_of[row] = index
+                tail = max(tail, positions[row] + 1 - blocks[-1] * SHARED_BLOCK)
+        packed = torch.tensor(members + start + list(prefixes) + group_of, dtype=torch.int32).to(device)
+        at_start, at_prefix, at_of = rows, rows + len(start), rows + len(start) + len(groups)
+        return cls(packed[:at_start], packed[at_start:at_prefix], packed[at_prefix:at_of], packed[at_of:],
+                   tuple(len(g) for g in groups), tuple(blocks), tail)
+
+
 @dataclass
 class GroupView:
     """Per-step view of one cache group: a block table row per sequence of the batch."""

@@ -273,6 +273,47 @@ def attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim
     return AttentionPlan(prompt=prompt, split=short_seqs, splits=splits, key_splits=key_splits)
 
 
+@dataclass(frozen=True)
+class SharedAttentionPlan:
+    """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows, common parts in at most ``prefix_parts`` runs
+    of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is shared, every row reads its own keys), what lies
+    behind in at most ``tail_parts`` of at least ``tail_run``."""
+
+    tiles: int
+    prefix_parts: int
+    prefix_run: int
+    tail_parts: int
+    tail_run: int
+
+
+SHARED_MIN_RUN = 4          # blocks of 64 keys: a tile of 16 keys for each of eight warps, twice
+SHARED_MAX_PARTS = 64
+
+
+def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,
+                     sms: Optional[int] = None) -> SharedAttentionPlan:
+    """The plan of attention over groups of rows with keys in common (``shared``: a :class:`SharedRows`)."""
+    return _shared_attention(dtype, num_heads // num_kv_heads, num_kv_heads, head_dim, shared.sizes, shared.blocks,
+                             shared.longest_tail, sms or kernels.sm_count())
+
+
+@lru_cache(maxsize=1024)
+def _shared_attention(dtype, fold, num_kv_heads, head_dim, sizes, blocks, longest_tail, sms) -> SharedAttentionPlan:
+    tile = kernels.attention_shared_tile(dtype)
+    target = 2 * sms                                            # blocks of threads that are resident at once
+    tiles = [-(-n * fold // tile) if n > 1 else 0 for n in sizes]
+    work = sum(t * b for t, b in zip(tiles, blocks)) * num_kv_heads
+    prefix_parts, prefix_run = 0, 1
+    if work:
+        prefix_run = max(SHARED_MIN_RUN, -(-work // target))
+        prefix_parts = min(SHARED_MAX_PARTS, -(-max(blocks) // prefix_run))
+    tail_blocks = -(-max(1, longest_tail) // 64)
+    work = sum(sizes) * -(-fold // tile) * num_kv_heads * tail_blocks
+    tail_run = max(SHARED_MIN_RUN, -(-work // target))
+    tail_parts = min(SHARED_MAX_PARTS, -(-tail_blocks // tail_run))
+    return SharedAttentionPlan(sum(tiles), prefix_parts, prefix_run, tail_parts, tail_run)
+
+
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,
              page_size: int = 16, sms: Optional[int] = None) -> str:
     """The plan of a built model as text: for every distinct layer and the head, the kernel of each operation at
