@@ -14,13 +14,16 @@
 //   attend_mma   bfloat16, tiles of 16 folded rows: every warp streams every eighth tile of 16 keys through a cp.async ring of its
 //                own into mma.sync.m16n8k16; scores and sums in 32 bits, the weights rounded to bfloat16 for their product with the
 //                values (as in this package's other attention kernels in bfloat16: relative 2^-9 of each, averaged over the keys).
+//   attend_tc    bfloat16, head sizes 64 and 128, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor cores.
 //   attend_f32   32-bit, tiles of 8 folded rows, multiply-adds only: a lane scores one key against the tile's rows, then owns a
 //                few columns of the values.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
-#include "common.cuh"
+#include "tma.cuh"
 
 namespace {
+
+using namespace tbtma;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMasked = -1.0e30f;
@@ -46,6 +49,7 @@ struct SharedParams {
     int tail_parts, tail_run;                 // the same behind it
     Paging paging;
     float scale_log2;
+    int* error;                               // set where a bounded wait ran out
 };
 
 // One block's work.
@@ -68,56 +72,59 @@ __device__ __forceinline__ int run_blocks(int blocks, int parts, int run) {
     return (blocks + n - 1) / n;
 }
 
-// Finds the work of block `index`; false if there is none.  Tiles of common parts first, then the parts behind, row by row.
+__device__ __forceinline__ int64_t common_blocks(const SharedParams& p) { return (int64_t)p.tiles * p.kv_heads * p.prefix_parts; }
+
+// The work of block `index` of those for the common parts (TILE folded rows a tile); false if there is none.
 template <int TILE>
-__device__ bool find_work(const SharedParams& p, int64_t index, Work& w) {
-    const int64_t of_prefix = (int64_t)p.tiles * p.kv_heads * p.prefix_parts;
-    if (index < of_prefix) {
-        const int part = (int)(index % p.prefix_parts);
-        const int64_t rest = index / p.prefix_parts;
-        w.kv_head = (int)(rest % p.kv_heads);
-        int tile = (int)(rest / p.kv_heads);
-        // which group: a warp counts the tiles of 32 groups at a time
-        const int lane = threadIdx.x & 31;
-        int group = -1;
-        for (int base = 0; base < p.groups; base += 32) {
-            const int g = base + lane;
-            int mine = 0;
-            if (g < p.groups) {
-                const int n = p.group_start[g + 1] - p.group_start[g];
-                if (n > 1) mine = (n * p.fold + TILE - 1) / TILE;
-            }
-            int up_to = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, up_to, o);
-                if (lane >= o) up_to += other;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, up_to > tile);
-            if (past) {
-                const int who = __ffs(past) - 1;
-                group = base + who;
-                tile -= __shfl_sync(0xffffffffu, up_to - mine, who);
-                break;
-            }
-            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+__device__ bool find_common(const SharedParams& p, int64_t index, Work& w) {
+    const int part = (int)(index % p.prefix_parts);
+    const int64_t rest = index / p.prefix_parts;
+    w.kv_head = (int)(rest % p.kv_heads);
+    int tile = (int)(rest / p.kv_heads);
+    // which group: a warp counts the tiles of 32 groups at a time
+    const int lane = threadIdx.x & 31;
+    int group = -1;
+    for (int base = 0; base < p.groups; base += 32) {
+        const int g = base + lane;
+        int mine = 0;
+        if (g < p.groups) {
+            const int n = p.group_start[g + 1] - p.group_start[g];
+            if (n > 1) mine = (n * p.fold + TILE - 1) / TILE;
         }
-        if (group < 0) return false;
-        const int blocks = common_keys(p, group) / kBlock;
-        if (blocks == 0) return false;
-        const int run = run_blocks(blocks, p.prefix_parts, p.prefix_run);
-        w.begin = part * run * kBlock;
-        w.end = min(blocks, (part + 1) * run) * kBlock;
-        if (w.begin >= w.end) return false;
-        w.first_member = p.group_start[group];
-        w.member_rows = p.group_start[group + 1] - w.first_member;
-        w.row = p.members[w.first_member];
-        w.folded = w.member_rows * p.fold;
-        w.first_folded = tile * TILE;
-        w.part = part;
-        return true;
+        int up_to = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, up_to, o);
+            if (lane >= o) up_to += other;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, up_to > tile);
+        if (past) {
+            const int who = __ffs(past) - 1;
+            group = base + who;
+            tile -= __shfl_sync(0xffffffffu, up_to - mine, who);
+            break;
+        }
+        tile -= __shfl_sync(0xffffffffu, up_to, 31);
     }
-    index -= of_prefix;
+    if (group < 0) return false;
+    const int blocks = common_keys(p, group) / kBlock;
+    if (blocks == 0) return false;
+    const int run = run_blocks(blocks, p.prefix_parts, p.prefix_run);
+    w.begin = part * run * kBlock;
+    w.end = min(blocks, (part + 1) * run) * kBlock;
+    if (w.begin >= w.end) return false;
+    w.first_member = p.group_start[group];
+    w.member_rows = p.group_start[group + 1] - w.first_member;
+    w.row = p.members[w.first_member];
+    w.folded = w.member_rows * p.fold;
+    w.first_folded = tile * TILE;
+    w.part = part;
+    return true;
+}
+
+// The work of block `index` of those for the keys behind, row by row.
+template <int TILE>
+__device__ bool find_tail(const SharedParams& p, int64_t index, Work& w) {
     const int part = (int)(index % p.tail_parts);
     int64_t rest = index / p.tail_parts;
     w.kv_head = (int)(rest % p.kv_heads);
@@ -138,6 +145,12 @@ __device__ bool find_work(const SharedParams& p, int64_t index, Work& w) {
     w.folded = p.fold;
     w.part = p.prefix_parts + part;
     return true;
+}
+
+template <int TILE>
+__device__ __forceinline__ bool find_work(const SharedParams& p, int64_t index, Work& w) {
+    const int64_t common = common_blocks(p);
+    return index < common ? find_common<TILE>(p, index, w) : find_tail<TILE>(p, index - common, w);
 }
 
 // Row of the batch and head of folded row `fr`.
@@ -186,7 +199,6 @@ constexpr int kWarps = D <= 64 ? 8 : D <= 128 ? 6 : 4;
 template <int D>
 constexpr int kStages = D > 64 && D <= 128 ? 2 : 3;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     const int bytes = valid ? 16 : 0;         // (0: the destination is filled with zeros)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
@@ -226,9 +238,9 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
     return (uint32_t)(row * (D * 2) + ((chunk ^ key) << 4));
 }
 
-template <int D>
+template <int D, int WARPS>
 __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* smem) {
-    constexpr int WARPS = kWarps<D>, STAGES = kStages<D>, CH = D / 8, PASSES = kKeys * CH / 32;
+    constexpr int STAGES = kStages<D>, CH = D / 8, PASSES = kKeys * CH / 32;
     constexpr uint32_t kTileBytes = kKeys * D * 2, kStageBytes = 2 * kTileBytes;
     constexpr bool QREG = D <= 128;           // the queries' fragments stay in registers
     constexpr int PITCH = D + 8;              // floats between rows of the sums that are put together (bank conflicts)
@@ -399,14 +411,384 @@ __global__ void __launch_bounds__(kWarps<D> * 32) shared_mma_kernel(const Shared
     pdl_wait();
     pdl_trigger();
     Work w;
-    if (find_work<kRows>(p, blockIdx.x, w)) attend_mma<D>(p, w, smem);
+    if (find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, kWarps<D>>(p, w, smem);
+}
+
+template <int D, int WARPS>
+constexpr size_t mma_bytes() {
+    constexpr size_t tiles = (size_t)kRows * D * 2 + (size_t)WARPS * kStages<D> * 2 * kKeys * D * 2;
+    constexpr size_t meet = (size_t)WARPS * kRows * (2 + D + 8) * sizeof(float);
+    return tiles > meet ? tiles : meet;
+}
+
+// ------------------------------------------------------------------------------------------------ bfloat16, tcgen05
+
+// Common parts of groups with more than 16 folded rows, head sizes 64 and 128: a tile of 128 folded rows against a run of blocks
+// of 64 keys.  Per block S = Q . K^T (tcgen05.mma, M128 x N64, both operands in shared memory as 64-number slices with the
+// 128-byte swizzle, S in 64 columns of tensor memory), the weights 2^(s - m) of a row by the thread that owns it, rounded to
+// bfloat16 into one of two buffers in tensor memory, and O += P . V (M128 x N D x K64, P from tensor memory), O in D columns.
+// No block needs a mask: a common part ends with a block, and what is beyond it belongs to the rows' own parts.
+// Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products; warp 5
+// brings keys and values, page by page, with cp.async.bulk.tensor into rings of their own.  All waits are bounded.
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 192;
+constexpr int kTcWarps = kTcThreads / 32;
+constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
+template <int D>
+constexpr int kTcStages = D == 64 ? 4 : 2;    // 64 KB of keys and values under way either way
+template <int D>
+struct TcShape {
+    static constexpr uint32_t kSlice = kBlock * 128;              // 64 keys x 64 numbers
+    static constexpr uint32_t kBlockBytes = (D / 64) * kSlice;    // a block of keys, or of values
+    static constexpr uint32_t kQSlice = kTcRows * 128, kQBytes = (D / 64) * kQSlice;
+    static constexpr size_t kBytes = (size_t)kQBytes + (size_t)2 * kTcStages<D> * kBlockBytes;
+};
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+// a tile of 128-byte rows with the 128-byte swizzle, 1024 bytes between groups of eight rows
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)lbo << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D = F32, A = B = BF16; b_mn: B is MN-major
+__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, int b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&r)[32]) {      // (tmem_wait_ld before the registers are used)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 template <int D>
-constexpr size_t mma_bytes() {
-    constexpr size_t tiles = (size_t)kRows * D * 2 + (size_t)kWarps<D> * kStages<D> * 2 * kKeys * D * 2;
-    constexpr size_t meet = (size_t)kWarps<D> * kRows * (2 + D + 8) * sizeof(float);
-    return tiles > meet ? tiles : meet;
+__device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMap* cache_map, unsigned char* smem) {
+    using Tiles = TcShape<D>;
+    constexpr int STAGES = kTcStages<D>;
+    constexpr uint32_t kSlice = Tiles::kSlice, kBlockBytes = Tiles::kBlockBytes;
+    // k_full, k_empty, v_full, v_empty [STAGES] each, s_full, s_free, p_ready[2], o_full[2] (of block j: those of j & 1)
+    __shared__ __align__(8) uint64_t bars[4 * STAGES + 6];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = min(kTcRows, w.folded - w.first_folded);
+    const int live_threads = (rows + 31) / 32 * 32;               // of the softmax warps: those with a row
+    const int n_blocks = (w.end - w.begin) / kBlock;
+    const int* table = p.table + (int64_t)w.row * p.table_stride;
+    const uint32_t q_tile = smem_u32(smem), ring = q_tile + Tiles::kQBytes;      // [stage][K | V]
+    const uint32_t k_full = smem_u32(&bars[0]), k_empty = smem_u32(&bars[STAGES]);
+    const uint32_t v_full = smem_u32(&bars[2 * STAGES]), v_empty = smem_u32(&bars[3 * STAGES]);
+    const uint32_t s_full = smem_u32(&bars[4 * STAGES]), s_free = s_full + 8;
+    auto p_ready = [&](int j) { return s_full + 16 + 8 * (j & 1); };
+    auto o_full = [&](int j) { return s_full + 32 + 8 * (j & 1); };
+    auto phase = [&](int j) { return (uint32_t)(j >> 1) & 1u; };
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(k_full + 8 * s, 1);
+            mbar_init(k_empty + 8 * s, 1);
+            mbar_init(v_full + 8 * s, 1);
+            mbar_init(v_empty + 8 * s, 1);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(s_free, live_threads);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(p_ready(b), live_threads);
+            mbar_init(o_full(b), 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_base_slot)), "r"(kTcColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp != 5) {
+        // the queries, while warp 5 already brings the first blocks
+        constexpr int CH = D / 8;
+        const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
+        for (int idx = threadIdx.x; idx < kTcRows * CH; idx += kTcThreads - 32) {
+            const int r = idx / CH, c = idx % CH;
+            const bool ok = r < rows;
+            const __nv_bfloat16* src = q;
+            if (ok) {
+                int row, head;
+                place_of(p, w, w.first_folded + r, row, head);
+                src = q + (int64_t)row * p.q_stride + (int64_t)head * D + c * 8;
+            }
+            cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), src, ok);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_smem();
+        asm volatile("bar.sync 1, 160;" ::: "memory");            // warps 0..4: the issuer reads the queries after this
+    }
+    const uint32_t tmem_base = tmem_base_slot;
+    const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + kBlock;
+    auto tmem_p = [&](int j) { return tmem_o + D + (j & 1) * (kBlock / 2); };
+
+    if (warp == 5) {
+        const int rows_per_copy = min(p.paging.size, kBlock), copies = kBlock / rows_per_copy;      // at most 8
+        bool ok = true;
+        for (int it = 0; it < n_blocks && ok; ++it) {
+            const int s = it % STAGES;
+            int page = 0, in_page = 0;
+            if (lane < copies) {
+                const int key = w.begin + it * kBlock + lane * rows_per_copy;
+                page = table[p.paging.page_of(key)];
+                in_page = p.paging.within(key);
+            }
+            const uint32_t dst = ring + s * 2 * kBlockBytes + (uint32_t)(lane * rows_per_copy) * 128;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                const uint32_t full = (which ? v_full : k_full) + 8 * s, empty = (which ? v_empty : k_empty) + 8 * s;
+                int go = 1;
+                if (lane == 0) {
+                    go = mbar_wait(empty, ((it / STAGES) & 1) ^ 1, &abort_flag) ? 1 : 0;
+                    if (go) mbar_expect_tx(full, kBlockBytes);
+                }
+                go = __shfl_sync(0xffffffffu, go, 0);             // also orders the announcement before the copies
+                if (!go) { ok = false; break; }
+                if (lane < copies) {
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_load_kv(dst + which * kBlockBytes + h * kSlice, cache_map, full, h * 64, in_page, w.kv_head, which, page);
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            abort_flag = 1;
+            atomicExch(p.error, 110);
+        }
+    } else if (warp == 4) {
+        if (lane == 0) {
+            constexpr uint32_t idesc_qk = idesc_bf16(kTcRows, kBlock, 0), idesc_pv = idesc_bf16(kTcRows, D, 1);
+            // (descriptors are moved by adding to their start-address field, bytes >> 4)
+            const uint64_t q_desc = desc_sw128(q_tile, 1), k_desc0 = desc_sw128(ring, 1);
+            const uint64_t v_desc0 = desc_sw128(ring + kBlockBytes, kSlice >> 4);
+            constexpr uint32_t kStageStep = (2 * kBlockBytes) >> 4;
+            auto issue_qk = [&](int s) {
+                tc_fence_after();
+                const uint64_t k_desc = k_desc0 + (uint32_t)s * kStageStep;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_ss(tmem_s, q_desc + (((kk >> 2) * Tiles::kQSlice + (kk & 3) * 32) >> 4),
+                            k_desc + (((kk >> 2) * kSlice + (kk & 3) * 32) >> 4), idesc_qk, kk != 0);
+                umma_commit(s_full);
+                umma_commit(k_empty + 8 * s);
+            };
+            int qs = 0, s = 0;
+            uint32_t q_parity = 0, parity = 0;
+            auto next_q = [&]() { if (++qs == STAGES) { qs = 0; q_parity ^= 1; } };
+            bool ok = mbar_wait(k_full + 8 * qs, q_parity, &abort_flag);
+            if (ok) issue_qk(qs);
+            next_q();
+            for (int j = 0; j < n_blocks && ok; ++j) {
+                if (j + 1 < n_blocks) {
+                    // as soon as the softmax warps hold S_j in registers the next block's scores may take its place
+                    if (!mbar_wait(k_full + 8 * qs, q_parity, &abort_flag) || !mbar_wait(s_free, j & 1, &abort_flag)) { ok = false; break; }
+                    issue_qk(qs);
+                    next_q();
+                }
+                if (!mbar_wait(v_full + 8 * s, parity, &abort_flag) || !mbar_wait(p_ready(j), phase(j), &abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t v_desc = v_desc0 + (uint32_t)s * kStageStep;
+#pragma unroll
+                for (int kk = 0; kk < kBlock / 16; ++kk)
+                    umma_ts(tmem_o, tmem_p(j) + kk * 8, v_desc + ((kk * 2048) >> 4), idesc_pv, kk != 0 || j != 0);
+                umma_commit(o_full(j));
+                umma_commit(v_empty + 8 * s);
+                if (++s == STAGES) { s = 0; parity ^= 1; }
+            }
+            if (!ok) {
+                abort_flag = 1;
+                atomicExch(p.error, 120);
+            }
+        }
+    } else if (warp * 32 < rows) {
+        const int r = warp * 32 + lane;                           // row of the tile = lane of tensor memory
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        // m: the maximum that the stored weights and O are scaled by; it is raised (and O rescaled) only when a block's exceeds it by
+        // more than 2^8, which keeps every weight at or below 256 and makes the rescaling rare
+        float m = kMasked, l = 0.0f;
+        bool ok = true;
+        // what P_j V_j read and wrote in tensor memory may be touched by this thread again (the fence orders it, the barrier alone does not)
+        auto product_done = [&](int j) {
+            if (!mbar_wait(o_full(j), phase(j), &abort_flag)) return false;
+            tc_fence_after();
+            return true;
+        };
+        const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+        for (int j = 0; j < n_blocks; ++j) {
+            if (!mbar_wait(s_full, j & 1, &abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t sc[2][32];
+            tmem_load_32(tmem_s + lane_base, sc[0]);
+            tmem_load_32(tmem_s + lane_base + 32, sc[1]);
+            tmem_wait_ld();
+            tc_fence_before();
+            mbar_arrive(s_free);                                  // S is in registers: the next block's scores may be computed
+            float mx[4] = {kMasked, kMasked, kMasked, kMasked};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(sc[0][i]), __uint_as_float(sc[0][i + 1]));
+                mx[2 + ((i >> 1) & 1)] = max3(mx[2 + ((i >> 1) & 1)], __uint_as_float(sc[1][i]), __uint_as_float(sc[1][i + 1]));
+            }
+            const float block_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+            if (__any_sync(0xffffffffu, block_max > m + 8.0f)) {
+                if (j > 0 && !product_done(j - 1)) { ok = false; break; }
+                const float m_new = fmaxf(m, block_max), correction = fast_exp2(m - m_new);
+                m = m_new;
+                l *= correction;
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t v[16];
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                              "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                            : "r"(tmem_o + lane_base + c * 16) : "memory");
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * correction);
+                        tmem_store_16(tmem_o + lane_base + c * 16, v);
+                    }
+                }
+            }
+            const uint64_t neg_m2 = pack2(-m, -m);
+            uint64_t ls[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float t0, t1;
+                    unpack2(fma2(pack2(__uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1])), scale2, neg_m2), t0, t1);
+                    const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
+                    ls[(i >> 1) & 3] = add2(ls[(i >> 1) & 3], pack2(p0, p1));
+                    sc[c][i >> 1] = pack_bf16(p0, p1);
+                }
+                if (c == 0 && j >= 2 && !product_done(j - 2)) { ok = false; break; }      // it has read this buffer
+                tmem_store_16(tmem_p(j) + lane_base + c * 16, sc[c]);
+            }
+            if (!ok) break;
+            float lo_sum, hi_sum;
+            unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), lo_sum, hi_sum);
+            l += lo_sum + hi_sum;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_ready(j));
+        }
+        if (ok && !product_done(n_blocks - 1)) ok = false;
+        if (ok) {
+            int row = 0, head = 0;
+            if (r < rows) place_of(p, w, w.first_folded + r, row, head);
+            const int64_t slot = slot_of(p, row, head, w.part);
+            float* to = p.part_a + slot * D;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t v[32];
+                tmem_load_32(tmem_o + lane_base + c * 32, v);
+                tmem_wait_ld();
+                if (r < rows) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(to + c * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            if (r < rows) p.part_ml[slot] = make_float2(m, l);
+            tc_fence_before();
+        } else {
+            abort_flag = 1;
+            atomicExch(p.error, 130);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTcColumns) : "memory");
+    }
+}
+
+// The common parts and the parts behind them in one launch: the latter's blocks run beside the former's.
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
+    extern __shared__ __align__(1024) unsigned char tc_smem[];
+    pdl_wait();
+    pdl_trigger();
+    Work w;
+    const int64_t common = common_blocks(p);
+    if (blockIdx.x < common) {
+        if (smem_u32(tc_smem) & 1023u) {                          // never expected: refuse rather than compute garbage
+            if (threadIdx.x == 0) atomicExch(p.error, 199);
+            return;
+        }
+        if (find_common<kTcRows>(p, blockIdx.x, w)) attend_tc<D>(p, w, &cache_map, tc_smem);
+    } else if (find_tail<kRows>(p, blockIdx.x - common, w)) {
+        attend_mma<D, kTcWarps>(p, w, tc_smem);
+    }
+}
+
+template <int D>
+constexpr size_t tc_bytes() {
+    constexpr size_t tail = mma_bytes<D, kTcWarps>();
+    return TcShape<D>::kBytes > tail ? TcShape<D>::kBytes : tail;
 }
 
 // ------------------------------------------------------------------------------------------------ 32-bit
@@ -587,10 +969,26 @@ int launch(Kernel kernel, int64_t blocks, int threads, size_t smem, const Shared
     return tb_launch_status();
 }
 
+template <int D>
+int launch_tc(const CUtensorMap& map, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
+    if (blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
+    const size_t smem = tc_bytes<D>();
+    const cudaError_t err = cudaFuncSetAttribute(shared_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return (int)err;
+    if (cudaError_t launched = tb_launch_pdl(shared_tc_kernel<D>, dim3((unsigned)blocks), dim3(kTcThreads), smem, stream, map, p))
+        return (int)launched;
+    return tb_launch_status();
+}
+
 }  // namespace
 
-// Folded rows of a tile: what `tiles` counts.
-TB_EXPORT int tb_attention_shared_tile(int dtype) { return dtype == TB_F32 ? kF32Rows : kRows; }
+// Folded rows of a tile: what `tiles` counts.  tensor: the form on the tcgen05 tensor cores.
+TB_EXPORT int tb_attention_shared_tile(int dtype, int tensor) { return dtype == TB_F32 ? kF32Rows : tensor ? kTcRows : kRows; }
+
+// Whether that form takes these sizes.
+TB_EXPORT int tb_attention_shared_tensor(int dtype, int head_dim, int page_size) {
+    return dtype == TB_BF16 && (head_dim == 64 || head_dim == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0;
+}
 
 // rows of q and out: [rows, heads * head_dim] with a stride; positions[b]: the last key of row b (-1: none); table: [rows, columns]
 // pages; members, group_start, prefix, group_of: the groups (SharedParams); tiles: the tiles of all groups of two rows or more,
@@ -601,7 +999,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
                                   const int* group_start, const int* prefix, const int* group_of, int rows, int groups, int heads,
                                   int kv_heads, int head_dim, int page_size, float scale, int tiles, int prefix_parts,
                                   int prefix_run, int tail_parts, int tail_run, float* part_a, float* part_ml,
-                                  int64_t part_floats, int dtype, cudaStream_t stream) {
+                                  int64_t part_floats, int tensor, int cache_pages, int* error, int dtype, cudaStream_t stream) {
     if (rows == 0) return 0;
     if (dtype != TB_F32 && dtype != TB_BF16) return TB_ERR_BAD_DTYPE;
     if (rows < 0 || groups < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || page_size < 1 || tiles < 0) return TB_ERR_BAD_SIZE;
@@ -612,6 +1010,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
     const int64_t parts = (int64_t)rows * heads * (prefix_parts + tail_parts);
     if (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim) return -5;
+    if (tensor && (!tb_attention_shared_tensor(dtype, head_dim, page_size) || error == nullptr)) return TB_ERR_BAD_SIZE;
     SharedParams p;
     p.q = q;
     p.out = out;
@@ -642,7 +1041,8 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.tail_run = tail_run;
     p.paging = tb_paging(page_size);
     p.scale_log2 = scale * kLog2e;
-    const int tile = tb_attention_shared_tile(dtype);
+    p.error = error;
+    const int tile = dtype == TB_F32 ? kF32Rows : kRows;                 // of the parts behind
     const int64_t blocks = (int64_t)tiles * kv_heads * prefix_parts +
                            (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
     int status;
@@ -650,14 +1050,18 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
         if (head_dim <= 64) status = launch(shared_f32_kernel<64>, blocks, kF32Warps * 32, f32_bytes<64>(), p, stream);
         else if (head_dim <= 128) status = launch(shared_f32_kernel<128>, blocks, kF32Warps * 32, f32_bytes<128>(), p, stream);
         else status = launch(shared_f32_kernel<256>, blocks, kF32Warps * 32, f32_bytes<256>(), p, stream);
+    } else if (tensor) {
+        CUtensorMap map;
+        if (!make_cache_map(&map, cache, cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
+        status = head_dim == 64 ? launch_tc<64>(map, blocks, p, stream) : launch_tc<128>(map, blocks, p, stream);
     } else if (head_dim <= 32) {
-        status = launch(shared_mma_kernel<32>, blocks, kWarps<32> * 32, mma_bytes<32>(), p, stream);
+        status = launch(shared_mma_kernel<32>, blocks, kWarps<32> * 32, mma_bytes<32, kWarps<32>>(), p, stream);
     } else if (head_dim <= 64) {
-        status = launch(shared_mma_kernel<64>, blocks, kWarps<64> * 32, mma_bytes<64>(), p, stream);
+        status = launch(shared_mma_kernel<64>, blocks, kWarps<64> * 32, mma_bytes<64, kWarps<64>>(), p, stream);
     } else if (head_dim <= 128) {
-        status = launch(shared_mma_kernel<128>, blocks, kWarps<128> * 32, mma_bytes<128>(), p, stream);
+        status = launch(shared_mma_kernel<128>, blocks, kWarps<128> * 32, mma_bytes<128, kWarps<128>>(), p, stream);
     } else {
-        status = launch(shared_mma_kernel<256>, blocks, kWarps<256> * 32, mma_bytes<256>(), p, stream);
+        status = launch(shared_mma_kernel<256>, blocks, kWarps<256> * 32, mma_bytes<256, kWarps<256>>(), p, stream);
     }
     if (status != 0) return status;
     const int64_t joins = ((int64_t)rows * heads + 3) / 4;

@@ -147,8 +147,24 @@ inline const CUtensorMap* cached_map_2d(const void* base, uint64_t rows, uint64_
 }
 
 // Tensor map of one cache entry [pages][K|V][kv head][key][head_dim] (head_dim a multiple of 64), boxes of 64 dims
-// of min(page_size, max_rows) keys of one head.  Maps are kept per (pointer, geometry): a cache entry lives as long
-// as its model.
+// of min(page_size, max_rows) keys of one head.
+inline bool make_cache_map(CUtensorMap* map, const void* cache, int pages, int num_kv_heads, int page_size, int max_rows,
+                           int head_dim) {
+    EncodeTiledFn fn = encode_tiled();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[5] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)num_kv_heads, 2,
+                                (cuuint64_t)pages};
+    const cuuint64_t row = (cuuint64_t)head_dim * 2;
+    const cuuint64_t strides[4] = {row, row * page_size, row * page_size * num_kv_heads,
+                                   row * page_size * num_kv_heads * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)(page_size < max_rows ? page_size : max_rows), 1, 1, 1};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(cache), dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The same, kept per (pointer, geometry): a cache entry lives as long as its model.
 inline const CUtensorMap* cache_map_for(const void* cache, int pages, int num_kv_heads, int page_size, int max_rows,
                                         int head_dim) {
     static std::mutex lock;
@@ -157,20 +173,8 @@ inline const CUtensorMap* cache_map_for(const void* cache, int pages, int num_kv
     const auto key = std::make_tuple(cache, pages, num_kv_heads, page_size, max_rows, head_dim);
     auto found = maps.find(key);
     if (found != maps.end()) return &found->second;
-    EncodeTiledFn fn = encode_tiled();
-    if (fn == nullptr) return nullptr;
     CUtensorMap map;
-    const cuuint64_t dims[5] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)num_kv_heads, 2,
-                                (cuuint64_t)pages};
-    const cuuint64_t row = (cuuint64_t)head_dim * 2;
-    const cuuint64_t strides[4] = {row, row * page_size, row * page_size * num_kv_heads,
-                                   row * page_size * num_kv_heads * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)(page_size < max_rows ? page_size : max_rows), 1, 1, 1};
-    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
-    if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(cache), dims, strides, box, elem,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return nullptr;
+    if (!make_cache_map(&map, cache, pages, num_kv_heads, page_size, max_rows, head_dim)) return nullptr;
     return &maps.emplace(key, map).first->second;
 }
 

@@ -298,9 +298,14 @@ def attention_rows(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, posi
     return out
 
 
-def attention_shared_tile(dtype: torch.dtype) -> int:
+def attention_shared_tensor(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    """Whether ``attention_shared`` has a form on the tcgen05 tensor cores for these sizes."""
+    return bool(load_library("attention_shared").tb_attention_shared_tensor(_i32(_code(dtype)), _i32(head_dim), _i32(page_size)))
+
+
+def attention_shared_tile(dtype: torch.dtype, tensor: bool = False) -> int:
     """Folded rows (rows of a group times query heads per kv head) that a block of ``attention_shared`` takes."""
-    return {torch.float32: 8, torch.bfloat16: 16}[dtype]
+    return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if tensor else 0))
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
@@ -321,6 +326,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
           and block_table.shape[0] == rows, "block table: a row a row of q, rows contiguous")
     _need(cache.is_contiguous() and tuple(cache.shape[1:]) == (2, num_kv_heads, page_size, head_dim), "cache layout")
     _need(shared.members.numel() == rows == shared.group_of.numel(), "shared: a place for every row")
+    _need(scale > 0.0, "the scale of the scores must be positive")
     parts = rows * num_heads * (choice.prefix_parts + choice.tail_parts)
     scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(load_library("attention_shared").tb_attention_shared(
@@ -329,8 +335,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
         _ptr(shared.prefix), _ptr(shared.group_of), _i32(rows), _i32(shared.prefix.numel()), _i32(num_heads),
         _i32(num_kv_heads), _i32(head_dim), _i32(page_size), _f32(scale), _i32(choice.tiles), _i32(choice.prefix_parts),
         _i32(choice.prefix_run), _i32(choice.tail_parts), _i32(choice.tail_run), _ptr(scratch),
-        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(_code(q.dtype)), _stream()),
-        "attention_shared")
+        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(1 if choice.tensor else 0),
+        _i32(cache.shape[0]), _ptr(_error_word(q.device)), _i32(_code(q.dtype)), _stream()), "attention_shared")
     return out
 
 

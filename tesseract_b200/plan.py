@@ -275,15 +275,16 @@ def attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim
 
 @dataclass(frozen=True)
 class SharedAttentionPlan:
-    """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows, common parts in at most ``prefix_parts`` runs
-    of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is shared, every row reads its own keys), what lies
-    behind in at most ``tail_parts`` of at least ``tail_run``."""
+    """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows (``tensor``: of 128, on the tcgen05 tensor
+    cores), common parts in at most ``prefix_parts`` runs of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is
+    shared, every row reads its own keys), what lies behind in at most ``tail_parts`` of at least ``tail_run``."""
 
     tiles: int
     prefix_parts: int
     prefix_run: int
     tail_parts: int
     tail_run: int
+    tensor: bool = False
 
 
 SHARED_MIN_RUN = 4          # blocks of 64 keys: a tile of 16 keys for each of eight warps, twice
@@ -293,25 +294,36 @@ SHARED_MAX_PARTS = 64
 def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,
                      sms: Optional[int] = None) -> SharedAttentionPlan:
     """The plan of attention over groups of rows with keys in common (``shared``: a :class:`SharedRows`)."""
-    return _shared_attention(dtype, num_heads // num_kv_heads, num_kv_heads, head_dim, shared.sizes, shared.blocks,
+    return _shared_attention(dtype, num_heads // num_kv_heads, num_kv_heads, head_dim, page_size, shared.sizes, shared.blocks,
                              shared.longest_tail, sms or kernels.sm_count())
 
 
+def _shared_runs(tiles: Sequence[int], blocks: Sequence[int], target: int) -> int:
+    """The shortest runs (in blocks) with which all tiles' runs are at most ``target``."""
+    run = max(SHARED_MIN_RUN, -(-sum(t * b for t, b in zip(tiles, blocks)) // target))
+    while run < max(blocks) and sum(t * -(-b // run) for t, b in zip(tiles, blocks)) > target:
+        run += 1
+    return run
+
+
 @lru_cache(maxsize=1024)
-def _shared_attention(dtype, fold, num_kv_heads, head_dim, sizes, blocks, longest_tail, sms) -> SharedAttentionPlan:
-    tile = kernels.attention_shared_tile(dtype)
-    target = 2 * sms                                            # blocks of threads that are resident at once
-    tiles = [-(-n * fold // tile) if n > 1 else 0 for n in sizes]
-    work = sum(t * b for t, b in zip(tiles, blocks)) * num_kv_heads
+def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, sizes, blocks, longest_tail, sms) -> SharedAttentionPlan:
+    target = max(1, 2 * sms // num_kv_heads)                    # blocks of threads that are resident at once, a kv head
+    shared_rows = [n * fold if b > 0 else 0 for n, b in zip(sizes, blocks)]
+    tensor = max(shared_rows) > 16 and kernels.attention_shared_tensor(dtype, head_dim, page_size)
+    tile = kernels.attention_shared_tile(dtype, tensor)
+    tiles = [-(-rows // tile) for rows in shared_rows]
     prefix_parts, prefix_run = 0, 1
-    if work:
-        prefix_run = max(SHARED_MIN_RUN, -(-work // target))
+    if any(tiles):
+        prefix_run = _shared_runs(tiles, blocks, target)
         prefix_parts = min(SHARED_MAX_PARTS, -(-max(blocks) // prefix_run))
     tail_blocks = -(-max(1, longest_tail) // 64)
-    work = sum(sizes) * -(-fold // tile) * num_kv_heads * tail_blocks
-    tail_run = max(SHARED_MIN_RUN, -(-work // target))
+    tail_tiles = sum(sizes) * -(-fold // kernels.attention_shared_tile(dtype))
+    tail_run = max(SHARED_MIN_RUN, -(-tail_tiles * tail_blocks // target))
     tail_parts = min(SHARED_MAX_PARTS, -(-tail_blocks // tail_run))
-    return SharedAttentionPlan(sum(tiles), prefix_parts, prefix_run, tail_parts, tail_run)
+    # (the kernel counts the tiles of every group of two rows or more, whether or not a whole block is shared)
+    counted = sum(-(-n * fold // tile) for n in sizes if n > 1)
+    return SharedAttentionPlan(counted, prefix_parts, prefix_run, tail_parts, tail_run, tensor)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,

@@ -172,6 +172,19 @@ def test_any_cut_gives_the_same_numbers(dtype):
     assert torch.equal(case.run(more), case.run(base))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [4, 5, 8, 9, 16, 24, 33, 70])
+def test_both_forms_in_bfloat16(rows, dim):
+    """The tensor cores' form (tiles of 128 folded rows) and the one of 16, at every count of rows, whichever the plan takes."""
+    case = Case([(1030, [1031 + 7 * i % 90 for i in range(rows)]), (192, [200, 250])], 8, 2, dim, seed=rows)
+    for tensor in (False, True):
+        tile = kernels.attention_shared_tile(torch.bfloat16, tensor)
+        tiles = sum(-(-n * 4 // tile) for n in (rows, 2))
+        for parts, run in ((1, 1), (5, 2)):
+            case.check(plan.SharedAttentionPlan(tiles, parts, run, 2, 1, tensor))
+    assert kernels.tcgen05_error() == 0
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_the_same_bits_every_time(dtype):
     case = Case([(900, [901 + 5 * i for i in range(40)])], 32, 8, 128, dtype=dtype, seed=9)
@@ -253,7 +266,7 @@ def test_refusals():
                         ("out", out.float()), ("out", out.cpu()), ("cache", case.cache.transpose(2, 3)), ("cache", case.cache.float()),
                         ("positions", case.positions.long()), ("positions", case.positions[:1]), ("block_table", case.table.long()),
                         ("block_table", case.table[:1]), ("page_size", 8), ("num_heads", 4), ("head_dim", 32),
-                        ("shared", small.shared)]:
+                        ("shared", small.shared), ("scale", 0.0), ("scale", -1.0), ("scale", math.nan)]:
         with pytest.raises(kernels.KernelError):
             kernels.attention_shared(**{**good, name: value})
     for dim in (8, 24, 272):
