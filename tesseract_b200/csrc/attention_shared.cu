@@ -37,8 +37,9 @@ struct SharedParams {
     const int* table;                         // [rows, table_stride]
     const int* members;                       // [rows]: the rows group by group
     const int* group_start;                   // [groups + 1]: where a group's rows begin in `members`
-    const int* prefix;                        // [groups]: keys in common
-    const int* group_of;                      // [rows]
+    const int* leader;                        // [groups]: the row through whose table the keys in common are read
+    const int* prefix;                        // [groups]: keys in common (whole blocks; 0 for a row alone)
+    const int* common;                        // [rows]: those of the row's group
     float* part_a;                            // [rows][heads][parts][head_dim]
     float2* part_ml;                          // [rows][heads][parts]
     int64_t q_stride, out_stride;
@@ -49,6 +50,7 @@ struct SharedParams {
     int tail_parts, tail_run;                 // the same behind it
     Paging paging;
     float scale_log2;
+    int tensor;                               // the common parts are attend_tc's
     int* error;                               // set where a bounded wait ran out
 };
 
@@ -61,9 +63,9 @@ struct Work {
     int part;                                 // slot of the partial result
 };
 
-__device__ __forceinline__ int common_keys(const SharedParams& p, int group) {
-    if (p.prefix_parts == 0 || p.group_start[group + 1] - p.group_start[group] < 2) return 0;
-    return min(p.prefix[group], p.table_keys) & ~(kBlock - 1);
+// Keys in common as the kernel takes them: none where nothing is shared, and no more than a table can name.
+__device__ __forceinline__ int common_keys(const SharedParams& p, int keys) {
+    return p.prefix_parts == 0 ? 0 : min(keys, p.table_keys) & ~(kBlock - 1);
 }
 
 // How `blocks` blocks of keys are cut: runs of the same number of blocks, at most `parts`.  Returns the blocks of a run.
@@ -81,15 +83,17 @@ __device__ bool find_common(const SharedParams& p, int64_t index, Work& w) {
     const int64_t rest = index / p.prefix_parts;
     w.kv_head = (int)(rest % p.kv_heads);
     int tile = (int)(rest / p.kv_heads);
-    // which group: a warp counts the tiles of 32 groups at a time
+    // which group: a warp counts the tiles of 32 groups at a time (all that is known of a group is loaded at once)
     const int lane = threadIdx.x & 31;
-    int group = -1;
     for (int base = 0; base < p.groups; base += 32) {
         const int g = base + lane;
-        int mine = 0;
+        int start = 0, n = 0, keys = 0, leader = 0, mine = 0;
         if (g < p.groups) {
-            const int n = p.group_start[g + 1] - p.group_start[g];
-            if (n > 1) mine = (n * p.fold + TILE - 1) / TILE;
+            start = p.group_start[g];
+            n = p.group_start[g + 1] - start;
+            keys = common_keys(p, p.prefix[g]);
+            leader = p.leader[g];
+            if (keys > 0) mine = (n * p.fold + TILE - 1) / TILE;
         }
         int up_to = mine;
 #pragma unroll
@@ -98,28 +102,25 @@ __device__ bool find_common(const SharedParams& p, int64_t index, Work& w) {
             if (lane >= o) up_to += other;
         }
         const unsigned past = __ballot_sync(0xffffffffu, up_to > tile);
-        if (past) {
-            const int who = __ffs(past) - 1;
-            group = base + who;
-            tile -= __shfl_sync(0xffffffffu, up_to - mine, who);
-            break;
+        if (past == 0) {
+            tile -= __shfl_sync(0xffffffffu, up_to, 31);
+            continue;
         }
-        tile -= __shfl_sync(0xffffffffu, up_to, 31);
+        const int who = __ffs(past) - 1;
+        tile -= __shfl_sync(0xffffffffu, up_to - mine, who);
+        const int blocks = __shfl_sync(0xffffffffu, keys, who) / kBlock;
+        const int run = run_blocks(blocks, p.prefix_parts, p.prefix_run);
+        w.begin = part * run * kBlock;
+        w.end = min(blocks, (part + 1) * run) * kBlock;
+        w.first_member = __shfl_sync(0xffffffffu, start, who);
+        w.member_rows = __shfl_sync(0xffffffffu, n, who);
+        w.row = __shfl_sync(0xffffffffu, leader, who);
+        w.folded = w.member_rows * p.fold;
+        w.first_folded = tile * TILE;
+        w.part = part;
+        return w.begin < w.end;
     }
-    if (group < 0) return false;
-    const int blocks = common_keys(p, group) / kBlock;
-    if (blocks == 0) return false;
-    const int run = run_blocks(blocks, p.prefix_parts, p.prefix_run);
-    w.begin = part * run * kBlock;
-    w.end = min(blocks, (part + 1) * run) * kBlock;
-    if (w.begin >= w.end) return false;
-    w.first_member = p.group_start[group];
-    w.member_rows = p.group_start[group + 1] - w.first_member;
-    w.row = p.members[w.first_member];
-    w.folded = w.member_rows * p.fold;
-    w.first_folded = tile * TILE;
-    w.part = part;
-    return true;
+    return false;
 }
 
 // The work of block `index` of those for the keys behind, row by row.
@@ -133,7 +134,7 @@ __device__ bool find_tail(const SharedParams& p, int64_t index, Work& w) {
     w.row = (int)(rest / tiles);
     if (w.row >= p.rows) return false;
     w.first_folded = (int)(rest % tiles) * TILE;
-    const int first = common_keys(p, p.group_of[w.row]);
+    const int first = common_keys(p, p.common[w.row]);
     const int last = min(p.positions[w.row] + 1, p.table_keys);
     if (last <= first) return false;
     const int blocks = (last - first + kBlock - 1) / kBlock;
@@ -405,13 +406,14 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
     leave_run<kRows, PITCH, WARPS>(p, w, ml, acc);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kWarps<D> * 32) shared_mma_kernel(const SharedParams p) {
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) shared_mma_kernel(const SharedParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     pdl_wait();
-    pdl_trigger();
+    pdl_trigger();                            // (only now: the kernels behind read what is older than this one without a wait of their own)
     Work w;
-    if (find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, kWarps<D>>(p, w, smem);
+    // (tensor: the common parts are the next kernel's)
+    if (p.tensor ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS>(p, w, smem);
 }
 
 template <int D, int WARPS>
@@ -432,7 +434,6 @@ constexpr size_t mma_bytes() {
 // brings keys and values, page by page, with cp.async.bulk.tensor into rings of their own.  All waits are bounded.
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 192;
-constexpr int kTcWarps = kTcThreads / 32;
 constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
 template <int D>
 constexpr int kTcStages = D == 64 ? 4 : 2;    // 64 KB of keys and values under way either way
@@ -559,19 +560,18 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     __syncthreads();
     tc_fence_after();
     if (warp != 5) {
-        // the queries, while warp 5 already brings the first blocks
-        constexpr int CH = D / 8;
-        const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
-        for (int idx = threadIdx.x; idx < kTcRows * CH; idx += kTcThreads - 32) {
-            const int r = idx / CH, c = idx % CH;
-            const bool ok = r < rows;
-            const __nv_bfloat16* src = q;
-            if (ok) {
+        // the queries, a thread a row, while warp 5 already brings the first blocks
+        const int r = threadIdx.x;
+        if (r < kTcRows) {
+            const __nv_bfloat16* src = (const __nv_bfloat16*)p.q;
+            if (r < rows) {
                 int row, head;
                 place_of(p, w, w.first_folded + r, row, head);
-                src = q + (int64_t)row * p.q_stride + (int64_t)head * D + c * 8;
+                src += (int64_t)row * p.q_stride + (int64_t)head * D;
             }
-            cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), src, ok);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+                cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), src + c * 8, r < rows);
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -662,6 +662,9 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         }
     } else if (warp * 32 < rows) {
         const int r = warp * 32 + lane;                           // row of the tile = lane of tensor memory
+        int row = 0, head = 0;
+        if (r < rows) place_of(p, w, w.first_folded + r, row, head);
+        const int64_t slot = slot_of(p, row, head, w.part);
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
         // m: the maximum that the stored weights and O are scaled by; it is raised (and O rescaled) only when a block's exceeds it by
         // more than 2^8, which keeps every weight at or below 256 and makes the rescaling rare
@@ -736,22 +739,29 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         }
         if (ok && !product_done(n_blocks - 1)) ok = false;
         if (ok) {
-            int row = 0, head = 0;
-            if (r < rows) place_of(p, w, w.first_folded + r, row, head);
-            const int64_t slot = slot_of(p, row, head, w.part);
-            float* to = p.part_a + slot * D;
+            // The row's sums go through shared memory (the queries and the rings are done with: the last product is) and from there
+            // as one bulk copy a row: stored from registers, 16 bytes a thread, the tile's 64 KB took 6 us.
+            constexpr uint32_t kPitch = D * 4 + 16;               // 16-byte stores of neighbouring rows lie on different banks
+            static_assert((size_t)kTcRows * kPitch <= TcShape<D>::kBytes, "the sums fit where the queries and the rings were");
+            const uint32_t staged = smem_u32(smem) + r * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t v[32];
                 tmem_load_32(tmem_o + lane_base + c * 32, v);
                 tmem_wait_ld();
-                if (r < rows) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(to + c * 32 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                }
+                for (int i = 0; i < 32; i += 4)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(staged + (c * 32 + i) * 4), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]) : "memory");
+            }
+            fence_async_smem();
+            if (r < rows) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                             ::"l"(p.part_a + slot * D), "r"(staged), "r"(D * 4) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
             if (r < rows) p.part_ml[slot] = make_float2(m, l);
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             tc_fence_before();
         } else {
             abort_flag = 1;
@@ -766,29 +776,20 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     }
 }
 
-// The common parts and the parts behind them in one launch: the latter's blocks run beside the former's.
+// Launched behind the kernel of the rows' own keys, whose blocks let it start once they have waited for what was in front of them:
+// so everything this kernel reads is there from the start, and its blocks fill the multiprocessors as those end.  What the
+// kernel behind reads of both is there once this one is done, so it waits for the one in front before it ends.
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
     extern __shared__ __align__(1024) unsigned char tc_smem[];
-    pdl_wait();
     pdl_trigger();
     Work w;
-    const int64_t common = common_blocks(p);
-    if (blockIdx.x < common) {
-        if (smem_u32(tc_smem) & 1023u) {                          // never expected: refuse rather than compute garbage
-            if (threadIdx.x == 0) atomicExch(p.error, 199);
-            return;
-        }
-        if (find_common<kTcRows>(p, blockIdx.x, w)) attend_tc<D>(p, w, &cache_map, tc_smem);
-    } else if (find_tail<kRows>(p, blockIdx.x - common, w)) {
-        attend_mma<D, kTcWarps>(p, w, tc_smem);
+    if (smem_u32(tc_smem) & 1023u) {                              // never expected: refuse rather than compute garbage
+        if (threadIdx.x == 0) atomicExch(p.error, 199);
+    } else if (find_common<kTcRows>(p, blockIdx.x, w)) {
+        attend_tc<D>(p, w, &cache_map, tc_smem);
     }
-}
-
-template <int D>
-constexpr size_t tc_bytes() {
-    constexpr size_t tail = mma_bytes<D, kTcWarps>();
-    return TcShape<D>::kBytes > tail ? TcShape<D>::kBytes : tail;
+    pdl_wait();
 }
 
 // ------------------------------------------------------------------------------------------------ 32-bit
@@ -916,17 +917,23 @@ constexpr size_t f32_bytes() {
 
 // ------------------------------------------------------------------------------------------------ the runs put together
 
-// A warp a (row, head): the weights of its runs 32 at a time, then the columns.
-template <typename T>
+// A warp a (row, head).  Its lanes read the maxima and sums of all runs at once (four a lane: kMaxParts), and their weights stay in
+// registers; then LANES lanes read a run's sums, 16 bytes each (for more than 128 columns twice), and 32 / LANES runs side by
+// side, eight loads under way a lane.  (One load of a maximum after the other, a run at a time, took 31 us for 64 rows of 32 heads of
+// 18 runs; this 5.)
+constexpr int kMaxParts = 128;
+template <typename T, int LANES>
 __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
-    pdl_wait();
-    pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (index >= (int64_t)p.rows * p.heads) return;
+    if (index >= (int64_t)p.rows * p.heads) {
+        pdl_wait();
+        return;
+    }
     const int row = (int)(index / p.heads), head = (int)(index % p.heads);
-    // the runs that the row has: the same rule as where they were made
-    const int common = common_keys(p, p.group_of[row]), last = min(p.positions[row] + 1, p.table_keys);
+    // The runs that the row has: the same rule as where they were made.  (The kernel in front lets this one start only once it has
+    // itself waited for what made the index arrays, so they may be read before its results are waited for.)
+    const int common = common_keys(p, p.common[row]), last = min(p.positions[row] + 1, p.table_keys);
     int of_prefix = 0, of_tail = 0;
     if (common > 0) {
         const int run = run_blocks(common / kBlock, p.prefix_parts, p.prefix_run);
@@ -937,24 +944,75 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
         of_tail = (blocks + run - 1) / run;
     }
     const int64_t slot = slot_of(p, row, head, 0);
-    const float2* ml = p.part_ml + slot;
-    auto slot_at = [&](int s) { return s < of_prefix ? s : p.prefix_parts + s - of_prefix; };
-    const int parts = of_prefix + of_tail;
-    float big = kMasked;
-    for (int s = lane; s < parts; s += 32) big = fmaxf(big, ml[slot_at(s)].x);
+    const int parts = of_prefix + of_tail, gap = p.prefix_parts - of_prefix;      // run s is in slot s, or s + gap behind the common part
+    float weight[kMaxParts / 32], sum = 0.0f, big = kMasked;
+    float2 ml[kMaxParts / 32];
+    pdl_wait();
+    pdl_trigger();
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 32; ++i) {
+        const int s = i * 32 + lane;
+        ml[i] = s < parts ? p.part_ml[slot + (s < of_prefix ? s : s + gap)] : make_float2(kMasked, 0.0f);
+        big = fmaxf(big, ml[i].x);
+    }
     big = warp_max(big);
-    float sum = 0.0f;
-    for (int s = 0; s < parts; ++s) {
-        const float2 v = ml[slot_at(s)];
-        sum += exp2f(v.x - big) * v.y;
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 32; ++i) {
+        weight[i] = i * 32 + lane < parts ? exp2f(ml[i].x - big) : 0.0f;
+        sum += weight[i] * ml[i].y;
+    }
+    sum = warp_sum(sum);
+    constexpr int AHEAD = 8;                                                      // loads under way
+    constexpr int ASIDE = 32 / LANES, TAKES = LANES == 32 ? 2 : 1;                // runs side by side; 16-byte columns of a lane
+    const int who = lane / LANES, col = (lane % LANES) * 4;
+    float4 a[TAKES];
+#pragma unroll
+    for (int c = 0; c < TAKES; ++c) a[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float* from = p.part_a + slot * p.head_dim;
+    for (int i = 0; i * 32 < parts; ++i) {
+        float chunk = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 32; ++k) chunk = k == i ? weight[k] : chunk;
+        const int here = min(32, parts - i * 32);
+        for (int s0 = 0; s0 < here; s0 += ASIDE * AHEAD) {
+            float4 v[AHEAD][TAKES];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int run = i * 32 + min(s0 + u * ASIDE + who, here - 1);     // (beyond the last: the last once more, with no weight)
+                const float* of_run = from + (int64_t)(run < of_prefix ? run : run + gap) * p.head_dim;
+#pragma unroll
+                for (int c = 0; c < TAKES; ++c)
+                    v[u][c] = *reinterpret_cast<const float4*>(of_run + min(col + c * 128, p.head_dim - 4));
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int s = s0 + u * ASIDE + who;
+                const float w = __shfl_sync(0xffffffffu, chunk, s & 31) * (s < here ? 1.0f : 0.0f);
+#pragma unroll
+                for (int c = 0; c < TAKES; ++c) {
+                    a[c].x = fmaf(w, v[u][c].x, a[c].x);
+                    a[c].y = fmaf(w, v[u][c].y, a[c].y);
+                    a[c].z = fmaf(w, v[u][c].z, a[c].z);
+                    a[c].w = fmaf(w, v[u][c].w, a[c].w);
+                }
+            }
+        }
     }
     const float inverse = parts > 0 ? 1.0f / sum : 0.0f;
     T* out = (T*)p.out + (int64_t)row * p.out_stride + (int64_t)head * p.head_dim;
-    for (int col = lane; col < p.head_dim; col += 32) {
-        float a = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < parts; ++s) a += exp2f(ml[slot_at(s)].x - big) * p.part_a[(slot + slot_at(s)) * p.head_dim + col];
-        Elem<T>::store(out + col, a * inverse);
+#pragma unroll
+    for (int c = 0; c < TAKES; ++c) {
+        float v[4] = {a[c].x, a[c].y, a[c].z, a[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int o = LANES; o < 32; o <<= 1) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o);
+            v[e] *= inverse;
+        }
+        if (who == 0 && col + c * 128 < p.head_dim) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Elem<T>::store(out + col + c * 128 + e, v[e]);
+        }
     }
 }
 
@@ -969,10 +1027,17 @@ int launch(Kernel kernel, int64_t blocks, int threads, size_t smem, const Shared
     return tb_launch_status();
 }
 
+// warps 2: blocks of two warps (where there are enough of them to fill the chip), else as many as share a multiprocessor in pairs.
+template <int D>
+int launch_mma(int warps, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
+    if (warps == 2) return launch(shared_mma_kernel<D, 2>, blocks, 64, mma_bytes<D, 2>(), p, stream);
+    return launch(shared_mma_kernel<D, kWarps<D>>, blocks, kWarps<D> * 32, mma_bytes<D, kWarps<D>>(), p, stream);
+}
+
 template <int D>
 int launch_tc(const CUtensorMap& map, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
     if (blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
-    const size_t smem = tc_bytes<D>();
+    const size_t smem = TcShape<D>::kBytes;
     const cudaError_t err = cudaFuncSetAttribute(shared_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return (int)err;
     if (cudaError_t launched = tb_launch_pdl(shared_tc_kernel<D>, dim3((unsigned)blocks), dim3(kTcThreads), smem, stream, map, p))
@@ -991,20 +1056,20 @@ TB_EXPORT int tb_attention_shared_tensor(int dtype, int head_dim, int page_size)
 }
 
 // rows of q and out: [rows, heads * head_dim] with a stride; positions[b]: the last key of row b (-1: none); table: [rows, columns]
-// pages; members, group_start, prefix, group_of: the groups (SharedParams); tiles: the tiles of all groups of two rows or more,
+// pages; members, group_start, leader, prefix, common: the groups (SharedParams); tiles: the tiles of all groups with keys in common,
 // ceil(rows of the group * heads / kv_heads / tile) each, no fewer.  prefix[g] is at most positions[b] + 1 for the rows of the group.
 // part_a, part_ml: rows * heads * (prefix_parts + tail_parts) * (head_dim and 2) floats.
 TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* cache,
                                   const int* positions, const int* table, int table_stride, int table_columns, const int* members,
-                                  const int* group_start, const int* prefix, const int* group_of, int rows, int groups, int heads,
+                                  const int* group_start, const int* leader, const int* prefix, const int* common, int rows, int groups, int heads,
                                   int kv_heads, int head_dim, int page_size, float scale, int tiles, int prefix_parts,
                                   int prefix_run, int tail_parts, int tail_run, float* part_a, float* part_ml,
-                                  int64_t part_floats, int tensor, int cache_pages, int* error, int dtype, cudaStream_t stream) {
+                                  int64_t part_floats, int warps, int tensor, int cache_pages, int* error, int dtype, cudaStream_t stream) {
     if (rows == 0) return 0;
     if (dtype != TB_F32 && dtype != TB_BF16) return TB_ERR_BAD_DTYPE;
     if (rows < 0 || groups < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || page_size < 1 || tiles < 0) return TB_ERR_BAD_SIZE;
     if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0) return TB_ERR_BAD_SIZE;
-    if (prefix_parts < 0 || tail_parts < 1 || prefix_run < 1 || tail_run < 1) return TB_ERR_BAD_SIZE;
+    if (prefix_parts < 0 || tail_parts < 1 || prefix_parts + tail_parts > kMaxParts || prefix_run < 1 || tail_run < 1) return TB_ERR_BAD_SIZE;
     const int element = dtype == TB_F32 ? 4 : 2;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)part_a) % 16 != 0) return TB_ERR_BAD_ALIGN;
     if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
@@ -1019,8 +1084,9 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.table = table;
     p.members = members;
     p.group_start = group_start;
+    p.leader = leader;
     p.prefix = prefix;
-    p.group_of = group_of;
+    p.common = common;
     p.part_a = part_a;
     p.part_ml = (float2*)part_ml;
     p.q_stride = q_stride;
@@ -1041,30 +1107,34 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.tail_run = tail_run;
     p.paging = tb_paging(page_size);
     p.scale_log2 = scale * kLog2e;
+    p.tensor = tensor;
     p.error = error;
     const int tile = dtype == TB_F32 ? kF32Rows : kRows;                 // of the parts behind
-    const int64_t blocks = (int64_t)tiles * kv_heads * prefix_parts +
-                           (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
+    const int64_t of_common = (int64_t)tiles * kv_heads * prefix_parts;
+    const int64_t blocks = (tensor ? 0 : of_common) + (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
     int status;
     if (dtype == TB_F32) {
         if (head_dim <= 64) status = launch(shared_f32_kernel<64>, blocks, kF32Warps * 32, f32_bytes<64>(), p, stream);
         else if (head_dim <= 128) status = launch(shared_f32_kernel<128>, blocks, kF32Warps * 32, f32_bytes<128>(), p, stream);
         else status = launch(shared_f32_kernel<256>, blocks, kF32Warps * 32, f32_bytes<256>(), p, stream);
-    } else if (tensor) {
-        CUtensorMap map;
-        if (!make_cache_map(&map, cache, cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
-        status = head_dim == 64 ? launch_tc<64>(map, blocks, p, stream) : launch_tc<128>(map, blocks, p, stream);
-    } else if (head_dim <= 32) {
-        status = launch(shared_mma_kernel<32>, blocks, kWarps<32> * 32, mma_bytes<32, kWarps<32>>(), p, stream);
-    } else if (head_dim <= 64) {
-        status = launch(shared_mma_kernel<64>, blocks, kWarps<64> * 32, mma_bytes<64, kWarps<64>>(), p, stream);
-    } else if (head_dim <= 128) {
-        status = launch(shared_mma_kernel<128>, blocks, kWarps<128> * 32, mma_bytes<128, kWarps<128>>(), p, stream);
     } else {
-        status = launch(shared_mma_kernel<256>, blocks, kWarps<256> * 32, mma_bytes<256, kWarps<256>>(), p, stream);
+        if (head_dim <= 32) status = launch_mma<32>(warps, blocks, p, stream);
+        else if (head_dim <= 64) status = launch_mma<64>(warps, blocks, p, stream);
+        else if (head_dim <= 128) status = launch_mma<128>(warps, blocks, p, stream);
+        else status = launch_mma<256>(warps, blocks, p, stream);
+        if (status == 0 && tensor && of_common > 0) {
+            CUtensorMap map;
+            if (!make_cache_map(&map, cache, cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
+            status = head_dim == 64 ? launch_tc<64>(map, of_common, p, stream) : launch_tc<128>(map, of_common, p, stream);
+        }
     }
     if (status != 0) return status;
     const int64_t joins = ((int64_t)rows * heads + 3) / 4;
-    return dtype == TB_F32 ? launch(shared_join_kernel<float>, joins, 128, 0, p, stream)
-                           : launch(shared_join_kernel<__nv_bfloat16>, joins, 128, 0, p, stream);
+    if (dtype == TB_F32)
+        return launch(head_dim <= 32 ? shared_join_kernel<float, 8> : head_dim <= 64 ? shared_join_kernel<float, 16>
+                                                                                     : shared_join_kernel<float, 32>,
+                      joins, 128, 0, p, stream);
+    return launch(head_dim <= 32 ? shared_join_kernel<__nv_bfloat16, 8> : head_dim <= 64 ? shared_join_kernel<__nv_bfloat16, 16>
+                                                                                         : shared_join_kernel<__nv_bfloat16, 32>,
+                  joins, 128, 0, p, stream);
 }

@@ -325,17 +325,17 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     _need(block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
           and block_table.shape[0] == rows, "block table: a row a row of q, rows contiguous")
     _need(cache.is_contiguous() and tuple(cache.shape[1:]) == (2, num_kv_heads, page_size, head_dim), "cache layout")
-    _need(shared.members.numel() == rows == shared.group_of.numel(), "shared: a place for every row")
+    _need(shared.members.numel() == rows == shared.common.numel(), "shared: a place for every row")
     _need(scale > 0.0, "the scale of the scores must be positive")
     parts = rows * num_heads * (choice.prefix_parts + choice.tail_parts)
     scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(load_library("attention_shared").tb_attention_shared(
         _ptr(q), _i64(q.stride(0)), _ptr(out), _i64(out.stride(0)), _ptr(cache), _ptr(positions), _ptr(block_table),
         _i32(block_table.stride(0)), _i32(block_table.shape[1]), _ptr(shared.members), _ptr(shared.group_start),
-        _ptr(shared.prefix), _ptr(shared.group_of), _i32(rows), _i32(shared.prefix.numel()), _i32(num_heads),
+        _ptr(shared.leader), _ptr(shared.prefix), _ptr(shared.common), _i32(rows), _i32(shared.prefix.numel()), _i32(num_heads),
         _i32(num_kv_heads), _i32(head_dim), _i32(page_size), _f32(scale), _i32(choice.tiles), _i32(choice.prefix_parts),
         _i32(choice.prefix_run), _i32(choice.tail_parts), _i32(choice.tail_run), _ptr(scratch),
-        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(1 if choice.tensor else 0),
+        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(choice.warps), _i32(1 if choice.tensor else 0),
         _i32(cache.shape[0]), _ptr(_error_word(q.device)), _i32(_code(q.dtype)), _stream()), "attention_shared")
     return out
 

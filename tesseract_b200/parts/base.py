@@ -45,6 +45,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Any, Callable, Dict, Generic, List, Mapping, Optional, Sequence, Tuple, Type, TypeVar
 
+import numpy as np
 import torch
 
 from ..config.spec import PartSpec
@@ -297,36 +298,43 @@ class SharedRows:
 
     members: torch.Tensor        # int32 [rows]: the rows, group by group
     group_start: torch.Tensor    # int32 [groups + 1]: where a group's rows begin in ``members``
-    prefix: torch.Tensor         # int32 [groups]: keys in common, none of them behind the position of a row of the group
-    group_of: torch.Tensor       # int32 [rows]
+    leader: torch.Tensor         # int32 [groups]: the row through whose block table the keys in common are read
+    prefix: torch.Tensor         # int32 [groups]: keys in common in whole blocks of 64 (0 for a row alone)
+    common: torch.Tensor         # int32 [rows]: those of the row's group
     sizes: Tuple[int, ...]       # host copies for decisions: rows of each group,
-    blocks: Tuple[int, ...]      # whole blocks of keys in common (0 for a row alone),
+    blocks: Tuple[int, ...]      # blocks of keys in common,
     longest_tail: int            # and the most keys that a row reads behind them
 
     @classmethod
     def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":
         """``groups``: the rows of each group; ``prefixes``: their keys in common; ``positions``: the position of every row
         (-1 for a row without keys)."""
-        rows = len(positions)
-        members = [row for group in groups for row in group]
-        if sorted(members) != list(range(rows)):
-            raise ValueError("every row of the step belongs to exactly one group")
-        if len(prefixes) != len(groups) or any(not group for group in groups):
-            raise ValueError("a group has rows and one number of keys in common")
-        group_of, start, blocks, tail = [0] * rows, [0], [], 0
-        for index, (group, prefix) in enumerate(zip(groups, prefixes)):
-            last = min(positions[row] for row in group)
-            if not 0 <= prefix <= last + 1:
-                raise ValueError(f"{prefix} keys in common, but a row of the group reads {last + 1}")
-            start.append(start[-1] + len(group))
-            blocks.append(prefix // SHARED_BLOCK if len(group) > 1 else 0)
-            for row in group:
-                group_of[row] = index
-                tail = max(tail, positions[row] + 1 - blocks[-1] * SHARED_BLOCK)
-        packed = torch.tensor(members + start + list(prefixes) + group_of, dtype=torch.int32).to(device)
-        at_start, at_prefix, at_of = rows, rows + len(start), rows + len(start) + len(groups)
-        return cls(packed[:at_start], packed[at_start:at_prefix], packed[at_prefix:at_of], packed[at_of:],
-                   tuple(len(g) for g in groups), tuple(blocks), tail)
+        arrays, sizes, blocks, tail = shared_arrays(groups, prefixes, positions)
+        packed = torch.from_numpy(np.concatenate(arrays)).to(device)
+        return cls(*packed.split([a.size for a in arrays]), sizes, blocks, tail)
+
+
+def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int]):
+    """The five arrays of :class:`SharedRows` on the host, int32, and its host copies."""
+    rows = len(positions)
+    members = [row for group in groups for row in group]
+    if sorted(members) != list(range(rows)):
+        raise ValueError("every row of the step belongs to exactly one group")
+    if len(prefixes) != len(groups) or any(not group for group in groups):
+        raise ValueError("a group has rows and one number of keys in common")
+    start, blocks, tail, common = [0], [], 0, [0] * rows
+    for group, prefix in zip(groups, prefixes):
+        last = min(positions[row] for row in group)
+        if not 0 <= prefix <= last + 1:
+            raise ValueError(f"{prefix} keys in common, but a row of the group reads {last + 1}")
+        start.append(start[-1] + len(group))
+        blocks.append(prefix // SHARED_BLOCK if len(group) > 1 else 0)
+        for row in group:
+            common[row] = blocks[-1] * SHARED_BLOCK
+            tail = max(tail, positions[row] + 1 - common[row])
+    arrays = [np.asarray(a, dtype=np.int32) for a in (members, start, [group[0] for group in groups],
+                                                      [b * SHARED_BLOCK for b in blocks], common)]
+    return arrays, tuple(len(g) for g in groups), tuple(blocks), tail
 
 
 @dataclass

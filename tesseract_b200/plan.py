@@ -285,6 +285,7 @@ class SharedAttentionPlan:
     tail_parts: int
     tail_run: int
     tensor: bool = False
+    warps: int = 0           # of a block: 2, or (0) as many as let two blocks share a multiprocessor
 
 
 SHARED_MIN_RUN = 4          # blocks of 64 keys: a tile of 16 keys for each of eight warps, twice
@@ -319,11 +320,13 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, sizes, blo
         prefix_parts = min(SHARED_MAX_PARTS, -(-max(blocks) // prefix_run))
     tail_blocks = -(-max(1, longest_tail) // 64)
     tail_tiles = sum(sizes) * -(-fold // kernels.attention_shared_tile(dtype))
-    tail_run = max(SHARED_MIN_RUN, -(-tail_tiles * tail_blocks // target))
+    # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
+    # are many
+    warps = 2 if dtype != torch.float32 and tail_tiles * tail_blocks > target else 0
+    resident = target if warps == 0 else 3 * target
+    tail_run = max(SHARED_MIN_RUN, -(-tail_tiles * tail_blocks // resident))
     tail_parts = min(SHARED_MAX_PARTS, -(-tail_blocks // tail_run))
-    # (the kernel counts the tiles of every group of two rows or more, whether or not a whole block is shared)
-    counted = sum(-(-n * fold // tile) for n in sizes if n > 1)
-    return SharedAttentionPlan(counted, prefix_parts, prefix_run, tail_parts, tail_run, tensor)
+    return SharedAttentionPlan(sum(tiles), prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,

@@ -180,8 +180,8 @@ def test_both_forms_in_bfloat16(rows, dim):
     for tensor in (False, True):
         tile = kernels.attention_shared_tile(torch.bfloat16, tensor)
         tiles = sum(-(-n * 4 // tile) for n in (rows, 2))
-        for parts, run in ((1, 1), (5, 2)):
-            case.check(plan.SharedAttentionPlan(tiles, parts, run, 2, 1, tensor))
+        for parts, run, warps in ((1, 1, 0), (5, 2, 2)):
+            case.check(plan.SharedAttentionPlan(tiles, parts, run, 2, 1, tensor, warps))
     assert kernels.tcgen05_error() == 0
 
 
