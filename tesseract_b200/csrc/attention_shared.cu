@@ -76,13 +76,13 @@ __device__ __forceinline__ int run_blocks(int blocks, int parts, int run) {
 
 __device__ __forceinline__ int64_t common_blocks(const SharedParams& p) { return (int64_t)p.tiles * p.kv_heads * p.prefix_parts; }
 
-// The work of block `index` of those for the common parts (TILE folded rows a tile); false if there is none.
+// The work of block `index` of those for the common parts (TILE folded rows a tile); false if there is none.  Heads go fastest,
+// first runs come first: short parts have no later ones, and the blocks that find nothing to do are the last to start.
 template <int TILE>
 __device__ bool find_common(const SharedParams& p, int64_t index, Work& w) {
-    const int part = (int)(index % p.prefix_parts);
-    const int64_t rest = index / p.prefix_parts;
-    w.kv_head = (int)(rest % p.kv_heads);
-    int tile = (int)(rest / p.kv_heads);
+    w.kv_head = (int)(index % p.kv_heads);
+    const int rest = (int)(index / p.kv_heads), part = rest / p.tiles;
+    int tile = rest % p.tiles;
     // which group: a warp counts the tiles of 32 groups at a time (all that is known of a group is loaded at once)
     const int lane = threadIdx.x & 31;
     for (int base = 0; base < p.groups; base += 32) {
@@ -126,14 +126,14 @@ __device__ bool find_common(const SharedParams& p, int64_t index, Work& w) {
 // The work of block `index` of those for the keys behind, row by row.
 template <int TILE>
 __device__ bool find_tail(const SharedParams& p, int64_t index, Work& w) {
-    const int part = (int)(index % p.tail_parts);
-    int64_t rest = index / p.tail_parts;
-    w.kv_head = (int)(rest % p.kv_heads);
-    rest /= p.kv_heads;
+    w.kv_head = (int)(index % p.kv_heads);
     const int tiles = (p.fold + TILE - 1) / TILE;
-    w.row = (int)(rest / tiles);
-    if (w.row >= p.rows) return false;
-    w.first_folded = (int)(rest % tiles) * TILE;
+    int rest = (int)(index / p.kv_heads);
+    w.first_folded = rest % tiles * TILE;
+    rest /= tiles;
+    w.row = rest % p.rows;
+    const int part = rest / p.rows;
+    if (part >= p.tail_parts) return false;
     const int first = common_keys(p, p.common[w.row]);
     const int last = min(p.positions[w.row] + 1, p.table_keys);
     if (last <= first) return false;
@@ -194,11 +194,12 @@ __device__ void leave_run(const SharedParams& p, const Work& w, const float* ml,
 
 constexpr int kKeys = 16;                     // keys of a warp's tile
 constexpr int kRows = 16;                     // folded rows of a block's tile
-// Warps and ring depth so that two blocks share a multiprocessor up to a padded head size of 128.
+// Warps and ring depth so that two blocks share a multiprocessor up to a padded head size of 128; blocks of two warps: eight, or four of
+// a head size of 128 (deeper rings: 16 rows of 4,000 keys, 32 heads of 128, 56.8 us with two stages and six blocks a multiprocessor).
 template <int D>
 constexpr int kWarps = D <= 64 ? 8 : D <= 128 ? 6 : 4;
-template <int D>
-constexpr int kStages = D > 64 && D <= 128 ? 2 : 3;
+template <int D, int WARPS>
+constexpr int kStages = D > 64 && D <= 128 && WARPS > 2 ? 2 : 3;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     const int bytes = valid ? 16 : 0;         // (0: the destination is filled with zeros)
@@ -239,9 +240,9 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
     return (uint32_t)(row * (D * 2) + ((chunk ^ key) << 4));
 }
 
-template <int D, int WARPS>
+template <int D, int WARPS, bool ONE>
 __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* smem) {
-    constexpr int STAGES = kStages<D>, CH = D / 8, PASSES = kKeys * CH / 32;
+    constexpr int STAGES = kStages<D, WARPS>, CH = D / 8, PASSES = kKeys * CH / 32, LOOKS = ONE ? 1 : PASSES;
     constexpr uint32_t kTileBytes = kKeys * D * 2, kStageBytes = 2 * kTileBytes;
     constexpr bool QREG = D <= 128;           // the queries' fragments stay in registers
     constexpr int PITCH = D + 8;              // floats between rows of the sums that are put together (bank conflicts)
@@ -266,27 +267,31 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
     const int64_t head_block = (int64_t)p.paging.size * p.head_dim;
     const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
     const __nv_bfloat16* base = (const __nv_bfloat16*)p.cache + (int64_t)w.kv_head * head_block;
-    // the pages of a tile's keys are looked up one tile ahead of its copies, which depend on them
-    auto look_up = [&](int key0, int (&pages)[PASSES]) {
+    // The page of a tile's keys is looked up one tile ahead of the copies, which depend on it.  Runs begin with a block, so with pages
+    // of a multiple of 16 keys a tile lies in one page, its keys one behind the other; otherwise (ONE false) every key has its own.
+    auto look_up = [&](int key0, int (&pages)[LOOKS]) {
 #pragma unroll
-        for (int pass = 0; pass < PASSES; ++pass) {
-            const int key = key0 + (pass * 32 + lane) / CH;
+        for (int pass = 0; pass < LOOKS; ++pass) {
+            const int key = ONE ? key0 : key0 + (pass * 32 + lane) / CH;
             pages[pass] = key < w.end ? table[p.paging.page_of(key)] : 0;
         }
     };
-    auto bring = [&](uint32_t dst, int key0, const int (&pages)[PASSES]) {
+    auto bring = [&](uint32_t dst, int key0, const int (&pages)[LOOKS]) {
+        const __nv_bfloat16* tile = nullptr;
+        if (ONE) tile = base + (int64_t)pages[0] * page_block + (int64_t)p.paging.within(key0) * p.head_dim;
 #pragma unroll
         for (int pass = 0; pass < PASSES; ++pass) {
             const int idx = pass * 32 + lane, r = idx / CH, c = idx % CH, key = key0 + r;
             const bool ok = key < w.end && c * 8 < p.head_dim;
             const __nv_bfloat16* src = base;
-            if (ok) src = base + (int64_t)pages[pass] * page_block + (int64_t)p.paging.within(key) * p.head_dim + c * 8;
+            if (ONE) src = ok ? tile + r * p.head_dim + c * 8 : base;
+            else if (ok) src = base + (int64_t)pages[pass % LOOKS] * page_block + (int64_t)p.paging.within(key) * p.head_dim + c * 8;
             const uint32_t offset = tile_offset<D>(r, c);
             cp_async16(dst + offset, src, ok);
             cp_async16(dst + kTileBytes + offset, src + v_offset, ok);
         }
     };
-    int next_pages[PASSES];
+    int next_pages[LOOKS];
     int load_key = w.begin + warp * kKeys;
     constexpr int STEP = WARPS * kKeys;
 #pragma unroll
@@ -336,13 +341,14 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
             mma_bf16(s[1], a, b[2], b[3]);
         }
         // this thread's scores: rows lane / 4 and lane / 4 + 8, keys 2 (lane % 4), + 1, + 8, + 9
+        const bool whole = key0 + kKeys <= w.end;
         float high[2] = {kMasked, kMasked};
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool there = key0 + nt * 8 + 2 * (lane & 3) + (e & 1) < w.end;
-                s[nt][e] = there ? s[nt][e] * p.scale_log2 : kMasked;
+                s[nt][e] *= p.scale_log2;
+                if (!whole && key0 + nt * 8 + 2 * (lane & 3) + (e & 1) >= w.end) s[nt][e] = -INFINITY;      // 2^(that - m) is 0
                 high[e >> 1] = fmaxf(high[e >> 1], s[nt][e]);
             }
         float correction[2];
@@ -368,8 +374,7 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
             float e4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                e4[e] = s[nt][e] > 0.5f * kMasked ? fast_exp2(s[nt][e] - m[e >> 1]) : 0.0f;
-                if (s[nt][e] != s[nt][e]) e4[e] = s[nt][e];        // a NaN score stays one
+                e4[e] = fast_exp2(s[nt][e] - m[e >> 1]);
                 l[e >> 1] += e4[e];
             }
             weights[2 * nt] = pack_bf16(e4[0], e4[1]);
@@ -406,19 +411,19 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
     leave_run<kRows, PITCH, WARPS>(p, w, ml, acc);
 }
 
-template <int D, int WARPS>
+template <int D, int WARPS, bool ONE>
 __global__ void __launch_bounds__(WARPS * 32) shared_mma_kernel(const SharedParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     pdl_wait();
     pdl_trigger();                            // (only now: the kernels behind read what is older than this one without a wait of their own)
     Work w;
     // (tensor: the common parts are the next kernel's)
-    if (p.tensor ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS>(p, w, smem);
+    if (p.tensor ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS, ONE>(p, w, smem);
 }
 
 template <int D, int WARPS>
 constexpr size_t mma_bytes() {
-    constexpr size_t tiles = (size_t)kRows * D * 2 + (size_t)WARPS * kStages<D> * 2 * kKeys * D * 2;
+    constexpr size_t tiles = (size_t)kRows * D * 2 + (size_t)WARPS * kStages<D, WARPS> * 2 * kKeys * D * 2;
     constexpr size_t meet = (size_t)WARPS * kRows * (2 + D + 8) * sizeof(float);
     return tiles > meet ? tiles : meet;
 }
@@ -1023,15 +1028,22 @@ int launch(Kernel kernel, int64_t blocks, int threads, size_t smem, const Shared
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) return (int)err;
     }
+    // (kernels that follow each other without a gap: one that asks for little shared memory must not leave the next one little)
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (err != cudaSuccess) return (int)err;
     if (cudaError_t err = tb_launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), smem, stream, p)) return (int)err;
     return tb_launch_status();
 }
 
 // warps 2: blocks of two warps (where there are enough of them to fill the chip), else as many as share a multiprocessor in pairs.
+template <int D, bool ONE>
+int launch_mma(int warps, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
+    if (warps == 2) return launch(shared_mma_kernel<D, 2, ONE>, blocks, 64, mma_bytes<D, 2>(), p, stream);
+    return launch(shared_mma_kernel<D, kWarps<D>, ONE>, blocks, kWarps<D> * 32, mma_bytes<D, kWarps<D>>(), p, stream);
+}
 template <int D>
 int launch_mma(int warps, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
-    if (warps == 2) return launch(shared_mma_kernel<D, 2>, blocks, 64, mma_bytes<D, 2>(), p, stream);
-    return launch(shared_mma_kernel<D, kWarps<D>>, blocks, kWarps<D> * 32, mma_bytes<D, kWarps<D>>(), p, stream);
+    return p.paging.size % kKeys == 0 ? launch_mma<D, true>(warps, blocks, p, stream) : launch_mma<D, false>(warps, blocks, p, stream);
 }
 
 template <int D>

@@ -303,15 +303,16 @@ class SharedRows:
     common: torch.Tensor         # int32 [rows]: those of the row's group
     sizes: Tuple[int, ...]       # host copies for decisions: rows of each group,
     blocks: Tuple[int, ...]      # blocks of keys in common,
-    longest_tail: int            # and the most keys that a row reads behind them
+    tails: Tuple[int, ...]       # and blocks (begun ones too) that each row reads behind them
+    plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
 
     @classmethod
     def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":
         """``groups``: the rows of each group; ``prefixes``: their keys in common; ``positions``: the position of every row
         (-1 for a row without keys)."""
-        arrays, sizes, blocks, tail = shared_arrays(groups, prefixes, positions)
+        arrays, sizes, blocks, tails = shared_arrays(groups, prefixes, positions)
         packed = torch.from_numpy(np.concatenate(arrays)).to(device)
-        return cls(*packed.split([a.size for a in arrays]), sizes, blocks, tail)
+        return cls(*packed.split([a.size for a in arrays]), sizes, blocks, tails)
 
 
 def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int]):
@@ -322,7 +323,7 @@ def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], posi
         raise ValueError("every row of the step belongs to exactly one group")
     if len(prefixes) != len(groups) or any(not group for group in groups):
         raise ValueError("a group has rows and one number of keys in common")
-    start, blocks, tail, common = [0], [], 0, [0] * rows
+    start, blocks, common = [0], [], [0] * rows
     for group, prefix in zip(groups, prefixes):
         last = min(positions[row] for row in group)
         if not 0 <= prefix <= last + 1:
@@ -331,10 +332,10 @@ def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], posi
         blocks.append(prefix // SHARED_BLOCK if len(group) > 1 else 0)
         for row in group:
             common[row] = blocks[-1] * SHARED_BLOCK
-            tail = max(tail, positions[row] + 1 - common[row])
     arrays = [np.asarray(a, dtype=np.int32) for a in (members, start, [group[0] for group in groups],
                                                       [b * SHARED_BLOCK for b in blocks], common)]
-    return arrays, tuple(len(g) for g in groups), tuple(blocks), tail
+    tails = tuple(-(-(last + 1 - keys) // SHARED_BLOCK) for last, keys in zip(positions, common))
+    return arrays, tuple(len(g) for g in groups), tuple(blocks), tails
 
 
 @dataclass

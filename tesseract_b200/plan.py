@@ -28,6 +28,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 from typing import List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import kernels
@@ -294,39 +295,47 @@ SHARED_MAX_PARTS = 64
 
 def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,
                      sms: Optional[int] = None) -> SharedAttentionPlan:
-    """The plan of attention over groups of rows with keys in common (``shared``: a :class:`SharedRows`)."""
-    return _shared_attention(dtype, num_heads // num_kv_heads, num_kv_heads, head_dim, page_size, shared.sizes, shared.blocks,
-                             shared.longest_tail, sms or kernels.sm_count())
+    """The plan of attention over groups of rows with keys in common (``shared``: a :class:`SharedRows`, which keeps its plans: the
+    layers of a step ask for the same one)."""
+    key = (dtype, num_heads, num_kv_heads, head_dim, page_size, sms)
+    choice = shared.plans.get(key)
+    if choice is None:
+        choice = _shared_attention(dtype, num_heads // num_kv_heads, num_kv_heads, head_dim, page_size, shared,
+                                   sms or kernels.sm_count())
+        shared.plans[key] = choice
+    return choice
 
 
-def _shared_runs(tiles: Sequence[int], blocks: Sequence[int], target: int) -> int:
-    """The shortest runs (in blocks) with which all tiles' runs are at most ``target``."""
-    run = max(SHARED_MIN_RUN, -(-sum(t * b for t, b in zip(tiles, blocks)) // target))
-    while run < max(blocks) and sum(t * -(-b // run) for t, b in zip(tiles, blocks)) > target:
-        run += 1
+def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int) -> int:
+    """The shortest runs (in blocks, ``SHARED_MIN_RUN`` at least) with which all tiles' runs are at most ``target``: one more, and the
+    chip goes round a second time for it."""
+    longest = int(blocks.max())
+    run = max(SHARED_MIN_RUN, -(-int((tiles * blocks).sum()) // target))
+    while run < longest and int((tiles * -(-blocks // run)).sum()) > target:
+        run += 1 + run // 16
     return run
 
 
-@lru_cache(maxsize=1024)
-def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, sizes, blocks, longest_tail, sms) -> SharedAttentionPlan:
-    target = max(1, 2 * sms // num_kv_heads)                    # blocks of threads that are resident at once, a kv head
-    shared_rows = [n * fold if b > 0 else 0 for n, b in zip(sizes, blocks)]
-    tensor = max(shared_rows) > 16 and kernels.attention_shared_tensor(dtype, head_dim, page_size)
+def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sms) -> SharedAttentionPlan:
+    sizes, blocks = np.asarray(shared.sizes), np.asarray(shared.blocks)
+    rows = np.where(blocks > 0, sizes * fold, 0)
+    tensor = int(rows.max()) > 16 and kernels.attention_shared_tensor(dtype, head_dim, page_size)
     tile = kernels.attention_shared_tile(dtype, tensor)
-    tiles = [-(-rows // tile) for rows in shared_rows]
+    tiles = -(-rows // tile)
+    target = max(1, 2 * sms // num_kv_heads)                    # large blocks of threads that are resident at once, a kv head
     prefix_parts, prefix_run = 0, 1
-    if any(tiles):
+    if tiles.any():
         prefix_run = _shared_runs(tiles, blocks, target)
-        prefix_parts = min(SHARED_MAX_PARTS, -(-max(blocks) // prefix_run))
-    tail_blocks = -(-max(1, longest_tail) // 64)
-    tail_tiles = sum(sizes) * -(-fold // kernels.attention_shared_tile(dtype))
+        prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
     # are many
-    warps = 2 if dtype != torch.float32 and tail_tiles * tail_blocks > target else 0
-    resident = target if warps == 0 else 3 * target
-    tail_run = max(SHARED_MIN_RUN, -(-tail_tiles * tail_blocks // resident))
-    tail_parts = min(SHARED_MAX_PARTS, -(-tail_blocks // tail_run))
-    return SharedAttentionPlan(sum(tiles), prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
+    tails = np.maximum(np.asarray(shared.tails), 1)
+    tail_tiles = np.full(tails.shape, -(-fold // kernels.attention_shared_tile(dtype)))
+    warps = 2 if dtype != torch.float32 and int(tail_tiles.sum()) > target else 0
+    small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
+    tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target)
+    tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
+    return SharedAttentionPlan(int(tiles.sum()), prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,
