@@ -16,6 +16,11 @@ pages are handed out again first.  ``admit`` with ``reserve_tokens`` sets aside 
 request's peak need in every group (src/engine/kv.rs:36-51), so an admitted request
 cannot run out; without a reservation pages come on demand and ``extend`` raises
 :class:`OutOfPages` when none is left.
+
+``fork`` gives a request continuations that go on from where it is: pages that are full are held by all of them together, the
+page that is still being filled and the fixed-size state are copied (as are the pages of groups that give pages back while a
+request lives, whose window moves on for each by itself), all copies of a call in one launch.  ``compact`` moves pages to the
+lowest ids.
 """
 
 from __future__ import annotations
@@ -46,6 +51,7 @@ class _Request:
     length: int = 0                            # tokens whose keys/values are stored
     pages: List[Dict[int, int]] = field(default_factory=list)   # per paged group: logical index -> page id
     first_live: List[int] = field(default_factory=list)         # per group: lowest logical page still held
+    family: object = field(default_factory=object)              # the same for a request and its continuations
 
 
 class CacheManager:
@@ -232,6 +238,139 @@ class CacheManager:
             g.tables[state.slot, :] = 0
         self.slots.release(request)
 
+    # ------------------------------------------------------------------ continuations
+    def _shareable_pages(self, group: _Group, length: int) -> int:
+        """Leading pages of a request of ``length`` tokens that nothing writes to any more and that stay while it lives."""
+        if group.need.live_span() is not None:
+            return 0
+        return length // group.need.positions_per_entry // self.page_size
+
+    def fork_pages(self, length: int, reserve_tokens: int) -> List[Tuple[int, int]]:
+        """Per paged group: the pages that a continuation of a request of ``length`` tokens shares, and those it draws of its own
+        until it has ``reserve_tokens``."""
+        out = []
+        for g in self.groups:
+            if g.pool is not None:
+                shared = self._shareable_pages(g, length)
+                out.append((shared, self.pages_for(g, reserve_tokens) - shared))
+        return out
+
+    def fork(self, pairs: Sequence[Tuple[Hashable, Hashable]], reserve_tokens: Optional[int] = None) -> bool:
+        """For every ``(parent, child)``: the new request ``child`` goes on from where ``parent`` is.  With ``reserve_tokens`` the
+        pages that each child may need up to that many tokens are set aside.  All of them, or none and False if they do not
+        fit now.  The copies are enqueued on the current stream, behind the step that filled the parents' last pages."""
+        pairs = list(pairs)
+        children = [child for _, child in pairs]
+        if len(set(children)) != len(children):
+            raise ValueError("a continuation is named twice")
+        for parent, child in pairs:
+            if parent not in self._requests:
+                raise ValueError(f"request {parent!r} is not live")
+            if child in self._requests:
+                raise ValueError(f"request {child!r} is already live")
+            if reserve_tokens is not None and reserve_tokens < self._requests[parent].length:
+                raise ValueError(f"request {parent!r} has more than {reserve_tokens} tokens already")
+        if len(pairs) > self.slots.free_slots:
+            return False
+        draws = [0] * len(self.groups)
+        for parent, _ in pairs:
+            state = self._requests[parent]
+            for index, g in enumerate(self.groups):
+                if g.pool is None:
+                    continue
+                shared = self._shareable_pages(g, state.length)
+                if reserve_tokens is not None:
+                    draws[index] += self.pages_for(g, reserve_tokens) - shared
+                else:
+                    draws[index] += sum(1 for logical in state.pages[index] if logical >= shared)
+        if any(g.pool is not None and draws[i] > g.pool.available_to_reserve for i, g in enumerate(self.groups)):
+            return False
+        moves: List[Tuple[List[int], List[int]]] = [([], []) for _ in self.groups]
+        for parent, child in pairs:
+            state = self._requests[parent]
+            slot = self.slots.allocate(child)
+            new = _Request(slot=slot, length=state.length, pages=[{} for _ in self.groups],
+                           first_live=list(state.first_live), family=state.family)
+            for index, g in enumerate(self.groups):
+                sources, targets = moves[index]
+                if g.pool is None:
+                    sources.append(state.slot)
+                    targets.append(slot)
+                    continue
+                shared = self._shareable_pages(g, state.length)
+                if reserve_tokens is None:
+                    g.pool.register(child)
+                else:
+                    g.pool.reserve(child, self.pages_for(g, reserve_tokens) - shared)
+                g.tables[slot, :] = 0
+                for logical, page in state.pages[index].items():
+                    if logical < shared:
+                        g.pool.share(child, page)
+                    else:
+                        sources.append(page)
+                        page = g.pool.allocate(child)
+                        targets.append(page)
+                        self._ever_used[index].add(page)
+                    new.pages[index][logical] = page
+                    g.tables[slot, logical] = page
+            self._requests[child] = new
+        self._copy(moves)
+        return True
+
+    def compact(self) -> int:
+        """Move the pages in use to the lowest ids of every group (one launch); returns how many moved.  The block tables of
+        steps that are built from now on name the new places."""
+        moves: List[Tuple[List[int], List[int]]] = []
+        for index, g in enumerate(self.groups):
+            renamed = g.pool.compact() if g.pool is not None else {}
+            moves.append((list(renamed), list(renamed.values())))
+            if not renamed:
+                continue
+            for state in self._requests.values():
+                held = state.pages[index]
+                for logical, page in held.items():
+                    if page in renamed:
+                        held[logical] = renamed[page]
+                        g.tables[state.slot, logical] = renamed[page]
+            self._ever_used[index].update(renamed.values())
+        self._copy(moves)
+        return sum(len(sources) for sources, _ in moves)
+
+    def _copy(self, moves: Sequence[Tuple[List[int], List[int]]]) -> None:
+        """Pages (or state slots) of every group from the first list's places to the second's, in all entries."""
+        todo = [(g.storage, sources, targets) for g, (sources, targets) in zip(self.groups, moves)
+                if g.storage is not None and g.storage.numel() and sources]
+        if todo and all(s.is_cuda and s.device.index == torch.cuda.current_device() for s, _, _ in todo):
+            kernels.copy_pages(todo)
+        else:
+            for storage, sources, targets in todo:
+                storage[:, targets] = storage[:, sources]
+
+    def rows_in_common(self, group_index: int, requests: Sequence[Hashable]) -> Tuple[List[List[int]], List[int]]:
+        """The rows of a step of ``requests`` (one a request) in groups whose first tokens lie in the same pages of a group of
+        the cache, and how many tokens that is; a request without such company is a group of its own."""
+        g = self.groups[group_index]
+        states = [self._requests[r] for r in requests]
+        if g.pool is None or g.need.live_span() is not None or g.need.positions_per_entry != 1:
+            return [[row] for row in range(len(states))], [0] * len(states)
+        families: Dict[int, List[int]] = {}
+        for row, state in enumerate(states):
+            families.setdefault(id(state.family), []).append(row)
+        groups, common = list(families.values()), []
+        for rows in groups:
+            if len(rows) == 1:
+                common.append(0)
+                continue
+            pages = min(states[row].length for row in rows) // self.page_size
+            tables = g.tables[[states[row].slot for row in rows], :pages]
+            same = (tables == tables[0]).all(axis=0)
+            common.append((pages if same.all() else int(same.argmin())) * self.page_size)
+        return groups, common
+
+    def has_company(self, requests: Sequence[Hashable]) -> bool:
+        """Whether two of ``requests`` are continuations of one prompt."""
+        return len({id(self._requests[r].family) for r in requests}) < len(requests)
+
     def _pinned_pages(self, group: _Group) -> int:
         """Leading pages that stay as long as the request lives (they hold positions that every later query reads)."""
         return -(-group.need.keep_first // self.page_size)
@@ -261,13 +400,15 @@ class CacheManager:
             if g.pool is None:
                 continue
             g.pool.check()
-            seen = set()
+            seen: Dict[int, int] = {}
             for request, state in self._requests.items():
-                for page in state.pages[index].values():
-                    if page in seen:
-                        raise AssertionError(f"page {page} is held twice")
-                    seen.add(page)
-                    if g.pool.owner_of(page) != request:
+                for logical, page in state.pages[index].items():
+                    seen[page] = seen.get(page, 0) + 1
+                    if request not in g.pool.holders_of(page):
                         raise AssertionError(f"page {page} ownership disagrees")
+                    if g.tables[state.slot, logical] != page:
+                        raise AssertionError(f"the block table of {request!r} disagrees at page {logical}")
+            if any(count != len(g.pool.holders_of(page)) for page, count in seen.items()):
+                raise AssertionError("a page has holders that no request's table names")
             if len(seen) != g.pool.used_pages:
                 raise AssertionError("pool holds pages that no request's table names")
