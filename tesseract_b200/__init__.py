@@ -7,11 +7,11 @@
 from .config import EngineConfig
 from .sampling.params import SamplingParams
 
-__all__ = ["LLM", "SamplingParams", "EngineConfig", "RequestOutput"]
+__all__ = ["LLM", "SamplingParams", "EngineConfig", "RequestOutput", "BeamOutput", "TokenScores"]
 
 
 def __getattr__(name):
-    if name in ("LLM", "RequestOutput"):
+    if name in ("LLM", "RequestOutput", "BeamOutput", "TokenScores"):
         from .engine import llm
 
         return getattr(llm, name)

@@ -26,13 +26,13 @@ lowest ids.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional, Sequence, Tuple
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
 
 from .. import kernels
-from ..parts.base import CacheBinding, PagedNeed, StateNeed
+from ..parts.base import CacheBinding, PagedKVNeed, PagedNeed, StateNeed
 from .pages import OutOfPages, PagePool, StateSlots
 
 
@@ -255,38 +255,42 @@ class CacheManager:
                 out.append((shared, self.pages_for(g, reserve_tokens) - shared))
         return out
 
-    def fork(self, pairs: Sequence[Tuple[Hashable, Hashable]], reserve_tokens: Optional[int] = None) -> bool:
-        """For every ``(parent, child)``: the new request ``child`` goes on from where ``parent`` is.  With ``reserve_tokens`` the
-        pages that each child may need up to that many tokens are set aside.  All of them, or none and False if they do not
+    def fork(self, pairs: Sequence[Tuple[Hashable, Hashable]], reserve_tokens: Union[int, Sequence[int], None] = None) -> bool:
+        """For every ``(parent, child)``: the new request ``child`` goes on from where ``parent`` is.  With ``reserve_tokens`` (a
+        number, or one a pair) the pages that each child may need up to that many tokens are set aside.  All of them, or none and False if they do not
         fit now.  The copies are enqueued on the current stream, behind the step that filled the parents' last pages."""
         pairs = list(pairs)
+        if reserve_tokens is None or isinstance(reserve_tokens, int):
+            reserve_tokens = [reserve_tokens] * len(pairs)
+        if len(reserve_tokens) != len(pairs):
+            raise ValueError("one number of tokens for all continuations, or one each")
         children = [child for _, child in pairs]
         if len(set(children)) != len(children):
             raise ValueError("a continuation is named twice")
-        for parent, child in pairs:
+        for (parent, child), reserve in zip(pairs, reserve_tokens):
             if parent not in self._requests:
                 raise ValueError(f"request {parent!r} is not live")
             if child in self._requests:
                 raise ValueError(f"request {child!r} is already live")
-            if reserve_tokens is not None and reserve_tokens < self._requests[parent].length:
-                raise ValueError(f"request {parent!r} has more than {reserve_tokens} tokens already")
+            if reserve is not None and reserve < self._requests[parent].length:
+                raise ValueError(f"request {parent!r} has more than {reserve} tokens already")
         if len(pairs) > self.slots.free_slots:
             return False
         draws = [0] * len(self.groups)
-        for parent, _ in pairs:
+        for (parent, _), reserve in zip(pairs, reserve_tokens):
             state = self._requests[parent]
             for index, g in enumerate(self.groups):
                 if g.pool is None:
                     continue
                 shared = self._shareable_pages(g, state.length)
-                if reserve_tokens is not None:
-                    draws[index] += self.pages_for(g, reserve_tokens) - shared
+                if reserve is not None:
+                    draws[index] += self.pages_for(g, reserve) - shared
                 else:
                     draws[index] += sum(1 for logical in state.pages[index] if logical >= shared)
         if any(g.pool is not None and draws[i] > g.pool.available_to_reserve for i, g in enumerate(self.groups)):
             return False
         moves: List[Tuple[List[int], List[int]]] = [([], []) for _ in self.groups]
-        for parent, child in pairs:
+        for (parent, child), reserve in zip(pairs, reserve_tokens):
             state = self._requests[parent]
             slot = self.slots.allocate(child)
             new = _Request(slot=slot, length=state.length, pages=[{} for _ in self.groups],
@@ -298,10 +302,10 @@ class CacheManager:
                     targets.append(slot)
                     continue
                 shared = self._shareable_pages(g, state.length)
-                if reserve_tokens is None:
+                if reserve is None:
                     g.pool.register(child)
                 else:
-                    g.pool.reserve(child, self.pages_for(g, reserve_tokens) - shared)
+                    g.pool.reserve(child, self.pages_for(g, reserve) - shared)
                 g.tables[slot, :] = 0
                 for logical, page in state.pages[index].items():
                     if logical < shared:
@@ -346,25 +350,28 @@ class CacheManager:
             for storage, sources, targets in todo:
                 storage[:, targets] = storage[:, sources]
 
-    def rows_in_common(self, group_index: int, requests: Sequence[Hashable]) -> Tuple[List[List[int]], List[int]]:
-        """The rows of a step of ``requests`` (one a request) in groups whose first tokens lie in the same pages of a group of
-        the cache, and how many tokens that is; a request without such company is a group of its own."""
-        g = self.groups[group_index]
+    def shares_keys(self, group_index: int) -> bool:
+        """Whether continuations hold full pages of this group together: keys and values of every token, an entry each."""
+        need = self.groups[group_index].need
+        return isinstance(need, PagedKVNeed) and need.live_span() is None
+
+    def rows_in_common(self, requests: Sequence[Hashable]) -> Tuple[List[List[int]], List[int]]:
+        """The rows of a step of ``requests`` (one a request) in groups whose first tokens lie in the same pages wherever full pages
+        are held together, and how many tokens that is; a request without such company is a group of its own."""
         states = [self._requests[r] for r in requests]
-        if g.pool is None or g.need.live_span() is not None or g.need.positions_per_entry != 1:
-            return [[row] for row in range(len(states))], [0] * len(states)
         families: Dict[int, List[int]] = {}
         for row, state in enumerate(states):
             families.setdefault(id(state.family), []).append(row)
         groups, common = list(families.values()), []
+        tables = [g.tables for i, g in enumerate(self.groups) if self.shares_keys(i)]
         for rows in groups:
-            if len(rows) == 1:
-                common.append(0)
-                continue
-            pages = min(states[row].length for row in rows) // self.page_size
-            tables = g.tables[[states[row].slot for row in rows], :pages]
-            same = (tables == tables[0]).all(axis=0)
-            common.append((pages if same.all() else int(same.argmin())) * self.page_size)
+            pages = min(states[row].length for row in rows) // self.page_size if len(rows) > 1 and tables else 0
+            for table in tables if pages else ():
+                mine = table[[states[row].slot for row in rows], :pages]
+                same = (mine == mine[0]).all(axis=0)
+                if not same.all():
+                    pages = int(same.argmin())
+            common.append(pages * self.page_size)
         return groups, common
 
     def has_company(self, requests: Sequence[Hashable]) -> bool:

@@ -53,6 +53,13 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--top-p", type=float, default=1.0)
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--ignore-eos", action="store_true")
+    p.add_argument("--beams", type=int, default=0, metavar="WIDTH",
+                   help="instead of sampling, the WIDTH most probable continuations that a beam search finds, with their log "
+                        "probabilities")
+    p.add_argument("--length-penalty", type=float, default=0.0,
+                   help="with --beams: rank by the log probability over the number of tokens to this power")
+    p.add_argument("--score", action="store_true",
+                   help="generate nothing: the log probability of every token of the prompts")
     p.add_argument("--no-cuda-graphs", action="store_true")
     p.add_argument("--check-weights", action="store_true",
                    help="after loading, read the final norm's weight back from the device and compare it with the "
@@ -79,6 +86,30 @@ def read_prompt_file(path: str):
             else:
                 prompts.append(line)
     return prompts
+
+
+def run_scored(llm, prompts, args, scratch) -> int:
+    """``--score`` and ``--beams``."""
+    if args.score:
+        for index, out in enumerate(llm.score(prompts)):
+            if args.json:
+                print(json.dumps({"request": index, "token_ids": out.token_ids, "logprobs": out.logprobs,
+                                  "entropies": out.entropies, "perplexity": out.perplexity}))
+            else:
+                print(f"[{index}] perplexity {out.perplexity:.4f}: " + " ".join(f"{v:.4f}" for v in out.logprobs))
+    else:
+        found = llm.beam_search(prompts, args.beams, args.max_tokens, length_penalty=args.length_penalty,
+                                ignore_eos=args.ignore_eos)
+        for index, outs in enumerate(found):
+            for rank, out in enumerate(outs):
+                if args.json:
+                    print(json.dumps({"request": index, "beam": rank, "token_ids": out.token_ids, "logprob": out.logprob,
+                                      "score": out.score, "finish_reason": out.finish_reason}))
+                else:
+                    print(f"[{index}.{rank}] {out.finish_reason} {out.logprob:.4f}: " + " ".join(map(str, out.token_ids)))
+    if scratch is not None:
+        scratch.cleanup()
+    return 0
 
 
 def main(argv=None) -> int:
@@ -128,6 +159,8 @@ def main(argv=None) -> int:
     if not prompts:
         print("no prompt given (--prompt, --prompt-ids, --prompt-file or --random-prompt)", file=sys.stderr)
         return 2
+    if args.score or args.beams:
+        return run_scored(llm, prompts, args, scratch)
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
                             seed=args.seed, ignore_eos=args.ignore_eos)
     started = time.time()

@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from .. import kernels
-from ..parts.base import GroupView, StepContext
+from ..parts.base import GroupView, SharedRows, StepContext
 from .step import StepEntry, Stepper
 
 
@@ -54,13 +54,17 @@ HOST_RING = 3          # pinned copies of a graph's metadata: a launch may be pr
 
 
 class _Graph:
-    """Persistent buffers and the captured graph for one (batch bucket, table width)."""
+    """Persistent buffers and the captured graph for one (batch bucket, table width), without or (``company``: the arrays of the
+    step that it is captured for) with rows that have keys in common: how the rows are grouped is data, so one graph serves every
+    grouping."""
 
-    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor):
+    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None):
         cache, device = stepper.cache, stepper.runtime.device
         self.batch, self.columns = batch, columns
         self.paged = [i for i, g in enumerate(cache.groups) if g.pool is not None]
-        ints = 4 * batch + len(self.paged) * batch * columns
+        # members, group starts, leaders, keys in common of each group and each row (parts.base.SharedRows)
+        together = [batch, batch + 1, batch, batch, batch] if company is not None else []
+        ints = 4 * batch + len(self.paged) * batch * columns + sum(together)
         ints = (ints + 1) // 2 * 2                                  # keep the float64 block 8-byte aligned
         self.nbytes = ints * 4 + batch * 4 + (batch % 2) * 4 + batch * 8
         self.hosts = [torch.zeros(self.nbytes, dtype=torch.uint8, pin_memory=True) for _ in range(HOST_RING)]
@@ -78,6 +82,10 @@ class _Graph:
             for _ in self.paged:
                 out["tables"].append(buffer[at:at + batch * columns * 4].view(torch.int32).view(batch, columns))
                 at += batch * columns * 4
+            out["together"] = []
+            for size in together:
+                out["together"].append(buffer[at:at + size * 4].view(torch.int32))
+                at += size * 4
             at = ints * 4
             out["temps"] = buffer[at:at + batch * 4].view(torch.float32)
             at += batch * 4 + (batch % 2) * 4
@@ -91,6 +99,8 @@ class _Graph:
             arrays = {k: (v.numpy() if not isinstance(v, list) else [t.numpy() for t in v]) for k, v in views.items()}
             arrays["slots"][:] = cache.scratch_slot
             arrays["feed"][:] = -1
+            if company is not None:
+                self.put_together(arrays, company[0])
             self.h_np.append(arrays)
         self.dev.copy_(self.hosts[0])
         arange = torch.arange(batch + 1, dtype=torch.int32, device=device)
@@ -98,8 +108,10 @@ class _Graph:
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=device)   # this step's token ids, chosen on the device
         groups: List[GroupView] = []
         tables = dict(zip(self.paged, self.d["tables"]))
+        shared = SharedRows(*self.d["together"], *company[1:], room=batch) if company is not None else None
         for index, g in enumerate(cache.groups):
-            groups.append(GroupView(tables.get(index), cache.page_size if g.pool is not None else 0))
+            groups.append(GroupView(tables.get(index), cache.page_size if g.pool is not None else 0,
+                                    shared if shared is not None and cache.shares_keys(index) else None))
         self.ctx = StepContext(
             num_rows=batch, num_seqs=batch, token_ids=self.tokens, positions=self.d["positions"],
             seq_of_row=arange[:batch], row_start=arange, seq_begin=self.d["positions"], state_slots=self.d["slots"],
@@ -109,6 +121,15 @@ class _Graph:
         self.logits: Optional[torch.Tensor] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self._capture(stepper)
+
+    @staticmethod
+    def put_together(arrays: dict, values) -> None:
+        """A step's grouping into the arrays; groups that it does not have begin behind the last row and hold none."""
+        for array, value in zip(arrays["together"], values):
+            array[:value.size] = value
+            array[value.size:] = 0
+        starts, used = arrays["together"][1], values[1]
+        starts[used.size:] = used[-1]
 
     def host_arrays(self) -> Tuple[int, dict]:
         """The next pinned metadata block of the ring, once the copy that last read it is done."""
@@ -180,7 +201,7 @@ class DecodeGraphs:
     def __init__(self, stepper: Stepper, max_batch: int):
         self.stepper = stepper
         self.max_batch = max_batch
-        self.graphs: Dict[Tuple[int, int], _Graph] = {}
+        self.graphs: Dict[Tuple[int, int, bool], _Graph] = {}
         self.replays = 0
         self.captures = 0
         self.kernels_replayed = 0
@@ -207,13 +228,17 @@ class DecodeGraphs:
         count = len(entries)
         lengths = [cache.length(e.request) for e in entries]
         pages = -(-(max(lengths) + 1) // cache.page_size)
-        key = (min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages)))
+        batch, columns = min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages))
+        company = stepper.company(entries, batch - count)
+        key = (batch, columns, company is not None)
         graph = self.graphs.get(key)
         if graph is None:
-            graph = _Graph(stepper, *key, self.sampled)
+            graph = _Graph(stepper, batch, columns, self.sampled, company)
             self.graphs[key] = graph
             self.captures += 1
         slot_index, h = graph.host_arrays()
+        if company is not None:
+            graph.put_together(h, company[0])
         slots = [cache.slot(e.request) for e in entries]
         h["tokens"][:count] = [int(e.tokens[0]) for e in entries]
         feed = [-1] * count

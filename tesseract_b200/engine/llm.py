@@ -20,6 +20,7 @@ import torch
 from ..config.engine_config import EngineConfig
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
+from .beam import BeamOutput, BeamSearch, TokenScores, score
 from .loading import load_model, make_stepper
 from .scheduler import FINISH_STOP, Request, Scheduler
 
@@ -102,14 +103,40 @@ class LLM:
         samples nothing; use it while no generation is in flight."""
         from .replay import TraceRunner
 
-        if self.scheduler.has_work():
-            raise RuntimeError("replay needs an idle engine: generation is in flight")
+        self._need_idle("replay")
         runner = TraceRunner(self.stepper)
         out = []
         for record in trace:
             logits = runner.step(record)
             out.append(None if logits is None else logits.cpu())
         return out
+
+    def beam_search(self, prompts: Sequence[Union[str, Sequence[int]]], width: int = 4, max_tokens: int = 128, *,
+                    length_penalty: float = 0.0, stop_token_ids: Sequence[int] = (), ignore_eos: bool = False
+                    ) -> List[List[BeamOutput]]:
+        """The ``width`` most probable continuations of every prompt that a beam search finds, best first (:class:`BeamSearch`: a
+        prompt's beams hold its cache pages together).  It drives this engine's own step function and cache; use it while no
+        generation is in flight."""
+        self._need_idle("beam search")
+        ends = frozenset(stop_token_ids) | (frozenset() if ignore_eos else frozenset(self.model.spec.eos_token_ids))
+        search = BeamSearch(self.stepper, width, max_tokens, end_ids=ends, length_penalty=length_penalty,
+                            portion=self.config.prefill_chunk_tokens)
+        outputs = search.run([self._encode(p) for p in prompts])
+        self._check_device_waits()
+        return outputs
+
+    def score(self, sequences: Sequence[Union[str, Sequence[int]]], alternatives: int = 0) -> List[TokenScores]:
+        """The model's log probability of every token of given sequences (all but each one's first), the entropy of what it expected
+        there, and with ``alternatives`` (up to 64) the tokens that it held most probable.  Use it while no generation is in
+        flight."""
+        self._need_idle("scoring")
+        out = [score(self.stepper, self._encode(s), alternatives, self.config.prefill_chunk_tokens) for s in sequences]
+        self._check_device_waits()
+        return out
+
+    def _need_idle(self, what: str) -> None:
+        if self.scheduler.has_work():
+            raise RuntimeError(f"{what} needs an idle engine: generation is in flight")
 
     def generate(self, prompts: Sequence[Union[str, Sequence[int]]],
                  sampling_params: Union[SamplingParams, Sequence[SamplingParams], None] = None) -> List[RequestOutput]:

@@ -18,7 +18,8 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
-from ..parts.base import GroupView, Runtime, StepContext
+from .. import plan
+from ..parts.base import GroupView, Runtime, SharedRows, StepContext, shared_arrays
 
 
 @dataclass
@@ -123,6 +124,18 @@ class Stepper:
                 raise StepError(f"request {entry.request!r} would pass the model's {self.max_positions} positions")
         return checked
 
+    def company(self, entries: Sequence[StepEntry], padding: int = 0):
+        """``parts.base.shared_arrays`` of a decode step in which continuations of one prompt have enough keys in common for those to
+        be read once (``padding`` rows behind it, which have nothing in common); None otherwise."""
+        cache = self.cache
+        requests = [e.request for e in entries]
+        if not cache.has_company(requests):
+            return None
+        groups, common = cache.rows_in_common(requests)
+        made = shared_arrays(groups + [[len(entries) + k] for k in range(padding)], common + [0] * padding,
+                             [cache.length(r) for r in requests] + [0] * padding)
+        return made if plan.sharing_pays(made[1], made[2]) else None
+
     # ------------------------------------------------------------------ the step
     def build_context(self, entries: Sequence[StepEntry], tokens: Optional[Sequence[Sequence[int]]] = None
                       ) -> Tuple[StepContext, Optional[torch.Tensor], int]:
@@ -150,11 +163,16 @@ class Stepper:
         paged = [i for i, g in enumerate(cache.groups) if g.pool is not None]
         for group_index in paged:
             arrays.append(cache.block_table_rows(group_index, slots, columns))
+        company = self.company(entries) if num_rows == num_seqs else None
+        if company is not None:
+            arrays += company[0]
         device = self._staging.upload(arrays)
         groups: List[GroupView] = []
         tables = dict(zip(paged, device[7:]))
+        shared = SharedRows(*device[-len(company[0]):], *company[1:]) if company is not None else None
         for index, g in enumerate(cache.groups):
-            groups.append(GroupView(block_table=tables.get(index), page_size=cache.page_size if g.pool else 0))
+            groups.append(GroupView(block_table=tables.get(index), page_size=cache.page_size if g.pool else 0,
+                                    shared=shared if shared is not None and cache.shares_keys(index) else None))
         ctx = StepContext(
             num_rows=num_rows, num_seqs=num_seqs, token_ids=device[0], positions=device[1], seq_of_row=device[2],
             row_start=device[3], seq_begin=device[4], state_slots=device[5], groups=groups,

@@ -79,6 +79,16 @@ class Attention(Mixer):
     def cache_need(self) -> PagedKVNeed:
         return PagedKVNeed(self.num_kv_heads, self.head_dim, self.window or None)
 
+    def _store(self, qkv: torch.Tensor, ctx: StepContext, cache: CacheBinding, inv_freq: Optional[torch.Tensor]) -> None:
+        """Positions on queries and keys (in place), new keys and values into their pages."""
+        rows = qkv.shape[0]
+        if inv_freq is None and self.position.kind != "none":
+            q_view = qkv[:, :self.q_width].view(rows, self.num_heads, self.head_dim)
+            k_view = qkv[:, self.q_width:self.q_width + self.kv_width].view(rows, self.num_kv_heads, self.head_dim)
+            self.position.apply(q_view, k_view, ctx.positions)
+        kernels.rope_kv_write(qkv, ctx.positions, ctx.seq_of_row, ctx.groups[cache.group].block_table, inv_freq, cache.storage,
+                              self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size, write_kv=cache.writes)
+
     def forward(self, x, ctx: StepContext, cache: Optional[CacheBinding], follow=None):
         if cache is None or cache.storage is None:
             raise RuntimeError("attention needs a paged key/value cache binding")
@@ -93,6 +103,15 @@ class Attention(Mixer):
         inv_freq = self.position.rotary_inv_freq
         rows = qkv.shape[0]
         attended = torch.empty((rows, self.q_width), dtype=qkv.dtype, device=qkv.device)
+        shared = group.shared if ctx.decode_only and not self.window else None
+        if shared is not None:
+            # decoded rows among which some have their first keys in common: those are read once
+            self._store(qkv, ctx, cache, inv_freq)
+            choice = plan.shared_attention(self.runtime.dtype, num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
+                                           head_dim=self.head_dim, page_size=cache.page_size, shared=shared)
+            kernels.attention_shared(qkv[:, :self.q_width], attended, cache.storage, ctx.positions, group.block_table, shared,
+                                     self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size, self.scale, choice)
+            return self.o_proj.forward(attended, follow=follow)
         new_tokens = ctx.host_new if len(ctx.host_new) == ctx.num_seqs else [ctx.max_new] * ctx.num_seqs
         choice = plan.attention(self.runtime.dtype, num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
                                 head_dim=self.head_dim, page_size=cache.page_size, new_tokens=new_tokens,
@@ -105,13 +124,7 @@ class Attention(Mixer):
                                           self.head_dim, cache.page_size, self.window, self.scale, inv_freq,
                                           cache.writes, choice.splits)
             return self.o_proj.forward(attended, follow=follow)
-        if inv_freq is None and self.position.kind != "none":
-            q_view = qkv[:, :self.q_width].view(rows, self.num_heads, self.head_dim)
-            k_view = qkv[:, self.q_width:self.q_width + self.kv_width].view(rows, self.num_kv_heads, self.head_dim)
-            self.position.apply(q_view, k_view, ctx.positions)
-        kernels.rope_kv_write(qkv, ctx.positions, ctx.seq_of_row, group.block_table, inv_freq, cache.storage,
-                              self.num_heads, self.num_kv_heads, self.head_dim, cache.page_size,
-                              write_kv=cache.writes)
+        self._store(qkv, ctx, cache, inv_freq)
         q = qkv[:, :self.q_width]
         if choice.rows:
             # the 32-bit path: a warp or, in steps of few rows, a block per (row, head), the same order of every reduction

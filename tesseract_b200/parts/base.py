@@ -304,6 +304,8 @@ class SharedRows:
     sizes: Tuple[int, ...]       # host copies for decisions: rows of each group,
     blocks: Tuple[int, ...]      # blocks of keys in common,
     tails: Tuple[int, ...]       # and blocks (begun ones too) that each row reads behind them
+    # rows and groups that the tensors have room for, where a captured step refills them (None: they hold just these)
+    room: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
 
     @classmethod
@@ -344,6 +346,9 @@ class GroupView:
 
     block_table: Optional[torch.Tensor]  # int32 [R, max_pages] on device; None for state groups
     page_size: int = 0
+    # a decode step with continuations of one prompt among its rows: which have their first keys in common, where reading those
+    # once pays (every row's block table names them too, so a part may ignore this)
+    shared: Optional["SharedRows"] = None
 
 
 @dataclass

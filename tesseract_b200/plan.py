@@ -293,6 +293,15 @@ SHARED_MIN_RUN = 4          # blocks of 64 keys: a tile of 16 keys for each of e
 SHARED_MAX_PARTS = 64
 
 
+SHARED_MIN_SAVED = 64       # blocks of 64 keys
+
+
+def sharing_pays(sizes: Sequence[int], blocks: Sequence[int]) -> bool:
+    """Whether a decode step reads common keys once a group (``sizes`` rows, ``blocks`` blocks of 64 keys in common each) rather than
+    once a row."""
+    return sum((n - 1) * b for n, b in zip(sizes, blocks)) >= SHARED_MIN_SAVED
+
+
 def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,
                      sms: Optional[int] = None) -> SharedAttentionPlan:
     """The plan of attention over groups of rows with keys in common (``shared``: a :class:`SharedRows`, which keeps its plans: the
@@ -335,7 +344,9 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target)
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
-    return SharedAttentionPlan(int(tiles.sum()), prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
+    # (tensors that are refilled: no grouping of so many rows has more tiles)
+    count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + shared.room // 2
+    return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,

@@ -182,7 +182,7 @@ def test_full_pages_are_held_together_and_the_page_being_filled_is_copied():
     assert cache.fork([("p", "x")])
     a, b = cache.pages_of("p"), cache.pages_of("x")
     assert a[0] == b[0] and a[1] == b[1] and a[2] != b[2] and cache.used_pages() == 4
-    assert cache.rows_in_common(0, ["p", "x"]) == ([[0, 1]], [8])
+    assert cache.rows_in_common(["p", "x"]) == ([[0, 1]], [8])
     assert cache.has_company(["p", "x"]) and not cache.has_company(["x"])
 
 
@@ -197,9 +197,9 @@ def test_rows_in_common_over_forks_of_forks_and_strangers():
     cache.extend("x", 8)
     cache.commit("x", 8)                                    # x: 17 tokens, p: 9
     cache.fork([("x", "y")])
-    assert cache.rows_in_common(0, ["x", "s", "y"]) == ([[0, 2], [1]], [16, 0])
-    assert cache.rows_in_common(0, ["y", "x", "p", "s"]) == ([[0, 1, 2], [3]], [8, 0])
-    assert cache.rows_in_common(1, ["x", "y"]) == ([[0], [1]], [0, 0])       # windows move on by themselves: nothing is shared
+    assert cache.rows_in_common(["x", "s", "y"]) == ([[0, 2], [1]], [16, 0])
+    assert cache.rows_in_common(["y", "x", "p", "s"]) == ([[0, 1, 2], [3]], [8, 0])
+    assert cache.shares_keys(0) and not cache.shares_keys(1)                # a window moves on for each by itself
     cache.check()
 
 
@@ -227,7 +227,8 @@ def test_forks_refuse_what_makes_no_sense():
     cache.admit("p")
     cache.extend("p", 6)
     cache.commit("p", 6)
-    for pairs, reserve in [([("q", "x")], None), ([("p", "p")], None), ([("p", "x"), ("p", "x")], None), ([("p", "x")], 5)]:
+    for pairs, reserve in [([("q", "x")], None), ([("p", "p")], None), ([("p", "x"), ("p", "x")], None), ([("p", "x")], 5),
+                           ([("p", "x"), ("p", "y")], [9])]:
         with pytest.raises(ValueError):
             cache.fork(pairs, reserve)
     assert cache.fork([]) and cache.compact() == 0
