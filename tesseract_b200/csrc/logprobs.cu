@@ -8,45 +8,45 @@
 // vocabulary has log probability NaN.
 //
 // Bound by HBM: 4 V bytes a row, read once.  A row is shared by a thread-block cluster of 1 to 8 blocks (a contiguous
-// part each); a block takes its part in chunks of 8,192 logits, sixteen a thread in registers, the next chunk's loads
-// under way meanwhile.  Of a chunk
+// part each); a block takes its part in chunks of sixteen logits a thread, in registers, the next chunk's loads under way
+// meanwhile.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
+// others' loads; few rows: blocks of 1,024, one chunk each at a vocabulary of 128,256.  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
 //     they meet once, at the end, in a fixed order, so a row's numbers do not depend on the timing;
 //   * a thread whose maximum exceeds the k-th best logit so far puts what exceeds it into a list in shared memory.  Once
 //     the first chunk is done few do: k numbers for the second chunk, k / 2 for the third.  A list that grows is cut to its k
 //     best (each entry's rank is the number of entries in front of it).
-//   * where more threads exceed it than the list could hold (the first chunk, or logits that rise with the id), a bound
-//     that at least k threads' maxima reach is found first, by halving the interval of the maxima's bit patterns; if equal
-//     numbers leave no bound that few enough reach, what lies above is taken and of the equal ones those of lowest id.
+//   * where more threads exceed it than the list could hold (the first chunk, or logits that rise with the id) a bound comes
+//     first: the k-th largest of 64 thread maxima (each warp's largest few), which k logits of the chunk reach.  Should more
+//     threads reach that than fit, the interval of the maxima's bit patterns is halved until few enough do; and if equal
+//     numbers leave no such bound, what lies above is taken and of the equal ones those of lowest id.
 #include "common.cuh"
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kPackets = 4;                        // 16-byte loads of a thread and chunk
 constexpr int kEach = 4 * kPackets;                // logits of a thread and chunk
-constexpr int kChunk = kEach * kThreads;
 constexpr int kMaxTop = 64;
 constexpr int kListed = 2048;                      // entries of the list
 constexpr int kRoom = (kListed - kMaxTop) / kEach; // threads that may add to a list of at most kMaxTop entries (124)
 static_assert(kRoom >= kMaxTop, "a bound that kMaxTop threads reach must fit");
 constexpr int kCut = 96;                           // a list this much longer than k is cut after a chunk
 constexpr int kMaxBlocks = 8;
+constexpr int kNobody = 0x7fffffff;                // the id of an entry that is none
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1024.0f;                   // e^x is 0 in 32 bits from here on down
 
 struct Shared {
     float value[kListed];
     int id[kListed];
-    float best_value[kMaxTop];
+    float best_value[kMaxTop];                     // k entries in order, behind those there are (-inf, kNobody)
     int best_id[kMaxTop];
-    float warp_stat[kWarps][3];
-    uint32_t warp_low[kWarps], warp_high[kWarps];
-    int warp_count[kWarps];
+    uint32_t sample[kMaxTop];                      // thread maxima, the largest of each warp
+    float warp_stat[32][3];
+    int warp_count[32];
     float stat[3];                                 // this block's m, S, T
+    uint32_t bound;
     int count;                                     // entries of the list
-    int kept;                                      // entries of best_*
 };
 
 // floats as unsigned numbers of the same order (-inf smallest; NaN never gets here)
@@ -56,6 +56,11 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 __device__ __forceinline__ float from_ordered(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ float exp2_of(float x) {       // 2^x, relative error about 2^-22, 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // (m, S, T) of two disjoint sets of numbers
@@ -67,11 +72,19 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float m2, flo
         return;
     }
     // (where e^(m - top) is 0, the distance must not make an infinity of what it is multiplied by; an infinite top gives NaN)
-    const float a = exp2f((m - top) * kLog2e), b = exp2f((m2 - top) * kLog2e);
+    const float a = exp2_of((m - top) * kLog2e), b = exp2_of((m2 - top) * kLog2e);
     const float da = fmaxf(m - top, kFar), db = fmaxf(m2 - top, kFar);
     t = (t + s * da) * a + (t2 + s2 * db) * b;
     s = s * a + s2 * b;
     m = top;
+}
+// The same over the first `count` (a power of two) lanes of a warp; every lane gets the result.
+__device__ __forceinline__ void join_lanes(float& m, float& s, float& t, int count) {
+    for (int o = 1; o < count; o <<= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
+        join(m, s, t, m2, s2, t2);
+    }
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -85,12 +98,17 @@ __device__ __forceinline__ uint32_t peer_u32(const void* local, uint32_t rank) {
     return v;
 }
 
-// Cuts the list to its k best, in order, in best_value / best_id: the rank of an entry is the number of entries in front of
+// The k best of the list's n entries, in order, into best_value / best_id: the rank of an entry is the number of entries in front of
 // it.  `share` threads count for one entry.  Every thread calls this; the list is whole (a barrier in front).
+template <int THREADS>
 __device__ __forceinline__ void cut(Shared& sh, int n, int k) {
     int share = 1;
-    while (share < 32 && n * share * 2 <= kThreads) share *= 2;
-    for (int base = 0; base < n; base += kThreads / share) {
+    while (share < 32 && n * share * 2 <= THREADS) share *= 2;
+    if ((int)threadIdx.x >= n && (int)threadIdx.x < k) {
+        sh.best_value[threadIdx.x] = -INFINITY;
+        sh.best_id[threadIdx.x] = kNobody;
+    }
+    for (int base = 0; base < n; base += THREADS / share) {
         const int e = base + (int)threadIdx.x / share, part = (int)threadIdx.x % share;
         const bool mine = e < n;
         const float v = mine ? sh.value[e] : 0.0f;
@@ -113,9 +131,10 @@ __device__ __forceinline__ void cut(Shared& sh, int n, int k) {
 }
 
 // The list of n entries becomes the k best alone.  Returns the value that a later logit has to exceed.
+template <int THREADS>
 __device__ __forceinline__ float recut(Shared& sh, int n, int k) {
     const int kept = min(n, k);
-    cut(sh, n, k);
+    cut<THREADS>(sh, n, k);
     if ((int)threadIdx.x < kept) {
         sh.value[threadIdx.x] = sh.best_value[threadIdx.x];
         sh.id[threadIdx.x] = sh.best_id[threadIdx.x];
@@ -126,6 +145,7 @@ __device__ __forceinline__ float recut(Shared& sh, int n, int k) {
     return bound;
 }
 
+template <int THREADS>
 __device__ __forceinline__ int sum_before(Shared& sh, int mine, int& all) {      // exclusive sum over the block's threads
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = mine;
@@ -139,7 +159,7 @@ __device__ __forceinline__ int sum_before(Shared& sh, int mine, int& all) {     
     __syncthreads();
     int before = incl - mine;
     all = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += sh.warp_count[w];
         all += sh.warp_count[w];
     }
@@ -147,10 +167,13 @@ __device__ __forceinline__ int sum_before(Shared& sh, int mine, int& all) {     
 }
 
 // grid: rows * blocks; the blocks of a row are one cluster.
-__global__ void __launch_bounds__(kThreads, 2)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __restrict__ tokens,
                 float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_value,
                 int* __restrict__ top_id, int vocab, int k, int blocks, int part) {
+    constexpr int WARPS = THREADS / 32, kChunk = kEach * THREADS;
+    constexpr int kSampled = kMaxTop / WARPS;      // thread maxima of a warp among the sample
     __shared__ Shared sh;
     pdl_trigger();
     const int64_t r = blockIdx.x / blocks;
@@ -163,7 +186,6 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const int end = last - first + ahead;          // logits are base[ahead .. end)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
     pdl_wait();                                    // the logits come from the kernel in front
     float given = NAN;
     if (block == 0 && threadIdx.x == 0) {
@@ -174,7 +196,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     auto fetch = [&](float4 (&held)[kPackets], int chunk) {
 #pragma unroll
         for (int u = 0; u < kPackets; ++u) {
-            const int i = chunk + (u * kThreads + (int)threadIdx.x) * 4;
+            const int i = chunk + (u * THREADS + (int)threadIdx.x) * 4;
             if (i >= ahead && i + 4 <= end) {
                 held[u] = __ldcs(reinterpret_cast<const float4*>(base + i));
             } else {
@@ -206,7 +228,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         top = top > -INFINITY ? top + 0.0f : -INFINITY;   // (sixteen NaNs; -0 is +0, as comparisons have it)
         if (top > m) {
             if (m > -INFINITY) {
-                const float d = m - top, a = exp2f(d * kLog2e);
+                const float d = m - top, a = exp2_of(d * kLog2e);
                 t = (t + s * fmaxf(d, kFar)) * a;
                 s *= a;
             }
@@ -215,12 +237,12 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         const float low = m > -INFINITY ? m : 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const float d = x[i] - low, e = exp2f(d * kLog2e);
+            const float d = x[i] - low, e = exp2_of(d * kLog2e);
             s += e;
             t += fmaxf(d, kFar) * e;               // (-inf adds nothing, a NaN comes in by e)
         }
         if (k == 0) continue;
-        auto id_of = [&](int i) { return first + chunk + ((i >> 2) * kThreads + (int)threadIdx.x) * 4 + (i & 3) - ahead; };
+        auto id_of = [&](int i) { return first + chunk + ((i >> 2) * THREADS + (int)threadIdx.x) * 4 + (i & 3) - ahead; };
         auto add = [&](bool wanted, int i) {
             if (!wanted) return;
             const int at = atomicAdd(&sh.count, 1);
@@ -238,34 +260,49 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
             cut_now = over >= k;
         } else {
             cut_now = true;
-            if (listed > k) bound = recut(sh, listed, k);
-            // a bound that at least k and at most kRoom threads' maxima reach
+            if (listed > k) bound = recut<THREADS>(sh, listed, k);
             const uint32_t mine = ordered(top), floor = ordered(bound);
-            uint32_t smallest = __reduce_min_sync(0xffffffffu, mine), largest = __reduce_max_sync(0xffffffffu, mine);
-            if (lane == 0) {
-                sh.warp_low[warp] = smallest;
-                sh.warp_high[warp] = largest;
+            // the sample: each warp's kSampled largest maxima (of different threads)
+            uint32_t rest = mine, largest = 0;
+#pragma unroll
+            for (int j = 0; j < kSampled; ++j) {
+                const uint32_t best = __reduce_max_sync(0xffffffffu, rest);
+                if (j == 0) largest = best;
+                if (lane == 0) sh.sample[warp * kSampled + j] = best;
+                if (lane == __ffs(__ballot_sync(0xffffffffu, rest == best)) - 1) rest = 0;
             }
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                smallest = min(smallest, sh.warp_low[w]);
-                largest = max(largest, sh.warp_high[w]);
-            }
-            // low_key: what at least k threads reach, or all that exceed the bound; high_key: what fewer than k reach
-            uint32_t low_key = max(smallest, floor + 1), high_key = largest + 1;
-            int reach;
-            while (high_key > low_key + 1) {
-                const uint32_t middle = low_key + (high_key - low_key) / 2;
-                reach = __syncthreads_count(mine >= middle);
-                if (reach < k) {
-                    high_key = middle;
-                } else {
-                    low_key = middle;
-                    if (reach <= kRoom) break;
+            // its k-th largest (equal ones by their place, so that exactly one has every rank), which k threads at least reach
+            if (threadIdx.x < kMaxTop) {
+                const uint32_t v = sh.sample[threadIdx.x];
+                int rank = 0;
+#pragma unroll 8
+                for (int j = 0; j < kMaxTop; ++j) {
+                    const uint32_t o = sh.sample[j];
+                    rank += o > v || (o == v && j < (int)threadIdx.x) ? 1 : 0;
                 }
+                if (rank == k - 1) sh.bound = v;
+                if (rank == 0) sh.warp_count[0] = (int)v;           // the block's largest
             }
-            reach = __syncthreads_count(mine >= low_key);
+            __syncthreads();
+            uint32_t low_key = max(sh.bound, floor + 1);
+            largest = (uint32_t)sh.warp_count[0];
+            int reach = __syncthreads_count(mine >= low_key);
+            if (reach > kRoom) {
+                // low_key: what at least k threads reach, or all that exceed the bound; high_key: what fewer than k reach
+                uint32_t high_key = largest + 1;
+                while (high_key > low_key + 1) {
+                    const uint32_t middle = low_key + (high_key - low_key) / 2;
+                    reach = __syncthreads_count(mine >= middle);
+                    if (reach < k) {
+                        high_key = middle;
+                    } else {
+                        low_key = middle;
+                        if (reach <= kRoom) break;
+                    }
+                }
+                reach = __syncthreads_count(mine >= low_key);
+            }
             const float cutoff = from_ordered(low_key);
             if (reach <= kRoom) {
                 if (mine >= low_key) {
@@ -285,7 +322,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
 #pragma unroll
                     for (int i = 0; i < kEach; ++i) equal += (i >> 2) == u && x[i] == cutoff ? 1 : 0;
                     int all;
-                    int at = taken + sum_before(sh, equal, all);
+                    int at = taken + sum_before<THREADS>(sh, equal, all);
 #pragma unroll
                     for (int i = 0; i < kEach; ++i) {
                         if ((i >> 2) == u && x[i] == cutoff) {
@@ -300,58 +337,52 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         __syncthreads();
         listed = sh.count;                         // (nothing is added before the next chunk's barrier)
         if (cut_now || listed > k + kCut) {
-            bound = recut(sh, listed, k);
+            bound = recut<THREADS>(sh, listed, k);
             listed = min(listed, k);
         }
     }
 
     // the block's sums, in the order of lanes and warps
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
-        join(m, s, t, m2, s2, t2);
-    }
+    join_lanes(m, s, t, 32);
     if (lane == 0) {
         sh.warp_stat[warp][0] = m;
         sh.warp_stat[warp][1] = s;
         sh.warp_stat[warp][2] = t;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWarps; ++w) join(m, s, t, sh.warp_stat[w][0], sh.warp_stat[w][1], sh.warp_stat[w][2]);
-        sh.stat[0] = m;
-        sh.stat[1] = s;
-        sh.stat[2] = t;
+    if (warp == 0) {
+        m = lane < WARPS ? sh.warp_stat[lane][0] : -INFINITY;
+        s = lane < WARPS ? sh.warp_stat[lane][1] : 0.0f;
+        t = lane < WARPS ? sh.warp_stat[lane][2] : 0.0f;
+        join_lanes(m, s, t, WARPS);
+        if (lane == 0) {
+            sh.stat[0] = m;
+            sh.stat[1] = s;
+            sh.stat[2] = t;
+        }
     }
-    if (k > 0) {
-        cut(sh, listed, k);
-        if (threadIdx.x == 0) sh.kept = min(listed, k);
-    }
+    if (k > 0) cut<THREADS>(sh, listed, k);
     if (blocks > 1) {
         cluster_sync();
         if (block == 0) {
-            if (threadIdx.x == 0) {
-                m = sh.stat[0], s = sh.stat[1], t = sh.stat[2];
-                for (int c = 1; c < blocks; ++c)
-                    join(m, s, t, __uint_as_float(peer_u32(&sh.stat[0], c)), __uint_as_float(peer_u32(&sh.stat[1], c)),
-                         __uint_as_float(peer_u32(&sh.stat[2], c)));
+            // the blocks' best together (k each, what is none of a block's behind all others: blocks * k <= 512), then the row's
+            for (int i = threadIdx.x; i < blocks * k; i += THREADS) {
+                sh.value[i] = __uint_as_float(peer_u32(&sh.best_value[i % k], i / k));
+                sh.id[i] = (int)peer_u32(&sh.best_id[i % k], i / k);
             }
-            if (k > 0) {
-                // the blocks' best together (each at most k: blocks * k <= kListed), then the row's
-                int n = 0;
-                for (int c = 0; c < blocks; ++c) {
-                    const int kept = (int)peer_u32(&sh.kept, c);
-                    for (int i = threadIdx.x; i < kept; i += kThreads) {
-                        sh.value[n + i] = __uint_as_float(peer_u32(&sh.best_value[i], c));
-                        sh.id[n + i] = (int)peer_u32(&sh.best_id[i], c);
-                    }
-                    n += kept;
-                }
-                __syncthreads();
-                cut(sh, n, k);
-                if (threadIdx.x == 0) sh.kept = min(n, k);
+            if (warp == 0) {
+                m = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[0], lane)) : -INFINITY;
+                s = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[1], lane)) : 0.0f;
+                t = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[2], lane)) : 0.0f;
+                join_lanes(m, s, t, kMaxBlocks);
             }
+            __syncthreads();
+            if ((int)threadIdx.x < k) {            // (what is no entry has no rank of its own)
+                sh.best_value[threadIdx.x] = -INFINITY;
+                sh.best_id[threadIdx.x] = kNobody;
+            }
+            __syncthreads();
+            if (k > 0) cut<THREADS>(sh, blocks * k, k);
             if (threadIdx.x == 0) {
                 sh.stat[0] = m;
                 sh.stat[1] = s;
@@ -368,55 +399,51 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         logprob[r] = (given - high) - log_sum;
         entropy[r] = log_sum - sh.stat[2] / sh.stat[1];
     }
-    const int kept = k > 0 ? sh.kept : 0;
-    for (int i = threadIdx.x; i < kept; i += kThreads) {
-        top_value[r * k + i] = (sh.best_value[i] - high) - log_sum;
-        top_id[r * k + i] = sh.best_id[i];
-    }
-    if (kept < k && warp == 0) {
-        // fewer than k logits above -inf: those at -inf (or NaN) follow, by id.  All but fewer than k are of that kind, so the
-        // first warp finds them within 2 k tokens.
-        int at = kept;
-        for (int i0 = 0; i0 < vocab && at < k; i0 += 32) {
-            const int i = i0 + lane;
-            const bool is = i < vocab && !(row[i] > -INFINITY);
-            const unsigned who = __ballot_sync(0xffffffffu, is);
-            const int place = at + __popc(who & ((1u << lane) - 1));
-            if (is && place < k) {
-                top_value[r * k + place] = (row[i] - high) - log_sum;
-                top_id[r * k + place] = i;
-            }
-            at += __popc(who);
+    if (warp != 0) return;
+    int kept = 0;
+    for (int i0 = 0; i0 < k; i0 += 32) {
+        const int i = i0 + lane;
+        const bool is = i < k && sh.best_id[i] != kNobody;
+        if (is) {
+            top_value[r * k + i] = (sh.best_value[i] - high) - log_sum;
+            top_id[r * k + i] = sh.best_id[i];
         }
+        kept += __popc(__ballot_sync(0xffffffffu, is));
+    }
+    // Fewer than k logits above -inf: those at -inf (or NaN) follow, by id.  All but fewer than k are of that kind, so they are found
+    // within 2 k tokens.
+    for (int i0 = 0; i0 < vocab && kept < k; i0 += 32) {
+        const int i = i0 + lane;
+        const bool is = i < vocab && !(row[i] > -INFINITY);
+        const unsigned who = __ballot_sync(0xffffffffu, is);
+        const int place = kept + __popc(who & ((1u << lane) - 1));
+        if (is && place < k) {
+            top_value[r * k + place] = (row[i] - high) - log_sum;
+            top_id[r * k + place] = i;
+        }
+        kept += __popc(who);
     }
 }
 
-// Blocks of a row: as many (up to the portable cluster size) as keep the grid within the two blocks a multiprocessor that fit,
-// and a chunk for each.
-int blocks_per_row(int rows, int vocab) {
+int sm_count() {
     static int sms = 0;
     if (sms == 0) {
         int device = 0;
         cudaGetDevice(&device);
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 1;
     }
-    int blocks = kMaxBlocks;
-    while (blocks > 1 && ((int64_t)rows * blocks > 2 * sms || vocab <= (blocks / 2) * kChunk)) blocks >>= 1;
-    return blocks;
+    return sms;
 }
 
-}  // namespace
-
-TB_EXPORT int tb_token_logprobs(const float* logits, int64_t stride, const int* tokens, float* logprob, float* entropy,
-                                float* top_value, int* top_id, int rows, int vocab, int top, cudaStream_t stream) {
-    if (rows == 0) return 0;
-    if (rows < 0 || vocab <= 0 || vocab > (1 << 30) || top < 0 || top > kMaxTop || top > vocab) return TB_ERR_BAD_SIZE;
-    const int blocks = blocks_per_row(rows, vocab);
+template <int THREADS>
+int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const float* logits, int64_t stride, const int* tokens,
+                float* logprob, float* entropy, float* top_value, int* top_id, int top) {
+    while (blocks > 1 && vocab <= (blocks / 2) * kEach * THREADS) blocks >>= 1;      // (a chunk for each)
     if ((int64_t)rows * blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
     const int part = ((vocab + blocks - 1) / blocks + 3) / 4 * 4;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(rows * blocks));
-    config.blockDim = dim3(kThreads);
+    config.blockDim = dim3(THREADS);
     config.stream = stream;
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -427,7 +454,22 @@ TB_EXPORT int tb_token_logprobs(const float* logits, int64_t stride, const int* 
     attribute[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attribute;
     config.numAttrs = 2;
-    const cudaError_t err = cudaLaunchKernelEx(&config, logprobs_kernel, logits, stride, tokens, logprob, entropy, top_value,
-                                               top_id, vocab, top, blocks, part);
+    const cudaError_t err = cudaLaunchKernelEx(&config, logprobs_kernel<THREADS>, logits, stride, tokens, logprob, entropy,
+                                               top_value, top_id, vocab, top, blocks, part);
     return err == cudaSuccess ? tb_launch_status() : (int)err;
+}
+
+}  // namespace
+
+TB_EXPORT int tb_token_logprobs(const float* logits, int64_t stride, const int* tokens, float* logprob, float* entropy,
+                                float* top_value, int* top_id, int rows, int vocab, int top, cudaStream_t stream) {
+    if (rows == 0) return 0;
+    if (rows < 0 || vocab <= 0 || vocab > (1 << 30) || top < 0 || top > kMaxTop || top > vocab) return TB_ERR_BAD_SIZE;
+    // few rows: large blocks, as many a row as keep one a multiprocessor; many: small ones, four a multiprocessor
+    const int64_t sms = sm_count();
+    if (rows * kMaxBlocks <= sms)
+        return launch_rows<1024>(rows, vocab, kMaxBlocks, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
+    int blocks = kMaxBlocks;
+    while (blocks > 1 && (int64_t)rows * blocks > 4 * sms) blocks >>= 1;
+    return launch_rows<256>(rows, vocab, blocks, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
 }

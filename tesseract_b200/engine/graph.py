@@ -201,7 +201,8 @@ class DecodeGraphs:
     def __init__(self, stepper: Stepper, max_batch: int):
         self.stepper = stepper
         self.max_batch = max_batch
-        self.graphs: Dict[Tuple[int, int, bool], _Graph] = {}
+        self.graphs: Dict[Tuple[int, int], _Graph] = {}
+        self.shared_graphs: Dict[Tuple[int, int], _Graph] = {}      # of steps whose rows have keys in common (Stepper.company)
         self.replays = 0
         self.captures = 0
         self.kernels_replayed = 0
@@ -230,11 +231,11 @@ class DecodeGraphs:
         pages = -(-(max(lengths) + 1) // cache.page_size)
         batch, columns = min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages))
         company = stepper.company(entries, batch - count)
-        key = (batch, columns, company is not None)
-        graph = self.graphs.get(key)
+        graphs = self.graphs if company is None else self.shared_graphs
+        graph = graphs.get((batch, columns))
         if graph is None:
             graph = _Graph(stepper, batch, columns, self.sampled, company)
-            self.graphs[key] = graph
+            graphs[batch, columns] = graph
             self.captures += 1
         slot_index, h = graph.host_arrays()
         if company is not None:
