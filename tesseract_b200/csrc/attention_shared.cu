@@ -19,6 +19,9 @@
 //                few columns of the values.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
+#include <new>
+#include <set>
+
 #include "tma.cuh"
 
 namespace {
@@ -1021,16 +1024,30 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
     }
 }
 
+// What a kernel is told once a device: the shared memory that it may ask for, and that the multiprocessors be set up for the largest
+// (kernels that follow each other without a gap: one that asks for little must not leave the next one little).
+int set_up(const void* kernel, size_t smem) {
+    static std::mutex lock;
+    static std::set<std::pair<const void*, int>> done;
+    int device = 0;
+    if (const cudaError_t err = cudaGetDevice(&device)) return (int)err;
+    std::lock_guard<std::mutex> guard(lock);
+    if (done.count({kernel, device})) return 0;
+    if (smem > 48 * 1024)
+        if (const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)err;
+    if (const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared))
+        return (int)err;
+    try {
+        done.insert({kernel, device});
+    } catch (const std::bad_alloc&) {         // (asked again next time)
+    }
+    return 0;
+}
+
 template <typename Kernel>
 int launch(Kernel kernel, int64_t blocks, int threads, size_t smem, const SharedParams& p, cudaStream_t stream) {
     if (blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
-    if (smem > 48 * 1024) {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return (int)err;
-    }
-    // (kernels that follow each other without a gap: one that asks for little shared memory must not leave the next one little)
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (err != cudaSuccess) return (int)err;
+    if (const int err = set_up((const void*)kernel, smem)) return err;
     if (cudaError_t err = tb_launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), smem, stream, p)) return (int)err;
     return tb_launch_status();
 }
@@ -1050,8 +1067,7 @@ template <int D>
 int launch_tc(const CUtensorMap& map, int64_t blocks, const SharedParams& p, cudaStream_t stream) {
     if (blocks > 0x7fffffff) return TB_ERR_BAD_SIZE;
     const size_t smem = TcShape<D>::kBytes;
-    const cudaError_t err = cudaFuncSetAttribute(shared_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (err != cudaSuccess) return (int)err;
+    if (const int err = set_up((const void*)shared_tc_kernel<D>, smem)) return err;
     if (cudaError_t launched = tb_launch_pdl(shared_tc_kernel<D>, dim3((unsigned)blocks), dim3(kTcThreads), smem, stream, map, p))
         return (int)launched;
     return tb_launch_status();

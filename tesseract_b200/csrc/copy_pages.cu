@@ -93,37 +93,43 @@ int piece_bytes(int64_t total) { return total >= (int64_t)(32 << 20) ? 16384 : 4
 
 constexpr int kErrBadPage = -6, kErrClash = -7, kErrMemory = -8;
 
-// store s: base[s], pitch[s] bytes from an entry to the next, size[s] bytes a page, entries[s] entries of pages[s] pages each;
-// counts[s] moves from sources[s][i] to targets[s][i].
-TB_EXPORT int tb_copy_pages(int num_stores, void* const* base, const int64_t* pitch, const int64_t* size, const int* entries,
-                            const int* pages, const int* counts, const int* const* sources, const int* const* targets,
-                            int* launches, cudaStream_t stream) {
+// packed: for every store its address, entries, pages, bytes of a page, moves, and the addresses of its sources and its targets
+// (int32).
+TB_EXPORT int tb_copy_pages(int num_stores, const int64_t* packed, int* launches, cudaStream_t stream) {
+    auto base = [&](int s) { return (char*)packed[s * 7]; };
+    auto entries = [&](int s) { return packed[s * 7 + 1]; };
+    auto pages = [&](int s) { return packed[s * 7 + 2]; };
+    auto size = [&](int s) { return packed[s * 7 + 3]; };
+    auto counts = [&](int s) { return (int)packed[s * 7 + 4]; };
+    auto sources = [&](int s) { return (const int*)packed[s * 7 + 5]; };
+    auto targets = [&](int s) { return (const int*)packed[s * 7 + 6]; };
     *launches = 0;
     std::vector<uint8_t> seen;
     int64_t total_bytes = 0;
     for (int s = 0; s < num_stores; ++s) {
-        if (entries[s] < 0 || pages[s] < 0 || size[s] < 0 || counts[s] < 0) return TB_ERR_BAD_SIZE;
+        if (entries(s) < 0 || pages(s) < 0 || pages(s) > 0x7fffffff || size(s) < 0 || packed[s * 7 + 4] < 0 || packed[s * 7 + 4] > 0x7fffffff)
+            return TB_ERR_BAD_SIZE;
         try {
-            seen.assign((size_t)pages[s], 0);
+            seen.assign((size_t)pages(s), 0);
         } catch (const std::bad_alloc&) {
             return kErrMemory;
         }
-        for (int i = 0; i < counts[s]; ++i) {
-            if (sources[s][i] < 0 || sources[s][i] >= pages[s] || targets[s][i] < 0 || targets[s][i] >= pages[s]) return kErrBadPage;
-            seen[(size_t)sources[s][i]] = 1;
+        for (int i = 0; i < counts(s); ++i) {
+            if (sources(s)[i] < 0 || sources(s)[i] >= pages(s) || targets(s)[i] < 0 || targets(s)[i] >= pages(s)) return kErrBadPage;
+            seen[(size_t)sources(s)[i]] = 1;
         }
-        for (int i = 0; i < counts[s]; ++i) {
-            uint8_t& mark = seen[(size_t)targets[s][i]];
+        for (int i = 0; i < counts(s); ++i) {
+            uint8_t& mark = seen[(size_t)targets(s)[i]];
             if (mark) return kErrClash;
             mark = 2;
         }
-        total_bytes += size[s] * counts[s] * entries[s];
+        total_bytes += size(s) * counts(s) * entries(s);
     }
     if (total_bytes == 0) return 0;
     // one launch takes up to kMaxStores stores and as many moves as its parameters hold; a store's moves may go on in the next
     int s = 0, done = 0;
     int64_t moves_left = 0;
-    for (int k = 0; k < num_stores; ++k) moves_left += counts[k];
+    for (int k = 0; k < num_stores; ++k) moves_left += counts(k);
     Params<kFewMoves> few;
     static thread_local Params<kManyMoves> many;       // (32 KB: too large to lay on a caller's stack unasked)
     while (s < num_stores) {
@@ -135,25 +141,25 @@ TB_EXPORT int tb_copy_pages(int num_stores, void* const* base, const int64_t* pi
         int used = 0, taken = 0;
         int64_t pieces = 0;
         while (s < num_stores && used < kMaxStores && taken < room) {
-            const int n = counts[s] - done < room - taken ? counts[s] - done : room - taken;
-            if (n > 0 && entries[s] > 0 && size[s] > 0) {
+            const int n = counts(s) - done < room - taken ? counts(s) - done : room - taken;
+            if (n > 0 && entries(s) > 0 && size(s) > 0) {
                 Store& store = stores[used++];
-                store.base = (char*)base[s];
-                store.pitch = pitch[s];
-                store.size = size[s];
-                const uint64_t all = (uint64_t)(uintptr_t)base[s] | (uint64_t)pitch[s] | (uint64_t)size[s];
+                store.base = base(s);
+                store.pitch = size(s) * pages(s);
+                store.size = size(s);
+                const uint64_t all = (uint64_t)(uintptr_t)base(s) | (uint64_t)size(s);
                 store.width = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
                 store.first_move = taken;
                 store.moves = n;
-                store.pieces = (int)((size[s] + piece - 1) / piece);
+                store.pieces = (int)((size(s) + piece - 1) / piece);
                 store.first_piece = pieces;
-                pieces += (int64_t)store.pieces * n * entries[s];
-                for (int i = 0; i < n; ++i) moves[taken + i] = make_int2(sources[s][done + i], targets[s][done + i]);
+                pieces += (int64_t)store.pieces * n * entries(s);
+                for (int i = 0; i < n; ++i) moves[taken + i] = make_int2(sources(s)[done + i], targets(s)[done + i]);
                 taken += n;
             }
             done += n;
             moves_left -= n;
-            if (done < counts[s]) break;
+            if (done < counts(s)) break;
             done = 0;
             ++s;
         }

@@ -13,13 +13,12 @@
 // others' loads; few rows: blocks of 1,024, one chunk each at a vocabulary of 128,256.  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
 //     they meet once, at the end, in a fixed order, so a row's numbers do not depend on the timing;
-//   * a thread whose maximum exceeds the k-th best logit so far puts what exceeds it into a list in shared memory.  Once
-//     the first chunk is done few do: k numbers for the second chunk, k / 2 for the third.  A list that grows is cut to its k
-//     best (each entry's rank is the number of entries in front of it).
-//   * where more threads exceed it than the list could hold (the first chunk, or logits that rise with the id) a bound comes
-//     first: the k-th largest of 64 thread maxima (each warp's largest few), which k logits of the chunk reach.  Should more
-//     threads reach that than fit, the interval of the maxima's bit patterns is halved until few enough do; and if equal
-//     numbers leave no such bound, what lies above is taken and of the equal ones those of lowest id.
+//   * every eight threads leave the largest of their 128 logits.  No block waits for anything inside the loop.
+// The alternatives come behind it: the k-th largest (or so) of those maxima is a bound that at least k logits reach, the few groups
+// of 128 that reach it are read once more (from L2), and what reaches it is ranked (an entry's rank is the number of entries in front
+// of it).  Where more logits reach the bound than the list holds (logits in order, a vocabulary of few groups, masks), the
+// interval of their bit patterns is halved, reading those groups each time, until few enough do; and if equal numbers leave no
+// such bound, what lies above is taken and of the equal ones those of lowest id.
 #include "common.cuh"
 
 namespace {
@@ -27,10 +26,9 @@ namespace {
 constexpr int kPackets = 4;                        // 16-byte loads of a thread and chunk
 constexpr int kEach = 4 * kPackets;                // logits of a thread and chunk
 constexpr int kMaxTop = 64;
-constexpr int kListed = 2048;                      // entries of the list
-constexpr int kRoom = (kListed - kMaxTop) / kEach; // threads that may add to a list of at most kMaxTop entries (124)
-static_assert(kRoom >= kMaxTop, "a bound that kMaxTop threads reach must fit");
-constexpr int kCut = 96;                           // a list this much longer than k is cut after a chunk
+constexpr int kListed = 512;                       // entries of the list
+constexpr int kGroup = 8;                          // threads whose largest logit is kept
+constexpr int kMaxGroups = 2048;                   // of a block (a longer part: of so many chunks together that they fit)
 constexpr int kMaxBlocks = 8;
 constexpr int kNobody = 0x7fffffff;                // the id of an entry that is none
 constexpr float kLog2e = 1.4426950408889634f;
@@ -41,12 +39,12 @@ struct Shared {
     int id[kListed];
     float best_value[kMaxTop];                     // k entries in order, behind those there are (-inf, kNobody)
     int best_id[kMaxTop];
-    uint32_t sample[kMaxTop];                      // thread maxima, the largest of each warp
+    uint32_t group[kMaxGroups];                    // the groups' largest logits, as `ordered` has them
+    int16_t reaching[kMaxGroups];                  // the groups that reach the bound
     float warp_stat[32][3];
-    int warp_count[32];
+    int warp_count[64];
     float stat[3];                                 // this block's m, S, T
-    uint32_t bound;
-    int count;                                     // entries of the list
+    int count, groups;                             // entries of the list, of `reaching`
 };
 
 // floats as unsigned numbers of the same order (-inf smallest; NaN never gets here)
@@ -130,19 +128,14 @@ __device__ __forceinline__ void cut(Shared& sh, int n, int k) {
     __syncthreads();
 }
 
-// The list of n entries becomes the k best alone.  Returns the value that a later logit has to exceed.
+// The sum over the block's threads with one barrier; two such sums that follow each other use places of their own (turn 0, 1).
 template <int THREADS>
-__device__ __forceinline__ float recut(Shared& sh, int n, int k) {
-    const int kept = min(n, k);
-    cut<THREADS>(sh, n, k);
-    if ((int)threadIdx.x < kept) {
-        sh.value[threadIdx.x] = sh.best_value[threadIdx.x];
-        sh.id[threadIdx.x] = sh.best_id[threadIdx.x];
-    }
-    if (threadIdx.x == 0) sh.count = kept;
-    const float bound = kept == k ? sh.best_value[k - 1] : -INFINITY;
+__device__ __forceinline__ int sum_of(Shared& sh, int mine, int turn) {
+    const int lane = threadIdx.x & 31;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) sh.warp_count[turn * 32 + (threadIdx.x >> 5)] = mine;
     __syncthreads();
-    return bound;
+    return __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? sh.warp_count[turn * 32 + lane] : 0);
 }
 
 template <int THREADS>
@@ -166,14 +159,133 @@ __device__ __forceinline__ int sum_before(Shared& sh, int mine, int& all) {     
     return before;
 }
 
+// Puts what may be among the k best of the block's logits into the list and returns how many that are (at least k, or all above
+// -inf if they are fewer; at most kListed).  The groups' largest logits, the block's m and zeroed counts are there.
+template <int THREADS>
+__device__ int find_best(Shared& sh, const float* base, int ahead, int end, int first, int chunks, int span, int k) {
+    constexpr int kChunk = kEach * THREADS, kGroups = THREADS / kGroup;
+    const int groups = (chunks + span - 1) / span * kGroups;
+    // low: what at least k logits reach, or all above -inf; high: what fewer than k groups (later: logits) reach
+    const uint32_t nothing = ordered(-INFINITY) + 1;
+    uint32_t low = nothing, high = sh.stat[0] > -INFINITY ? ordered(sh.stat[0] + 0.0f) + 1 : nothing;
+    int turn = 0;
+    while (high > low + 1) {
+        const uint32_t middle = low + (high - low) / 2;
+        int mine = 0;
+        for (int g = threadIdx.x; g < groups; g += THREADS) mine += sh.group[g] >= middle ? 1 : 0;
+        const int reach = sum_of<THREADS>(sh, mine, turn);
+        turn ^= 1;
+        if (reach < k) {
+            high = middle;
+        } else {
+            low = middle;
+            if (reach <= k + k / 4) break;
+        }
+    }
+    for (int g = threadIdx.x; g < groups; g += THREADS)
+        if (sh.group[g] >= low) sh.reaching[atomicAdd(&sh.groups, 1)] = (int16_t)g;
+    __syncthreads();
+    const int reaching = sh.groups;
+    // every logit of the groups that reach `low`, a group of threads each: take(logit, id)
+    auto walk = [&](auto take) {
+        for (int e = threadIdx.x / kGroup; e < reaching; e += kGroups) {
+            const int g = sh.reaching[e], c0 = g / kGroups * span, thread = g % kGroups * kGroup + (int)threadIdx.x % kGroup;
+            for (int c = c0; c < min(chunks, c0 + span); ++c) {
+                float x[kEach];
+#pragma unroll
+                for (int u = 0; u < kPackets; ++u) {
+                    const int i = c * kChunk + (u * THREADS + thread) * 4;
+                    if (i >= ahead && i + 4 <= end) {
+                        *reinterpret_cast<float4*>(x + 4 * u) = *reinterpret_cast<const float4*>(base + i);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[4 * u + j] = i + j >= ahead && i + j < end ? base[i + j] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    take(x[i], first + c * kChunk + ((i >> 2) * THREADS + thread) * 4 + (i & 3) - ahead);
+            }
+        }
+    };
+    auto add = [&](float x, int id) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kListed) {
+            sh.value[at] = x;
+            sh.id[at] = id;
+        }
+    };
+    float cutoff = from_ordered(low);
+    walk([&](float x, int id) { if (x >= cutoff) add(x, id); });
+    __syncthreads();
+    int n = sh.count;
+    if (n <= kListed) return n;
+    // more than the list holds
+    high = ordered(sh.stat[0] + 0.0f) + 1;
+    while (high > low + 1) {
+        const uint32_t middle = low + (high - low) / 2;
+        const float at_least = from_ordered(middle);
+        __syncthreads();                           // (everyone has read the count)
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        int mine = 0;
+        walk([&](float x, int) { mine += x >= at_least ? 1 : 0; });
+        __syncwarp();
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if ((threadIdx.x & 31) == 0) atomicAdd(&sh.count, mine);
+        __syncthreads();
+        n = sh.count;
+        if (n < k) {
+            high = middle;
+        } else {
+            low = middle;
+            if (n <= kListed) break;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    cutoff = from_ordered(low);
+    if (high > low + 1) {
+        walk([&](float x, int id) { if (x >= cutoff) add(x, id); });
+        __syncthreads();
+        return sh.count;
+    }
+    // fewer than k logits are larger than `cutoff`, more than fit equal to it: the larger ones, and of the equal ones the first k by
+    // id (packets of a lower u come first, then lower threads)
+    walk([&](float x, int id) { if (x > cutoff) add(x, id); });
+    int taken = 0;
+    for (int c = 0; c < chunks && taken < k; ++c) {
+        for (int u = 0; u < kPackets && taken < k; ++u) {
+            const int i = c * kChunk + (u * THREADS + (int)threadIdx.x) * 4;
+            float x[4];
+            int equal = 0, all;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = i + j >= ahead && i + j < end ? base[i + j] : -INFINITY;
+                equal += x[j] == cutoff ? 1 : 0;
+            }
+            int at = taken + sum_before<THREADS>(sh, equal, all);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (x[j] != cutoff) continue;
+                if (at < k) add(x[j], first + i + j - ahead);
+                ++at;
+            }
+            taken += all;
+        }
+    }
+    __syncthreads();
+    return sh.count;
+}
+
 // grid: rows * blocks; the blocks of a row are one cluster.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __restrict__ tokens,
                 float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_value,
                 int* __restrict__ top_id, int vocab, int k, int blocks, int part) {
-    constexpr int WARPS = THREADS / 32, kChunk = kEach * THREADS;
-    constexpr int kSampled = kMaxTop / WARPS;      // thread maxima of a warp among the sample
+    constexpr int WARPS = THREADS / 32, kChunk = kEach * THREADS, kGroups = THREADS / kGroup;
     __shared__ Shared sh;
     pdl_trigger();
     const int64_t r = blockIdx.x / blocks;
@@ -185,7 +297,6 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const float* base = row + first - ahead;       // (only packets that lie wholly inside the part are read as such)
     const int end = last - first + ahead;          // logits are base[ahead .. end)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) sh.count = 0;
     pdl_wait();                                    // the logits come from the kernel in front
     float given = NAN;
     if (block == 0 && threadIdx.x == 0) {
@@ -198,7 +309,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         for (int u = 0; u < kPackets; ++u) {
             const int i = chunk + (u * THREADS + (int)threadIdx.x) * 4;
             if (i >= ahead && i + 4 <= end) {
-                held[u] = __ldcs(reinterpret_cast<const float4*>(base + i));
+                held[u] = *reinterpret_cast<const float4*>(base + i);
             } else {
                 held[u].x = i >= ahead && i < end ? base[i] : -INFINITY;
                 held[u].y = i + 1 >= ahead && i + 1 < end ? base[i + 1] : -INFINITY;
@@ -208,11 +319,14 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         }
     };
 
-    float m = -INFINITY, s = 0.0f, t = 0.0f, bound = -INFINITY;
-    int listed = 0;                                // entries of the list, as every thread knows them between two chunks
+    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    const int chunks = (end + kChunk - 1) / kChunk;
+    const int span = max(1, (chunks * kGroups + kMaxGroups - 1) / kMaxGroups);       // chunks that a group's largest is taken over (1 up to 1M logits)
+    const int group = threadIdx.x / kGroup;
+    float largest = -INFINITY;
     float4 next[kPackets];
     fetch(next, 0);
-    for (int chunk = 0; chunk < end; chunk += kChunk) {
+    for (int c = 0; c < chunks; ++c) {
         float x[kEach];
 #pragma unroll
         for (int u = 0; u < kPackets; ++u) {
@@ -221,7 +335,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
             x[4 * u + 2] = next[u].z;
             x[4 * u + 3] = next[u].w;
         }
-        if (chunk + kChunk < end) fetch(next, chunk + kChunk);
+        if (c + 1 < chunks) fetch(next, (c + 1) * kChunk);
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
@@ -242,103 +356,12 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
             t += fmaxf(d, kFar) * e;               // (-inf adds nothing, a NaN comes in by e)
         }
         if (k == 0) continue;
-        auto id_of = [&](int i) { return first + chunk + ((i >> 2) * THREADS + (int)threadIdx.x) * 4 + (i & 3) - ahead; };
-        auto add = [&](bool wanted, int i) {
-            if (!wanted) return;
-            const int at = atomicAdd(&sh.count, 1);
-            sh.value[at] = x[i];
-            sh.id[at] = id_of(i);
-        };
-        const int over = __syncthreads_count(top > bound);
-        if (over == 0) continue;
-        bool cut_now;
-        if (over * kEach + listed <= kListed) {
-            if (top > bound) {
+        largest = fmaxf(largest, top);
+        if ((c + 1) % span == 0 || c + 1 == chunks) {
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) add(x[i] > bound, i);
-            }
-            cut_now = over >= k;
-        } else {
-            cut_now = true;
-            if (listed > k) bound = recut<THREADS>(sh, listed, k);
-            const uint32_t mine = ordered(top), floor = ordered(bound);
-            // the sample: each warp's kSampled largest maxima (of different threads)
-            uint32_t rest = mine, largest = 0;
-#pragma unroll
-            for (int j = 0; j < kSampled; ++j) {
-                const uint32_t best = __reduce_max_sync(0xffffffffu, rest);
-                if (j == 0) largest = best;
-                if (lane == 0) sh.sample[warp * kSampled + j] = best;
-                if (lane == __ffs(__ballot_sync(0xffffffffu, rest == best)) - 1) rest = 0;
-            }
-            __syncthreads();
-            // its k-th largest (equal ones by their place, so that exactly one has every rank), which k threads at least reach
-            if (threadIdx.x < kMaxTop) {
-                const uint32_t v = sh.sample[threadIdx.x];
-                int rank = 0;
-#pragma unroll 8
-                for (int j = 0; j < kMaxTop; ++j) {
-                    const uint32_t o = sh.sample[j];
-                    rank += o > v || (o == v && j < (int)threadIdx.x) ? 1 : 0;
-                }
-                if (rank == k - 1) sh.bound = v;
-                if (rank == 0) sh.warp_count[0] = (int)v;           // the block's largest
-            }
-            __syncthreads();
-            uint32_t low_key = max(sh.bound, floor + 1);
-            largest = (uint32_t)sh.warp_count[0];
-            int reach = __syncthreads_count(mine >= low_key);
-            if (reach > kRoom) {
-                // low_key: what at least k threads reach, or all that exceed the bound; high_key: what fewer than k reach
-                uint32_t high_key = largest + 1;
-                while (high_key > low_key + 1) {
-                    const uint32_t middle = low_key + (high_key - low_key) / 2;
-                    reach = __syncthreads_count(mine >= middle);
-                    if (reach < k) {
-                        high_key = middle;
-                    } else {
-                        low_key = middle;
-                        if (reach <= kRoom) break;
-                    }
-                }
-                reach = __syncthreads_count(mine >= low_key);
-            }
-            const float cutoff = from_ordered(low_key);
-            if (reach <= kRoom) {
-                if (mine >= low_key) {
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) add(x[i] >= cutoff && x[i] > bound, i);
-                }
-            } else {
-                // more threads than fit have `cutoff` as their maximum, fewer than k a larger one: all that is larger, and of
-                // what is equal to it the first k by id (packets of a lower u come first, then lower threads)
-                if (top > cutoff) {
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) add(x[i] > cutoff, i);
-                }
-                int taken = 0;
-                for (int u = 0; u < kPackets && taken < k; ++u) {
-                    int equal = 0;
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) equal += (i >> 2) == u && x[i] == cutoff ? 1 : 0;
-                    int all;
-                    int at = taken + sum_before<THREADS>(sh, equal, all);
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) {
-                        if ((i >> 2) == u && x[i] == cutoff) {
-                            add(at < k, i);
-                            ++at;
-                        }
-                    }
-                    taken += all;
-                }
-            }
-        }
-        __syncthreads();
-        listed = sh.count;                         // (nothing is added before the next chunk's barrier)
-        if (cut_now || listed > k + kCut) {
-            bound = recut<THREADS>(sh, listed, k);
-            listed = min(listed, k);
+            for (int o = 1; o < kGroup; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            if (threadIdx.x % kGroup == 0) sh.group[c / span * kGroups + group] = ordered(largest);
+            largest = -INFINITY;
         }
     }
 
@@ -359,9 +382,14 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
             sh.stat[0] = m;
             sh.stat[1] = s;
             sh.stat[2] = t;
+            sh.count = sh.groups = 0;
         }
     }
-    if (k > 0) cut<THREADS>(sh, listed, k);
+    __syncthreads();
+    if (k > 0) {
+        const int n = find_best<THREADS>(sh, base, ahead, end, first, chunks, span, k);
+        cut<THREADS>(sh, n, k);
+    }
     if (blocks > 1) {
         cluster_sync();
         if (block == 0) {

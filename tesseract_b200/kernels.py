@@ -9,6 +9,7 @@ loaded, or a kernel refuses a size, the call raises.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import numpy as np
@@ -75,6 +76,10 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
+def _raw_stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
@@ -88,6 +93,15 @@ def _cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise KernelError("kernel arguments must live on a CUDA device")
+
+
+@lru_cache(maxsize=None)
+def _entry(library: str, name: str, *types):
+    """The C entry ``name`` with its argument types declared: a call of thirty arguments then takes plain integers, which costs the
+    host a third less than a ctypes object for each."""
+    entry = getattr(load_library(library), name)
+    entry.argtypes = types
+    return entry
 
 
 SS_STRIDE = 16      # rows per tile / per CTA in the small side arrays that one kernel leaves for the next
@@ -163,33 +177,32 @@ def copy_pages(moves) -> None:
     travel in the launch: nothing has to outlive the call."""
     global launch_count
     count = len(moves)
-    base, pitch, size = (_pointer * count)(), (_i64 * count)(), (_i64 * count)()
-    entries, pages, counts = (_i32 * count)(), (_i32 * count)(), (_i32 * count)()
-    sources, targets = (_pointer * count)(), (_pointer * count)()
+    packed = []                                          # five numbers and two addresses a store
     kept = []                                            # the index arrays live until the call returns
     device = None
-    for i, (store, source, target) in enumerate(moves):
-        _cuda(store)
-        _need(store.dim() >= 2 and store.is_contiguous(), "copy_pages takes contiguous stores [entries, pages, ...]")
+    for store, source, target in moves:
+        if not (store.is_cuda and store.dim() >= 2 and store.is_contiguous()):
+            raise KernelError("copy_pages takes contiguous stores [entries, pages, ...] on a CUDA device")
         if device is None:
-            device = store.device
-            _need(device.index == torch.cuda.current_device(), "copy_pages runs on the current device")
-        _need(store.device == device, "copy_pages takes stores of one device")
+            device = store.get_device()
+            _need(device == torch.cuda.current_device(), "copy_pages runs on the current device")
+        elif store.get_device() != device:
+            raise KernelError("copy_pages takes stores of one device")
         source, target = _host_indices(source), _host_indices(target)
-        _need(source.size == target.size, "copy_pages takes as many targets as sources")
-        for j in range(i):
-            _need(moves[j][0].data_ptr() != store.data_ptr() or not store.numel(), "copy_pages takes a store once a call")
+        if source.size != target.size:
+            raise KernelError("copy_pages takes as many targets as sources")
         kept.append((source, target))
-        shape = store.shape
-        entries[i], pages[i] = shape[0], shape[1]
+        entries, pages = store.shape[0], store.shape[1]
         # (from the sizes: a tensor without numbers, or an extent of one, may have any stride)
-        size[i] = store.numel() // (shape[0] * shape[1]) * store.element_size() if store.numel() else 0
-        pitch[i] = size[i] * shape[1]
-        base[i], counts[i] = store.data_ptr(), source.size
-        sources[i], targets[i] = source.ctypes.data, target.ctypes.data
+        numbers = store.numel()
+        packed += (store.data_ptr(), entries, pages, numbers // (entries * pages) * store.element_size() if numbers else 0,
+                   source.size, source.ctypes.data, target.ctypes.data)
+    if count > 1 and len(set(packed[::7])) < sum(1 for p in packed[::7] if p) + any(p == 0 for p in packed[::7]):
+        raise KernelError("copy_pages takes a store once a call")
     launches = _i32(0)
-    status = load_library("copy_pages").tb_copy_pages(_i32(count), base, pitch, size, entries, pages, counts, sources, targets,
-                                                      ctypes.byref(launches), _stream())
+    status = _entry("copy_pages", "tb_copy_pages", _i32, _pointer, _pointer, _pointer)(
+        count, (_i64 * len(packed))(*packed), ctypes.addressof(launches),
+        torch._C._cuda_getCurrentRawStream(device) if device is not None else 0)
     launch_count -= 1                                    # (_check counts one; a call may launch none or several)
     _check(status, "copy_pages")
     launch_count += launches.value
@@ -200,6 +213,8 @@ def _host_indices(indices) -> np.ndarray:
         _need(not indices.is_cuda, "page indices are host lists or arrays")
         indices = indices.numpy()
     array = np.asarray(indices)
+    if array.dtype == np.int32 and array.ndim == 1 and array.flags.c_contiguous:
+        return array
     if array.size == 0:
         return np.empty(0, dtype=np.int32)
     _need(array.ndim == 1 and array.dtype.kind in "iu", "page indices are one-dimensional lists of integers")
@@ -316,27 +331,28 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     gives zeros) through row ``b`` of ``block_table``, a group's keys in common through its first member's.
     ``q``/``out``: ``[B, num_heads*head_dim]`` views; ``choice``: ``plan.shared_attention``'s answer for ``shared``."""
     _cuda(q, out, cache, positions, block_table, shared.members)
-    rows = q.shape[0]
-    _need(q.dtype == out.dtype == cache.dtype, "attention dtypes disagree")
-    _need(q.dim() == 2 and q.shape[1] == num_heads * head_dim and out.shape == q.shape and q.stride(1) == 1
-          and out.stride(1) == 1, "q/out layout")
+    rows, width = q.shape
+    dtype = q.dtype
+    _need(dtype == out.dtype == cache.dtype, "attention dtypes disagree")
+    _need(width == num_heads * head_dim and out.shape == q.shape and q.stride(1) == 1 and out.stride(1) == 1, "q/out layout")
     _need(positions.dtype == torch.int32 and block_table.dtype == torch.int32, "positions and block_table must be int32")
     _need(positions.is_contiguous() and positions.numel() == rows, "one position a row")
     _need(block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
           and block_table.shape[0] == rows, "block table: a row a row of q, rows contiguous")
-    _need(cache.is_contiguous() and tuple(cache.shape[1:]) == (2, num_kv_heads, page_size, head_dim), "cache layout")
+    _need(cache.is_contiguous() and cache.shape[1:] == (2, num_kv_heads, page_size, head_dim), "cache layout")
     _need(shared.members.numel() == rows == shared.common.numel(), "shared: a place for every row")
     _need(scale > 0.0, "the scale of the scores must be positive")
     parts = rows * num_heads * (choice.prefix_parts + choice.tail_parts)
     scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
-    _check(load_library("attention_shared").tb_attention_shared(
-        _ptr(q), _i64(q.stride(0)), _ptr(out), _i64(out.stride(0)), _ptr(cache), _ptr(positions), _ptr(block_table),
-        _i32(block_table.stride(0)), _i32(block_table.shape[1]), _ptr(shared.members), _ptr(shared.group_start),
-        _ptr(shared.leader), _ptr(shared.prefix), _ptr(shared.common), _i32(rows), _i32(shared.prefix.numel()), _i32(num_heads),
-        _i32(num_kv_heads), _i32(head_dim), _i32(page_size), _f32(scale), _i32(choice.tiles), _i32(choice.prefix_parts),
-        _i32(choice.prefix_run), _i32(choice.tail_parts), _i32(choice.tail_run), _ptr(scratch),
-        _pointer(scratch.data_ptr() + 4 * parts * head_dim), _i64(parts * head_dim), _i32(choice.warps), _i32(1 if choice.tensor else 0),
-        _i32(cache.shape[0]), _ptr(_error_word(q.device)), _i32(_code(q.dtype)), _stream()), "attention_shared")
+    at = scratch.data_ptr()
+    _check(_entry("attention_shared", "tb_attention_shared", _pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32,
+                  *[_pointer] * 5, *[_i32] * 6, _f32, *[_i32] * 5, _pointer, _pointer, _i64, _i32, _i32, _i32, _pointer, _i32,
+                  _pointer)(
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], *shared.addresses(), rows, shared.prefix.numel(), num_heads, num_kv_heads,
+        head_dim, page_size, scale, choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, at,
+        at + 4 * parts * head_dim, parts * head_dim, choice.warps, choice.tensor, cache.shape[0],
+        _error_word(q.device).data_ptr(), _code(dtype), _raw_stream()), "attention_shared")
     return out
 
 
@@ -409,17 +425,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int
     rows, vocab = logits.shape
     _need(tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows,
           "tokens must be contiguous int32 [S]")
-    _need(logits.device == tokens.device, "token_logprobs takes tensors of one device")
-    _need(0 <= alternatives <= min(MAX_ALTERNATIVES, vocab),
-          f"token_logprobs gives up to {MAX_ALTERNATIVES} alternatives, and no more than the vocabulary has tokens")
     device = logits.device
+    _need(device == tokens.device, "token_logprobs takes tensors of one device")
+    if not 0 <= alternatives <= min(MAX_ALTERNATIVES, vocab):
+        raise KernelError(f"token_logprobs gives up to {MAX_ALTERNATIVES} alternatives, and no more than the vocabulary has tokens")
     logprob = torch.empty(rows, dtype=torch.float32, device=device)
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
     values = torch.empty((rows, alternatives), dtype=torch.float32, device=device)
     ids = torch.empty((rows, alternatives), dtype=torch.int32, device=device)
-    _check(load_library("logprobs").tb_token_logprobs(_ptr(logits), _i64(logits.stride(0)), _ptr(tokens), _ptr(logprob),
-                                                      _ptr(entropy), _ptr(values), _ptr(ids), _i32(rows), _i32(vocab),
-                                                      _i32(alternatives), _stream()), "token_logprobs")
+    _check(_entry("logprobs", "tb_token_logprobs", _pointer, _i64, *[_pointer] * 5, _i32, _i32, _i32, _pointer)(
+        logits.data_ptr(), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), values.data_ptr(),
+        ids.data_ptr(), rows, vocab, alternatives, _raw_stream()), "token_logprobs")
     return logprob, entropy, values, ids
 
 

@@ -308,6 +308,10 @@ class SharedRows:
     room: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
 
+    def addresses(self) -> Tuple[int, ...]:
+        return (self.members.data_ptr(), self.group_start.data_ptr(), self.leader.data_ptr(), self.prefix.data_ptr(),
+                self.common.data_ptr())
+
     @classmethod
     def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":
         """``groups``: the rows of each group; ``prefixes``: their keys in common; ``positions``: the position of every row
