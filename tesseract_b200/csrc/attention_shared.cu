@@ -54,6 +54,7 @@ struct SharedParams {
     Paging paging;
     float scale_log2;
     int tensor;                               // the common parts are attend_tc's
+    int direct;                               // one run a row and nothing in common: the results go to `out` at once
     int* error;                               // set where a bounded wait ran out
 };
 
@@ -135,6 +136,8 @@ __device__ bool find_tail(const SharedParams& p, int64_t index, Work& w) {
     w.first_folded = rest % tiles * TILE;
     rest /= tiles;
     w.row = rest % p.rows;
+    w.member_rows = 0;
+    w.folded = p.fold;
     const int part = rest / p.rows;
     if (part >= p.tail_parts) return false;
     const int first = common_keys(p, p.common[w.row]);
@@ -145,8 +148,6 @@ __device__ bool find_tail(const SharedParams& p, int64_t index, Work& w) {
     w.begin = first + part * run * kBlock;
     w.end = min(last, w.begin + run * kBlock);
     if (w.begin >= w.end) return false;
-    w.member_rows = 0;
-    w.folded = p.fold;
     w.part = p.prefix_parts + part;
     return true;
 }
@@ -168,9 +169,14 @@ __device__ __forceinline__ int64_t slot_of(const SharedParams& p, int row, int h
     return ((int64_t)row * p.heads + head) * (p.prefix_parts + p.tail_parts) + part;
 }
 
+template <typename T>
+__device__ __forceinline__ void store_out(const SharedParams& p, int row, int head, int col, float v) {
+    Elem<T>::store((T*)p.out + (int64_t)row * p.out_stride + (int64_t)head * p.head_dim + col, v);
+}
+
 // The warps' results of a tile, (m, l) in `ml` [warps][TILE][2] and sums in `acc` [warps][TILE][PITCH], put together in the
 // order of the warps and left as the run's.  Every warp has written its own (a barrier in front).
-template <int TILE, int PITCH, int WARPS>
+template <typename T, int TILE, int PITCH, int WARPS>
 __device__ void leave_run(const SharedParams& p, const Work& w, const float* ml, const float* acc) {
     const int rows = min(TILE, w.folded - w.first_folded);
     for (int idx = threadIdx.x; idx < rows * p.head_dim; idx += WARPS * 32) {
@@ -187,9 +193,23 @@ __device__ void leave_run(const SharedParams& p, const Work& w, const float* ml,
         }
         int row, head;
         place_of(p, w, w.first_folded + r, row, head);
+        if (p.direct) {
+            store_out<T>(p, row, head, col, a / l);
+            continue;
+        }
         const int64_t slot = slot_of(p, row, head, w.part);
         p.part_a[slot * p.head_dim + col] = a;
         if (col == 0) p.part_ml[slot] = make_float2(big, l);
+    }
+}
+
+// The zeros of a row without keys, where nothing behind this kernel writes them.
+template <typename T, int TILE>
+__device__ void leave_nothing(const SharedParams& p, const Work& w) {
+    const int rows = min(TILE, w.folded - w.first_folded);
+    for (int idx = threadIdx.x; idx < rows * p.head_dim; idx += blockDim.x) {
+        const int r = idx / p.head_dim;
+        store_out<T>(p, w.row, w.kv_head * p.fold + w.first_folded + r, idx - r * p.head_dim, 0.0f);
     }
 }
 
@@ -411,7 +431,7 @@ __device__ void attend_mma(const SharedParams& p, const Work& w, unsigned char* 
                 make_float2(o[dt][2 * i], o[dt][2 * i + 1]);
     }
     __syncthreads();
-    leave_run<kRows, PITCH, WARPS>(p, w, ml, acc);
+    leave_run<__nv_bfloat16, kRows, PITCH, WARPS>(p, w, ml, acc);
 }
 
 template <int D, int WARPS, bool ONE>
@@ -422,6 +442,7 @@ __global__ void __launch_bounds__(WARPS * 32) shared_mma_kernel(const SharedPara
     Work w;
     // (tensor: the common parts are the next kernel's)
     if (p.tensor ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS, ONE>(p, w, smem);
+    else if (p.direct) leave_nothing<__nv_bfloat16, kRows>(p, w);
 }
 
 template <int D, int WARPS>
@@ -803,108 +824,150 @@ __global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------ 32-bit
 
 constexpr int kF32Rows = 8;                   // folded rows of a tile
-constexpr int kF32Warps = 8;
-constexpr int kF32Keys = 32;                  // keys of a warp's tile: a lane scores one
+constexpr int kF32Warps = 4;
+constexpr int kF32Keys = 32;                  // keys of a warp's tile
+constexpr int kF32Aside = 4;                  // keys whose scores are summed side by side: with eight rows one sum a lane
 
-// D: head size padded to 64, 128 or 256.
+// N neighbouring numbers (2, 4 or 8) from or to 8- or 16-byte boundaries.
+template <int N>
+__device__ __forceinline__ void load_n(const float* from, float (&v)[N]) {
+    if constexpr (N == 2) {
+        const float2 t = *reinterpret_cast<const float2*>(from);
+        v[0] = t.x;
+        v[1] = t.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(from + i);
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_n(float* to, const float (&v)[N]) {
+    if constexpr (N == 2) {
+        *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(v + i);
+    }
+}
+
+// D: head size padded to 64, 128 or 256.  A lane owns a few neighbouring columns of queries, keys and values, so keys and values
+// are read whole rows at a time.  Its products for four keys and eight rows are 32 partial sums, which the lanes exchange in five
+// rounds, half as many each, until every lane has one score: 31 exchanges for 32 scores.  (A lane a key instead, its row read 16
+// bytes at a time: 131 us for 16 rows at 4,096 keys of 32 heads of 128, bound by the cache lines that each load touches.)
 template <int D>
 __device__ void attend_f32(const SharedParams& p, const Work& w, float* smem) {
-    constexpr int COLS = D / 32;              // columns of the values that a lane owns: lane, lane + 32, ...
+    constexpr int COLS = D / 32;              // (the head size is a multiple of 16, so a lane's columns are all there or none)
+    constexpr int GROUPS = kF32Keys / kF32Aside;
+    static_assert(kF32Rows * kF32Aside == 32, "a score a lane");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = min(kF32Rows, w.folded - w.first_folded);
-    const int dim = p.head_dim;
-    float* queries = smem;                                               // [kF32Rows][D], zeros beyond the rows
-    float* weights = queries + kF32Rows * D + warp * (kF32Keys * kF32Rows);      // [key][row] of this warp
-    const float* q = (const float*)p.q;
-    for (int idx = threadIdx.x; idx < kF32Rows * D; idx += kF32Warps * 32) {
-        const int r = idx / D, col = idx % D;
-        float v = 0.0f;
-        if (r < rows && col < dim) {
+    const int dim = p.head_dim, col = lane * COLS;
+    const bool owns = col < dim;
+    float* weights = smem + warp * (kF32Keys * kF32Rows);                            // [key][row] of this warp
+    int64_t* places = reinterpret_cast<int64_t*>(smem + kF32Warps * kF32Keys * kF32Rows) + warp * kF32Keys;    // where its keys lie
+    float query[kF32Rows][COLS];
+#pragma unroll
+    for (int r = 0; r < kF32Rows; ++r) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) query[r][c] = 0.0f;
+        if (r < rows && owns) {
             int row, head;
             place_of(p, w, w.first_folded + r, row, head);
-            v = q[(int64_t)row * p.q_stride + (int64_t)head * dim + col];
+            load_n((const float*)p.q + (int64_t)row * p.q_stride + (int64_t)head * dim + col, query[r]);
         }
-        queries[idx] = v;
     }
-    __syncthreads();
     const int* table = p.table + (int64_t)w.row * p.table_stride;
     const int64_t head_block = (int64_t)p.paging.size * dim;
     const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
-    const float* base = (const float*)p.cache + (int64_t)w.kv_head * head_block;
-    float m[kF32Rows], l[kF32Rows], o[kF32Rows][COLS];
+    const float* keys = (const float*)p.cache + (int64_t)w.kv_head * head_block + (owns ? col : 0);
+    const float* values = keys + v_offset;
+    // of row lane % 8: the maximum, and the sum over the keys that this lane weighs
+    float m = kMasked, l = 0.0f, o[kF32Rows][COLS];
 #pragma unroll
-    for (int r = 0; r < kF32Rows; ++r) {
-        m[r] = kMasked;
-        l[r] = 0.0f;
+    for (int r = 0; r < kF32Rows; ++r)
 #pragma unroll
         for (int c = 0; c < COLS; ++c) o[r][c] = 0.0f;
-    }
     for (int key0 = w.begin + warp * kF32Keys; key0 < w.end; key0 += kF32Warps * kF32Keys) {
-        const int key = key0 + lane;
-        const bool there = key < w.end;
-        int64_t at = 0;                       // (a lane without a key reads page 0, which is always there)
-        if (there) at = (int64_t)table[p.paging.page_of(key)] * page_block + (int64_t)p.paging.within(key) * dim;
-        const float* k = base + at;
-        float s[kF32Rows];
+        const int key = min(key0 + lane, w.end - 1);              // (beyond the end: the last key once more, masked below)
+        places[lane] = (int64_t)table[p.paging.page_of(key)] * page_block + (int64_t)p.paging.within(key) * dim;
+        __syncwarp();
+        float score[GROUPS];
 #pragma unroll
-        for (int r = 0; r < kF32Rows; ++r) s[r] = 0.0f;
-#pragma unroll 4
-        for (int d = 0; d < dim; d += 4) {
-            const float4 kv = *reinterpret_cast<const float4*>(k + d);
+        for (int g = 0; g < GROUPS; ++g) {
+            float k[kF32Aside][COLS], part[32];
 #pragma unroll
-            for (int r = 0; r < kF32Rows; ++r) {
-                const float4 qv = *reinterpret_cast<const float4*>(queries + r * D + d);
-                s[r] = fmaf(qv.x, kv.x, s[r]);
-                s[r] = fmaf(qv.y, kv.y, s[r]);
-                s[r] = fmaf(qv.z, kv.z, s[r]);
-                s[r] = fmaf(qv.w, kv.w, s[r]);
+            for (int a = 0; a < kF32Aside; ++a) load_n(keys + places[g * kF32Aside + a], k[a]);
+#pragma unroll
+            for (int a = 0; a < kF32Aside; ++a)
+#pragma unroll
+                for (int r = 0; r < kF32Rows; ++r) {
+                    float sum = query[r][0] * k[a][0];
+#pragma unroll
+                    for (int c = 1; c < COLS; ++c) sum = fmaf(query[r][c], k[a][c], sum);
+                    part[a * kF32Rows + r] = sum;
+                }
+            // round o: a lane keeps the sums whose number has its bit o, and gives the others away
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const bool upper = lane & o;
+#pragma unroll
+                for (int i = 0; i < o; ++i) {
+                    const float mine = upper ? part[i + o] : part[i], other = upper ? part[i] : part[i + o];
+                    part[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+                }
             }
+            score[g] = part[0] * p.scale_log2;                    // of key g * 4 + lane / 8 and row lane % 8
+        }
+        float high = kMasked;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            if (key0 + g * kF32Aside + lane / kF32Rows >= w.end) score[g] = -INFINITY;        // 2^(that - m) is 0
+            high = fmaxf(high, score[g]);
+        }
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+        const float m_new = fmaxf(m, high), correction = exp2f(m - m_new);
+        m = m_new;
+        l *= correction;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const float weight = exp2f(score[g] - m_new);
+            l += weight;
+            weights[g * 32 + lane] = weight;
         }
 #pragma unroll
         for (int r = 0; r < kF32Rows; ++r) {
-            const float score = there ? s[r] * p.scale_log2 : kMasked;
-            const float m_new = fmaxf(m[r], warp_max(score));
-            const float correction = exp2f(m[r] - m_new);
-            m[r] = m_new;
-            const float weight = there ? exp2f(score - m_new) : 0.0f;
-            l[r] = l[r] * correction + weight;             // (this lane's keys; the lanes meet at the end)
+            const float c_r = __shfl_sync(0xffffffffu, correction, r);
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) o[r][c] *= correction;
-            weights[lane * kF32Rows + r] = weight;
+            for (int c = 0; c < COLS; ++c) o[r][c] *= c_r;
         }
         __syncwarp();
         const int count = min(kF32Keys, w.end - key0);
-#pragma unroll 4
+#pragma unroll(COLS <= 2 ? 8 : 4)
         for (int j = 0; j < count; ++j) {
-            const float* v = base + v_offset + __shfl_sync(0xffffffffu, at, j);
-            float weight[kF32Rows];
+            float weight[kF32Rows], value[COLS];
+            load_n(values + places[j], value);
+            load_n(weights + j * kF32Rows, weight);
 #pragma unroll
-            for (int r = 0; r < kF32Rows; r += 4)
-                *reinterpret_cast<float4*>(weight + r) = *reinterpret_cast<const float4*>(weights + j * kF32Rows + r);
+            for (int c = 0; c < COLS; ++c)
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                const float value = c * 32 + lane < dim ? v[c * 32 + lane] : 0.0f;
-#pragma unroll
-                for (int r = 0; r < kF32Rows; ++r) o[r][c] = fmaf(weight[r], value, o[r][c]);
-            }
+                for (int r = 0; r < kF32Rows; ++r) o[r][c] = fmaf(weight[r], value[c], o[r][c]);
         }
         __syncwarp();
     }
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
     __syncthreads();
     float* ml = smem;
     float* acc = ml + kF32Warps * kF32Rows * 2;
-#pragma unroll
-    for (int r = 0; r < kF32Rows; ++r) {
-        const float sum = warp_sum(l[r]);
-        if (lane == 0) {
-            ml[(warp * kF32Rows + r) * 2] = m[r];
-            ml[(warp * kF32Rows + r) * 2 + 1] = sum;
-        }
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[(warp * kF32Rows + r) * D + c * 32 + lane] = o[r][c];
+    if (lane < kF32Rows) {
+        ml[(warp * kF32Rows + lane) * 2] = m;
+        ml[(warp * kF32Rows + lane) * 2 + 1] = l;
     }
+#pragma unroll
+    for (int r = 0; r < kF32Rows; ++r) store_n(acc + (warp * kF32Rows + r) * D + col, o[r]);
     __syncthreads();
-    leave_run<kF32Rows, D, kF32Warps>(p, w, ml, acc);
+    leave_run<float, kF32Rows, D, kF32Warps>(p, w, ml, acc);
 }
 
 template <int D>
@@ -914,11 +977,12 @@ __global__ void __launch_bounds__(kF32Warps * 32) shared_f32_kernel(const Shared
     pdl_trigger();
     Work w;
     if (find_work<kF32Rows>(p, blockIdx.x, w)) attend_f32<D>(p, w, f32_smem);
+    else if (p.direct) leave_nothing<float, kF32Rows>(p, w);
 }
 
 template <int D>
 constexpr size_t f32_bytes() {
-    constexpr size_t tiles = (size_t)kF32Rows * D + (size_t)kF32Warps * kF32Keys * kF32Rows;
+    constexpr size_t tiles = (size_t)kF32Warps * kF32Keys * (kF32Rows + 2);      // weights, and where the keys lie
     constexpr size_t meet = (size_t)kF32Warps * kF32Rows * (2 + D);
     return (tiles > meet ? tiles : meet) * sizeof(float);
 }
@@ -1086,7 +1150,8 @@ TB_EXPORT int tb_attention_shared_tensor(int dtype, int head_dim, int page_size)
 // rows of q and out: [rows, heads * head_dim] with a stride; positions[b]: the last key of row b (-1: none); table: [rows, columns]
 // pages; members, group_start, leader, prefix, common: the groups (SharedParams); tiles: the tiles of all groups with keys in common,
 // ceil(rows of the group * heads / kv_heads / tile) each, no fewer.  prefix[g] is at most positions[b] + 1 for the rows of the group.
-// part_a, part_ml: rows * heads * (prefix_parts + tail_parts) * (head_dim and 2) floats.
+// part_a, part_ml: rows * heads * (prefix_parts + tail_parts) * (head_dim and 2) floats; none where nothing is in common and every
+// row is one run.
 TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* cache,
                                   const int* positions, const int* table, int table_stride, int table_columns, const int* members,
                                   const int* group_start, const int* leader, const int* prefix, const int* common, int rows, int groups, int heads,
@@ -1101,8 +1166,8 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     const int element = dtype == TB_F32 ? 4 : 2;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)part_a) % 16 != 0) return TB_ERR_BAD_ALIGN;
     if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
-    const int64_t parts = (int64_t)rows * heads * (prefix_parts + tail_parts);
-    if (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim) return -5;
+    const int64_t parts = prefix_parts == 0 && tail_parts == 1 ? 0 : (int64_t)rows * heads * (prefix_parts + tail_parts);
+    if (parts > 0 && (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim)) return -5;
     if (tensor && (!tb_attention_shared_tensor(dtype, head_dim, page_size) || error == nullptr)) return TB_ERR_BAD_SIZE;
     SharedParams p;
     p.q = q;
@@ -1136,6 +1201,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.paging = tb_paging(page_size);
     p.scale_log2 = scale * kLog2e;
     p.tensor = tensor;
+    p.direct = prefix_parts == 0 && tail_parts == 1;
     p.error = error;
     const int tile = dtype == TB_F32 ? kF32Rows : kRows;                 // of the parts behind
     const int64_t of_common = (int64_t)tiles * kv_heads * prefix_parts;
@@ -1156,7 +1222,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
             status = head_dim == 64 ? launch_tc<64>(map, of_common, p, stream) : launch_tc<128>(map, of_common, p, stream);
         }
     }
-    if (status != 0) return status;
+    if (status != 0 || p.direct) return status;
     const int64_t joins = ((int64_t)rows * heads + 3) / 4;
     if (dtype == TB_F32)
         return launch(head_dim <= 32 ? shared_join_kernel<float, 8> : head_dim <= 64 ? shared_join_kernel<float, 16>

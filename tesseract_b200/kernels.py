@@ -342,9 +342,10 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     _need(cache.is_contiguous() and cache.shape[1:] == (2, num_kv_heads, page_size, head_dim), "cache layout")
     _need(shared.members.numel() == rows == shared.common.numel(), "shared: a place for every row")
     _need(scale > 0.0, "the scale of the scores must be positive")
-    parts = rows * num_heads * (choice.prefix_parts + choice.tail_parts)
-    scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
-    at = scratch.data_ptr()
+    parts, at = rows * num_heads * (choice.prefix_parts + choice.tail_parts), 0
+    if choice.prefix_parts or choice.tail_parts > 1:
+        scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
+        at = scratch.data_ptr()
     _check(_entry("attention_shared", "tb_attention_shared", _pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32,
                   *[_pointer] * 5, *[_i32] * 6, _f32, *[_i32] * 5, _pointer, _pointer, _i64, _i32, _i32, _i32, _pointer, _i32,
                   _pointer)(

@@ -303,7 +303,8 @@ class SharedRows:
     common: torch.Tensor         # int32 [rows]: those of the row's group
     sizes: Tuple[int, ...]       # host copies for decisions: rows of each group,
     blocks: Tuple[int, ...]      # blocks of keys in common,
-    tails: Tuple[int, ...]       # and blocks (begun ones too) that each row reads behind them
+    tails: Tuple[int, ...]       # blocks (begun ones too) that each row reads behind them,
+    row_blocks: Tuple[int, ...]  # and blocks that it has in common with its group
     # rows and groups that the tensors have room for, where a captured step refills them (None: they hold just these)
     room: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
@@ -316,9 +317,9 @@ class SharedRows:
     def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":
         """``groups``: the rows of each group; ``prefixes``: their keys in common; ``positions``: the position of every row
         (-1 for a row without keys)."""
-        arrays, sizes, blocks, tails = shared_arrays(groups, prefixes, positions)
+        arrays, *host = shared_arrays(groups, prefixes, positions)
         packed = torch.from_numpy(np.concatenate(arrays)).to(device)
-        return cls(*packed.split([a.size for a in arrays]), sizes, blocks, tails)
+        return cls(*packed.split([a.size for a in arrays]), *host)
 
 
 def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int]):
@@ -341,7 +342,7 @@ def shared_arrays(groups: Sequence[Sequence[int]], prefixes: Sequence[int], posi
     arrays = [np.asarray(a, dtype=np.int32) for a in (members, start, [group[0] for group in groups],
                                                       [b * SHARED_BLOCK for b in blocks], common)]
     tails = tuple(-(-(last + 1 - keys) // SHARED_BLOCK) for last, keys in zip(positions, common))
-    return arrays, tuple(len(g) for g in groups), tuple(blocks), tails
+    return arrays, tuple(len(g) for g in groups), tuple(blocks), tails, tuple(keys // SHARED_BLOCK for keys in common)
 
 
 @dataclass

@@ -289,11 +289,18 @@ class SharedAttentionPlan:
     warps: int = 0           # of a block: 2, or (0) as many as let two blocks share a multiprocessor
 
 
-SHARED_MIN_RUN = 4          # blocks of 64 keys: a tile of 16 keys for each of eight warps, twice
+# Blocks of 64 keys in a run: a tile of 16 keys for each of eight warps, twice; in 32 bits one of 32 for each of four.
+SHARED_MIN_RUN = {torch.bfloat16: 4, torch.float32: 2}
 SHARED_MAX_PARTS = 64
 
 
-SHARED_MIN_SAVED = 64       # blocks of 64 keys
+# Blocks of 64 keys that rows need not read themselves from where on common parts are taken by themselves: below, one launch over
+# every row's own keys is faster (4 rows of 32 heads of 64 at 200 keys: 4.5 us on the device, 7.0 with a launch to put parts together).
+SHARED_MIN_SAVED = 64
+# Tiles of 16 folded rows times blocks of common keys from where on the tensor cores' form is faster, whose launch takes 10 us (32
+# heads on 8, device time with and without: 64 rows at 2,048 keys of 64 11.1 and 11.6 us, at 8,192 15.9 and 18.9, 128 rows at
+# 16,384 24.4 and 44.2; of 128, 32 rows at 1,024 11.6 and 11.3, 64 at 2,048 13.1 and 19.0, 128 at 16,384 34.8 and 91.8).
+SHARED_TENSOR_MIN = {64: 128, 128: 48}
 
 
 def sharing_pays(sizes: Sequence[int], blocks: Sequence[int]) -> bool:
@@ -315,11 +322,11 @@ def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, h
     return choice
 
 
-def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int) -> int:
-    """The shortest runs (in blocks, ``SHARED_MIN_RUN`` at least) with which all tiles' runs are at most ``target``: one more, and the
+def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int, shortest: int) -> int:
+    """The shortest runs (in blocks, ``shortest`` at least) with which all tiles' runs are at most ``target``: one more, and the
     chip goes round a second time for it."""
     longest = int(blocks.max())
-    run = max(SHARED_MIN_RUN, -(-int((tiles * blocks).sum()) // target))
+    run = max(shortest, -(-int((tiles * blocks).sum()) // target))
     while run < longest and int((tiles * -(-blocks // run)).sum()) > target:
         run += 1 + run // 16
     return run
@@ -327,22 +334,28 @@ def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int) -> int:
 
 def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sms) -> SharedAttentionPlan:
     sizes, blocks = np.asarray(shared.sizes), np.asarray(shared.blocks)
+    tails = np.asarray(shared.tails)
+    if not sharing_pays(shared.sizes, shared.blocks):           # every row reads its own
+        tails = tails + np.asarray(shared.row_blocks)
+        blocks = np.zeros_like(blocks)
     rows = np.where(blocks > 0, sizes * fold, 0)
-    tensor = int(rows.max()) > 16 and kernels.attention_shared_tensor(dtype, head_dim, page_size)
+    work = int((-(-rows // 16) * blocks).sum())
+    tensor = work > SHARED_TENSOR_MIN.get(head_dim, 0) and kernels.attention_shared_tensor(dtype, head_dim, page_size)
     tile = kernels.attention_shared_tile(dtype, tensor)
     tiles = -(-rows // tile)
-    target = max(1, 2 * sms // num_kv_heads)                    # large blocks of threads that are resident at once, a kv head
+    # large blocks of threads that are resident at once, a kv head (those of the 32-bit form are half as large)
+    target = max(1, (4 if dtype == torch.float32 and head_dim <= 128 else 2) * sms // num_kv_heads)
     prefix_parts, prefix_run = 0, 1
     if tiles.any():
-        prefix_run = _shared_runs(tiles, blocks, target)
+        prefix_run = _shared_runs(tiles, blocks, target, SHARED_MIN_RUN[dtype])
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
     # are many
-    tails = np.maximum(np.asarray(shared.tails), 1)
+    tails = np.maximum(tails, 1)
     tail_tiles = np.full(tails.shape, -(-fold // kernels.attention_shared_tile(dtype)))
     warps = 2 if dtype != torch.float32 and int(tail_tiles.sum()) > target else 0
     small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
-    tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target)
+    tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
     # (tensors that are refilled: no grouping of so many rows has more tiles)
     count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + shared.room // 2

@@ -186,6 +186,18 @@ def test_both_forms_in_bfloat16(rows, dim):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_share_nothing_in_one_launch(dtype):
+    """No common part and one run a row: the results are written at once, the zeros of rows without keys too."""
+    for dim in (48, 64, 128):
+        case = Case([(0, [0]), (128, [200, 140]), (0, [1]), (0, [0, 70, 0])], 8, 2, dim, dtype=dtype, seed=4)
+        before = kernels.launch_count
+        got = case.check(plan.SharedAttentionPlan(0, 0, 1, 1, 1))
+        assert kernels.launch_count == before + 1
+        rows = case.shared.members.tolist()
+        assert not bool(got[[rows[0], rows[4], rows[6]]].any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_the_same_bits_every_time(dtype):
     case = Case([(900, [901 + 5 * i for i in range(40)])], 32, 8, 128, dtype=dtype, seed=9)
     first = case.run().clone()
