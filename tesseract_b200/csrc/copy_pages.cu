@@ -93,33 +93,45 @@ int piece_bytes(int64_t total) { return total >= (int64_t)(32 << 20) ? 16384 : 4
 
 constexpr int kErrBadPage = -6, kErrClash = -7, kErrMemory = -8;
 
-// packed: for every store its address, entries, pages, bytes of a page, moves, and the addresses of its sources and its targets
-// (int32).
-TB_EXPORT int tb_copy_pages(int num_stores, const int64_t* packed, int* launches, cudaStream_t stream) {
-    auto base = [&](int s) { return (char*)packed[s * 7]; };
-    auto entries = [&](int s) { return packed[s * 7 + 1]; };
-    auto pages = [&](int s) { return packed[s * 7 + 2]; };
-    auto size = [&](int s) { return packed[s * 7 + 3]; };
-    auto counts = [&](int s) { return (int)packed[s * 7 + 4]; };
-    auto sources = [&](int s) { return (const int*)packed[s * 7 + 5]; };
-    auto targets = [&](int s) { return (const int*)packed[s * 7 + 6]; };
-    *launches = 0;
+// packed: for every store its address, entries, pages, bytes of a page and moves; then, as 32-bit numbers, every store's sources and
+// targets.  Returns (launches << 16) + status.
+TB_EXPORT int tb_copy_pages(int num_stores, const int64_t* packed, cudaStream_t stream) {
+    auto base = [&](int s) { return (char*)packed[s * 5]; };
+    auto entries = [&](int s) { return packed[s * 5 + 1]; };
+    auto pages = [&](int s) { return packed[s * 5 + 2]; };
+    auto size = [&](int s) { return packed[s * 5 + 3]; };
+    auto counts = [&](int s) { return (int)packed[s * 5 + 4]; };
+    int at_store = 0;
+    const int* indices = (const int*)(packed + 5 * (int64_t)num_stores);
+    // (asked in the order of the stores, twice)
+    auto sources = [&](int s) {
+        if (s < at_store) {
+            at_store = 0;
+            indices = (const int*)(packed + 5 * (int64_t)num_stores);
+        }
+        for (; at_store < s; ++at_store) indices += 2 * (int64_t)counts(at_store);
+        return indices;
+    };
+    auto targets = [&](int s) { return sources(s) + counts(s); };
+    int launches = 0;
     std::vector<uint8_t> seen;
     int64_t total_bytes = 0;
     for (int s = 0; s < num_stores; ++s) {
-        if (entries(s) < 0 || pages(s) < 0 || pages(s) > 0x7fffffff || size(s) < 0 || packed[s * 7 + 4] < 0 || packed[s * 7 + 4] > 0x7fffffff)
+        if (entries(s) < 0 || pages(s) < 0 || pages(s) > 0x7fffffff || size(s) < 0 || packed[s * 5 + 4] < 0 || packed[s * 5 + 4] > 0x3fffffff)
             return TB_ERR_BAD_SIZE;
+        const int n = counts(s);
+        const int *source = sources(s), *target = targets(s);
         try {
             seen.assign((size_t)pages(s), 0);
         } catch (const std::bad_alloc&) {
             return kErrMemory;
         }
-        for (int i = 0; i < counts(s); ++i) {
-            if (sources(s)[i] < 0 || sources(s)[i] >= pages(s) || targets(s)[i] < 0 || targets(s)[i] >= pages(s)) return kErrBadPage;
-            seen[(size_t)sources(s)[i]] = 1;
+        for (int i = 0; i < n; ++i) {
+            if (source[i] < 0 || source[i] >= pages(s) || target[i] < 0 || target[i] >= pages(s)) return kErrBadPage;
+            seen[(size_t)source[i]] = 1;
         }
-        for (int i = 0; i < counts(s); ++i) {
-            uint8_t& mark = seen[(size_t)targets(s)[i]];
+        for (int i = 0; i < n; ++i) {
+            uint8_t& mark = seen[(size_t)target[i]];
             if (mark) return kErrClash;
             mark = 2;
         }
@@ -154,7 +166,8 @@ TB_EXPORT int tb_copy_pages(int num_stores, const int64_t* packed, int* launches
                 store.pieces = (int)((size(s) + piece - 1) / piece);
                 store.first_piece = pieces;
                 pieces += (int64_t)store.pieces * n * entries(s);
-                for (int i = 0; i < n; ++i) moves[taken + i] = make_int2(sources(s)[done + i], targets(s)[done + i]);
+                const int *source = sources(s) + done, *target = targets(s) + done;
+                for (int i = 0; i < n; ++i) moves[taken + i] = make_int2(source[i], target[i]);
                 taken += n;
             }
             done += n;
@@ -167,8 +180,8 @@ TB_EXPORT int tb_copy_pages(int num_stores, const int64_t* packed, int* launches
         (small ? few.count : many.count) = used;
         (small ? few.piece : many.piece) = piece;
         const int status = small ? launch(few, pieces, stream) : launch(many, pieces, stream);
-        if (status != 0) return status;
-        ++*launches;
+        if (status != 0) return (launches << 16) + status;
+        ++launches;
     }
-    return 0;
+    return launches << 16;
 }

@@ -10,7 +10,8 @@
 // Bound by HBM: 4 V bytes a row, read once.  A row is shared by a thread-block cluster of 1 to 8 blocks (a contiguous
 // part each); a block takes its part in chunks of sixteen logits a thread, in registers, the next chunk's loads under way
 // meanwhile.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
-// others' loads; few rows: blocks of 1,024, one chunk each at a vocabulary of 128,256.  Of a chunk
+// others' loads (1,536 rows of 128,256 logits, one alternative: 143 us, 85 % of the measured copy rate; without alternatives 119);
+// few rows: blocks of 1,024, one chunk each at that vocabulary.  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
 //     they meet once, at the end, in a fixed order, so a row's numbers do not depend on the timing;
 //   * every eight threads leave the largest of their 128 logits.  No block waits for anything inside the loop.
@@ -42,7 +43,8 @@ struct Shared {
     uint32_t group[kMaxGroups];                    // the groups' largest logits, as `ordered` has them
     int16_t reaching[kMaxGroups];                  // the groups that reach the bound
     float warp_stat[32][3];
-    int warp_count[64];
+    int warp_count[32];
+    uint32_t bound;
     float stat[3];                                 // this block's m, S, T
     int count, groups;                             // entries of the list, of `reaching`
 };
@@ -61,27 +63,21 @@ __device__ __forceinline__ float exp2_of(float x) {       // 2^x, relative error
     return y;
 }
 
-// (m, S, T) of two disjoint sets of numbers
-__device__ __forceinline__ void join(float& m, float& s, float& t, float m2, float s2, float t2) {
-    const float top = fmaxf(m, m2);
-    if (!(top > -INFINITY)) {                      // nothing in either (a NaN in s or t stays)
-        s += s2;
-        t += t2;
-        return;
+// (m, S, T) of a warp's lanes together, in every lane; a lane with nothing brings (-inf, 0, 0).  Every lane is brought to the common
+// maximum once and then S and T are summed.
+__device__ __forceinline__ void meet(float& m, float& s, float& t) {
+    const float top = from_ordered(__reduce_max_sync(0xffffffffu, ordered(m)));
+    if (top > -INFINITY) {                         // (nothing anywhere: S and T are 0, or NaN, as they are)
+        // (where e^(m - top) is 0, the distance must not make an infinity of what it is multiplied by; an infinite top gives NaN)
+        const float d = m - top, a = exp2_of(d * kLog2e);
+        t = (t + s * fmaxf(d, kFar)) * a;
+        s *= a;
     }
-    // (where e^(m - top) is 0, the distance must not make an infinity of what it is multiplied by; an infinite top gives NaN)
-    const float a = exp2_of((m - top) * kLog2e), b = exp2_of((m2 - top) * kLog2e);
-    const float da = fmaxf(m - top, kFar), db = fmaxf(m2 - top, kFar);
-    t = (t + s * da) * a + (t2 + s2 * db) * b;
-    s = s * a + s2 * b;
     m = top;
-}
-// The same over the first `count` (a power of two) lanes of a warp; every lane gets the result.
-__device__ __forceinline__ void join_lanes(float& m, float& s, float& t, int count) {
-    for (int o = 1; o < count; o <<= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
-        join(m, s, t, m2, s2, t2);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
     }
 }
 
@@ -97,17 +93,20 @@ __device__ __forceinline__ uint32_t peer_u32(const void* local, uint32_t rank) {
 }
 
 // The k best of the list's n entries, in order, into best_value / best_id: the rank of an entry is the number of entries in front of
-// it.  `share` threads count for one entry.  Every thread calls this; the list is whole (a barrier in front).
+// it.  Every thread calls this; the list is whole (a barrier in front).
+// (Not inlined: the second call finds its instructions there.)
 template <int THREADS>
-__device__ __forceinline__ void cut(Shared& sh, int n, int k) {
-    int share = 1;
-    while (share < 32 && n * share * 2 <= THREADS) share *= 2;
+__device__ __noinline__ void cut(Shared& sh, int n, int k) {
+    int shift = 3;                                 // 2^shift threads count for one entry
+    while (shift > 0 && (n << shift) > THREADS) --shift;
+    const int share = 1 << shift;
     if ((int)threadIdx.x >= n && (int)threadIdx.x < k) {
         sh.best_value[threadIdx.x] = -INFINITY;
         sh.best_id[threadIdx.x] = kNobody;
     }
-    for (int base = 0; base < n; base += THREADS / share) {
-        const int e = base + (int)threadIdx.x / share, part = (int)threadIdx.x % share;
+    const int warp_first = threadIdx.x & ~31;      // (a warp without an entry has nothing to do)
+    for (int base = 0; base + (warp_first >> shift) < n; base += THREADS >> shift) {
+        const int e = base + ((int)threadIdx.x >> shift), part = (int)threadIdx.x & (share - 1);
         const bool mine = e < n;
         const float v = mine ? sh.value[e] : 0.0f;
         const int id = mine ? sh.id[e] : 0;
@@ -126,16 +125,6 @@ __device__ __forceinline__ void cut(Shared& sh, int n, int k) {
         }
     }
     __syncthreads();
-}
-
-// The sum over the block's threads with one barrier; two such sums that follow each other use places of their own (turn 0, 1).
-template <int THREADS>
-__device__ __forceinline__ int sum_of(Shared& sh, int mine, int turn) {
-    const int lane = threadIdx.x & 31;
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sh.warp_count[turn * 32 + (threadIdx.x >> 5)] = mine;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? sh.warp_count[turn * 32 + lane] : 0);
 }
 
 template <int THREADS>
@@ -167,21 +156,36 @@ __device__ int find_best(Shared& sh, const float* base, int ahead, int end, int 
     const int groups = (chunks + span - 1) / span * kGroups;
     // low: what at least k logits reach, or all above -inf; high: what fewer than k groups (later: logits) reach
     const uint32_t nothing = ordered(-INFINITY) + 1;
-    uint32_t low = nothing, high = sh.stat[0] > -INFINITY ? ordered(sh.stat[0] + 0.0f) + 1 : nothing;
-    int turn = 0;
-    while (high > low + 1) {
-        const uint32_t middle = low + (high - low) / 2;
-        int mine = 0;
-        for (int g = threadIdx.x; g < groups; g += THREADS) mine += sh.group[g] >= middle ? 1 : 0;
-        const int reach = sum_of<THREADS>(sh, mine, turn);
-        turn ^= 1;
-        if (reach < k) {
-            high = middle;
-        } else {
-            low = middle;
-            if (reach <= k + k / 4) break;
+    if (threadIdx.x < 32) {
+        // one warp looks for the bound (a barrier a round cost the block four times as much): it begins at the smallest of its lanes'
+        // largest, or for k above 32 second largest, groups, which 32, or 64, groups reach
+        const int lane = threadIdx.x;
+        uint32_t one = 0, two = 0;
+#pragma unroll 4
+        for (int g = lane; g < groups; g += 32) {
+            const uint32_t v = sh.group[g];
+            two = max(two, min(one, v));
+            one = max(one, v);
         }
+        uint32_t low = max(nothing, __reduce_min_sync(0xffffffffu, k <= 32 ? one : two));
+        uint32_t high = __reduce_max_sync(0xffffffffu, one) + 1;
+        while (high > low + 1) {
+            const uint32_t middle = low + (high - low) / 2;
+            int reach = 0;
+#pragma unroll 8
+            for (int g = lane; g < groups; g += 32) reach += sh.group[g] >= middle ? 1 : 0;
+            reach = __reduce_add_sync(0xffffffffu, reach);
+            if (reach < k) {
+                high = middle;
+            } else {
+                low = middle;
+                if (reach <= k + k / 4) break;
+            }
+        }
+        if (lane == 0) sh.bound = low;
     }
+    __syncthreads();
+    uint32_t low = sh.bound, high;
     for (int g = threadIdx.x; g < groups; g += THREADS)
         if (sh.group[g] >= low) sh.reaching[atomicAdd(&sh.groups, 1)] = (int16_t)g;
     __syncthreads();
@@ -298,12 +302,6 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const int end = last - first + ahead;          // logits are base[ahead .. end)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();                                    // the logits come from the kernel in front
-    float given = NAN;
-    if (block == 0 && threadIdx.x == 0) {
-        const int token = tokens[r];
-        if (token >= 0 && token < vocab) given = row[token];
-    }
-
     auto fetch = [&](float4 (&held)[kPackets], int chunk) {
 #pragma unroll
         for (int u = 0; u < kPackets; ++u) {
@@ -325,7 +323,9 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const int group = threadIdx.x / kGroup;
     float largest = -INFINITY;
     float4 next[kPackets];
+    const int token = block == 0 && threadIdx.x == 0 ? tokens[r] : -1;
     fetch(next, 0);
+    const float given = token >= 0 && token < vocab ? row[token] : NAN;
     for (int c = 0; c < chunks; ++c) {
         float x[kEach];
 #pragma unroll
@@ -365,8 +365,8 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         }
     }
 
-    // the block's sums, in the order of lanes and warps
-    join_lanes(m, s, t, 32);
+    // the block's sums, in an order of lanes and warps that is always the same
+    meet(m, s, t);
     if (lane == 0) {
         sh.warp_stat[warp][0] = m;
         sh.warp_stat[warp][1] = s;
@@ -377,7 +377,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         m = lane < WARPS ? sh.warp_stat[lane][0] : -INFINITY;
         s = lane < WARPS ? sh.warp_stat[lane][1] : 0.0f;
         t = lane < WARPS ? sh.warp_stat[lane][2] : 0.0f;
-        join_lanes(m, s, t, WARPS);
+        meet(m, s, t);
         if (lane == 0) {
             sh.stat[0] = m;
             sh.stat[1] = s;
@@ -394,15 +394,17 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
         cluster_sync();
         if (block == 0) {
             // the blocks' best together (k each, what is none of a block's behind all others: blocks * k <= 512), then the row's
-            for (int i = threadIdx.x; i < blocks * k; i += THREADS) {
-                sh.value[i] = __uint_as_float(peer_u32(&sh.best_value[i % k], i / k));
-                sh.id[i] = (int)peer_u32(&sh.best_id[i % k], i / k);
+            for (int i = threadIdx.x; i < blocks * kMaxTop; i += THREADS) {
+                const int c = i / kMaxTop, j = i % kMaxTop;
+                if (j >= k) continue;
+                sh.value[c * k + j] = __uint_as_float(peer_u32(&sh.best_value[j], c));
+                sh.id[c * k + j] = (int)peer_u32(&sh.best_id[j], c);
             }
             if (warp == 0) {
                 m = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[0], lane)) : -INFINITY;
                 s = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[1], lane)) : 0.0f;
                 t = lane < blocks ? __uint_as_float(peer_u32(&sh.stat[2], lane)) : 0.0f;
-                join_lanes(m, s, t, kMaxBlocks);
+                meet(m, s, t);
             }
             __syncthreads();
             if ((int)threadIdx.x < k) {            // (what is no entry has no rank of its own)
@@ -493,11 +495,16 @@ TB_EXPORT int tb_token_logprobs(const float* logits, int64_t stride, const int* 
                                 float* top_value, int* top_id, int rows, int vocab, int top, cudaStream_t stream) {
     if (rows == 0) return 0;
     if (rows < 0 || vocab <= 0 || vocab > (1 << 30) || top < 0 || top > kMaxTop || top > vocab) return TB_ERR_BAD_SIZE;
-    // few rows: large blocks, as many a row as keep one a multiprocessor; many: small ones, four a multiprocessor
+    // Few rows: blocks of 1,024, as many a row as leave each a multiprocessor of its own; up to two rows a multiprocessor one of 512
+    // each, beyond one of 256.  (128,256 logits, twenty alternatives, device time of blocks of 256 / 512 / 1,024 at their best split:
+    // 64 rows 20.1 / 15.0 / 14.7 us, 256 rows 31.3 / 28.6 / 34.6, 1,536 rows 145 / 153 / 183.)
     const int64_t sms = sm_count();
-    if (rows * kMaxBlocks <= sms)
-        return launch_rows<1024>(rows, vocab, kMaxBlocks, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
-    int blocks = kMaxBlocks;
-    while (blocks > 1 && (int64_t)rows * blocks > 4 * sms) blocks >>= 1;
-    return launch_rows<256>(rows, vocab, blocks, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
+    if (rows <= sms) {
+        int blocks = kMaxBlocks;
+        while (rows * blocks > sms) blocks >>= 1;
+        return launch_rows<1024>(rows, vocab, blocks, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
+    }
+    if (rows <= 2 * sms)
+        return launch_rows<512>(rows, vocab, 1, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
+    return launch_rows<256>(rows, vocab, 1, stream, logits, stride, tokens, logprob, entropy, top_value, top_id, top);
 }

@@ -9,7 +9,7 @@ loaded, or a kernel refuses a size, the call raises.
 from __future__ import annotations
 
 import ctypes
-from functools import lru_cache
+import struct
 from typing import Optional
 
 import numpy as np
@@ -95,12 +95,17 @@ def _cuda(*tensors: torch.Tensor) -> None:
             raise KernelError("kernel arguments must live on a CUDA device")
 
 
-@lru_cache(maxsize=None)
-def _entry(library: str, name: str, *types):
+_entries = {}
+
+
+def _entry(library: str, name: str, types):
     """The C entry ``name`` with its argument types declared: a call of thirty arguments then takes plain integers, which costs the
     host a third less than a ctypes object for each."""
-    entry = getattr(load_library(library), name)
-    entry.argtypes = types
+    entry = _entries.get(name)
+    if entry is None:
+        entry = getattr(load_library(library), name)
+        entry.argtypes = types
+        _entries[name] = entry
     return entry
 
 
@@ -176,36 +181,36 @@ def copy_pages(moves) -> None:
     call that breaks this, or names a page outside a store, raises :class:`KernelError` and copies nothing.  The indices
     travel in the launch: nothing has to outlive the call."""
     global launch_count
-    count = len(moves)
-    packed = []                                          # five numbers and two addresses a store
-    kept = []                                            # the index arrays live until the call returns
-    device = None
+    header, indices, device = [], [], -1
     for store, source, target in moves:
         if not (store.is_cuda and store.dim() >= 2 and store.is_contiguous()):
             raise KernelError("copy_pages takes contiguous stores [entries, pages, ...] on a CUDA device")
-        if device is None:
+        if device != store.get_device():
+            _need(device < 0, "copy_pages takes stores of one device")
             device = store.get_device()
             _need(device == torch.cuda.current_device(), "copy_pages runs on the current device")
-        elif store.get_device() != device:
-            raise KernelError("copy_pages takes stores of one device")
         source, target = _host_indices(source), _host_indices(target)
         if source.size != target.size:
             raise KernelError("copy_pages takes as many targets as sources")
-        kept.append((source, target))
-        entries, pages = store.shape[0], store.shape[1]
+        entries, pages = store.shape[:2]
         # (from the sizes: a tensor without numbers, or an extent of one, may have any stride)
         numbers = store.numel()
-        packed += (store.data_ptr(), entries, pages, numbers // (entries * pages) * store.element_size() if numbers else 0,
-                   source.size, source.ctypes.data, target.ctypes.data)
-    if count > 1 and len(set(packed[::7])) < sum(1 for p in packed[::7] if p) + any(p == 0 for p in packed[::7]):
-        raise KernelError("copy_pages takes a store once a call")
-    launches = _i32(0)
-    status = _entry("copy_pages", "tb_copy_pages", _i32, _pointer, _pointer, _pointer)(
-        count, (_i64 * len(packed))(*packed), ctypes.addressof(launches),
-        torch._C._cuda_getCurrentRawStream(device) if device is not None else 0)
+        header += (store.data_ptr(), entries, pages, numbers // (entries * pages) * store.element_size() if numbers else 0, source.size)
+        indices += (source.tobytes(), target.tobytes())
+    if len(moves) > 1:
+        addresses = [a for a in header[::5] if a]
+        _need(len(set(addresses)) == len(addresses), "copy_pages takes a store once a call")
+    if not header:
+        return
+    done = _entry("copy_pages", "tb_copy_pages", _COPY_PAGES)(
+        len(moves), b"".join([struct.pack(f"{len(header)}q", *header), *indices]), torch._C._cuda_getCurrentRawStream(device))
     launch_count -= 1                                    # (_check counts one; a call may launch none or several)
-    _check(status, "copy_pages")
-    launch_count += launches.value
+    _check(done if done < 0 else done & 0xffff, "copy_pages")
+    launch_count += done >> 16
+
+
+_COPY_PAGES = (_i32, ctypes.c_char_p, _pointer)
+_INT32 = np.dtype(np.int32)
 
 
 def _host_indices(indices) -> np.ndarray:
@@ -213,14 +218,14 @@ def _host_indices(indices) -> np.ndarray:
         _need(not indices.is_cuda, "page indices are host lists or arrays")
         indices = indices.numpy()
     array = np.asarray(indices)
-    if array.dtype == np.int32 and array.ndim == 1 and array.flags.c_contiguous:
+    if array.dtype is _INT32 and array.ndim == 1:
         return array
     if array.size == 0:
         return np.empty(0, dtype=np.int32)
     _need(array.ndim == 1 and array.dtype.kind in "iu", "page indices are one-dimensional lists of integers")
     if array.dtype != np.int32:
         _need(int(array.min()) >= 0 and int(array.max()) < 2 ** 31, "a page outside its store")
-    return np.ascontiguousarray(array, dtype=np.int32)
+    return array.astype(np.int32)
 
 
 def silu_mul(gate_up: torch.Tensor, out: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
@@ -323,6 +328,10 @@ def attention_shared_tile(dtype: torch.dtype, tensor: bool = False) -> int:
     return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if tensor else 0))
 
 
+_ATTENTION_SHARED = (_pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32, *[_pointer] * 5, *[_i32] * 6, _f32,
+                     *[_i32] * 5, _pointer, _pointer, _i64, _i32, _i32, _i32, _pointer, _i32, _pointer)
+
+
 def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
                      shared, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, choice
                      ) -> torch.Tensor:
@@ -346,9 +355,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     if choice.prefix_parts or choice.tail_parts > 1:
         scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
         at = scratch.data_ptr()
-    _check(_entry("attention_shared", "tb_attention_shared", _pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32,
-                  *[_pointer] * 5, *[_i32] * 6, _f32, *[_i32] * 5, _pointer, _pointer, _i64, _i32, _i32, _i32, _pointer, _i32,
-                  _pointer)(
+    _check(_entry("attention_shared", "tb_attention_shared", _ATTENTION_SHARED)(
         q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
         block_table.stride(0), block_table.shape[1], *shared.addresses(), rows, shared.prefix.numel(), num_heads, num_kv_heads,
         head_dim, page_size, scale, choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, at,
@@ -411,6 +418,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tenso
 
 
 MAX_ALTERNATIVES = 64
+_TOKEN_LOGPROBS = (_pointer, _i64, *[_pointer] * 5, _i32, _i32, _i32, _pointer)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int = 0) -> tuple:
@@ -434,7 +442,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
     values = torch.empty((rows, alternatives), dtype=torch.float32, device=device)
     ids = torch.empty((rows, alternatives), dtype=torch.int32, device=device)
-    _check(_entry("logprobs", "tb_token_logprobs", _pointer, _i64, *[_pointer] * 5, _i32, _i32, _i32, _pointer)(
+    _check(_entry("logprobs", "tb_token_logprobs", _TOKEN_LOGPROBS)(
         logits.data_ptr(), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), values.data_ptr(),
         ids.data_ptr(), rows, vocab, alternatives, _raw_stream()), "token_logprobs")
     return logprob, entropy, values, ids
