@@ -200,7 +200,10 @@ class CacheManager:
                 grown[:, :g.tables.shape[1]] = g.tables
                 g.tables = grown
             first_needed = self._first_needed_page(g, state.length)
-            for logical in range(max(first_needed, state.first_live[index]), last + 1):
+            begin = max(first_needed, state.first_live[index])
+            if g.need.live_span() is None:
+                begin = max(begin, len(held))         # (nothing has been given back: the pages up to there are held)
+            for logical in range(begin, last + 1):
                 if logical in held:
                     continue
                 page = g.pool.allocate(request)       # may raise OutOfPages
@@ -286,7 +289,7 @@ class CacheManager:
                 if reserve is not None:
                     draws[index] += self.pages_for(g, reserve) - shared
                 else:
-                    draws[index] += sum(1 for logical in state.pages[index] if logical >= shared)
+                    draws[index] += len(state.pages[index]) - shared
         if any(g.pool is not None and draws[i] > g.pool.available_to_reserve for i, g in enumerate(self.groups)):
             return False
         moves: List[Tuple[List[int], List[int]]] = [([], []) for _ in self.groups]
@@ -306,17 +309,19 @@ class CacheManager:
                     g.pool.register(child)
                 else:
                     g.pool.reserve(child, self.pages_for(g, reserve) - shared)
-                g.tables[slot, :] = 0
-                for logical, page in state.pages[index].items():
-                    if logical < shared:
-                        g.pool.share(child, page)
-                    else:
-                        sources.append(page)
-                        page = g.pool.allocate(child)
-                        targets.append(page)
-                        self._ever_used[index].add(page)
-                    new.pages[index][logical] = page
+                held = dict(state.pages[index])
+                own = [logical for logical in held if logical >= shared] if shared == 0 else list(range(shared, len(held)))
+                if shared:                       # (of such a group every page from the first on is held)
+                    g.pool.share(child, [held[logical] for logical in range(shared)])
+                g.tables[slot, :] = g.tables[state.slot, :]
+                for logical in own:
+                    sources.append(held[logical])
+                    page = g.pool.allocate(child)
+                    targets.append(page)
+                    self._ever_used[index].add(page)
+                    held[logical] = page
                     g.tables[slot, logical] = page
+                new.pages[index] = held
             self._requests[child] = new
         self._copy(moves)
         return True

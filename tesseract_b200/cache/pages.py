@@ -18,7 +18,9 @@ release (src/engine/recurrent.rs:6-38).
 
 from __future__ import annotations
 
-from typing import Dict, Hashable, List, Optional
+from typing import Dict, Hashable, List, Optional, Sequence, Set
+
+import numpy as np
 
 
 class OutOfPages(RuntimeError):
@@ -33,10 +35,10 @@ class PagePool:
         self.first_page = first_page
         # LIFO: the last element is handed out first; start so that low ids go first.
         self._free: List[int] = list(range(first_page + num_pages - 1, first_page - 1, -1))
-        self._holders: Dict[int, List[Hashable]] = {}      # page -> who holds it, the longest-standing holder first
+        self._refs = np.zeros(num_pages, dtype=np.int32)    # holders of each page (from first_page on)
         self._quota: Dict[Hashable, int] = {}
-        self._held: Dict[Hashable, int] = {}                # pages drawn by the owner (and not given back)
-        self._borrowed: Dict[Hashable, set] = {}            # pages that it shares and others drew
+        self._drawn: Dict[Hashable, Set[int]] = {}          # pages drawn by the owner (and not given back)
+        self._borrowed: Dict[Hashable, Set[int]] = {}       # pages that it shares and others drew
         self._reserved_unallocated = 0
 
     # ---------------------------------------------------------------- queries
@@ -46,138 +48,145 @@ class PagePool:
 
     @property
     def used_pages(self) -> int:
-        return len(self._holders)
+        return self.num_pages - len(self._free)
 
     @property
     def available_to_reserve(self) -> int:
         return len(self._free) - self._reserved_unallocated
 
     def held_by(self, owner: Hashable) -> int:
-        return self._held.get(owner, 0) + len(self._borrowed.get(owner, ()))
+        return len(self._drawn.get(owner, ())) + len(self._borrowed.get(owner, ()))
 
     def owner_of(self, page: int) -> Optional[Hashable]:
-        holders = self._holders.get(page)
+        holders = self.holders_of(page)
         return holders[0] if holders else None
 
     def holders_of(self, page: int) -> List[Hashable]:
-        return list(self._holders.get(page, ()))
+        """Who holds the page: the one who drew it, if it has not ended, then those who share it."""
+        return ([owner for owner, pages in self._drawn.items() if page in pages]
+                + [owner for owner, pages in self._borrowed.items() if page in pages])
 
     # ---------------------------------------------------------------- reservations
     def reserve(self, owner: Hashable, pages: int) -> bool:
         """Set aside ``pages`` pages for ``owner`` (its peak simultaneous need)."""
-        if owner in self._quota or owner in self._held:
+        if owner in self._quota:
             return False
         if pages > self.available_to_reserve:
             return False
-        self._quota[owner] = pages
-        self._held[owner] = 0
+        self._enter(owner, pages)
         self._reserved_unallocated += pages
         return True
 
     def register(self, owner: Hashable) -> None:
         """Admit ``owner`` without a reservation: its pages come on demand."""
-        if owner in self._held:
+        if owner in self._quota:
             raise ValueError(f"{owner!r} is already registered in this pool")
-        self._quota[owner] = 0
-        self._held[owner] = 0
+        self._enter(owner, 0)
+
+    def _enter(self, owner: Hashable, quota: int) -> None:
+        self._quota[owner] = quota
+        self._drawn[owner] = set()
+        self._borrowed[owner] = set()
 
     # ---------------------------------------------------------------- pages
     def allocate(self, owner: Hashable) -> int:
-        if owner not in self._held:
+        if owner not in self._quota:
             raise KeyError(f"{owner!r} is not registered in this pool")
-        held, quota = self._held[owner], self._quota[owner]
-        if held < quota:
+        drawn = self._drawn[owner]
+        if len(drawn) < self._quota[owner]:
             self._reserved_unallocated -= 1   # drawing on the owner's own reservation
         elif self.available_to_reserve <= 0:
             raise OutOfPages(f"cache pool exhausted: {self.num_pages} pages, {len(self._free)} free, "
                              f"{self._reserved_unallocated} reserved for other requests")
         page = self._free.pop()
-        self._holders[page] = [owner]
-        self._held[owner] = held + 1
+        self._refs[page - self.first_page] = 1
+        drawn.add(page)
         return page
 
-    def share(self, owner: Hashable, page: int) -> None:
-        """``owner`` holds ``page`` too, beside whoever holds it now."""
-        if owner not in self._held:
+    def share(self, owner: Hashable, pages: Sequence[int]) -> None:
+        """``owner`` holds ``pages`` too, beside whoever holds them now."""
+        if owner not in self._quota:
             raise KeyError(f"{owner!r} is not registered in this pool")
-        holders = self._holders.get(page)
-        if holders is None:
-            raise ValueError(f"page {page} is free")
-        if owner in holders:
-            raise ValueError(f"page {page} is already held by {owner!r}")
-        holders.append(owner)
-        self._borrowed.setdefault(owner, set()).add(page)
+        new = set(pages)
+        if len(new) != len(pages) or not new.isdisjoint(self._drawn[owner]) or not new.isdisjoint(self._borrowed[owner]):
+            raise ValueError(f"a page is already held by {owner!r}, or named twice")
+        places = np.asarray(pages, dtype=np.int64) - self.first_page
+        if places.size and (places.min() < 0 or places.max() >= self.num_pages or not self._refs[places].all()):
+            raise ValueError("a page to be shared is free")
+        self._refs[places] += 1
+        self._borrowed[owner] |= new
 
     def give_back(self, owner: Hashable, page: int) -> None:
         """Return one page while the owner lives on (a window has passed it)."""
-        holders = self._holders.get(page, ())
-        if owner not in holders:
+        drawn, borrowed = self._drawn.get(owner, ()), self._borrowed.get(owner, ())
+        if page in borrowed:
+            borrowed.remove(page)             # (another's draw: no reservation of the owner covers it)
+        elif page not in drawn:
             raise ValueError(f"page {page} is not held by {owner!r}")
-        if page in self._borrowed.get(owner, ()):
-            self._borrowed[owner].remove(page)              # (another's draw: no reservation of the owner covers it)
-            self._let_go(owner, page)
-            return
-        if len(holders) > 1:
+        elif self._refs[page - self.first_page] > 1:
             # (the reservation would be owed a page that is not free)
             raise ValueError(f"page {page} is shared and cannot be given back by the one who drew it before it ends")
-        self._let_go(owner, page)
-        held = self._held[owner]
-        self._held[owner] = held - 1
-        if held <= self._quota[owner]:
-            self._reserved_unallocated += 1   # the reservation covers the peak, so it is owed again
+        else:
+            if len(drawn) <= self._quota[owner]:
+                self._reserved_unallocated += 1   # the reservation covers the peak, so it is owed again
+            drawn.remove(page)
+        self._let_go([page])
 
-    def _let_go(self, owner: Hashable, page: int) -> None:
-        holders = self._holders[page]
-        holders.remove(owner)
-        if not holders:
-            del self._holders[page]
-            self._free.append(page)
+    def _let_go(self, pages: Sequence[int]) -> None:
+        """One holder less for each page; those without one are free, in the order given."""
+        places = np.asarray(pages, dtype=np.int64) - self.first_page
+        self._refs[places] -= 1
+        self._free.extend((places[self._refs[places] == 0] + self.first_page).tolist())
 
     def release(self, owner: Hashable, pages: List[int]) -> None:
         """The owner ends: it lets go of its remaining pages and its reservation is dropped."""
-        if owner not in self._held:
+        if owner not in self._quota:
             return
-        borrowed = self._borrowed.pop(owner, set())
-        drawn = 0
-        for page in pages:
-            if owner not in self._holders.get(page, ()):
-                raise ValueError(f"page {page} is not held by {owner!r}")
-            drawn += page not in borrowed
-            self._let_go(owner, page)
-        held = self._held.pop(owner) - drawn + len(borrowed) - (len(pages) - drawn)
-        quota = self._quota.pop(owner)
-        if held != 0:
-            raise ValueError(f"{owner!r} ended while still holding {held} pages not named in the release")
-        self._reserved_unallocated -= max(0, quota - drawn)
+        drawn, borrowed = self._drawn[owner], self._borrowed[owner]
+        named = set(pages)
+        if len(named) != len(pages) or not named <= drawn | borrowed:
+            raise ValueError(f"a page named in the release is not held by {owner!r}, or named twice")
+        if len(named) != len(drawn) + len(borrowed):
+            raise ValueError(f"{owner!r} ended while still holding {len(drawn) + len(borrowed) - len(named)} pages not named in "
+                             f"the release")
+        self._reserved_unallocated -= max(0, self._quota.pop(owner) - len(drawn))
+        del self._drawn[owner], self._borrowed[owner]
+        if pages:
+            self._let_go(pages)
 
     def compact(self) -> Dict[int, int]:
         """Rename the held pages so that they have the lowest ids, and hand out free ones from the lowest on again.  Returns where
         the pages that move go (free ids all: no page moves to where another one was)."""
-        end = self.first_page + len(self._holders)
-        targets = [page for page in range(self.first_page, end) if page not in self._holders]
-        sources = sorted(page for page in self._holders if page >= end)
+        end = self.first_page + self.used_pages
+        held = self._refs > 0
+        targets = (np.flatnonzero(~held[:self.used_pages]) + self.first_page).tolist()
+        sources = (np.flatnonzero(held[self.used_pages:]) + end).tolist()
         moves = dict(zip(sources, targets))
-        for source, target in moves.items():
-            self._holders[target] = self._holders.pop(source)
-        for owner, pages in self._borrowed.items():
-            self._borrowed[owner] = {moves.get(page, page) for page in pages}
+        if moves:
+            at, to = np.asarray(sources) - self.first_page, np.asarray(targets) - self.first_page
+            self._refs[to] = self._refs[at]
+            self._refs[at] = 0
+            for holdings in (self._drawn, self._borrowed):
+                for owner, pages in holdings.items():
+                    holdings[owner] = {moves.get(page, page) for page in pages}
         self._free = list(range(self.first_page + self.num_pages - 1, end - 1, -1))
         return moves
 
     def check(self) -> None:
-        """Invariants: every page is free or owned, exactly once; reservations are honoured."""
-        ids = list(self._free) + list(self._holders)
-        if sorted(ids) != list(range(self.first_page, self.first_page + self.num_pages)):
-            raise AssertionError("a page was lost, duplicated, or freed twice")
-        counts: Dict[Hashable, int] = {}
-        for page, holders in self._holders.items():
-            if not holders or len(set(holders)) != len(holders):
-                raise AssertionError(f"page {page} has no holder, or one twice")
-            for owner in holders:
-                counts[owner] = counts.get(owner, 0) + 1
-        if any(counts.get(o, 0) != self.held_by(o) for o in self._held) or any(o not in self._held for o in counts):
+        """Invariants: every page is free or held, its holders counted right; reservations are honoured."""
+        refs = np.zeros(self.num_pages, dtype=np.int32)
+        for owner in self._quota:
+            drawn, borrowed = self._drawn[owner], self._borrowed[owner]
+            if not drawn.isdisjoint(borrowed):
+                raise AssertionError(f"{owner!r} holds a page twice")
+            refs[np.asarray(sorted(drawn | borrowed), dtype=np.int64) - self.first_page] += 1
+        if sum(len(d) for d in self._drawn.values()) != len(set().union(*self._drawn.values())):
+            raise AssertionError("a page was drawn twice")
+        if not (refs == self._refs).all():
             raise AssertionError("held counts disagree with ownership")
-        expected = sum(max(0, self._quota[o] - self._held[o]) for o in self._held)
+        if sorted(self._free) != (np.flatnonzero(refs == 0) + self.first_page).tolist():
+            raise AssertionError("a page was lost, duplicated, or freed twice")
+        expected = sum(max(0, self._quota[o] - len(self._drawn[o])) for o in self._quota)
         if expected != self._reserved_unallocated or self._reserved_unallocated > len(self._free):
             raise AssertionError("reservation accounting is inconsistent")
 

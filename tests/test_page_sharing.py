@@ -18,7 +18,7 @@ def test_a_shared_page_is_free_when_its_last_holder_lets_go():
     pool.register("a")
     pool.register("b")
     page = pool.allocate("a")
-    pool.share("b", page)
+    pool.share("b", [page])
     assert pool.holders_of(page) == ["a", "b"] and pool.used_pages == 1 and pool.held_by("b") == 1
     pool.check()
     pool.release("a", [page])
@@ -34,15 +34,20 @@ def test_sharing_refuses_free_pages_strangers_and_a_second_time():
     pool.register("a")
     page = pool.allocate("a")
     with pytest.raises(KeyError):
-        pool.share("b", page)
+        pool.share("b", [page])
     with pytest.raises(ValueError):
-        pool.share("a", page)
+        pool.share("a", [page])
     pool.register("b")
     with pytest.raises(ValueError):
-        pool.share("b", page + 1)
-    pool.share("b", page)
+        pool.share("b", [page + 1])
     with pytest.raises(ValueError):
-        pool.share("b", page)
+        pool.share("b", [page, page])
+    for outside in (-1, 4):
+        with pytest.raises(ValueError):
+            pool.share("b", [outside])
+    pool.share("b", [page])
+    with pytest.raises(ValueError):
+        pool.share("b", [page])
     with pytest.raises(ValueError):
         pool.give_back("a", page)          # shared: its reservation would be owed a page that is not free
     pool.give_back("b", page)              # a borrowed page may be let go of
@@ -56,7 +61,7 @@ def test_reservations_count_what_an_owner_draws():
     pages = [pool.allocate("a") for _ in range(3)]
     assert pool.reserve("b", 4)
     for page in pages[:2]:
-        pool.share("b", page)
+        pool.share("b", [page])
     assert pool.available_to_reserve == 0
     own = [pool.allocate("b") for _ in range(4)]
     pool.check()
@@ -72,7 +77,7 @@ def test_compaction_takes_the_lowest_ids_and_moves_to_free_places_alone():
     for owner in "abc":
         pool.register(owner)
     pages = {o: [pool.allocate(o) for _ in range(2)] for o in "abc"}
-    pool.share("c", pages["b"][0])
+    pool.share("c", [pages["b"][0]])
     pool.release("a", pages["a"])
     moves = pool.compact()
     assert moves == {5: 1, 6: 2}
