@@ -113,6 +113,10 @@ class CacheManager:
                 self.bindings.append(tuple(made))
             else:
                 self.bindings.append(made[0])
+        # bytes that a block of 64 tokens takes in an entry of the groups that continuations hold together (the largest)
+        self.shared_block_bytes = max((64 * 2 * g.need.num_kv_heads * g.need.head_dim
+                                       * torch.empty((), dtype=g.need.dtype or dtype).element_size()
+                                       for i, g in enumerate(self.groups) if self.shares_keys(i)), default=0)
         self._requests: Dict[Hashable, _Request] = {}
         self.pages_reused = 0          # pages handed out that an earlier owner had given back
         self._ever_used: List[set] = [set() for _ in self.groups]

@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_c
     } else if (find_common<kTcRows>(p, blockIdx.x, w)) {
         attend_tc<D>(p, w, &cache_map, tc_smem);
     }
-    pdl_wait();
+    if (blockIdx.x == 0) pdl_wait();          // (one block is enough; those without work must not stand in the others' way)
 }
 
 // ------------------------------------------------------------------------------------------------ 32-bit

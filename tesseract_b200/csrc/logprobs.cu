@@ -8,8 +8,8 @@
 // vocabulary has log probability NaN.
 //
 // Bound by HBM: 4 V bytes a row, read once.  A row is shared by a thread-block cluster of 1 to 8 blocks (a contiguous
-// part each); a block takes its part in chunks of sixteen logits a thread, in registers, the next chunk's loads under way
-// meanwhile.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
+// part each); a block takes its part in chunks of sixteen logits a thread, two chunks' asynchronous copies under way while one is
+// worked on in registers.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
 // others' loads (1,536 rows of 128,256 logits, one alternative: 143 us, 85 % of the measured copy rate; without alternatives 119);
 // few rows: blocks of 1,024, one chunk each at that vocabulary.  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
@@ -30,6 +30,7 @@ constexpr int kMaxTop = 64;
 constexpr int kListed = 512;                       // entries of the list
 constexpr int kGroup = 8;                          // threads whose largest logit is kept
 constexpr int kMaxGroups = 2048;                   // of a block (a longer part: of so many chunks together that they fit)
+constexpr int kSlots = 2;                          // chunks under way
 constexpr int kMaxBlocks = 8;
 constexpr int kNobody = 0x7fffffff;                // the id of an entry that is none
 constexpr float kLog2e = 1.4426950408889634f;
@@ -40,7 +41,7 @@ struct Shared {
     int id[kListed];
     float best_value[kMaxTop];                     // k entries in order, behind those there are (-inf, kNobody)
     int best_id[kMaxTop];
-    uint32_t group[kMaxGroups];                    // the groups' largest logits, as `ordered` has them
+    alignas(16) uint32_t group[kMaxGroups];        // the groups' largest logits, as `ordered` has them
     int16_t reaching[kMaxGroups];                  // the groups that reach the bound
     float warp_stat[32][3];
     int warp_count[32];
@@ -151,21 +152,29 @@ __device__ __forceinline__ int sum_before(Shared& sh, int mine, int& all) {     
 // Puts what may be among the k best of the block's logits into the list and returns how many that are (at least k, or all above
 // -inf if they are fewer; at most kListed).  The groups' largest logits, the block's m and zeroed counts are there.
 template <int THREADS>
-__device__ int find_best(Shared& sh, const float* base, int ahead, int end, int first, int chunks, int span, int k) {
+__device__ int find_best(Shared& sh, const float* base, int ahead, int end, int first, int chunks, int span, int groups,
+                         int k) {
     constexpr int kChunk = kEach * THREADS, kGroups = THREADS / kGroup;
-    const int groups = (chunks + span - 1) / span * kGroups;
     // low: what at least k logits reach, or all above -inf; high: what fewer than k groups (later: logits) reach
     const uint32_t nothing = ordered(-INFINITY) + 1;
     if (threadIdx.x < 32) {
         // one warp looks for the bound (a barrier a round cost the block four times as much): it begins at the smallest of its lanes'
         // largest, or for k above 32 second largest, groups, which 32, or 64, groups reach
         const int lane = threadIdx.x;
+        // (four at a time: what is behind the last is 0 up to a multiple of 128)
+        const uint4* four = reinterpret_cast<const uint4*>(sh.group);
         uint32_t one = 0, two = 0;
-#pragma unroll 4
-        for (int g = lane; g < groups; g += 32) {
-            const uint32_t v = sh.group[g];
+        auto meet_one = [&](uint32_t v) {
             two = max(two, min(one, v));
             one = max(one, v);
+        };
+#pragma unroll 4
+        for (int g = lane; g * 4 < groups; g += 32) {
+            const uint4 v = four[g];
+            meet_one(v.x);
+            meet_one(v.y);
+            meet_one(v.z);
+            meet_one(v.w);
         }
         uint32_t low = max(nothing, __reduce_min_sync(0xffffffffu, k <= 32 ? one : two));
         uint32_t high = __reduce_max_sync(0xffffffffu, one) + 1;
@@ -173,7 +182,10 @@ __device__ int find_best(Shared& sh, const float* base, int ahead, int end, int 
             const uint32_t middle = low + (high - low) / 2;
             int reach = 0;
 #pragma unroll 8
-            for (int g = lane; g < groups; g += 32) reach += sh.group[g] >= middle ? 1 : 0;
+            for (int g = lane; g * 4 < groups; g += 32) {
+                const uint4 v = four[g];
+                reach += (v.x >= middle ? 1 : 0) + (v.y >= middle ? 1 : 0) + (v.z >= middle ? 1 : 0) + (v.w >= middle ? 1 : 0);
+            }
             reach = __reduce_add_sync(0xffffffffu, reach);
             if (reach < k) {
                 high = middle;
@@ -290,6 +302,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
                 float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_value,
                 int* __restrict__ top_id, int vocab, int k, int blocks, int part) {
     constexpr int WARPS = THREADS / 32, kChunk = kEach * THREADS, kGroups = THREADS / kGroup;
+    extern __shared__ float4 ring[];               // [kSlots][kPackets][THREADS]
     __shared__ Shared sh;
     pdl_trigger();
     const int64_t r = blockIdx.x / blocks;
@@ -302,17 +315,21 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const int end = last - first + ahead;          // logits are base[ahead .. end)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();                                    // the logits come from the kernel in front
-    auto fetch = [&](float4 (&held)[kPackets], int chunk) {
+    // A chunk's packets on their way into this thread's own places of ring slot c % kSlots (nobody else reads them: no barrier).  A slot
+    // is free as soon as its chunk is in registers, so kSlots chunks are under way while one is worked on.
+    auto fetch = [&](int c) {
 #pragma unroll
         for (int u = 0; u < kPackets; ++u) {
-            const int i = chunk + (u * THREADS + (int)threadIdx.x) * 4;
+            const int i = c * kChunk + (u * THREADS + (int)threadIdx.x) * 4;
+            float4* to = ring + (c % kSlots * kPackets + u) * THREADS + threadIdx.x;
             if (i >= ahead && i + 4 <= end) {
-                held[u] = *reinterpret_cast<const float4*>(base + i);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                             ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(base + i) : "memory");
             } else {
-                held[u].x = i >= ahead && i < end ? base[i] : -INFINITY;
-                held[u].y = i + 1 >= ahead && i + 1 < end ? base[i + 1] : -INFINITY;
-                held[u].z = i + 2 >= ahead && i + 2 < end ? base[i + 2] : -INFINITY;
-                held[u].w = i + 3 >= ahead && i + 3 < end ? base[i + 3] : -INFINITY;
+                to->x = i >= ahead && i < end ? base[i] : -INFINITY;
+                to->y = i + 1 >= ahead && i + 1 < end ? base[i + 1] : -INFINITY;
+                to->z = i + 2 >= ahead && i + 2 < end ? base[i + 2] : -INFINITY;
+                to->w = i + 3 >= ahead && i + 3 < end ? base[i + 3] : -INFINITY;
             }
         }
     };
@@ -321,21 +338,24 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     const int chunks = (end + kChunk - 1) / kChunk;
     const int span = max(1, (chunks * kGroups + kMaxGroups - 1) / kMaxGroups);       // chunks that a group's largest is taken over (1 up to 1M logits)
     const int group = threadIdx.x / kGroup;
+    const int groups = (chunks + span - 1) / span * kGroups;
+    if ((int)threadIdx.x < ((groups + 127) & ~127) - groups) sh.group[groups + threadIdx.x] = 0;
     float largest = -INFINITY;
-    float4 next[kPackets];
     const int token = block == 0 && threadIdx.x == 0 ? tokens[r] : -1;
-    fetch(next, 0);
+#pragma unroll
+    for (int c = 0; c < kSlots; ++c) {
+        if (c < chunks) fetch(c);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     const float given = token >= 0 && token < vocab ? row[token] : NAN;
     for (int c = 0; c < chunks; ++c) {
         float x[kEach];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
 #pragma unroll
-        for (int u = 0; u < kPackets; ++u) {
-            x[4 * u] = next[u].x;
-            x[4 * u + 1] = next[u].y;
-            x[4 * u + 2] = next[u].z;
-            x[4 * u + 3] = next[u].w;
-        }
-        if (c + 1 < chunks) fetch(next, (c + 1) * kChunk);
+        for (int u = 0; u < kPackets; ++u)
+            *reinterpret_cast<float4*>(x + 4 * u) = ring[(c % kSlots * kPackets + u) * THREADS + threadIdx.x];
+        if (c + kSlots < chunks) fetch(c + kSlots);
+        asm volatile("cp.async.commit_group;" ::: "memory");
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
@@ -387,7 +407,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
     }
     __syncthreads();
     if (k > 0) {
-        const int n = find_best<THREADS>(sh, base, ahead, end, first, chunks, span, k);
+        const int n = find_best<THREADS>(sh, base, ahead, end, first, chunks, span, groups, k);
         cut<THREADS>(sh, n, k);
     }
     if (blocks > 1) {
@@ -474,7 +494,18 @@ int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const floa
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(rows * blocks));
     config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = (size_t)kSlots * kPackets * THREADS * sizeof(float4);
     config.stream = stream;
+    // (with the list and the groups more than a kernel may have unasked: told once a device)
+    static bool told[64];
+    int device = 0;
+    if (const cudaError_t err = cudaGetDevice(&device)) return (int)err;
+    if (device < 0 || device >= 64 || !told[device]) {
+        if (const cudaError_t err = cudaFuncSetAttribute(logprobs_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         (int)config.dynamicSmemBytes))
+            return (int)err;
+        if (device >= 0 && device < 64) told[device] = true;
+    }
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
     attribute[0].val.clusterDim.x = blocks;

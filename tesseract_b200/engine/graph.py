@@ -56,7 +56,7 @@ HOST_RING = 3          # pinned copies of a graph's metadata: a launch may be pr
 class _Graph:
     """Persistent buffers and the captured graph for one (batch bucket, table width), without or (``company``: the arrays of the
     step that it is captured for) with rows that have keys in common: how the rows are grouped is data, so one graph serves every
-    grouping."""
+    grouping with as many such groups."""
 
     def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None):
         cache, device = stepper.cache, stepper.runtime.device
@@ -202,7 +202,7 @@ class DecodeGraphs:
         self.stepper = stepper
         self.max_batch = max_batch
         self.graphs: Dict[Tuple[int, int], _Graph] = {}
-        self.shared_graphs: Dict[Tuple[int, int], _Graph] = {}      # of steps whose rows have keys in common (Stepper.company)
+        self.shared_graphs: Dict[Tuple[int, int, int], _Graph] = {}     # of steps whose rows have keys in common (Stepper.company)
         self.replays = 0
         self.captures = 0
         self.kernels_replayed = 0
@@ -231,11 +231,13 @@ class DecodeGraphs:
         pages = -(-(max(lengths) + 1) // cache.page_size)
         batch, columns = min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages))
         company = stepper.company(entries, batch - count)
-        graphs = self.graphs if company is None else self.shared_graphs
-        graph = graphs.get((batch, columns))
+        # (with company also by the groups that have keys in common: they bound what a captured launch must be laid out for)
+        graphs, key = ((self.graphs, (batch, columns)) if company is None
+                       else (self.shared_graphs, (batch, columns, sum(1 for b in company[2] if b))))
+        graph = graphs.get(key)
         if graph is None:
             graph = _Graph(stepper, batch, columns, self.sampled, company)
-            graphs[batch, columns] = graph
+            graphs[key] = graph
             self.captures += 1
         slot_index, h = graph.host_arrays()
         if company is not None:

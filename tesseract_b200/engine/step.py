@@ -134,7 +134,7 @@ class Stepper:
         groups, common = cache.rows_in_common(requests)
         made = shared_arrays(groups + [[len(entries) + k] for k in range(padding)], common + [0] * padding,
                              [cache.length(r) for r in requests] + [0] * padding)
-        return made if plan.sharing_pays(made[1], made[2]) else None
+        return made if plan.sharing_pays(made[1], made[2], cache.shared_block_bytes) else None
 
     # ------------------------------------------------------------------ the step
     def build_context(self, entries: Sequence[StepEntry], tokens: Optional[Sequence[Sequence[int]]] = None

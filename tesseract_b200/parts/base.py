@@ -305,7 +305,8 @@ class SharedRows:
     blocks: Tuple[int, ...]      # blocks of keys in common,
     tails: Tuple[int, ...]       # blocks (begun ones too) that each row reads behind them,
     row_blocks: Tuple[int, ...]  # and blocks that it has in common with its group
-    # rows and groups that the tensors have room for, where a captured step refills them (None: they hold just these)
+    # rows that the tensors have room for, where a captured step refills them with other groupings of as many groups with keys in
+    # common (None: they hold just these)
     room: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
 

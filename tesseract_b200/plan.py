@@ -295,18 +295,28 @@ SHARED_MAX_PARTS = 64
 
 
 # Blocks of 64 keys that rows need not read themselves from where on common parts are taken by themselves: below, one launch over
-# every row's own keys is faster (4 rows of 32 heads of 64 at 200 keys: 4.5 us on the device, 7.0 with a launch to put parts together).
+# every row's own keys is faster (4 rows of 32 heads of 64 at 200 keys: 4.2 us on the device, 7.0 with a launch to put parts together).
 SHARED_MIN_SAVED = 64
+# The same in bytes of keys and values from where on a decode step takes ``attention_shared`` at all: below, the kernel that rotates,
+# writes and attends in one launch is faster, as it finds the common pages in L2 (a step of the 1B sizes with and without, 8 rows
+# at 2,048 keys, 29 MB: 0.757 and 0.702 ms; 32 at 2,048, 130 MB: 0.992 and 1.068; 32 at 8,192, 520 MB: 1.136 and 1.931; of 8 layers
+# of the 8B sizes, 16 rows at 1,024, 63 MB: 1.058 and 1.050; 4 at 8,192, 101 MB: 0.975 and 1.013; 32 at 8,192: 1.179 and 2.105).
+SHARED_MIN_BYTES = 96 << 20
 # Tiles of 16 folded rows times blocks of common keys from where on the tensor cores' form is faster, whose launch takes 10 us (32
 # heads on 8, device time with and without: 64 rows at 2,048 keys of 64 11.1 and 11.6 us, at 8,192 15.9 and 18.9, 128 rows at
 # 16,384 24.4 and 44.2; of 128, 32 rows at 1,024 11.6 and 11.3, 64 at 2,048 13.1 and 19.0, 128 at 16,384 34.8 and 91.8).
 SHARED_TENSOR_MIN = {64: 128, 128: 48}
 
 
-def sharing_pays(sizes: Sequence[int], blocks: Sequence[int]) -> bool:
-    """Whether a decode step reads common keys once a group (``sizes`` rows, ``blocks`` blocks of 64 keys in common each) rather than
-    once a row."""
-    return sum((n - 1) * b for n, b in zip(sizes, blocks)) >= SHARED_MIN_SAVED
+def saved_blocks(sizes: Sequence[int], blocks: Sequence[int]) -> int:
+    """Blocks of 64 keys that the rows of groups (``sizes`` rows, ``blocks`` blocks in common each) need not read a second time."""
+    return sum((n - 1) * b for n, b in zip(sizes, blocks))
+
+
+def sharing_pays(sizes: Sequence[int], blocks: Sequence[int], block_bytes: int) -> bool:
+    """Whether a decode step reads common keys once a group rather than once a row, with ``block_bytes`` of keys and values in a
+    block of 64 of one layer."""
+    return saved_blocks(sizes, blocks) * block_bytes >= max(1, SHARED_MIN_BYTES)
 
 
 def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,
@@ -335,7 +345,7 @@ def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int, shortest: i
 def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sms) -> SharedAttentionPlan:
     sizes, blocks = np.asarray(shared.sizes), np.asarray(shared.blocks)
     tails = np.asarray(shared.tails)
-    if not sharing_pays(shared.sizes, shared.blocks):           # every row reads its own
+    if saved_blocks(shared.sizes, shared.blocks) < SHARED_MIN_SAVED:        # every row reads its own
         tails = tails + np.asarray(shared.row_blocks)
         blocks = np.zeros_like(blocks)
     rows = np.where(blocks > 0, sizes * fold, 0)
@@ -345,10 +355,6 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     tiles = -(-rows // tile)
     # large blocks of threads that are resident at once, a kv head (those of the 32-bit form are half as large)
     target = max(1, (4 if dtype == torch.float32 and head_dim <= 128 else 2) * sms // num_kv_heads)
-    prefix_parts, prefix_run = 0, 1
-    if tiles.any():
-        prefix_run = _shared_runs(tiles, blocks, target, SHARED_MIN_RUN[dtype])
-        prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
     # are many
     tails = np.maximum(tails, 1)
@@ -357,8 +363,15 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
-    # (tensors that are refilled: no grouping of so many rows has more tiles)
-    count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + shared.room // 2
+    prefix_parts, prefix_run = 0, 1
+    if tiles.any():
+        room = target
+        if not tensor and warps == 0:           # (in one launch with the rows' own)
+            room = max(target // 2, target - int((tail_tiles * -(-tails // tail_run)).sum()))
+        prefix_run = _shared_runs(tiles, blocks, room, SHARED_MIN_RUN[dtype])
+        prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
+    # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles)
+    count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + int((blocks > 0).sum())
     return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
 
 

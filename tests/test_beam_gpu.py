@@ -52,7 +52,8 @@ def engine(folder, dtype="float32", **options):
 def test_beams_in_32_bits_are_the_plain_searchs(model_folders, monkeypatch, name, length, width, steps, graphs, share):
     from tesseract_b200 import plan
 
-    monkeypatch.setattr(plan, "SHARED_MIN_SAVED", 0 if share else 10 ** 9)
+    monkeypatch.setattr(plan, "SHARED_MIN_SAVED", 0)
+    monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 0 if share else 1 << 60)
     folder = model_folders(name)
     config, tensors = llama.load_folder(folder)
     prompts = [random_tokens(config["vocab_size"], length, seed=length), random_tokens(config["vocab_size"], length // 2, seed=1)]
@@ -71,6 +72,8 @@ def test_beams_in_32_bits_are_the_plain_searchs(model_folders, monkeypatch, name
         assert [o.score for o in outs] == sorted((o.score for o in outs), reverse=True)
     assert llm.stepper.cache.used_pages() == 0
     llm.stepper.cache.check()
+    if graphs:
+        assert bool(llm.stepper.graphs.shared_graphs) == (share and length >= 64)      # (a whole block in common)
 
 
 @pytest.mark.parametrize("graphs", [True, False])
@@ -79,6 +82,7 @@ def test_beams_in_bfloat16_are_scored_as_the_plain_model_scores_them(model_folde
     from tesseract_b200 import plan
 
     monkeypatch.setattr(plan, "SHARED_MIN_SAVED", 0)
+    monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 0)
     folder = model_folders(name)
     config, tensors = llama.load_folder(folder)
     length = 100

@@ -69,6 +69,29 @@ def test_rows_apart_and_off_the_boundary(vocab, apart):
     check(whole[:, 1:], tokens_for(6, vocab), 9)
 
 
+@pytest.mark.parametrize("rows, vocab", [(1, 3000001), (300, 1100003)])
+def test_vocabularies_of_more_groups_than_are_kept(rows, vocab):
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randn(rows, vocab, generator=gen, device="cuda")
+    tokens = tokens_for(rows, vocab)
+    got = kernels.token_logprobs(logits, tokens, 40)
+    for r in {0, rows // 2, rows - 1}:
+        logs = torch.log_softmax(logits[r].double(), dim=0)
+        order = torch.sort(logits[r], descending=True, stable=True).indices[:40]
+        bound = (16 * vocab / 4096 + 60) * U * 30
+        assert torch.equal(got[3][r].long(), order)
+        assert float((got[2][r].double() - logs[order]).abs().max()) <= bound
+        assert abs(float(got[0][r]) - float(logs[int(tokens[r])])) <= bound
+        assert abs(float(got[1][r]) + float((logs.exp() * logs).sum())) <= bound
+
+
+@pytest.mark.parametrize("rows", [140, 150, 290, 300, 600])
+def test_every_size_of_block(rows):
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randn(rows, 9001, generator=gen, device="cuda") * 2
+    check(logits, tokens_for(rows, 9001), 17)
+
+
 @pytest.mark.parametrize("rows", [1, 30, 400])
 def test_the_same_numbers_at_every_split(rows):
     """How many blocks share a row depends on the rows: alternatives are the same tokens whichever."""

@@ -1,0 +1,94 @@
+"""How attention over rows with keys in common is cut, and what of its kernel a run cannot show (no GPU needed)."""
+
+import os
+import re
+
+import pytest
+import torch
+
+from tesseract_b200 import kernels, plan
+from tesseract_b200.parts.base import SharedRows, shared_arrays
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tesseract_b200", "csrc")
+SMS = 148
+
+
+def choose(groups, heads=32, kv_heads=8, dim=128, dtype=torch.bfloat16, page=16, room=None):
+    rows, members, prefixes, positions = 0, [], [], []
+    for prefix, counts in groups:
+        members.append(list(range(rows, rows + len(counts))))
+        prefixes.append(prefix)
+        positions += [n - 1 for n in counts]
+        rows += len(counts)
+    shared = SharedRows.of(members, prefixes, positions, "cpu")
+    shared.room = room
+    return shared, plan.shared_attention(dtype, num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, page_size=page, shared=shared,
+                                         sms=SMS)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 256])
+@pytest.mark.parametrize("groups", [
+    [(0, [1])], [(0, [0])], [(200, [205] * 4)], [(2048, [2100] * 16)], [(32768, [32900] * 64)], [(0, [70000])],
+    [(300 * k, [300 * k + 10 * j for j in range(1, 2 + k)]) for k in range(1, 9)], [(131072, [131073, 131080])], [(64, [65] * 500)],
+])
+def test_runs_cover_every_key_and_fit_the_chip(groups, dim, dtype):
+    shared, choice = choose(groups, dim=dim, dtype=dtype)
+    fold, kv_heads = 4, 8
+    assert 1 <= choice.tail_parts <= plan.SHARED_MAX_PARTS and 0 <= choice.prefix_parts <= plan.SHARED_MAX_PARTS
+    if choice.prefix_parts == 0:
+        assert choice.tiles == 0 and not choice.tensor
+        assert plan.saved_blocks(shared.sizes, shared.blocks) < plan.SHARED_MIN_SAVED
+    else:
+        tile = kernels.attention_shared_tile(dtype, choice.tensor)
+        assert choice.tiles == sum(-(-n * fold // tile) for n, b in zip(shared.sizes, shared.blocks) if b)
+        runs = [(-(-n * fold // tile), -(-b // choice.prefix_run)) for n, b in zip(shared.sizes, shared.blocks) if b]
+        assert choice.prefix_parts == min(plan.SHARED_MAX_PARTS, max(r for _, r in runs))
+        # at most what is resident at once, unless every tile is one run already
+        assert sum(t * r for t, r in runs) * kv_heads <= 4 * SMS or max(r for _, r in runs) == 1
+        assert choice.tensor == (dtype == torch.bfloat16 and dim in (64, 128) and
+                                 sum(-(-n * fold // 16) * b for n, b in zip(shared.sizes, shared.blocks)) > plan.SHARED_TENSOR_MIN[dim])
+
+
+def test_what_is_shared_and_what_not():
+    assert choose([(200, [205] * 4)])[1].prefix_parts == 0            # three rows times three blocks: every row reads its own
+    assert choose([(2048, [2100] * 16)])[1].prefix_parts > 0
+    assert choose([(4096, [5000])])[1].prefix_parts == 0              # alone
+    block = 64 * 8 * 64 * 2 * 2
+    assert not plan.sharing_pays((8,), (32,), block) and plan.sharing_pays((32,), (32,), block)
+    assert not plan.sharing_pays((1, 1), (0, 0), block) and not plan.sharing_pays((4,), (100,), 0)
+
+
+def test_a_captured_plan_has_tiles_for_every_grouping_of_as_many_groups():
+    for room in (8, 16, 32):
+        _, choice = choose([(4096, [4200] * (room // 2)), (2048, [2100] * (room - room // 2))], room=room)
+        tile = kernels.attention_shared_tile(torch.bfloat16, choice.tensor)
+        for first in range(0, room + 1):
+            assert choice.tiles >= -(-first * 4 // tile) + -(-(room - first) * 4 // tile)
+
+
+def test_arrays_of_a_step():
+    arrays, sizes, blocks, tails, row_blocks = shared_arrays([[2, 0], [1], [3]], [130, 500, 0], [140, 600, 129, -1])
+    members, start, leader, prefix, common = [a.tolist() for a in arrays]
+    assert members == [2, 0, 1, 3] and start == [0, 2, 3, 4] and leader == [2, 1, 3]
+    assert prefix == [128, 0, 0] and common == [128, 0, 128, 0]       # whole blocks, and nothing for a row alone
+    assert sizes == (2, 1, 1) and blocks == (2, 0, 0) and tails == (1, 10, 1, 0) and row_blocks == (2, 0, 2, 0)
+
+
+def test_tensor_memory_that_a_product_used_is_touched_behind_a_fence():
+    """attend_tc: a softmax thread that waited for a product's commit reads or writes what the product used only behind
+    ``tcgen05.fence::after_thread_sync``."""
+    with open(os.path.join(CSRC, "attention_shared.cu")) as handle:
+        code = re.sub(r"//[^\n]*", "", handle.read())
+    softmax = code[code.index("const uint32_t lane_base"):code.index("__global__ void __launch_bounds__(kTcThreads, 2)")]
+    waiting, waits, touches = False, 0, 0
+    for event in re.finditer(r"(?P<wait>mbar_wait\((?:o_full|s_full))|(?P<fence>tc_fence_after\(\))|"
+                             r"(?P<touch>tmem_(?:load|store)\w*\(tmem_[ops]\b|\"r\"\(tmem_o)", softmax):
+        if event["wait"]:
+            waiting, waits = True, waits + 1
+        elif event["fence"]:
+            waiting = False
+        else:
+            touches += 1
+            assert not waiting
+    assert waits == 2 and touches >= 5                                # (o_full is waited for in product_done alone)
