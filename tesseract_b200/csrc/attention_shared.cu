@@ -169,6 +169,12 @@ __device__ __forceinline__ int64_t slot_of(const SharedParams& p, int row, int h
     return ((int64_t)row * p.heads + head) * (p.prefix_parts + p.tail_parts) + part;
 }
 
+// Waits, with a limit, for copies that are under way when something has been given up.
+__device__ __noinline__ void settle(uint32_t bar, uint32_t parity) {
+    for (uint32_t spin = 0; spin < kSpinLimit && !mbar_try_wait(bar, parity); ++spin) {
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void store_out(const SharedParams& p, int row, int head, int col, float v) {
     Elem<T>::store((T*)p.out + (int64_t)row * p.out_stride + (int64_t)head * p.head_dim + col, v);
@@ -551,7 +557,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     // k_full, k_empty, v_full, v_empty [STAGES] each, s_full, s_free, p_ready[2], o_full[2] (of block j: those of j & 1)
     __shared__ __align__(8) uint64_t bars[4 * STAGES + 6];
     __shared__ uint32_t tmem_base_slot;
-    __shared__ int abort_flag;
+    __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = min(kTcRows, w.folded - w.first_folded);
     const int live_threads = (rows + 31) / 32 * 32;               // of the softmax warps: those with a row
@@ -585,6 +591,11 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                      ::"r"(smem_u32(&tmem_base_slot)), "r"(kTcColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // where a thread's query lies, and the page of a lane's keys in the first block: looked up while the rest is set up
+    const int rows_per_copy = min(p.paging.size, kBlock), copies = kBlock / rows_per_copy;          // keys and copies of a block: at most 8
+    int row = 0, head = 0, next_page = 0;
+    if (threadIdx.x < rows) place_of(p, w, w.first_folded + threadIdx.x, row, head);
+    if (warp == 5 && lane < copies) next_page = table[p.paging.page_of(w.begin + lane * rows_per_copy)];
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -592,12 +603,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         // the queries, a thread a row, while warp 5 already brings the first blocks
         const int r = threadIdx.x;
         if (r < kTcRows) {
-            const __nv_bfloat16* src = (const __nv_bfloat16*)p.q;
-            if (r < rows) {
-                int row, head;
-                place_of(p, w, w.first_folded + r, row, head);
-                src += (int64_t)row * p.q_stride + (int64_t)head * D;
-            }
+            const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (int64_t)row * p.q_stride + (int64_t)head * D;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)
                 cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), src + c * 8, r < rows);
@@ -612,16 +618,13 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     auto tmem_p = [&](int j) { return tmem_o + D + (j & 1) * (kBlock / 2); };
 
     if (warp == 5) {
-        const int rows_per_copy = min(p.paging.size, kBlock), copies = kBlock / rows_per_copy;      // at most 8
         bool ok = true;
+        int asked[2] = {0, 0};                                    // blocks of keys, and of values, that copies were issued for
         for (int it = 0; it < n_blocks && ok; ++it) {
             const int s = it % STAGES;
-            int page = 0, in_page = 0;
-            if (lane < copies) {
-                const int key = w.begin + it * kBlock + lane * rows_per_copy;
-                page = table[p.paging.page_of(key)];
-                in_page = p.paging.within(key);
-            }
+            const int key = w.begin + it * kBlock + lane * rows_per_copy, page = next_page;
+            const int in_page = p.paging.within(key);
+            if (lane < copies && it + 1 < n_blocks) next_page = table[p.paging.page_of(key + kBlock)];
             const uint32_t dst = ring + s * 2 * kBlockBytes + (uint32_t)(lane * rows_per_copy) * 128;
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
@@ -638,11 +641,17 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                     for (int h = 0; h < D / 64; ++h)
                         tma_load_kv(dst + which * kBlockBytes + h * kSlice, cache_map, full, h * 64, in_page, w.kv_head, which, page);
                 }
+                ++asked[which];
             }
         }
         if (!ok && lane == 0) {
             abort_flag = 1;
             atomicExch(p.error, 110);
+        }
+        if (!ok || abort_flag) {                                  // (no copy lands in a block that has left)
+            for (int which = 0; which < 2; ++which)
+                for (int it = max(0, asked[which] - STAGES); it < asked[which]; ++it)
+                    settle((which ? v_full : k_full) + 8 * (it % STAGES), (it / STAGES) & 1);
         }
     } else if (warp == 4) {
         if (lane == 0) {
@@ -691,8 +700,6 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         }
     } else if (warp * 32 < rows) {
         const int r = warp * 32 + lane;                           // row of the tile = lane of tensor memory
-        int row = 0, head = 0;
-        if (r < rows) place_of(p, w, w.first_folded + r, row, head);
         const int64_t slot = slot_of(p, row, head, w.part);
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
         // m: the maximum that the stored weights and O are scaled by; it is raised (and O rescaled) only when a block's exceeds it by
