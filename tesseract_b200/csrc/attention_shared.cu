@@ -465,10 +465,11 @@ constexpr size_t mma_bytes() {
 // 128-byte swizzle, S in 64 columns of tensor memory), the weights 2^(s - m) of a row by the thread that owns it, rounded to
 // bfloat16 into one of two buffers in tensor memory, and O += P . V (M128 x N D x K64, P from tensor memory), O in D columns.
 // No block needs a mask: a common part ends with a block, and what is beyond it belongs to the rows' own parts.
-// Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products; warp 5
-// brings keys and values, page by page, with cp.async.bulk.tensor into rings of their own.  All waits are bounded.
+// Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products for the
+// scores and one lane of warp 6 those with the values; warp 5 brings keys and values, page by page, with cp.async.bulk.tensor into
+// rings of their own.  All waits are bounded.
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 192;
+constexpr int kTcThreads = 224;
 constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
 template <int D>
 constexpr int kTcStages = D == 64 ? 4 : 2;    // 64 KB of keys and values under way either way
@@ -599,7 +600,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp != 5) {
+    if (warp < 5) {
         // the queries, a thread a row, while warp 5 already brings the first blocks
         const int r = threadIdx.x;
         if (r < kTcRows) {
@@ -616,6 +617,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     const uint32_t tmem_base = tmem_base_slot;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + kBlock;
     auto tmem_p = [&](int j) { return tmem_o + D + (j & 1) * (kBlock / 2); };
+    constexpr uint32_t kStageStep = (2 * kBlockBytes) >> 4;       // a ring stage further, in the units of a descriptor's address
 
     if (warp == 5) {
         bool ok = true;
@@ -655,12 +657,18 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         }
     } else if (warp == 4) {
         if (lane == 0) {
-            constexpr uint32_t idesc_qk = idesc_bf16(kTcRows, kBlock, 0), idesc_pv = idesc_bf16(kTcRows, D, 1);
+            constexpr uint32_t idesc_qk = idesc_bf16(kTcRows, kBlock, 0);
             // (descriptors are moved by adding to their start-address field, bytes >> 4)
             const uint64_t q_desc = desc_sw128(q_tile, 1), k_desc0 = desc_sw128(ring, 1);
-            const uint64_t v_desc0 = desc_sw128(ring + kBlockBytes, kSlice >> 4);
-            constexpr uint32_t kStageStep = (2 * kBlockBytes) >> 4;
-            auto issue_qk = [&](int s) {
+            int s = 0;
+            uint32_t parity = 0;
+            bool ok = true;
+            for (int j = 0; j < n_blocks; ++j) {
+                // as soon as the softmax warps hold S_{j-1} in registers the next block's scores may take its place
+                if (!mbar_wait(k_full + 8 * s, parity, &abort_flag) || (j > 0 && !mbar_wait(s_free, (j - 1) & 1, &abort_flag))) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
                 const uint64_t k_desc = k_desc0 + (uint32_t)s * kStageStep;
 #pragma unroll
@@ -669,21 +677,25 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                             k_desc + (((kk >> 2) * kSlice + (kk & 3) * 32) >> 4), idesc_qk, kk != 0);
                 umma_commit(s_full);
                 umma_commit(k_empty + 8 * s);
-            };
-            int qs = 0, s = 0;
-            uint32_t q_parity = 0, parity = 0;
-            auto next_q = [&]() { if (++qs == STAGES) { qs = 0; q_parity ^= 1; } };
-            bool ok = mbar_wait(k_full + 8 * qs, q_parity, &abort_flag);
-            if (ok) issue_qk(qs);
-            next_q();
-            for (int j = 0; j < n_blocks && ok; ++j) {
-                if (j + 1 < n_blocks) {
-                    // as soon as the softmax warps hold S_j in registers the next block's scores may take its place
-                    if (!mbar_wait(k_full + 8 * qs, q_parity, &abort_flag) || !mbar_wait(s_free, j & 1, &abort_flag)) { ok = false; break; }
-                    issue_qk(qs);
-                    next_q();
+                if (++s == STAGES) { s = 0; parity ^= 1; }
+            }
+            if (!ok) {
+                abort_flag = 1;
+                atomicExch(p.error, 120);
+            }
+        }
+    } else if (warp == 6) {
+        if (lane == 0) {
+            constexpr uint32_t idesc_pv = idesc_bf16(kTcRows, D, 1);
+            const uint64_t v_desc0 = desc_sw128(ring + kBlockBytes, kSlice >> 4);
+            int s = 0;
+            uint32_t parity = 0;
+            bool ok = true;
+            for (int j = 0; j < n_blocks; ++j) {
+                if (!mbar_wait(v_full + 8 * s, parity, &abort_flag) || !mbar_wait(p_ready(j), phase(j), &abort_flag)) {
+                    ok = false;
+                    break;
                 }
-                if (!mbar_wait(v_full + 8 * s, parity, &abort_flag) || !mbar_wait(p_ready(j), phase(j), &abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint64_t v_desc = v_desc0 + (uint32_t)s * kStageStep;
 #pragma unroll
@@ -695,7 +707,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
             }
             if (!ok) {
                 abort_flag = 1;
-                atomicExch(p.error, 120);
+                atomicExch(p.error, 125);
             }
         }
     } else if (warp * 32 < rows) {
