@@ -11,12 +11,15 @@
 //
 // What a block does: one tile of folded rows (the `fold` query heads of a kv head, row after row of the group, or of one row
 // behind the common part) against one run of keys of one kv head.
-//   attend_mma   bfloat16, tiles of 16 folded rows: every warp streams every eighth tile of 16 keys through a cp.async ring of its
+//   attend_mma   bfloat16, tiles of 16 folded rows: the warps take turns at tiles of 16 keys, each through a cp.async ring of its
 //                own into mma.sync.m16n8k16; scores and sums in 32 bits, the weights rounded to bfloat16 for their product with the
 //                values (as in this package's other attention kernels in bfloat16: relative 2^-9 of each, averaged over the keys).
-//   attend_tc    bfloat16, head sizes 64 and 128, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor cores.
-//   attend_f32   32-bit, tiles of 8 folded rows, multiply-adds only: a lane scores one key against the tile's rows, then owns a
-//                few columns of the values.
+//                Bound by HBM: 16 rows of 4,000 keys of their own, 32 heads on 8 of 128, 262 MB in 47.3 us = 5.5 TB/s, 0.86 of the
+//                measured copy rate; below some 10 MB by the chain of a launch, its look-ups and the first copies (4 to 12 us).
+//   attend_tc    bfloat16, head sizes 64 and 128, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor
+//                cores, see there.  A tile of 16 would read a common part from L2 once for every 16 folded rows.
+//   attend_f32   32-bit, tiles of 8 folded rows, multiply-adds only, see there.
+// Which form and how many runs: plan.shared_attention, with both sides' times beside its rule.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
 #include <new>
@@ -468,6 +471,12 @@ constexpr size_t mma_bytes() {
 // Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products for the
 // scores and one lane of warp 6 those with the values; warp 5 brings keys and values, page by page, with cp.async.bulk.tensor into
 // rings of their own.  All waits are bounded.
+// 64 rows, 32 heads on 8 of 128, 32,768 keys in common: 50.6 us with the join behind it (134 MB, 20.8 us at the measured copy rate;
+// 34 GFLOP, 20.2 us at the measured matrix rate).  Two blocks of 128 rows a multiprocessor read the same keys (L2 hit rate 46 %), and
+// the chain of a block of keys bounds it: scores, their way to registers, maximum, weights, their way back, product; counters show
+// the tensor pipe at 38 %, the special-function pipe at 38 % and the issue slots at 32 %.  Two tiles in one block of threads with
+// 512 columns took 68.1 us, two threads a row 1.3 us longer than one, both products' issue by one lane 53.3; products with the
+// values by a warp of their own cost head size 64 something (64 rows, 65,536 keys: 68.0 us, 66.5 with one lane).
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 224;
 constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
@@ -871,8 +880,10 @@ __device__ __forceinline__ void store_n(float* to, const float (&v)[N]) {
 
 // D: head size padded to 64, 128 or 256.  A lane owns a few neighbouring columns of queries, keys and values, so keys and values
 // are read whole rows at a time.  Its products for four keys and eight rows are 32 partial sums, which the lanes exchange in five
-// rounds, half as many each, until every lane has one score: 31 exchanges for 32 scores.  (A lane a key instead, its row read 16
-// bytes at a time: 131 us for 16 rows at 4,096 keys of 32 heads of 128, bound by the cache lines that each load touches.)
+// rounds, half as many each, until every lane has one score: 31 exchanges for 32 scores.  16 rows of 32 heads on 8 of 128 at 4,096
+// keys in common: 66.6 us, 1.1 GFLOP, 16 TFLOP/s of plain multiply-adds; bound by the instructions of the exchanges and by their
+// latency (issue slots 33 %), not by the 42 MB.  (A lane a key instead, its row read 16 bytes at a time: 131 us, bound by the cache
+// lines that each load touches.)
 template <int D>
 __device__ void attend_f32(const SharedParams& p, const Work& w, float* smem) {
     constexpr int COLS = D / 32;              // (the head size is a multiple of 16, so a lane's columns are all there or none)
@@ -1010,8 +1021,8 @@ constexpr size_t f32_bytes() {
 
 // A warp a (row, head).  Its lanes read the maxima and sums of all runs at once (four a lane: kMaxParts), and their weights stay in
 // registers; then LANES lanes read a run's sums, 16 bytes each (for more than 128 columns twice), and 32 / LANES runs side by
-// side, eight loads under way a lane.  (One load of a maximum after the other, a run at a time, took 31 us for 64 rows of 32 heads of
-// 18 runs; this 5.)
+// side, eight loads under way a lane.  64 rows of 32 heads of 128 and 19 runs, 20 MB, most of it still in L2: 5 us.  (One load of a
+// maximum after the other, a run at a time, took 31.)
 constexpr int kMaxParts = 128;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {

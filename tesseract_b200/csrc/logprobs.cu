@@ -10,8 +10,9 @@
 // Bound by HBM: 4 V bytes a row, read once.  A row is shared by a thread-block cluster of 1 to 8 blocks (a contiguous
 // part each); a block takes its part in chunks of sixteen logits a thread, two chunks' asynchronous copies under way while one is
 // worked on in registers.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
-// others' loads (1,536 rows of 128,256 logits, one alternative: 143 us, 85 % of the measured copy rate; without alternatives 119);
-// few rows: blocks of 1,024, one chunk each at that vocabulary.  Of a chunk
+// others' loads (1,536 rows of 128,256 logits, one alternative: 133 us, 0.92 of the measured copy rate; 143 where the clocks have fallen
+// under minutes of load); few rows: blocks of 1,024, one chunk each at that vocabulary (64 rows, 20 alternatives: 14.1 us, of which
+// the 33 MB are 5.1, the rest the start, the bound, the second reading and the exchange of a cluster).  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
 //     they meet once, at the end, in a fixed order, so a row's numbers do not depend on the timing;
 //   * every eight threads leave the largest of their 128 logits.  No block waits for anything inside the loop.
