@@ -18,7 +18,7 @@
 //                measured copy rate; below some 10 MB by the chain of a launch, its look-ups and the first copies (4 to 12 us).
 //   attend_tc    bfloat16, head sizes 64 and 128, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor
 //                cores, see there.  A tile of 16 would read a common part from L2 once for every 16 folded rows.
-//   attend_f32   32-bit, tiles of 8 folded rows, multiply-adds only, see there.
+//   attend_f32, attend_f32_wide   32-bit, tiles of 8 and of 32 folded rows, multiply-adds only, see there.
 // Which form and how many runs: plan.shared_attention, with both sides' times beside its rule.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
@@ -56,7 +56,7 @@ struct SharedParams {
     int tail_parts, tail_run;                 // the same behind it
     Paging paging;
     float scale_log2;
-    int tensor;                               // the common parts are attend_tc's
+    int wide;                                 // the common parts are a kernel's of their own (attend_tc, attend_f32_wide)
     int direct;                               // one run a row and nothing in common: the results go to `out` at once
     int* error;                               // set where a bounded wait ran out
 };
@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(WARPS * 32) shared_mma_kernel(const SharedPara
     pdl_wait();
     pdl_trigger();                            // (only now: the kernels behind read what is older than this one without a wait of their own)
     Work w;
-    // (tensor: the common parts are the next kernel's)
-    if (p.tensor ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS, ONE>(p, w, smem);
+    // (wide: the common parts are the next kernel's)
+    if (p.wide ? find_tail<kRows>(p, blockIdx.x, w) : find_work<kRows>(p, blockIdx.x, w)) attend_mma<D, WARPS, ONE>(p, w, smem);
     else if (p.direct) leave_nothing<__nv_bfloat16, kRows>(p, w);
 }
 
@@ -556,6 +556,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 
@@ -851,162 +856,222 @@ __global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------ 32-bit
 
-constexpr int kF32Rows = 8;                   // folded rows of a tile
+constexpr int kF32Rows = 8;                   // folded rows of a warp
 constexpr int kF32Warps = 4;
-constexpr int kF32Keys = 32;                  // keys of a warp's tile
-constexpr int kF32Aside = 4;                  // keys whose scores are summed side by side: with eight rows one sum a lane
-
-// N neighbouring numbers (2, 4 or 8) from or to 8- or 16-byte boundaries.
-template <int N>
-__device__ __forceinline__ void load_n(const float* from, float (&v)[N]) {
-    if constexpr (N == 2) {
-        const float2 t = *reinterpret_cast<const float2*>(from);
-        v[0] = t.x;
-        v[1] = t.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(from + i);
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_n(float* to, const float (&v)[N]) {
-    if constexpr (N == 2) {
-        *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(v + i);
-    }
-}
-
-// D: head size padded to 64, 128 or 256.  A lane owns a few neighbouring columns of queries, keys and values, so keys and values
-// are read whole rows at a time.  Its products for four keys and eight rows are 32 partial sums, which the lanes exchange in five
-// rounds, half as many each, until every lane has one score: 31 exchanges for 32 scores.  16 rows of 32 heads on 8 of 128 at 4,096
-// keys in common: 66.6 us, 1.1 GFLOP, 16 TFLOP/s of plain multiply-adds; bound by the instructions of the exchanges and by their
-// latency (issue slots 33 %), not by the 42 MB.  (A lane a key instead, its row read 16 bytes at a time: 131 us, bound by the cache
-// lines that each load touches.)
+constexpr int kF32Keys = 32;                  // keys of a tile
+constexpr int kF32Aside = 4;                  // keys whose scores a warp sums side by side: with eight rows one a lane
+// Columns of a lane.  (8 for 128 too, where two blocks share a multiprocessor instead of three: 64 rows at 2,048 keys 95.0 us instead of
+// 96.3, but 8 rows 25.8 instead of 21.2.)
 template <int D>
-__device__ void attend_f32(const SharedParams& p, const Work& w, float* smem) {
-    constexpr int COLS = D / 32;              // (the head size is a multiple of 16, so a lane's columns are all there or none)
-    constexpr int GROUPS = kF32Keys / kF32Aside;
-    static_assert(kF32Rows * kF32Aside == 32, "a score a lane");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = min(kF32Rows, w.folded - w.first_folded);
-    const int dim = p.head_dim, col = lane * COLS;
-    const bool owns = col < dim;
-    float* weights = smem + warp * (kF32Keys * kF32Rows);                            // [key][row] of this warp
-    int64_t* places = reinterpret_cast<int64_t*>(smem + kF32Warps * kF32Keys * kF32Rows) + warp * kF32Keys;    // where its keys lie
-    float query[kF32Rows][COLS];
+constexpr int kColsF32 = D == 256 ? 8 : 4;
+
+// D: head size padded to 64, 128 or 256.  COLS columns of queries, keys and values are a lane's (one group of four neighbours, or
+// two), so keys and values are read whole rows at a time, and one 16-byte load serves 32 multiply-adds; where fewer than 32 lanes
+// have a row between them, the parts of a warp take keys of their own.  A lane's products for its keys and the eight rows are
+// partial sums, which the lanes exchange in rounds, half as many each, until every lane has one score: as many exchanges for 32 scores
+// as lanes share a row, less one.  Rows go in packed pairs.
+template <int D, int COLS>
+struct RowsF32 {
+    static constexpr int kCols = COLS, kLanes = D / COLS, kParts = 32 / kLanes;
+    static constexpr int kApart = kLanes * 4;                     // from a lane's first group of columns to its second
+    uint64_t query[kF32Rows / 2][kCols], o[kF32Rows / 2][kCols];
+    // of row lane % 8: the maximum, and the sum over the keys that this lane weighs
+    float m, l;
+
+    // A lane's columns of a row, `from` the first of them, zeros from column `left` on (a multiple of four).
+    static __device__ __forceinline__ void load(const float* from, int left, float (&v)[kCols]) {
 #pragma unroll
-    for (int r = 0; r < kF32Rows; ++r) {
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) query[r][c] = 0.0f;
-        if (r < rows && owns) {
-            int row, head;
-            place_of(p, w, w.first_folded + r, row, head);
-            load_n((const float*)p.q + (int64_t)row * p.q_stride + (int64_t)head * dim + col, query[r]);
+        for (int i = 0; i < kCols / 4; ++i) {
+            float4 four = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i * kApart < left) four = *reinterpret_cast<const float4*>(from + i * kApart);
+            *reinterpret_cast<float4*>(v + i * 4) = four;
         }
     }
-    const int* table = p.table + (int64_t)w.row * p.table_stride;
-    const int64_t head_block = (int64_t)p.paging.size * dim;
-    const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
-    const float* keys = (const float*)p.cache + (int64_t)w.kv_head * head_block + (owns ? col : 0);
-    const float* values = keys + v_offset;
-    // of row lane % 8: the maximum, and the sum over the keys that this lane weighs
-    float m = kMasked, l = 0.0f, o[kF32Rows][COLS];
+
+    __device__ __forceinline__ void begin(const SharedParams& p, const Work& w, int first, int rows, int col) {
+        m = kMasked;
+        l = 0.0f;
 #pragma unroll
-    for (int r = 0; r < kF32Rows; ++r)
+        for (int pair = 0; pair < kF32Rows / 2; ++pair) {
+            float q[2][kCols];
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) o[r][c] = 0.0f;
-    for (int key0 = w.begin + warp * kF32Keys; key0 < w.end; key0 += kF32Warps * kF32Keys) {
-        const int key = min(key0 + lane, w.end - 1);              // (beyond the end: the last key once more, masked below)
-        places[lane] = (int64_t)table[p.paging.page_of(key)] * page_block + (int64_t)p.paging.within(key) * dim;
-        __syncwarp();
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) q[i][c] = 0.0f;
+                const int r = (pair * 2 + i) ^ (threadIdx.x & 7);  // (`tile` says why)
+                if (r < rows) {
+                    int row, head;
+                    place_of(p, w, first + r, row, head);
+                    load((const float*)p.q + (int64_t)row * p.q_stride + (int64_t)head * p.head_dim + col, p.head_dim - col, q[i]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                query[pair][c] = pack2(q[0][c], q[1][c]);
+                o[pair][c] = 0;
+            }
+        }
+    }
+
+    // `count` of KEYS keys; key(j) and value(j): this lane's columns of the j-th (those beyond `count` are masked); weights: room for
+    // KEYS x 8 numbers of this warp.
+    template <int KEYS, typename Key, typename Value>
+    __device__ __forceinline__ void tile(float* weights, int count, float scale, Key key, Value value) {
+        constexpr int GROUPS = KEYS / kF32Aside, MINE = kF32Aside / kParts;
+        static_assert(kF32Rows * MINE == kLanes, "a score a lane");
+        const int lane = threadIdx.x & 31, mine = lane / kLanes;
+        // Exchanges without a choice: in round r a lane keeps the lower half of its sums and gives the upper away, as lanes whose number
+        // has bit r hold their keys (rounds of 8 and more) and query rows (below) with that bit turned over.
+        const int turned = (lane >> 3) & (MINE - 1);
         float score[GROUPS];
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            float k[kF32Aside][COLS], part[32];
+            float k[MINE][kCols];
+            uint64_t part[kLanes / 2];                            // pairs of rows, key by key
 #pragma unroll
-            for (int a = 0; a < kF32Aside; ++a) load_n(keys + places[g * kF32Aside + a], k[a]);
+            for (int a = 0; a < MINE; ++a) key(g * kF32Aside + mine * MINE + (a ^ turned), k[a]);
 #pragma unroll
-            for (int a = 0; a < kF32Aside; ++a)
+            for (int a = 0; a < MINE; ++a)
 #pragma unroll
-                for (int r = 0; r < kF32Rows; ++r) {
-                    float sum = query[r][0] * k[a][0];
+                for (int c = 0; c < kCols; ++c) {
+                    const uint64_t twice = pack2(k[a][c], k[a][c]);
 #pragma unroll
-                    for (int c = 1; c < COLS; ++c) sum = fmaf(query[r][c], k[a][c], sum);
-                    part[a * kF32Rows + r] = sum;
+                    for (int pair = 0; pair < kF32Rows / 2; ++pair) {
+                        uint64_t& sum = part[a * (kF32Rows / 2) + pair];
+                        sum = c == 0 ? mul2(query[pair][c], twice) : fma2(query[pair][c], twice, sum);
+                    }
                 }
-            // round o: a lane keeps the sums whose number has its bit o, and gives the others away
+            float lo, hi;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const bool upper = lane & o;
+            for (int r = kLanes / 2; r > 1; r >>= 1) {
 #pragma unroll
-                for (int i = 0; i < o; ++i) {
-                    const float mine = upper ? part[i + o] : part[i], other = upper ? part[i] : part[i + o];
-                    part[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+                for (int i = 0; i < r / 2; ++i) {
+                    unpack2(part[i + r / 2], lo, hi);
+                    part[i] = add2(part[i], pack2(__shfl_xor_sync(0xffffffffu, lo, r), __shfl_xor_sync(0xffffffffu, hi, r)));
                 }
             }
-            score[g] = part[0] * p.scale_log2;                    // of key g * 4 + lane / 8 and row lane % 8
+            unpack2(part[0], lo, hi);
+            score[g] = (lo + __shfl_xor_sync(0xffffffffu, hi, 1)) * scale;           // of key g * 4 + lane / 8 and row lane % 8
         }
         float high = kMasked;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            if (key0 + g * kF32Aside + lane / kF32Rows >= w.end) score[g] = -INFINITY;        // 2^(that - m) is 0
+            if (g * kF32Aside + lane / kF32Rows >= count) score[g] = -INFINITY;      // 2^(that - m) is 0
             high = fmaxf(high, score[g]);
         }
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
-        const float m_new = fmaxf(m, high), correction = exp2f(m - m_new);
-        m = m_new;
-        l *= correction;
+        const float m_new = fmaxf(m, high);
+        if (__any_sync(0xffffffffu, m_new != m)) {
+            const float correction = exp2f(m - m_new);
+            m = m_new;
+            l *= correction;
+#pragma unroll
+            for (int pair = 0; pair < kF32Rows / 2; ++pair) {
+                const uint64_t c_r = pack2(__shfl_sync(0xffffffffu, correction, pair * 2), __shfl_sync(0xffffffffu, correction, pair * 2 + 1));
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) o[pair][c] = mul2(o[pair][c], c_r);
+            }
+        }
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            const float weight = exp2f(score[g] - m_new);
+            const float weight = exp2f(score[g] - m);
             l += weight;
             weights[g * 32 + lane] = weight;
         }
-#pragma unroll
-        for (int r = 0; r < kF32Rows; ++r) {
-            const float c_r = __shfl_sync(0xffffffffu, correction, r);
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) o[r][c] *= c_r;
-        }
         __syncwarp();
-        const int count = min(kF32Keys, w.end - key0);
-#pragma unroll(COLS <= 2 ? 8 : 4)
-        for (int j = 0; j < count; ++j) {
-            float weight[kF32Rows], value[COLS];
-            load_n(values + places[j], value);
-            load_n(weights + j * kF32Rows, weight);
+#pragma unroll(kCols == 4 ? 8 : 2)
+        for (int j = mine; j < count; j += kParts) {
+            float v[kCols];
+            value(j, v);
+            const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(weights + j * kF32Rows);
+            const ulonglong2 w1 = *reinterpret_cast<const ulonglong2*>(weights + j * kF32Rows + 4);
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int r = 0; r < kF32Rows; ++r) o[r][c] = fmaf(weight[r], value[c], o[r][c]);
+            for (int c = 0; c < kCols; ++c) {
+                const uint64_t twice = pack2(v[c], v[c]);
+                o[0][c] = fma2(w0.x, twice, o[0][c]);
+                o[1][c] = fma2(w0.y, twice, o[1][c]);
+                o[2][c] = fma2(w1.x, twice, o[2][c]);
+                o[3][c] = fma2(w1.y, twice, o[3][c]);
+            }
         }
-        __syncwarp();
+        __syncwarp();                                             // (what has been read may be written again)
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 8);
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
+
+    // The lanes' shares of l together, and the parts' of o.
+    __device__ __forceinline__ void end() {
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+#pragma unroll
+        for (int r = kLanes; r < 32; r <<= 1)
+#pragma unroll
+            for (int pair = 0; pair < kF32Rows / 2; ++pair)
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) o[pair][c] = add2(o[pair][c], __shfl_xor_sync(0xffffffffu, o[pair][c], r));
+    }
+
+    __device__ __forceinline__ void store(int row, float* to, int left) const {      // row: known when this is compiled
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+            float v[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) unpack2(o[row / 2][c + i], v[i][0], v[i][1]);
+            if (c / 4 * kApart < left)
+                *reinterpret_cast<float4*>(to + c / 4 * kApart) = make_float4(v[0][row & 1], v[1][row & 1], v[2][row & 1], v[3][row & 1]);
+        }
+    }
+};
+
+// A tile of eight folded rows against a run of keys, whose tiles of 32 the four warps take in turns, straight from memory: for few
+// rows, where the latency of a load after the look-up before it is what a call waits for (8 beams at 1,111 keys of 32 heads of 64:
+// 13 us).  (A lane a key instead, its row read 16 bytes at a time: 131 us for 16 rows at 4,096 keys of 32 heads of 128 where this
+// took 67, bound by the cache lines that each load touches.)
+template <int D>
+__device__ void attend_f32(const SharedParams& p, const Work& w, float* smem) {
+    using Rows = RowsF32<D, kColsF32<D>>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int dim = p.head_dim, col = lane % Rows::kLanes * 4;
+    float* weights = smem + warp * (kF32Keys * kF32Rows);                            // [key][row] of this warp
+    int64_t* places = reinterpret_cast<int64_t*>(smem + kF32Warps * kF32Keys * kF32Rows) + warp * kF32Keys;    // where its keys lie
+    Rows rows;
+    rows.begin(p, w, w.first_folded, min(kF32Rows, w.folded - w.first_folded), col);
+    const int* table = p.table + (int64_t)w.row * p.table_stride;
+    const int64_t head_block = (int64_t)p.paging.size * dim;
+    const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block;
+    const float* keys = (const float*)p.cache + (int64_t)w.kv_head * head_block + col;
+    const float* values = keys + (int64_t)p.kv_heads * head_block;
+    for (int key0 = w.begin + warp * kF32Keys; key0 < w.end; key0 += kF32Warps * kF32Keys) {
+        const int key = min(key0 + lane, w.end - 1);              // (beyond the end: the last key once more, masked)
+        places[lane] = (int64_t)table[p.paging.page_of(key)] * page_block + (int64_t)p.paging.within(key) * dim;
+        __syncwarp();
+        rows.template tile<kF32Keys>(weights, w.end - key0 < kF32Keys ? w.end - key0 : kF32Keys, p.scale_log2,
+                                     [&](int j, float (&v)[Rows::kCols]) { Rows::load(keys + places[j], dim - col, v); },
+                                     [&](int j, float (&v)[Rows::kCols]) { Rows::load(values + places[j], dim - col, v); });
+    }
+    rows.end();
     __syncthreads();
     float* ml = smem;
     float* acc = ml + kF32Warps * kF32Rows * 2;
     if (lane < kF32Rows) {
-        ml[(warp * kF32Rows + lane) * 2] = m;
-        ml[(warp * kF32Rows + lane) * 2 + 1] = l;
+        ml[(warp * kF32Rows + lane) * 2] = rows.m;
+        ml[(warp * kF32Rows + lane) * 2 + 1] = rows.l;
     }
+    if (lane < Rows::kLanes) {
 #pragma unroll
-    for (int r = 0; r < kF32Rows; ++r) store_n(acc + (warp * kF32Rows + r) * D + col, o[r]);
+        for (int r = 0; r < kF32Rows; ++r) rows.store(r, acc + (warp * kF32Rows + r) * D + col, D);
+    }
     __syncthreads();
     leave_run<float, kF32Rows, D, kF32Warps>(p, w, ml, acc);
 }
 
 template <int D>
-__global__ void __launch_bounds__(kF32Warps * 32) shared_f32_kernel(const SharedParams p) {
+__global__ void __launch_bounds__(kF32Warps * 32, D <= 128 ? 4 : 2) shared_f32_kernel(const SharedParams p) {
     extern __shared__ __align__(128) float f32_smem[];
     pdl_wait();
     pdl_trigger();
     Work w;
-    if (find_work<kF32Rows>(p, blockIdx.x, w)) attend_f32<D>(p, w, f32_smem);
+    // (wide: the common parts are the next kernel's)
+    if (p.wide ? find_tail<kF32Rows>(p, blockIdx.x, w) : find_work<kF32Rows>(p, blockIdx.x, w)) attend_f32<D>(p, w, f32_smem);
     else if (p.direct) leave_nothing<float, kF32Rows>(p, w);
 }
 
@@ -1015,6 +1080,98 @@ constexpr size_t f32_bytes() {
     constexpr size_t tiles = (size_t)kF32Warps * kF32Keys * (kF32Rows + 2);      // weights, and where the keys lie
     constexpr size_t meet = (size_t)kF32Warps * kF32Rows * (2 + D);
     return (tiles > meet ? tiles : meet) * sizeof(float);
+}
+
+// Common parts of groups with more folded rows: four warps with eight rows each against the same keys and values, which go through
+// shared memory once for all of them, in asynchronous copies.  32 rows of 32 heads on 8 of 128 at 8,192 keys: 142 us, 4.3 GFLOP,
+// 30 TFLOP/s of some 74 that the multiply-adds have (353 us with tiles of eight rows).  Bound by instructions: of 62 for a key and
+// eight rows 32 are packed multiply-adds, which take the pipe two cycles each, 12 the exchanges, the rest loads and doubled operands;
+// with a choice between two sums in front of each exchange it took 162.
+constexpr int kWideRows = kF32Warps * kF32Rows;
+template <int D>
+constexpr int kWideKeys = D <= 128 ? 32 : 16;
+template <int D>
+constexpr int kWideStages = D == 64 ? 3 : 2;
+template <int D>
+constexpr size_t wide_bytes() {
+    return ((size_t)kWideStages<D> * 2 * kWideKeys<D> * D + (size_t)kF32Warps * kWideKeys<D> * kF32Rows) * sizeof(float);
+}
+
+template <int D>
+__device__ void attend_f32_wide(const SharedParams& p, const Work& w, float* smem) {
+    using Rows = RowsF32<D, kColsF32<D>>;
+    constexpr int KEYS = kWideKeys<D>, STAGES = kWideStages<D>, CH = D / 4, PASSES = KEYS * CH / (kF32Warps * 32);
+    constexpr int kTile = KEYS * D;                               // numbers of a tile of keys, or of values
+    static_assert(kBlock % KEYS == 0, "a common part ends with a tile: no key is masked");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int dim = p.head_dim, col = lane % Rows::kLanes * 4;
+    const int first = w.first_folded + warp * kF32Rows, here = min(kF32Rows, w.folded - first);     // (0 or less: none for this warp)
+    float* weights = smem + STAGES * 2 * kTile + warp * (KEYS * kF32Rows);
+    const int* table = p.table + (int64_t)w.row * p.table_stride;
+    const int64_t head_block = (int64_t)p.paging.size * dim;
+    const int64_t page_block = 2 * (int64_t)p.kv_heads * head_block, v_offset = (int64_t)p.kv_heads * head_block;
+    const float* base = (const float*)p.cache + (int64_t)w.kv_head * head_block;
+    const int tiles = (w.end - w.begin) / KEYS;
+    // a lane's key of a tile: its page is looked up one tile ahead of the copies
+    auto look_up = [&](int t) { return t < tiles && lane < KEYS ? table[p.paging.page_of(w.begin + t * KEYS + lane)] : 0; };
+    auto bring = [&](int t, int page) {
+        const int64_t place = (int64_t)page * page_block + (int64_t)p.paging.within(w.begin + t * KEYS + (lane < KEYS ? lane : 0)) * dim;
+        const uint32_t dst = smem_u32(smem + (t % STAGES) * 2 * kTile);
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+            const int idx = pass * (kF32Warps * 32) + (int)threadIdx.x, key = idx / CH, c = idx % CH;
+            const float* src = base + __shfl_sync(0xffffffffu, place, key) + c * 4;
+            const bool ok = c * 4 < dim;
+            cp_async16(dst + idx * 16, ok ? src : base, ok);
+            cp_async16(dst + kTile * 4 + idx * 16, ok ? src + v_offset : base, ok);
+        }
+    };
+    int page = look_up(0);
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) {
+        if (t < tiles) bring(t, page);
+        cp_async_commit();
+        page = look_up(t + 1);
+    }
+    Rows rows;
+    rows.begin(p, w, first, here, col);
+    for (int t = 0; t < tiles; ++t) {
+        cp_async_wait<STAGES - 2>();
+        __syncthreads();                                          // tile t is there, and nobody reads tile t - 1 any more
+        if (t + STAGES - 1 < tiles) {
+            bring(t + STAGES - 1, page);
+            page = look_up(t + STAGES);
+        }
+        cp_async_commit();
+        const float* keys = smem + (t % STAGES) * 2 * kTile + col;
+        if (here > 0)
+            rows.template tile<KEYS>(weights, KEYS, p.scale_log2, [&](int j, float (&v)[Rows::kCols]) { Rows::load(keys + j * D, D, v); },
+                                     [&](int j, float (&v)[Rows::kCols]) { Rows::load(keys + kTile + j * D, D, v); });
+    }
+    if (here <= 0) return;
+    rows.end();
+    int64_t slot = 0;
+    if (lane < here) {
+        int row, head;
+        place_of(p, w, first + lane, row, head);
+        slot = slot_of(p, row, head, w.part);
+        p.part_ml[slot] = make_float2(rows.m, rows.l);
+    }
+#pragma unroll
+    for (int r = 0; r < kF32Rows; ++r) {
+        const int64_t to = __shfl_sync(0xffffffffu, slot, r);
+        if (r < here && lane < Rows::kLanes) rows.store(r, p.part_a + to * dim + col, dim - col);
+    }
+}
+
+// (launched as shared_tc_kernel is)
+template <int D>
+__global__ void __launch_bounds__(kF32Warps * 32, D == 64 ? 4 : D == 128 ? 3 : 2) shared_f32_wide_kernel(const SharedParams p) {
+    extern __shared__ __align__(128) float f32_smem[];
+    pdl_trigger();
+    Work w;
+    if (find_common<kWideRows>(p, blockIdx.x, w)) attend_f32_wide<D>(p, w, f32_smem);
+    if (blockIdx.x == 0) pdl_wait();
 }
 
 // ------------------------------------------------------------------------------------------------ the runs put together
@@ -1169,11 +1326,14 @@ int launch_tc(const CUtensorMap& map, int64_t blocks, const SharedParams& p, cud
 
 }  // namespace
 
-// Folded rows of a tile: what `tiles` counts.  tensor: the form on the tcgen05 tensor cores.
-TB_EXPORT int tb_attention_shared_tile(int dtype, int tensor) { return dtype == TB_F32 ? kF32Rows : tensor ? kTcRows : kRows; }
+// Folded rows of a tile: what `tiles` counts.  wide: the form for groups of more folded rows.
+TB_EXPORT int tb_attention_shared_tile(int dtype, int wide) {
+    return dtype == TB_F32 ? (wide ? kWideRows : kF32Rows) : wide ? kTcRows : kRows;
+}
 
-// Whether that form takes these sizes.
-TB_EXPORT int tb_attention_shared_tensor(int dtype, int head_dim, int page_size) {
+// Whether that form takes these sizes (bfloat16: on the tcgen05 tensor cores).
+TB_EXPORT int tb_attention_shared_wide(int dtype, int head_dim, int page_size) {
+    if (dtype == TB_F32) return 1;
     return dtype == TB_BF16 && (head_dim == 64 || head_dim == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0;
 }
 
@@ -1187,7 +1347,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
                                   const int* group_start, const int* leader, const int* prefix, const int* common, int rows, int groups, int heads,
                                   int kv_heads, int head_dim, int page_size, float scale, int tiles, int prefix_parts,
                                   int prefix_run, int tail_parts, int tail_run, float* part_a, float* part_ml,
-                                  int64_t part_floats, int warps, int tensor, int cache_pages, int* error, int dtype, cudaStream_t stream) {
+                                  int64_t part_floats, int warps, int wide, int cache_pages, int* error, int dtype, cudaStream_t stream) {
     if (rows == 0) return 0;
     if (dtype != TB_F32 && dtype != TB_BF16) return TB_ERR_BAD_DTYPE;
     if (rows < 0 || groups < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || page_size < 1 || tiles < 0) return TB_ERR_BAD_SIZE;
@@ -1198,7 +1358,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
     const int64_t parts = prefix_parts == 0 && tail_parts == 1 ? 0 : (int64_t)rows * heads * (prefix_parts + tail_parts);
     if (parts > 0 && (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim)) return -5;
-    if (tensor && (!tb_attention_shared_tensor(dtype, head_dim, page_size) || error == nullptr)) return TB_ERR_BAD_SIZE;
+    if (wide && (!tb_attention_shared_wide(dtype, head_dim, page_size) || error == nullptr)) return TB_ERR_BAD_SIZE;
     SharedParams p;
     p.q = q;
     p.out = out;
@@ -1230,23 +1390,28 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.tail_run = tail_run;
     p.paging = tb_paging(page_size);
     p.scale_log2 = scale * kLog2e;
-    p.tensor = tensor;
+    p.wide = wide;
     p.direct = prefix_parts == 0 && tail_parts == 1;
     p.error = error;
     const int tile = dtype == TB_F32 ? kF32Rows : kRows;                 // of the parts behind
     const int64_t of_common = (int64_t)tiles * kv_heads * prefix_parts;
-    const int64_t blocks = (tensor ? 0 : of_common) + (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
+    const int64_t blocks = (wide ? 0 : of_common) + (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
     int status;
     if (dtype == TB_F32) {
         if (head_dim <= 64) status = launch(shared_f32_kernel<64>, blocks, kF32Warps * 32, f32_bytes<64>(), p, stream);
         else if (head_dim <= 128) status = launch(shared_f32_kernel<128>, blocks, kF32Warps * 32, f32_bytes<128>(), p, stream);
         else status = launch(shared_f32_kernel<256>, blocks, kF32Warps * 32, f32_bytes<256>(), p, stream);
+        if (status == 0 && wide && of_common > 0) {
+            if (head_dim <= 64) status = launch(shared_f32_wide_kernel<64>, of_common, kF32Warps * 32, wide_bytes<64>(), p, stream);
+            else if (head_dim <= 128) status = launch(shared_f32_wide_kernel<128>, of_common, kF32Warps * 32, wide_bytes<128>(), p, stream);
+            else status = launch(shared_f32_wide_kernel<256>, of_common, kF32Warps * 32, wide_bytes<256>(), p, stream);
+        }
     } else {
         if (head_dim <= 32) status = launch_mma<32>(warps, blocks, p, stream);
         else if (head_dim <= 64) status = launch_mma<64>(warps, blocks, p, stream);
         else if (head_dim <= 128) status = launch_mma<128>(warps, blocks, p, stream);
         else status = launch_mma<256>(warps, blocks, p, stream);
-        if (status == 0 && tensor && of_common > 0) {
+        if (status == 0 && wide && of_common > 0) {
             CUtensorMap map;
             if (!make_cache_map(&map, cache, cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
             status = head_dim == 64 ? launch_tc<64>(map, of_common, p, stream) : launch_tc<128>(map, of_common, p, stream);

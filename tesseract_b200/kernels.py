@@ -318,14 +318,14 @@ def attention_rows(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, posi
     return out
 
 
-def attention_shared_tensor(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
-    """Whether ``attention_shared`` has a form on the tcgen05 tensor cores for these sizes."""
-    return bool(load_library("attention_shared").tb_attention_shared_tensor(_i32(_code(dtype)), _i32(head_dim), _i32(page_size)))
+def attention_shared_wide(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    """Whether ``attention_shared`` has a form for groups of many folded rows (bfloat16: on the tcgen05 tensor cores) for these sizes."""
+    return bool(load_library("attention_shared").tb_attention_shared_wide(_i32(_code(dtype)), _i32(head_dim), _i32(page_size)))
 
 
-def attention_shared_tile(dtype: torch.dtype, tensor: bool = False) -> int:
+def attention_shared_tile(dtype: torch.dtype, wide: bool = False) -> int:
     """Folded rows (rows of a group times query heads per kv head) that a block of ``attention_shared`` takes."""
-    return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if tensor else 0))
+    return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if wide else 0))
 
 
 _ATTENTION_SHARED = (_pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32, *[_pointer] * 5, *[_i32] * 6, _f32,
@@ -359,7 +359,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
         q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
         block_table.stride(0), block_table.shape[1], *shared.addresses(), rows, shared.prefix.numel(), num_heads, num_kv_heads,
         head_dim, page_size, scale, choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, at,
-        at + 4 * parts * head_dim, parts * head_dim, choice.warps, choice.tensor, cache.shape[0],
+        at + 4 * parts * head_dim, parts * head_dim, choice.warps, choice.wide, cache.shape[0],
         _error_word(q.device).data_ptr(), _code(dtype), _raw_stream()), "attention_shared")
     return out
 

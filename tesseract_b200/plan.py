@@ -276,8 +276,8 @@ def attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim
 
 @dataclass(frozen=True)
 class SharedAttentionPlan:
-    """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows (``tensor``: of 128, on the tcgen05 tensor
-    cores), common parts in at most ``prefix_parts`` runs of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is
+    """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows (``wide``: larger tiles, in bfloat16 on
+    the tcgen05 tensor cores), common parts in at most ``prefix_parts`` runs of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is
     shared, every row reads its own keys), what lies behind in at most ``tail_parts`` of at least ``tail_run``."""
 
     tiles: int
@@ -285,7 +285,7 @@ class SharedAttentionPlan:
     prefix_run: int
     tail_parts: int
     tail_run: int
-    tensor: bool = False
+    wide: bool = False
     warps: int = 0           # of a block: 2, or (0) as many as let two blocks share a multiprocessor
 
 
@@ -302,10 +302,15 @@ SHARED_MIN_SAVED = 64
 # at 2,048 keys, 29 MB: 0.757 and 0.702 ms; 32 at 2,048, 130 MB: 0.992 and 1.068; 32 at 8,192, 520 MB: 1.136 and 1.931; of 8 layers
 # of the 8B sizes, 16 rows at 1,024, 63 MB: 1.058 and 1.050; 4 at 8,192, 101 MB: 0.975 and 1.013; 32 at 8,192: 1.179 and 2.105).
 SHARED_MIN_BYTES = 96 << 20
-# Tiles of 16 folded rows times blocks of common keys from where on the tensor cores' form is faster, whose launch takes 10 us (32
-# heads on 8, device time with and without: 64 rows at 2,048 keys of 64 11.1 and 11.6 us, at 8,192 15.9 and 18.9, 128 rows at
-# 16,384 24.4 and 44.2; of 128, 32 rows at 1,024 11.6 and 11.3, 64 at 2,048 13.1 and 19.0, 128 at 16,384 34.8 and 91.8).
-SHARED_TENSOR_MIN = {64: 128, 128: 48}
+# Tiles of 16 folded rows times blocks of common keys from where on the form with the larger tiles is faster, by head size (32 heads
+# on 8 unless it says otherwise, device time with the small tiles and with the large).  bfloat16, whose launch takes 10 us: 64 rows at
+# 2,048 keys of 64 11.1 and 11.6 us, at 8,192 15.9 and 18.9 the other way, 128 rows at 16,384 44.2 and 24.4; of 128, 32 rows at 1,024
+# 11.3 and 11.6, 64 at 2,048 19.0 and 13.1, 128 at 16,384 91.8 and 34.8.  32 bits: 4 rows at 2,048 keys of 64 12.1 and 13.8, 8 16.6
+# and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 heads on 2 of 256, 8 rows at 8,192 keys 32.7 and
+# 34.9, 32 at 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
+SHARED_WIDE_MIN = {torch.bfloat16: {64: 128, 128: 48}, torch.float32: {64: 48, 128: 48, 256: 192}}
+# Blocks of threads of the 32-bit form that share a multiprocessor, small tiles and large, by the head size that they are made for.
+SHARED_F32_RESIDENT = {False: {64: 4, 128: 4, 256: 2}, True: {64: 4, 128: 3, 256: 2}}
 
 
 def saved_blocks(sizes: Sequence[int], blocks: Sequence[int]) -> int:
@@ -350,29 +355,33 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
         blocks = np.zeros_like(blocks)
     rows = np.where(blocks > 0, sizes * fold, 0)
     work = int((-(-rows // 16) * blocks).sum())
-    tensor = work > SHARED_TENSOR_MIN.get(head_dim, 0) and kernels.attention_shared_tensor(dtype, head_dim, page_size)
-    tile = kernels.attention_shared_tile(dtype, tensor)
+    padded = 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256            # (a kernel's head size, in 32 bits)
+    wide = work > SHARED_WIDE_MIN[dtype].get(padded, 0) and kernels.attention_shared_wide(dtype, head_dim, page_size)
+    tile = kernels.attention_shared_tile(dtype, wide)
     tiles = -(-rows // tile)
-    # large blocks of threads that are resident at once, a kv head (those of the 32-bit form are half as large)
-    target = max(1, (4 if dtype == torch.float32 and head_dim <= 128 else 2) * sms // num_kv_heads)
+    # (large) blocks of threads that are resident at once, a kv head
+    target = max(1, (SHARED_F32_RESIDENT[False][padded] if dtype == torch.float32 else 2) * sms // num_kv_heads)
     # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
     # are many
     tails = np.maximum(tails, 1)
     tail_tiles = np.full(tails.shape, -(-fold // kernels.attention_shared_tile(dtype)))
     warps = 2 if dtype != torch.float32 and int(tail_tiles.sum()) > target else 0
     small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
+    shortest = 1 if wide and dtype == torch.float32 else SHARED_MIN_RUN[dtype]
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
     prefix_parts, prefix_run = 0, 1
     if tiles.any():
         room = target
-        if not tensor and warps == 0:           # (in one launch with the rows' own)
+        if not wide and warps == 0:             # (in one launch with the rows' own)
             room = max(target // 2, target - int((tail_tiles * -(-tails // tail_run)).sum()))
-        prefix_run = _shared_runs(tiles, blocks, room, SHARED_MIN_RUN[dtype])
+        elif dtype == torch.float32:
+            room = max(1, SHARED_F32_RESIDENT[True][padded] * sms // num_kv_heads)
+        prefix_run = _shared_runs(tiles, blocks, room, shortest)
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles)
     count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + int((blocks > 0).sum())
-    return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, tensor, warps)
+    return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, wide, warps)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,

@@ -172,16 +172,18 @@ def test_any_cut_gives_the_same_numbers(dtype):
     assert torch.equal(case.run(more), case.run(base))
 
 
-@pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("rows", [4, 5, 8, 9, 16, 24, 33, 70])
-def test_both_forms_in_bfloat16(rows, dim):
-    """The tensor cores' form (tiles of 128 folded rows) and the one of 16, at every count of rows, whichever the plan takes."""
-    case = Case([(1030, [1031 + 7 * i % 90 for i in range(rows)]), (192, [200, 250])], 8, 2, dim, seed=rows)
-    for tensor in (False, True):
-        tile = kernels.attention_shared_tile(torch.bfloat16, tensor)
-        tiles = sum(-(-n * 4 // tile) for n in (rows, 2))
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 16), (torch.float32, 64),
+                                        (torch.float32, 80), (torch.float32, 128), (torch.float32, 208), (torch.float32, 256)])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 8, 9, 16, 24, 33, 70])
+def test_both_forms(rows, dtype, dim):
+    """The form with the larger tiles (in bfloat16 the tensor cores') and the other, at every count of rows, whichever the plan takes."""
+    case = Case([(1030, [1031 + 7 * i % 90 for i in range(rows)]), (192, [200, 250])], 8, 2, dim, dtype=dtype, seed=rows)
+    alone = rows == 1                                # (a row alone has nothing in common with another)
+    for wide in (False, True):
+        tile = kernels.attention_shared_tile(dtype, wide)
+        tiles = sum(-(-n * 4 // tile) for n in ((2,) if alone else (rows, 2)))
         for parts, run, warps in ((1, 1, 0), (5, 2, 2)):
-            case.check(plan.SharedAttentionPlan(tiles, parts, run, 2, 1, tensor, warps))
+            case.check(plan.SharedAttentionPlan(tiles, parts, run, 2, 1, wide, warps))
     assert kernels.tcgen05_error() == 0
 
 

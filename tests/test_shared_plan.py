@@ -37,17 +37,18 @@ def test_runs_cover_every_key_and_fit_the_chip(groups, dim, dtype):
     fold, kv_heads = 4, 8
     assert 1 <= choice.tail_parts <= plan.SHARED_MAX_PARTS and 0 <= choice.prefix_parts <= plan.SHARED_MAX_PARTS
     if choice.prefix_parts == 0:
-        assert choice.tiles == 0 and not choice.tensor
+        assert choice.tiles == 0 and not choice.wide
         assert plan.saved_blocks(shared.sizes, shared.blocks) < plan.SHARED_MIN_SAVED
     else:
-        tile = kernels.attention_shared_tile(dtype, choice.tensor)
+        tile = kernels.attention_shared_tile(dtype, choice.wide)
         assert choice.tiles == sum(-(-n * fold // tile) for n, b in zip(shared.sizes, shared.blocks) if b)
         runs = [(-(-n * fold // tile), -(-b // choice.prefix_run)) for n, b in zip(shared.sizes, shared.blocks) if b]
         assert choice.prefix_parts == min(plan.SHARED_MAX_PARTS, max(r for _, r in runs))
         # at most what is resident at once, unless every tile is one run already
         assert sum(t * r for t, r in runs) * kv_heads <= 4 * SMS or max(r for _, r in runs) == 1
-        assert choice.tensor == (dtype == torch.bfloat16 and dim in (64, 128) and
-                                 sum(-(-n * fold // 16) * b for n, b in zip(shared.sizes, shared.blocks)) > plan.SHARED_TENSOR_MIN[dim])
+        least = plan.SHARED_WIDE_MIN[dtype].get(64 if dim <= 64 else 128 if dim <= 128 else 256, 0)
+        assert choice.wide == ((dtype == torch.float32 or dim in (64, 128)) and
+                               sum(-(-n * fold // 16) * b for n, b in zip(shared.sizes, shared.blocks)) > least)
 
 
 def test_what_is_shared_and_what_not():
@@ -62,7 +63,7 @@ def test_what_is_shared_and_what_not():
 def test_a_captured_plan_has_tiles_for_every_grouping_of_as_many_groups():
     for room in (8, 16, 32):
         _, choice = choose([(4096, [4200] * (room // 2)), (2048, [2100] * (room - room // 2))], room=room)
-        tile = kernels.attention_shared_tile(torch.bfloat16, choice.tensor)
+        tile = kernels.attention_shared_tile(torch.bfloat16, choice.wide)
         for first in range(0, room + 1):
             assert choice.tiles >= -(-first * 4 // tile) + -(-(room - first) * 4 // tile)
 
