@@ -18,7 +18,7 @@ import torch
 from .. import kernels
 from ..sampling.sampler import InvalidLogits
 from .scheduler import FINISH_LENGTH, FINISH_STOP, RequestRejected
-from .step import StepEntry, Stepper
+from .step import StepEntry, StepError, Stepper
 
 
 @dataclass
@@ -255,6 +255,8 @@ def score(stepper: Stepper, sequence: Sequence[int], alternatives: int = 0, port
     sequence = [int(t) for t in sequence]
     if not sequence:
         raise RequestRejected("the sequence is empty")
+    if not 0 <= sequence[-1] < stepper.vocab_size:                   # (which no step runs)
+        raise StepError(f"token id {sequence[-1]} is outside the vocabulary of {stepper.vocab_size}")
     if len(sequence) > stepper.max_positions:
         raise RequestRejected(f"the sequence has {len(sequence)} tokens, the model {stepper.max_positions} positions")
     request = ("score", id(sequence))

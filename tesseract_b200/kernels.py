@@ -178,7 +178,8 @@ def copy_pages(moves) -> None:
 
     A store is a contiguous tensor ``[entries, pages, ...]`` of any type (cache pages, or state slots); ``sources`` and
     ``targets`` are host lists or arrays of page indices.  No target may be named twice or be a source of the same store; a
-    call that breaks this, or names a page outside a store, raises :class:`KernelError` and copies nothing.  The indices
+    call that breaks this, names a page outside a store, or takes stores that lie on each other raises :class:`KernelError` and copies
+    nothing.  The indices
     travel in the launch: nothing has to outlive the call."""
     global launch_count
     header, indices, device = [], [], -1
@@ -198,8 +199,9 @@ def copy_pages(moves) -> None:
         header += (store.data_ptr(), entries, pages, numbers // (entries * pages) * store.element_size() if numbers else 0, source.size)
         indices += (source.tobytes(), target.tobytes())
     if len(moves) > 1:
-        addresses = [a for a in header[::5] if a]
-        _need(len(set(addresses)) == len(addresses), "copy_pages takes a store once a call")
+        # (moves of stores that lie on each other would have no order)
+        spans = sorted((header[i], header[i] + header[i + 1] * header[i + 2] * header[i + 3]) for i in range(0, len(header), 5) if header[i])
+        _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "copy_pages takes a store once a call, and none that lies on another")
     if not header:
         return
     done = _entry("copy_pages", "tb_copy_pages", _COPY_PAGES)(

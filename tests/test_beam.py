@@ -10,7 +10,7 @@ import torch
 
 import tesseract_b200.parts  # noqa: F401
 from tesseract_b200.cache import CacheManager
-from tesseract_b200.engine.beam import BeamSearch, TokenScores
+from tesseract_b200.engine.beam import BeamSearch, TokenScores, score
 from tesseract_b200.engine.scheduler import RequestRejected
 from tesseract_b200.parts import PagedKVNeed, StateNeed
 from tesseract_b200.sampling import InvalidLogits
@@ -144,6 +144,14 @@ def test_refusals():
     with pytest.raises(RequestRejected, match="no room"):
         HostSearch(stepper, 2, 20).run([[1] * 8])
     assert stepper.cache.slots.free_slots == 3
+
+
+@pytest.mark.parametrize("sequence", [[], [1, 2, VOCAB], [1, 2, -1], [VOCAB], [1] * 51])
+def test_scoring_refuses_what_no_step_would_run(sequence):
+    stepper = FakeStepper(max_positions=50)
+    with pytest.raises((RequestRejected, ValueError)):
+        score(stepper, sequence)
+    assert stepper.cache.used_pages() == 0 and stepper.cache.slots.free_slots == 16 and not stepper.rows
 
 
 def test_logits_without_a_probability_fail_and_leave_nothing_behind():

@@ -124,5 +124,9 @@ def test_refuses_what_is_not_a_store():
             kernels.copy_pages([(bad, [0], [1])])
     with pytest.raises(kernels.KernelError, match="once"):
         kernels.copy_pages([(store, [0], [1]), (store, [2], [3])])
+    with pytest.raises(kernels.KernelError, match="once"):
+        kernels.copy_pages([(store[1:], [0], [1]), (store[:3], [2], [3])])
+    kernels.copy_pages([(store[2:], [0], [1]), (store[:2], [2], [3])])        # side by side
+    assert torch.equal(store[2:, 1], store[2:, 0]) and torch.equal(store[:2, 3], store[:2, 2])
     with pytest.raises(kernels.KernelError, match="host"):
         kernels.copy_pages([(store, torch.tensor([0], device="cuda"), [1])])
