@@ -471,17 +471,18 @@ constexpr size_t mma_bytes() {
 // Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products for the
 // scores and one lane of warp 6 those with the values; warp 5 brings keys and values, page by page, with cp.async.bulk.tensor into
 // rings of their own.  All waits are bounded.
-// 64 rows, 32 heads on 8 of 128, 32,768 keys in common: 50.6 us with the join behind it (134 MB, 20.8 us at the measured copy rate;
-// 34 GFLOP, 20.2 us at the measured matrix rate).  Two blocks of 128 rows a multiprocessor read the same keys (L2 hit rate 46 %), and
-// the chain of a block of keys bounds it: scores, their way to registers, maximum, weights, their way back, product; counters show
-// the tensor pipe at 38 %, the special-function pipe at 38 % and the issue slots at 32 %.  Two tiles in one block of threads with
-// 512 columns took 68.1 us, two threads a row 1.3 us longer than one, both products' issue by one lane 53.3; products with the
-// values by a warp of their own cost head size 64 something (64 rows, 65,536 keys: 68.0 us, 66.5 with one lane).
+// 64 rows, 32 heads on 8 of 128, 32,768 keys in common: 49.5 us with the join behind it (134 MB, 20.8 us at the measured copy rate;
+// 34 GFLOP, 20.2 us at the measured matrix rate).  A block of 64 keys takes a softmax warp some 2,080 cycles, two blocks of threads a
+// multiprocessor: 1,050 for the weights (both blocks' exponentials are 1,024 of the special-function unit), 570 waiting for scores
+// (two tiles read the same keys through L2, 8.6 TB/s), 160 for a buffer of weights, the rest on the way to and from tensor memory.
+// Tried: two tiles in one block of threads with 512 columns (68.1 us), two threads a row (1.3 longer), both products' issue by one lane
+// (53.3), a part of the exponentials on the multiply-add pipe (51.7; head size 64 71 instead of 66), queries in tensor memory (no
+// change; with the weights in the scores' place, as head size 128 needs then, 56.7), all keys found in L2 (47.7).
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 224;
 constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
 template <int D>
-constexpr int kTcStages = D == 64 ? 4 : 2;    // 64 KB of keys and values under way either way
+constexpr int kTcStages = D == 64 ? 4 : 2;    // of the keys' ring and of the values'; 64 KB under way either way (a third for keys of 128 changes nothing)
 template <int D>
 struct TcShape {
     static constexpr uint32_t kSlice = kBlock * 128;              // 64 keys x 64 numbers
@@ -578,21 +579,16 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     const int live_threads = (rows + 31) / 32 * 32;               // of the softmax warps: those with a row
     const int n_blocks = (w.end - w.begin) / kBlock;
     const int* table = p.table + (int64_t)w.row * p.table_stride;
-    const uint32_t q_tile = smem_u32(smem), ring = q_tile + Tiles::kQBytes;      // [stage][K | V]
-    const uint32_t k_full = smem_u32(&bars[0]), k_empty = smem_u32(&bars[STAGES]);
-    const uint32_t v_full = smem_u32(&bars[2 * STAGES]), v_empty = smem_u32(&bars[3 * STAGES]);
-    const uint32_t s_full = smem_u32(&bars[4 * STAGES]), s_free = s_full + 8;
+    const uint32_t q_tile = smem_u32(smem), key_tiles = q_tile + Tiles::kQBytes, value_tiles = key_tiles + STAGES * kBlockBytes;
+    const uint32_t k_full = smem_u32(&bars[0]), k_empty = k_full + 8 * STAGES;
+    const uint32_t v_full = k_empty + 8 * STAGES, v_empty = v_full + 8 * STAGES;
+    const uint32_t s_full = v_empty + 8 * STAGES, s_free = s_full + 8;
     auto p_ready = [&](int j) { return s_full + 16 + 8 * (j & 1); };
     auto o_full = [&](int j) { return s_full + 32 + 8 * (j & 1); };
     auto phase = [&](int j) { return (uint32_t)(j >> 1) & 1u; };
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(k_full + 8 * s, 1);
-            mbar_init(k_empty + 8 * s, 1);
-            mbar_init(v_full + 8 * s, 1);
-            mbar_init(v_empty + 8 * s, 1);
-        }
+        for (int s = 0; s < 4 * STAGES; ++s) mbar_init(k_full + 8 * s, 1);
         mbar_init(s_full, 1);
         mbar_init(s_free, live_threads);
         for (int b = 0; b < 2; ++b) {
@@ -608,9 +604,9 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     }
     // where a thread's query lies, and the page of a lane's keys in the first block: looked up while the rest is set up
     const int rows_per_copy = min(p.paging.size, kBlock), copies = kBlock / rows_per_copy;          // keys and copies of a block: at most 8
-    int row = 0, head = 0, next_page = 0;
+    int row = 0, head = 0, first_page = 0;
     if (threadIdx.x < rows) place_of(p, w, w.first_folded + threadIdx.x, row, head);
-    if (warp == 5 && lane < copies) next_page = table[p.paging.page_of(w.begin + lane * rows_per_copy)];
+    if (warp == 5 && lane < copies) first_page = table[p.paging.page_of(w.begin + lane * rows_per_copy)];
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -631,49 +627,58 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     const uint32_t tmem_base = tmem_base_slot;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + kBlock;
     auto tmem_p = [&](int j) { return tmem_o + D + (j & 1) * (kBlock / 2); };
-    constexpr uint32_t kStageStep = (2 * kBlockBytes) >> 4;       // a ring stage further, in the units of a descriptor's address
+    constexpr uint32_t kStageStep = kBlockBytes >> 4;       // a ring stage further, in the units of a descriptor's address
 
     if (warp == 5) {
         bool ok = true;
-        int asked[2] = {0, 0};                                    // blocks of keys, and of values, that copies were issued for
-        for (int it = 0; it < n_blocks && ok; ++it) {
+        int asked_keys = 0, asked_values = 0;                     // blocks that copies were issued for
+        // block `it` of keys (or values) into its slot, from the pages that the lanes' keys lie in
+        auto bring = [&](int it, int page, uint32_t full, uint32_t empty, uint32_t tiles, int which, int& asked) {
             const int s = it % STAGES;
-            const int key = w.begin + it * kBlock + lane * rows_per_copy, page = next_page;
-            const int in_page = p.paging.within(key);
-            if (lane < copies && it + 1 < n_blocks) next_page = table[p.paging.page_of(key + kBlock)];
-            const uint32_t dst = ring + s * 2 * kBlockBytes + (uint32_t)(lane * rows_per_copy) * 128;
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                const uint32_t full = (which ? v_full : k_full) + 8 * s, empty = (which ? v_empty : k_empty) + 8 * s;
-                int go = 1;
-                if (lane == 0) {
-                    go = mbar_wait(empty, ((it / STAGES) & 1) ^ 1, &abort_flag) ? 1 : 0;
-                    if (go) mbar_expect_tx(full, kBlockBytes);
-                }
-                go = __shfl_sync(0xffffffffu, go, 0);             // also orders the announcement before the copies
-                if (!go) { ok = false; break; }
-                if (lane < copies) {
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-                        tma_load_kv(dst + which * kBlockBytes + h * kSlice, cache_map, full, h * 64, in_page, w.kv_head, which, page);
-                }
-                ++asked[which];
+            int go = 1;
+            if (lane == 0) {
+                go = mbar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, &abort_flag) ? 1 : 0;
+                if (go) mbar_expect_tx(full + 8 * s, kBlockBytes);
             }
+            go = __shfl_sync(0xffffffffu, go, 0);                 // also orders the announcement before the copies
+            if (!go) return false;
+            if (lane < copies) {
+                const uint32_t dst = tiles + s * kBlockBytes + (uint32_t)(lane * rows_per_copy) * 128;
+                const int in_page = p.paging.within(w.begin + it * kBlock + lane * rows_per_copy);
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h)
+                    tma_load_kv(dst + h * kSlice, cache_map, full + 8 * s, h * 64, in_page, w.kv_head, which, page);
+            }
+            ++asked;
+            return true;
+        };
+        // Keys go one block ahead of values: they are asked for that much earlier,
+        // and pages are looked up one block ahead of that.
+        auto look_up = [&](int it) {
+            return lane < copies && it < n_blocks ? table[p.paging.page_of(w.begin + it * kBlock + lane * rows_per_copy)] : 0;
+        };
+        int page = first_page, next_page = look_up(1);
+        ok = bring(0, page, k_full, k_empty, key_tiles, 0, asked_keys);
+        for (int it = 0; it < n_blocks && ok; ++it) {
+            const int behind = look_up(it + 2);
+            if (it + 1 < n_blocks) ok = bring(it + 1, next_page, k_full, k_empty, key_tiles, 0, asked_keys);
+            ok = ok && bring(it, page, v_full, v_empty, value_tiles, 1, asked_values);
+            page = next_page;
+            next_page = behind;
         }
         if (!ok && lane == 0) {
             abort_flag = 1;
             atomicExch(p.error, 110);
         }
         if (!ok || abort_flag) {                                  // (no copy lands in a block that has left)
-            for (int which = 0; which < 2; ++which)
-                for (int it = max(0, asked[which] - STAGES); it < asked[which]; ++it)
-                    settle((which ? v_full : k_full) + 8 * (it % STAGES), (it / STAGES) & 1);
+            for (int it = max(0, asked_keys - STAGES); it < asked_keys; ++it) settle(k_full + 8 * (it % STAGES), (it / STAGES) & 1);
+            for (int it = max(0, asked_values - STAGES); it < asked_values; ++it) settle(v_full + 8 * (it % STAGES), (it / STAGES) & 1);
         }
     } else if (warp == 4) {
         if (lane == 0) {
             constexpr uint32_t idesc_qk = idesc_bf16(kTcRows, kBlock, 0);
             // (descriptors are moved by adding to their start-address field, bytes >> 4)
-            const uint64_t q_desc = desc_sw128(q_tile, 1), k_desc0 = desc_sw128(ring, 1);
+            const uint64_t q_desc = desc_sw128(q_tile, 1), k_desc0 = desc_sw128(key_tiles, 1);
             int s = 0;
             uint32_t parity = 0;
             bool ok = true;
@@ -701,7 +706,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     } else if (warp == 6) {
         if (lane == 0) {
             constexpr uint32_t idesc_pv = idesc_bf16(kTcRows, D, 1);
-            const uint64_t v_desc0 = desc_sw128(ring + kBlockBytes, kSlice >> 4);
+            const uint64_t v_desc0 = desc_sw128(value_tiles, kSlice >> 4);
             int s = 0;
             uint32_t parity = 0;
             bool ok = true;
@@ -728,8 +733,8 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         const int r = warp * 32 + lane;                           // row of the tile = lane of tensor memory
         const int64_t slot = slot_of(p, row, head, w.part);
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-        // m: the maximum that the stored weights and O are scaled by; it is raised (and O rescaled) only when a block's exceeds it by
-        // more than 2^8, which keeps every weight at or below 256 and makes the rescaling rare
+        // m: the maximum that the stored weights and O are scaled by; it is raised (and O rescaled) only when a block's weights leave
+        // their range, which is rare
         float m = kMasked, l = 0.0f;
         bool ok = true;
         // what P_j V_j read and wrote in tensor memory may be touched by this thread again (the fence orders it, the barrier alone does not)
@@ -748,14 +753,35 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
             tmem_wait_ld();
             tc_fence_before();
             mbar_arrive(s_free);                                  // S is in registers: the next block's scores may be computed
-            float mx[4] = {kMasked, kMasked, kMasked, kMasked};
+            // The weights against the maximum so far, whose block's sum shows whether that is still near enough: a weight above 2^16
+            // cannot hide in it, and up to there neither the weights in bfloat16 nor the sums in 32 bits lose anything.  Only
+            // otherwise, and in the first block, is the block's maximum looked for and are the weights taken (again) against that.
+            uint32_t weights[32];
+            float block_sum = 0.0f;
+            auto weigh = [&]() {
+                const uint64_t neg_m2 = pack2(-m, -m);
+                uint64_t ls[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(sc[0][i]), __uint_as_float(sc[0][i + 1]));
-                mx[2 + ((i >> 1) & 1)] = max3(mx[2 + ((i >> 1) & 1)], __uint_as_float(sc[1][i]), __uint_as_float(sc[1][i + 1]));
-            }
-            const float block_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-            if (__any_sync(0xffffffffu, block_max > m + 8.0f)) {
+                for (int i = 0; i < 64; i += 2) {
+                    float t0, t1;
+                    unpack2(fma2(pack2(__uint_as_float(sc[i >> 5][i & 31]), __uint_as_float(sc[i >> 5][(i & 31) + 1])), scale2, neg_m2), t0, t1);
+                    const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
+                    ls[(i >> 1) & 3] = add2(ls[(i >> 1) & 3], pack2(p0, p1));
+                    weights[i >> 1] = pack_bf16(p0, p1);
+                }
+                float lo, hi;
+                unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), lo, hi);
+                block_sum = lo + hi;
+            };
+            if (j > 0) weigh();
+            if (j == 0 || __any_sync(0xffffffffu, block_sum > 65536.0f)) {
+                float mx[4] = {kMasked, kMasked, kMasked, kMasked};
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(sc[0][i]), __uint_as_float(sc[0][i + 1]));
+                    mx[2 + ((i >> 1) & 1)] = max3(mx[2 + ((i >> 1) & 1)], __uint_as_float(sc[1][i]), __uint_as_float(sc[1][i + 1]));
+                }
+                const float block_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
                 if (j > 0 && !product_done(j - 1)) { ok = false; break; }
                 const float m_new = fmaxf(m, block_max), correction = fast_exp2(m - m_new);
                 m = m_new;
@@ -775,26 +801,12 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                         tmem_store_16(tmem_o + lane_base + c * 16, v);
                     }
                 }
+                weigh();
             }
-            const uint64_t neg_m2 = pack2(-m, -m);
-            uint64_t ls[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float t0, t1;
-                    unpack2(fma2(pack2(__uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1])), scale2, neg_m2), t0, t1);
-                    const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
-                    ls[(i >> 1) & 3] = add2(ls[(i >> 1) & 3], pack2(p0, p1));
-                    sc[c][i >> 1] = pack_bf16(p0, p1);
-                }
-                if (c == 0 && j >= 2 && !product_done(j - 2)) { ok = false; break; }      // it has read this buffer
-                tmem_store_16(tmem_p(j) + lane_base + c * 16, sc[c]);
-            }
-            if (!ok) break;
-            float lo_sum, hi_sum;
-            unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), lo_sum, hi_sum);
-            l += lo_sum + hi_sum;
+            if (j >= 2 && !product_done(j - 2)) { ok = false; break; }               // it has read this buffer
+            tmem_store_16(tmem_p(j) + lane_base, weights);
+            tmem_store_16(tmem_p(j) + lane_base + 16, weights + 16);
+            l += block_sum;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(p_ready(j));
