@@ -22,6 +22,7 @@
 // Which form and how many runs: plan.shared_attention, with both sides' times beside its rule.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
+#include <cstring>
 #include <new>
 #include <set>
 
@@ -1354,40 +1355,57 @@ TB_EXPORT int tb_attention_shared_wide(int dtype, int head_dim, int page_size) {
 // ceil(rows of the group * heads / kv_heads / tile) each, no fewer.  prefix[g] is at most positions[b] + 1 for the rows of the group.
 // part_a, part_ml: rows * heads * (prefix_parts + tail_parts) * (head_dim and 2) floats; none where nothing is in common and every
 // row is one run.
-TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* cache,
-                                  const int* positions, const int* table, int table_stride, int table_columns, const int* members,
-                                  const int* group_start, const int* leader, const int* prefix, const int* common, int rows, int groups, int heads,
-                                  int kv_heads, int head_dim, int page_size, float scale, int tiles, int prefix_parts,
-                                  int prefix_run, int tail_parts, int tail_run, float* part_a, float* part_ml,
-                                  int64_t part_floats, int warps, int wide, int cache_pages, int* error, int dtype, cudaStream_t stream) {
+// The arguments come as one run of bytes (as declared here, nothing between them): a call of so many cost the host 3 us more.
+struct SharedCall {
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    const void* cache;
+    const int *positions, *table, *members, *group_start, *leader, *prefix, *common;
+    float *part_a, *part_ml;
+    int64_t part_floats;
+    int* error;
+    int table_stride, table_columns, rows, groups, heads, kv_heads, head_dim, page_size;
+    int tiles, prefix_parts, prefix_run, tail_parts, tail_run, warps, wide, cache_pages, dtype;
+    float scale;
+};
+static_assert(sizeof(SharedCall) == 16 * 8 + 18 * 4, "nothing between the arguments");
+
+TB_EXPORT int tb_attention_shared(const void* packed, cudaStream_t stream) {
+    SharedCall call;
+    memcpy(&call, packed, sizeof(call));
+    const int rows = call.rows, groups = call.groups, heads = call.heads, kv_heads = call.kv_heads, head_dim = call.head_dim;
+    const int page_size = call.page_size, tiles = call.tiles, prefix_parts = call.prefix_parts, tail_parts = call.tail_parts;
+    const int warps = call.warps, wide = call.wide, dtype = call.dtype;
     if (rows == 0) return 0;
     if (dtype != TB_F32 && dtype != TB_BF16) return TB_ERR_BAD_DTYPE;
     if (rows < 0 || groups < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || page_size < 1 || tiles < 0) return TB_ERR_BAD_SIZE;
     if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0) return TB_ERR_BAD_SIZE;
-    if (prefix_parts < 0 || tail_parts < 1 || prefix_parts + tail_parts > kMaxParts || prefix_run < 1 || tail_run < 1) return TB_ERR_BAD_SIZE;
+    if (prefix_parts < 0 || tail_parts < 1 || prefix_parts + tail_parts > kMaxParts || call.prefix_run < 1 || call.tail_run < 1) return TB_ERR_BAD_SIZE;
     const int element = dtype == TB_F32 ? 4 : 2;
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)part_a) % 16 != 0) return TB_ERR_BAD_ALIGN;
-    if ((q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
+    if (((uintptr_t)call.q | (uintptr_t)call.out | (uintptr_t)call.cache | (uintptr_t)call.part_a) % 16 != 0) return TB_ERR_BAD_ALIGN;
+    if ((call.q_stride * element) % 16 != 0) return TB_ERR_BAD_ALIGN;
     const int64_t parts = prefix_parts == 0 && tail_parts == 1 ? 0 : (int64_t)rows * heads * (prefix_parts + tail_parts);
-    if (parts > 0 && (part_a == nullptr || part_ml == nullptr || part_floats < parts * head_dim)) return -5;
-    if (wide && (!tb_attention_shared_wide(dtype, head_dim, page_size) || error == nullptr)) return TB_ERR_BAD_SIZE;
+    if (parts > 0 && (call.part_a == nullptr || call.part_ml == nullptr || call.part_floats < parts * head_dim)) return -5;
+    if (wide && (!tb_attention_shared_wide(dtype, head_dim, page_size) || call.error == nullptr)) return TB_ERR_BAD_SIZE;
     SharedParams p;
-    p.q = q;
-    p.out = out;
-    p.cache = cache;
-    p.positions = positions;
-    p.table = table;
-    p.members = members;
-    p.group_start = group_start;
-    p.leader = leader;
-    p.prefix = prefix;
-    p.common = common;
-    p.part_a = part_a;
-    p.part_ml = (float2*)part_ml;
-    p.q_stride = q_stride;
-    p.out_stride = out_stride;
-    p.table_stride = table_stride;
-    const int64_t keys = (int64_t)table_columns * page_size;
+    p.q = call.q;
+    p.out = call.out;
+    p.cache = call.cache;
+    p.positions = call.positions;
+    p.table = call.table;
+    p.members = call.members;
+    p.group_start = call.group_start;
+    p.leader = call.leader;
+    p.prefix = call.prefix;
+    p.common = call.common;
+    p.part_a = call.part_a;
+    p.part_ml = (float2*)call.part_ml;
+    p.q_stride = call.q_stride;
+    p.out_stride = call.out_stride;
+    p.table_stride = call.table_stride;
+    const int64_t keys = (int64_t)call.table_columns * page_size;
     p.table_keys = (int)(keys < 0x7fffff00 ? keys : 0x7fffff00);
     p.rows = rows;
     p.groups = groups;
@@ -1397,14 +1415,14 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
     p.head_dim = head_dim;
     p.tiles = tiles;
     p.prefix_parts = prefix_parts;
-    p.prefix_run = prefix_run;
+    p.prefix_run = call.prefix_run;
     p.tail_parts = tail_parts;
-    p.tail_run = tail_run;
+    p.tail_run = call.tail_run;
     p.paging = tb_paging(page_size);
-    p.scale_log2 = scale * kLog2e;
+    p.scale_log2 = call.scale * kLog2e;
     p.wide = wide;
     p.direct = prefix_parts == 0 && tail_parts == 1;
-    p.error = error;
+    p.error = call.error;
     const int tile = dtype == TB_F32 ? kF32Rows : kRows;                 // of the parts behind
     const int64_t of_common = (int64_t)tiles * kv_heads * prefix_parts;
     const int64_t blocks = (wide ? 0 : of_common) + (int64_t)rows * ((p.fold + tile - 1) / tile) * kv_heads * tail_parts;
@@ -1425,7 +1443,7 @@ TB_EXPORT int tb_attention_shared(const void* q, int64_t q_stride, void* out, in
         else status = launch_mma<256>(warps, blocks, p, stream);
         if (status == 0 && wide && of_common > 0) {
             CUtensorMap map;
-            if (!make_cache_map(&map, cache, cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
+            if (!make_cache_map(&map, call.cache, call.cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
             status = head_dim == 64 ? launch_tc<64>(map, of_common, p, stream) : launch_tc<128>(map, of_common, p, stream);
         }
     }

@@ -13,7 +13,7 @@
 // Bound by HBM: every byte is read once and written once.  A block copies one piece of one page with 16-byte loads, all
 // of a thread's loads in flight before its first store.  1,500 pages of a 32-bit cache moved down, 1.57 GB read and written: 244 us,
 // the measured copy rate (6.4 TB/s); states and last pages of 31 forks, 2.21 GB: 334 us, 6.6 TB/s.  A fork of a few pages is bound
-// by the host: 7.6 us a call, of which the launch is 2.
+// by the host: 7.5 us a call, of which the launch is 2.
 #include <new>
 #include <vector>
 

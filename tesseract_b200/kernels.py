@@ -330,8 +330,8 @@ def attention_shared_tile(dtype: torch.dtype, wide: bool = False) -> int:
     return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if wide else 0))
 
 
-_ATTENTION_SHARED = (_pointer, _i64, _pointer, _i64, _pointer, _pointer, _pointer, _i32, _i32, *[_pointer] * 5, *[_i32] * 6, _f32,
-                     *[_i32] * 5, _pointer, _pointer, _i64, _i32, _i32, _i32, _pointer, _i32, _pointer)
+_ATTENTION_SHARED = (ctypes.c_char_p, _pointer)
+_SHARED_CALL = struct.Struct("=QqQq10QqQ17if")      # the fields of attention_shared.cu's SharedCall
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
@@ -357,12 +357,13 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     if choice.prefix_parts or choice.tail_parts > 1:
         scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
         at = scratch.data_ptr()
-    _check(_entry("attention_shared", "tb_attention_shared", _ATTENTION_SHARED)(
+    call = _SHARED_CALL.pack(
         q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0), block_table.shape[1], *shared.addresses(), rows, shared.prefix.numel(), num_heads, num_kv_heads,
-        head_dim, page_size, scale, choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, at,
-        at + 4 * parts * head_dim, parts * head_dim, choice.warps, choice.wide, cache.shape[0],
-        _error_word(q.device).data_ptr(), _code(dtype), _raw_stream()), "attention_shared")
+        *shared.addresses(), at, at + 4 * parts * head_dim, parts * head_dim, _error_word(q.device).data_ptr(),
+        block_table.stride(0), block_table.shape[1], rows, shared.prefix.numel(), num_heads, num_kv_heads, head_dim, page_size,
+        choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, choice.warps, choice.wide,
+        cache.shape[0], _code(dtype), scale)
+    _check(_entry("attention_shared", "tb_attention_shared", _ATTENTION_SHARED)(call, _raw_stream()), "attention_shared")
     return out
 
 
@@ -436,14 +437,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int
     rows, vocab = logits.shape
     _need(tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.numel() == rows,
           "tokens must be contiguous int32 [S]")
-    device = logits.device
-    _need(device == tokens.device, "token_logprobs takes tensors of one device")
+    _need(logits.device == tokens.device, "token_logprobs takes tensors of one device")
     if not 0 <= alternatives <= min(MAX_ALTERNATIVES, vocab):
         raise KernelError(f"token_logprobs gives up to {MAX_ALTERNATIVES} alternatives, and no more than the vocabulary has tokens")
-    logprob = torch.empty(rows, dtype=torch.float32, device=device)
-    entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    values = torch.empty((rows, alternatives), dtype=torch.float32, device=device)
-    ids = torch.empty((rows, alternatives), dtype=torch.int32, device=device)
+    # (new_empty: half a microsecond less each than torch.empty)
+    logprob, entropy, values = logits.new_empty(rows), logits.new_empty(rows), logits.new_empty((rows, alternatives))
+    ids = tokens.new_empty((rows, alternatives))
     _check(_entry("logprobs", "tb_token_logprobs", _TOKEN_LOGPROBS)(
         logits.data_ptr(), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), values.data_ptr(),
         ids.data_ptr(), rows, vocab, alternatives, _raw_stream()), "token_logprobs")
