@@ -16,7 +16,7 @@
 //                values (as in this package's other attention kernels in bfloat16: relative 2^-9 of each, averaged over the keys).
 //                Bound by HBM: 16 rows of 4,000 keys of their own, 32 heads on 8 of 128, 262 MB in 47.3 us = 5.5 TB/s, 0.86 of the
 //                measured copy rate; below some 10 MB by the chain of a launch, its look-ups and the first copies (4 to 12 us).
-//   attend_tc    bfloat16, head sizes 64 and 128, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor
+//   attend_tc    bfloat16, common parts of groups with more folded rows: tiles of 128 on the tcgen05 tensor
 //                cores, see there.  A tile of 16 would read a common part from L2 once for every 16 folded rows.
 //   attend_f32, attend_f32_wide   32-bit, tiles of 8 and of 32 folded rows, multiply-adds only, see there.
 // Which form and how many runs: plan.shared_attention, with both sides' times beside its rule.
@@ -464,15 +464,16 @@ constexpr size_t mma_bytes() {
 
 // ------------------------------------------------------------------------------------------------ bfloat16, tcgen05
 
-// Common parts of groups with more than 16 folded rows, head sizes 64 and 128: a tile of 128 folded rows against a run of blocks
-// of 64 keys.  Per block S = Q . K^T (tcgen05.mma, M128 x N64, both operands in shared memory as 64-number slices with the
+// Common parts of groups with more than a few folded rows, head sizes up to 64, 128 and 256: a tile of 128 folded rows against a run of blocks
+// of 64 keys.  (Head sizes between are filled up with zeros, 80 for one: 20 heads on 4, 64 rows at 32,768 keys 45 us, 338 with tiles of
+// 16; 8 heads on 2 of 256 45 and 365.)  Per block S = Q . K^T (tcgen05.mma, M128 x N64, both operands in shared memory as 64-number slices with the
 // 128-byte swizzle, S in 64 columns of tensor memory), the weights 2^(s - m) of a row by the thread that owns it, rounded to
 // bfloat16 into one of two buffers in tensor memory, and O += P . V (M128 x N D x K64, P from tensor memory), O in D columns.
 // No block needs a mask: a common part ends with a block, and what is beyond it belongs to the rows' own parts.
 // Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products for the
 // scores and one lane of warp 6 those with the values; warp 5 brings keys and values, page by page, with cp.async.bulk.tensor into
 // rings of their own.  All waits are bounded.
-// 64 rows, 32 heads on 8 of 128, 32,768 keys in common: 49.5 us with the join behind it (134 MB, 20.8 us at the measured copy rate;
+// 64 rows, 32 heads on 8 of 128, 32,768 keys in common: 48.4 us with the join behind it (134 MB, 20.8 us at the measured copy rate;
 // 34 GFLOP, 20.2 us at the measured matrix rate).  A block of 64 keys takes a softmax warp some 2,080 cycles, two blocks of threads a
 // multiprocessor: 1,050 for the weights (both blocks' exponentials are 1,024 of the special-function unit), 570 waiting for scores
 // (two tiles read the same keys through L2, 8.6 TB/s), 160 for a buffer of weights, the rest on the way to and from tensor memory.
@@ -481,11 +482,13 @@ constexpr size_t mma_bytes() {
 // change; with the weights in the scores' place, as head size 128 needs then, 56.7), all keys found in L2 (47.7).
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 224;
-constexpr uint32_t kTcColumns = 256;          // tensor memory of a block: S 64, O up to 128, two buffers of P of 32
 template <int D>
 constexpr int kTcStages = D == 64 ? 4 : 2;    // of the keys' ring and of the values'; 64 KB under way either way (a third for keys of 128 changes nothing)
 template <int D>
+constexpr int kTcBlocks = D == 256 ? 1 : 2;   // that share a multiprocessor
+template <int D>
 struct TcShape {
+    static constexpr uint32_t kColumns = D == 256 ? 512 : 256;    // of tensor memory: S 64, O D, two buffers of P of 32
     static constexpr uint32_t kSlice = kBlock * 128;              // 64 keys x 64 numbers
     static constexpr uint32_t kBlockBytes = (D / 64) * kSlice;    // a block of keys, or of values
     static constexpr uint32_t kQSlice = kTcRows * 128, kQBytes = (D / 64) * kQSlice;
@@ -576,6 +579,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int dim = p.head_dim;               // (queries and, by the tensor map, keys and values are zeros from there up to D)
     const int rows = min(kTcRows, w.folded - w.first_folded);
     const int live_threads = (rows + 31) / 32 * 32;               // of the softmax warps: those with a row
     const int n_blocks = (w.end - w.begin) / kBlock;
@@ -600,7 +604,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     }
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&tmem_base_slot)), "r"(kTcColumns) : "memory");
+                     ::"r"(smem_u32(&tmem_base_slot)), "r"(Tiles::kColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // where a thread's query lies, and the page of a lane's keys in the first block: looked up while the rest is set up
@@ -615,10 +619,10 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         // the queries, a thread a row, while warp 5 already brings the first blocks
         const int r = threadIdx.x;
         if (r < kTcRows) {
-            const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (int64_t)row * p.q_stride + (int64_t)head * D;
+            const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + (int64_t)row * p.q_stride + (int64_t)head * dim;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)
-                cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), src + c * 8, r < rows);
+                cp_async16(q_tile + (c >> 3) * Tiles::kQSlice + sw128(r, c & 7), c * 8 < dim ? src + c * 8 : src, r < rows && c * 8 < dim);
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -706,7 +710,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
         }
     } else if (warp == 6) {
         if (lane == 0) {
-            constexpr uint32_t idesc_pv = idesc_bf16(kTcRows, D, 1);
+            const uint32_t idesc_pv = idesc_bf16(kTcRows, dim, 1);
             const uint64_t v_desc0 = desc_sw128(value_tiles, kSlice >> 4);
             int s = 0;
             uint32_t parity = 0;
@@ -790,6 +794,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                 if (j > 0) {
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c) {
+                        if (c * 16 >= dim) break;
                         uint32_t v[16];
                         asm volatile(
                             "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -821,6 +826,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
             const uint32_t staged = smem_u32(smem) + r * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
+                if (c * 32 >= dim) break;
                 uint32_t v[32];
                 tmem_load_32(tmem_o + lane_base + c * 32, v);
                 tmem_wait_ld();
@@ -832,7 +838,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
             fence_async_smem();
             if (r < rows) {
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                             ::"l"(p.part_a + slot * D), "r"(staged), "r"(D * 4) : "memory");
+                             ::"l"(p.part_a + slot * dim), "r"(staged), "r"(dim * 4) : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
             if (r < rows) p.part_ml[slot] = make_float2(m, l);
@@ -847,7 +853,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     __syncthreads();
     if (warp == 4) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTcColumns) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Tiles::kColumns) : "memory");
     }
 }
 
@@ -855,7 +861,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
 // so everything this kernel reads is there from the start, and its blocks fill the multiprocessors as those end.  What the
 // kernel behind reads of both is there once this one is done, so it waits for the one in front before it ends.
 template <int D>
-__global__ void __launch_bounds__(kTcThreads, 2) shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
+__global__ void __launch_bounds__(kTcThreads, kTcBlocks<D>) shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
     extern __shared__ __align__(1024) unsigned char tc_smem[];
     pdl_trigger();
     Work w;
@@ -1347,7 +1353,7 @@ TB_EXPORT int tb_attention_shared_tile(int dtype, int wide) {
 // Whether that form takes these sizes (bfloat16: on the tcgen05 tensor cores).
 TB_EXPORT int tb_attention_shared_wide(int dtype, int head_dim, int page_size) {
     if (dtype == TB_F32) return 1;
-    return dtype == TB_BF16 && (head_dim == 64 || head_dim == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0;
+    return dtype == TB_BF16 && head_dim <= 256 && page_size >= 8 && (page_size & (page_size - 1)) == 0;
 }
 
 // rows of q and out: [rows, heads * head_dim] with a stride; positions[b]: the last key of row b (-1: none); table: [rows, columns]
@@ -1444,7 +1450,8 @@ TB_EXPORT int tb_attention_shared(const void* packed, cudaStream_t stream) {
         if (status == 0 && wide && of_common > 0) {
             CUtensorMap map;
             if (!make_cache_map(&map, call.cache, call.cache_pages, kv_heads, page_size, kBlock, head_dim)) return TB_ERR_BAD_SIZE;
-            status = head_dim == 64 ? launch_tc<64>(map, of_common, p, stream) : launch_tc<128>(map, of_common, p, stream);
+            status = head_dim <= 64 ? launch_tc<64>(map, of_common, p, stream)
+                     : head_dim <= 128 ? launch_tc<128>(map, of_common, p, stream) : launch_tc<256>(map, of_common, p, stream);
         }
     }
     if (status != 0 || p.direct) return status;

@@ -146,8 +146,8 @@ inline const CUtensorMap* cached_map_2d(const void* base, uint64_t rows, uint64_
     return &mine;
 }
 
-// Tensor map of one cache entry [pages][K|V][kv head][key][head_dim] (head_dim a multiple of 64), boxes of 64 dims
-// of min(page_size, max_rows) keys of one head.
+// Tensor map of one cache entry [pages][K|V][kv head][key][head_dim] (head_dim a multiple of 16), boxes of 64 dims
+// of min(page_size, max_rows) keys of one head (zeros behind the last dim).
 inline bool make_cache_map(CUtensorMap* map, const void* cache, int pages, int num_kv_heads, int page_size, int max_rows,
                            int head_dim) {
     EncodeTiledFn fn = encode_tiled();

@@ -302,15 +302,23 @@ SHARED_MIN_SAVED = 64
 # at 2,048 keys, 29 MB: 0.757 and 0.702 ms; 32 at 2,048, 130 MB: 0.992 and 1.068; 32 at 8,192, 520 MB: 1.136 and 1.931; of 8 layers
 # of the 8B sizes, 16 rows at 1,024, 63 MB: 1.058 and 1.050; 4 at 8,192, 101 MB: 0.975 and 1.013; 32 at 8,192: 1.179 and 2.105).
 SHARED_MIN_BYTES = 96 << 20
-# Tiles of 16 folded rows times blocks of common keys from where on the form with the larger tiles is faster, by head size (32 heads
-# on 8 unless it says otherwise, device time with the small tiles and with the large).  bfloat16, whose launch takes 10 us: 64 rows at
-# 2,048 keys of 64 11.1 and 11.6 us, at 8,192 15.9 and 18.9 the other way, 128 rows at 16,384 44.2 and 24.4; of 128, 32 rows at 1,024
-# 11.3 and 11.6, 64 at 2,048 19.0 and 13.1, 128 at 16,384 91.8 and 34.8.  32 bits: 4 rows at 2,048 keys of 64 12.1 and 13.8, 8 16.6
-# and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 heads on 2 of 256, 8 rows at 8,192 keys 32.7 and
+# Where the form with the larger tiles is faster by more than the 3 us of host time that its launch costs.  bfloat16 (a tile of it works
+# for 128 rows whatever it holds): tiles of 16 folded rows of a group beyond the first two, or the first (at head sizes above 128, where
+# small tiles hold few keys, all of them and two more), times its blocks of common keys, kv heads and head size.  Device time with small tiles and with large: 32 heads on 8 of 64, 8 rows at 8,192 keys 12.4 and 14.5 us, 16 at 2,048 11.5 and
+# 11.2, 16 at 8,192 19.9 and 16.9, 64 at 8,192 100.8 and 22.9, 16 groups of 4 at 8,192 51.6 and 65.9; of 128, 4 rows at 8,192 15.8 and
+# 18.0, 8 at 2,048 13.9 and 12.4, 64 at 8,192 114 and 32, 16 groups of 4 at 8,192 96.6 and 98.7; 20 on 4 of 80, 8 rows at 2,048 10.9 and
+# 12.0, 8 at 8,192 16.3 and 15.5, 64 at 32,768 338 and 45; 8 on 2 of 256, 2 rows at 8,192 17.8 and 15.2, 64 at 32,768 365 and 45; 4 on 2 of
+# 16, 64 rows at 8,192 10.2 and 11.7, at 32,768 22.9 and 16.1.
+SHARED_WIDE_FREE = {64: 2, 128: 1, 256: -2}
+SHARED_WIDE_MIN = 49152
+# 32 bits: all tiles of 16 folded rows times blocks of common keys, by head size.  32 heads on 8 of 64, 4 rows at 2,048 keys 12.1 and 13.8,
+# 8 16.6 and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 on 2 of 256, 8 rows at 8,192 keys 32.7 and
 # 34.9, 32 at 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
-SHARED_WIDE_MIN = {torch.bfloat16: {64: 128, 128: 48}, torch.float32: {64: 48, 128: 48, 256: 192}}
-# Blocks of threads of the 32-bit form that share a multiprocessor, small tiles and large, by the head size that they are made for.
-SHARED_F32_RESIDENT = {False: {64: 4, 128: 4, 256: 2}, True: {64: 4, 128: 3, 256: 2}}
+SHARED_WIDE_MIN_F32 = {64: 48, 128: 48, 256: 192}
+# Blocks of threads that share a multiprocessor, by the head size that they are made for: of the form with the larger tiles, and of
+# the 32-bit one with the small.
+SHARED_WIDE_RESIDENT = {torch.bfloat16: {64: 2, 128: 2, 256: 1}, torch.float32: {64: 4, 128: 3, 256: 2}}
+SHARED_F32_RESIDENT = {64: 4, 128: 4, 256: 2}
 
 
 def saved_blocks(sizes: Sequence[int], blocks: Sequence[int]) -> int:
@@ -354,18 +362,22 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
         tails = tails + np.asarray(shared.row_blocks)
         blocks = np.zeros_like(blocks)
     rows = np.where(blocks > 0, sizes * fold, 0)
-    work = int((-(-rows // 16) * blocks).sum())
-    padded = 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256            # (a kernel's head size, in 32 bits)
-    wide = work > SHARED_WIDE_MIN[dtype].get(padded, 0) and kernels.attention_shared_wide(dtype, head_dim, page_size)
+    sixteens = -(-rows // 16)
+    padded = 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256            # (a kernel's head size)
+    if dtype == torch.float32:
+        wide = int((sixteens * blocks).sum()) > SHARED_WIDE_MIN_F32[padded]
+    else:
+        wide = int((np.where(sixteens > 0, np.maximum(sixteens - SHARED_WIDE_FREE[padded], 0), 0) * blocks).sum()) * num_kv_heads * head_dim > SHARED_WIDE_MIN
+    wide = wide and kernels.attention_shared_wide(dtype, head_dim, page_size)
     tile = kernels.attention_shared_tile(dtype, wide)
     tiles = -(-rows // tile)
     # (large) blocks of threads that are resident at once, a kv head
-    target = max(1, (SHARED_F32_RESIDENT[False][padded] if dtype == torch.float32 else 2) * sms // num_kv_heads)
-    # rows' own keys, a block of threads each: large blocks where they are few, small ones (and all of them at once) where they
-    # are many
+    target = max(1, (SHARED_F32_RESIDENT[padded] if dtype == torch.float32 else 2) * sms // num_kv_heads)
+    # rows' own keys, a block of threads each: large blocks where they are few or share a launch with common parts, small ones (and
+    # all of them at once) where they are many
     tails = np.maximum(tails, 1)
     tail_tiles = np.full(tails.shape, -(-fold // kernels.attention_shared_tile(dtype)))
-    warps = 2 if dtype != torch.float32 and int(tail_tiles.sum()) > target else 0
+    warps = 2 if dtype != torch.float32 and int(tail_tiles.sum()) > target and (wide or not tiles.any()) else 0
     small = 4 if head_dim <= 64 else 2 if head_dim <= 128 else 1        # as many small ones are resident beside a large one's room
     shortest = 1 if wide and dtype == torch.float32 else SHARED_MIN_RUN[dtype]
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
@@ -373,10 +385,11 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     prefix_parts, prefix_run = 0, 1
     if tiles.any():
         room = target
-        if not wide and warps == 0:             # (in one launch with the rows' own)
-            room = max(target // 2, target - int((tail_tiles * -(-tails // tail_run)).sum()))
-        elif dtype == torch.float32:
-            room = max(1, SHARED_F32_RESIDENT[True][padded] * sms // num_kv_heads)
+        if wide:
+            room = max(1, SHARED_WIDE_RESIDENT[dtype][padded] * sms // num_kv_heads)
+        else:                                   # in one launch with the rows' own: at once with them where those leave half of the chip
+            left = target - int((tail_tiles * -(-tails // tail_run)).sum())
+            room = left if 2 * left >= target else target
         prefix_run = _shared_runs(tiles, blocks, room, shortest)
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles)

@@ -172,10 +172,10 @@ def test_any_cut_gives_the_same_numbers(dtype):
     assert torch.equal(case.run(more), case.run(base))
 
 
-@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 16), (torch.float32, 64),
-                                        (torch.float32, 80), (torch.float32, 128), (torch.float32, 208), (torch.float32, 256)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [16, 48, 64, 80, 112, 128, 144, 192, 208, 256])
 @pytest.mark.parametrize("rows", [1, 2, 4, 5, 8, 9, 16, 24, 33, 70])
-def test_both_forms(rows, dtype, dim):
+def test_both_forms(rows, dim, dtype):
     """The form with the larger tiles (in bfloat16 the tensor cores') and the other, at every count of rows, whichever the plan takes."""
     case = Case([(1030, [1031 + 7 * i % 90 for i in range(rows)]), (192, [200, 250])], 8, 2, dim, dtype=dtype, seed=rows)
     alone = rows == 1                                # (a row alone has nothing in common with another)

@@ -46,9 +46,19 @@ def test_runs_cover_every_key_and_fit_the_chip(groups, dim, dtype):
         assert choice.prefix_parts == min(plan.SHARED_MAX_PARTS, max(r for _, r in runs))
         # at most what is resident at once, unless every tile is one run already
         assert sum(t * r for t, r in runs) * kv_heads <= 4 * SMS or max(r for _, r in runs) == 1
-        least = plan.SHARED_WIDE_MIN[dtype].get(64 if dim <= 64 else 128 if dim <= 128 else 256, 0)
-        assert choice.wide == ((dtype == torch.float32 or dim in (64, 128)) and
-                               sum(-(-n * fold // 16) * b for n, b in zip(shared.sizes, shared.blocks)) > least)
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim, groups, wide", [
+    (torch.bfloat16, 32, 8, 64, [(8192, [8200] * 8)], False), (torch.bfloat16, 32, 8, 64, [(8192, [8200] * 16)], True),
+    (torch.bfloat16, 32, 8, 64, [(8192, [8200] * 4)] * 16, False), (torch.bfloat16, 32, 8, 128, [(8192, [8200] * 4)] * 16, False),
+    (torch.bfloat16, 32, 8, 128, [(2048, [2100] * 16)], True), (torch.bfloat16, 32, 8, 64, [(2048, [2100] * 16)], False), (torch.bfloat16, 20, 4, 80, [(32768, [32800] * 64)], True),
+    (torch.bfloat16, 8, 2, 256, [(8192, [8200] * 2)], True), (torch.bfloat16, 4, 2, 16, [(8192, [8200] * 64)], False),
+    (torch.float32, 32, 8, 64, [(2048, [2100] * 4)], False), (torch.float32, 32, 8, 64, [(2048, [2100] * 8)], True),
+])
+def test_which_form_takes_the_keys_in_common(dtype, heads, kv_heads, dim, groups, wide):
+    _, choice = choose(groups, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype)
+    assert choice.wide == wide and choice.prefix_parts > 0
+    assert choice.wide or choice.warps == 0                           # (common parts want the large blocks)
 
 
 def test_what_is_shared_and_what_not():
@@ -81,7 +91,7 @@ def test_tensor_memory_that_a_product_used_is_touched_behind_a_fence():
     ``tcgen05.fence::after_thread_sync``."""
     with open(os.path.join(CSRC, "attention_shared.cu")) as handle:
         code = re.sub(r"//[^\n]*", "", handle.read())
-    softmax = code[code.index("const uint32_t lane_base"):code.index("__global__ void __launch_bounds__(kTcThreads, 2)")]
+    softmax = code[code.index("const uint32_t lane_base"):code.index("__global__ void __launch_bounds__(kTcThreads")]
     waiting, waits, touches = False, 0, 0
     for event in re.finditer(r"(?P<wait>mbar_wait\((?:o_full|s_full))|(?P<fence>tc_fence_after\(\))|"
                              r"(?P<touch>tmem_(?:load|store)\w*\(tmem_[ops]\b|\"r\"\(tmem_o)", softmax):
