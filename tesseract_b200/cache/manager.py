@@ -264,8 +264,8 @@ class CacheManager:
 
     def fork(self, pairs: Sequence[Tuple[Hashable, Hashable]], reserve_tokens: Union[int, Sequence[int], None] = None) -> bool:
         """For every ``(parent, child)``: the new request ``child`` goes on from where ``parent`` is.  With ``reserve_tokens`` (a
-        number, or one a pair) the pages that each child may need up to that many tokens are set aside.  All of them, or none and False if they do not
-        fit now.  The copies are enqueued on the current stream, behind the step that filled the parents' last pages."""
+        number, or one a pair) the pages that each child may need up to that many tokens are set aside.  All of them, or none and
+        False if they do not fit now.  The copies are enqueued on the current stream, behind the step that filled the parents' last pages."""
         pairs = list(pairs)
         if reserve_tokens is None or isinstance(reserve_tokens, int):
             reserve_tokens = [reserve_tokens] * len(pairs)

@@ -464,12 +464,13 @@ constexpr size_t mma_bytes() {
 
 // ------------------------------------------------------------------------------------------------ bfloat16, tcgen05
 
-// Common parts of groups with more than a few folded rows, head sizes up to 64, 128 and 256: a tile of 128 folded rows against a run of blocks
-// of 64 keys.  (Head sizes between are filled up with zeros, 80 for one: 20 heads on 4, 64 rows at 32,768 keys 45 us, 338 with tiles of
-// 16; 8 heads on 2 of 256 45 and 365.)  Per block S = Q . K^T (tcgen05.mma, M128 x N64, both operands in shared memory as 64-number slices with the
-// 128-byte swizzle, S in 64 columns of tensor memory), the weights 2^(s - m) of a row by the thread that owns it, rounded to
-// bfloat16 into one of two buffers in tensor memory, and O += P . V (M128 x N D x K64, P from tensor memory), O in D columns.
-// No block needs a mask: a common part ends with a block, and what is beyond it belongs to the rows' own parts.
+// Common parts of groups with more than a few folded rows, head sizes up to 64, 128 and 256: a tile of 128 folded rows against a run
+// of blocks of 64 keys.  (Head sizes between are filled up with zeros, 80 for one: 20 heads on 4, 64 rows at 32,768 keys 45 us, 338
+// with tiles of 16; 8 heads on 2 of 256 45 and 365.)  Per block S = Q . K^T (tcgen05.mma, M128 x N64, both operands in shared memory
+// as 64-number slices with the 128-byte swizzle, S in 64 columns of tensor memory), the weights 2^(s - m) of a row by the thread
+// that owns it, rounded to bfloat16 into one of two buffers in tensor memory, and O += P . V (M128 x N D x K64, P from tensor
+// memory), O in D columns.  No block needs a mask: a common part ends with a block, and what is beyond it belongs to the rows' own
+// parts.
 // Warps 0-3: softmax, a thread a row (warps whose rows do not exist leave at once); one lane of warp 4 issues the products for the
 // scores and one lane of warp 6 those with the values; warp 5 brings keys and values, page by page, with cp.async.bulk.tensor into
 // rings of their own.  All waits are bounded.
@@ -483,7 +484,7 @@ constexpr size_t mma_bytes() {
 constexpr int kTcRows = 128;
 constexpr int kTcThreads = 224;
 template <int D>
-constexpr int kTcStages = D == 64 ? 4 : 2;    // of the keys' ring and of the values'; 64 KB under way either way (a third for keys of 128 changes nothing)
+constexpr int kTcStages = D == 64 ? 4 : 2;    // of the keys' ring and of the values': 128 KB a multiprocessor (a third for keys of 128 changes nothing)
 template <int D>
 constexpr int kTcBlocks = D == 256 ? 1 : 2;   // that share a multiprocessor
 template <int D>
@@ -861,7 +862,8 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
 // so everything this kernel reads is there from the start, and its blocks fill the multiprocessors as those end.  What the
 // kernel behind reads of both is there once this one is done, so it waits for the one in front before it ends.
 template <int D>
-__global__ void __launch_bounds__(kTcThreads, kTcBlocks<D>) shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
+__global__ void __launch_bounds__(kTcThreads, kTcBlocks<D>)
+shared_tc_kernel(const __grid_constant__ CUtensorMap cache_map, const SharedParams p) {
     extern __shared__ __align__(1024) unsigned char tc_smem[];
     pdl_trigger();
     Work w;

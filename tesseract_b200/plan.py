@@ -277,8 +277,8 @@ def attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim
 @dataclass(frozen=True)
 class SharedAttentionPlan:
     """How ``attention_shared`` cuts a step: ``tiles`` tiles of all groups' folded rows (``wide``: larger tiles, in bfloat16 on
-    the tcgen05 tensor cores), common parts in at most ``prefix_parts`` runs of at least ``prefix_run`` blocks of 64 keys each (0 parts: nothing is
-    shared, every row reads its own keys), what lies behind in at most ``tail_parts`` of at least ``tail_run``."""
+    the tcgen05 tensor cores), common parts in at most ``prefix_parts`` runs of at least ``prefix_run`` blocks of 64 keys each (0
+    parts: nothing is shared, every row reads its own keys), what lies behind in at most ``tail_parts`` of at least ``tail_run``."""
 
     tiles: int
     prefix_parts: int
@@ -302,18 +302,19 @@ SHARED_MIN_SAVED = 64
 # at 2,048 keys, 29 MB: 0.757 and 0.702 ms; 32 at 2,048, 130 MB: 0.992 and 1.068; 32 at 8,192, 520 MB: 1.136 and 1.931; of 8 layers
 # of the 8B sizes, 16 rows at 1,024, 63 MB: 1.058 and 1.050; 4 at 8,192, 101 MB: 0.975 and 1.013; 32 at 8,192: 1.179 and 2.105).
 SHARED_MIN_BYTES = 96 << 20
-# Where the form with the larger tiles is faster by more than the 3 us of host time that its launch costs.  bfloat16 (a tile of it works
-# for 128 rows whatever it holds): tiles of 16 folded rows of a group beyond the first two, or the first (at head sizes above 128, where
-# small tiles hold few keys, all of them and two more), times its blocks of common keys, kv heads and head size.  Device time with small tiles and with large: 32 heads on 8 of 64, 8 rows at 8,192 keys 12.4 and 14.5 us, 16 at 2,048 11.5 and
-# 11.2, 16 at 8,192 19.9 and 16.9, 64 at 8,192 100.8 and 22.9, 16 groups of 4 at 8,192 51.6 and 65.9; of 128, 4 rows at 8,192 15.8 and
-# 18.0, 8 at 2,048 13.9 and 12.4, 64 at 8,192 114 and 32, 16 groups of 4 at 8,192 96.6 and 98.7; 20 on 4 of 80, 8 rows at 2,048 10.9 and
-# 12.0, 8 at 8,192 16.3 and 15.5, 64 at 32,768 338 and 45; 8 on 2 of 256, 2 rows at 8,192 17.8 and 15.2, 64 at 32,768 365 and 45; 4 on 2 of
+# Where the form with the larger tiles is faster by more than the 3 us of host time that its launch costs.  bfloat16 (a tile of it
+# works for 128 rows whatever it holds): tiles of 16 folded rows of a group beyond the first two, or the first (at head sizes above
+# 128, where small tiles hold few keys, all of them and two more), times its blocks of common keys, kv heads and head size.  Device
+# time with small tiles and with large: 32 heads on 8 of 64, 8 rows at 8,192 keys 12.4 and 14.5 us, 16 at 2,048 11.5 and 11.2, 16 at
+# 8,192 19.9 and 16.9, 64 at 8,192 100.8 and 22.9, 16 groups of 4 at 8,192 51.6 and 65.9; of 128, 4 rows at 8,192 15.8 and 18.0, 8 at
+# 2,048 13.9 and 12.4, 64 at 8,192 114 and 32, 16 groups of 4 at 8,192 96.6 and 98.7; 20 on 4 of 80, 8 rows at 2,048 10.9 and 12.0, 8
+# at 8,192 16.3 and 15.5, 64 at 32,768 338 and 45; 8 on 2 of 256, 2 rows at 8,192 17.8 and 15.2, 64 at 32,768 365 and 45; 4 on 2 of
 # 16, 64 rows at 8,192 10.2 and 11.7, at 32,768 22.9 and 16.1.
 SHARED_WIDE_FREE = {64: 2, 128: 1, 256: -2}
 SHARED_WIDE_MIN = 49152
-# 32 bits: all tiles of 16 folded rows times blocks of common keys, by head size.  32 heads on 8 of 64, 4 rows at 2,048 keys 12.1 and 13.8,
-# 8 16.6 and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 on 2 of 256, 8 rows at 8,192 keys 32.7 and
-# 34.9, 32 at 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
+# 32 bits: all tiles of 16 folded rows times blocks of common keys, by head size.  32 heads on 8 of 64, 4 rows at 2,048 keys 12.1 and
+# 13.8, 8 16.6 and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 on 2 of 256, 8 rows at 8,192 keys
+# 32.7 and 34.9, 32 at 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
 SHARED_WIDE_MIN_F32 = {64: 48, 128: 48, 256: 192}
 # Blocks of threads that share a multiprocessor, by the head size that they are made for: of the form with the larger tiles, and of
 # the 32-bit one with the small.
@@ -367,7 +368,8 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     if dtype == torch.float32:
         wide = int((sixteens * blocks).sum()) > SHARED_WIDE_MIN_F32[padded]
     else:
-        wide = int((np.where(sixteens > 0, np.maximum(sixteens - SHARED_WIDE_FREE[padded], 0), 0) * blocks).sum()) * num_kv_heads * head_dim > SHARED_WIDE_MIN
+        beyond = np.where(sixteens > 0, np.maximum(sixteens - SHARED_WIDE_FREE[padded], 0), 0)
+        wide = int((beyond * blocks).sum()) * num_kv_heads * head_dim > SHARED_WIDE_MIN
     wide = wide and kernels.attention_shared_wide(dtype, head_dim, page_size)
     tile = kernels.attention_shared_tile(dtype, wide)
     tiles = -(-rows // tile)
