@@ -55,10 +55,11 @@ HOST_RING = 3          # pinned copies of a graph's metadata: a launch may be pr
 
 class _Graph:
     """Persistent buffers and the captured graph for one (batch bucket, table width), without or (``company``: the arrays of the
-    step that it is captured for) with rows that have keys in common: how the rows are grouped is data, so one graph serves every
-    grouping with as many such groups."""
+    step that it is captured for) with rows that have keys in common: which rows are grouped is data, so one graph serves every
+    grouping into groups of the same sizes, or (``any_sizes``) into as many groups of any size, whose launches are laid out for more
+    tiles than most have."""
 
-    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None):
+    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None, any_sizes: bool = False):
         cache, device = stepper.cache, stepper.runtime.device
         self.batch, self.columns = batch, columns
         self.paged = [i for i, g in enumerate(cache.groups) if g.pool is not None]
@@ -108,7 +109,7 @@ class _Graph:
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=device)   # this step's token ids, chosen on the device
         groups: List[GroupView] = []
         tables = dict(zip(self.paged, self.d["tables"]))
-        shared = SharedRows(*self.d["together"], *company[1:], room=batch) if company is not None else None
+        shared = SharedRows(*self.d["together"], *company[1:], room=batch if any_sizes else None) if company is not None else None
         for index, g in enumerate(cache.groups):
             groups.append(GroupView(tables.get(index), cache.page_size if g.pool is not None else 0,
                                     shared if shared is not None and cache.shares_keys(index) else None))
@@ -195,6 +196,9 @@ class DecodeLaunch:
         return self.host_tokens[:self.count].tolist()
 
 
+GROUPINGS = 8          # graphs of one batch and table width for groups of exact sizes
+
+
 class DecodeGraphs:
     """Chooses, captures and replays decode graphs for a :class:`Stepper`."""
 
@@ -202,7 +206,8 @@ class DecodeGraphs:
         self.stepper = stepper
         self.max_batch = max_batch
         self.graphs: Dict[Tuple[int, int], _Graph] = {}
-        self.shared_graphs: Dict[Tuple[int, int, int], _Graph] = {}     # of steps whose rows have keys in common (Stepper.company)
+        # of steps whose rows have keys in common (Stepper.company): by those groups' sizes, or (`_grouping`) their number
+        self.shared_graphs: Dict[Tuple[int, int, object], _Graph] = {}
         self.replays = 0
         self.captures = 0
         self.kernels_replayed = 0
@@ -216,6 +221,17 @@ class DecodeGraphs:
     def eligible(self, entries: Sequence[StepEntry]) -> bool:
         return (self.safe and len(entries) <= self.max_batch
                 and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries))
+
+    def _grouping(self, batch: int, columns: int, company) -> Tuple[int, int, object]:
+        """The key of a step with company: the sizes of the groups that have keys in common, which a captured launch is laid out for
+        (beams keep theirs), or, where a batch has met many, their number, which bounds them."""
+        sizes = tuple(sorted(n for n, blocks in zip(company[1], company[2]) if blocks))
+        key = (batch, columns, sizes)
+        if key not in self.shared_graphs:
+            met = sum(1 for other in self.shared_graphs if other[:2] == key[:2] and not isinstance(other[2], int))
+            if met >= GROUPINGS:
+                return (batch, columns, len(sizes))
+        return key
 
     def launch(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float],
                previous: Optional[DecodeLaunch] = None, fed: Optional[Sequence[bool]] = None) -> DecodeLaunch:
@@ -231,12 +247,10 @@ class DecodeGraphs:
         pages = -(-(max(lengths) + 1) // cache.page_size)
         batch, columns = min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages))
         company = stepper.company(entries, batch - count)
-        # (with company also by the groups that have keys in common: they bound what a captured launch must be laid out for)
-        graphs, key = ((self.graphs, (batch, columns)) if company is None
-                       else (self.shared_graphs, (batch, columns, sum(1 for b in company[2] if b))))
+        graphs, key = (self.graphs, (batch, columns)) if company is None else (self.shared_graphs, self._grouping(batch, columns, company))
         graph = graphs.get(key)
         if graph is None:
-            graph = _Graph(stepper, batch, columns, self.sampled, company)
+            graph = _Graph(stepper, batch, columns, self.sampled, company, company is not None and isinstance(key[2], int))
             graphs[key] = graph
             self.captures += 1
         slot_index, h = graph.host_arrays()

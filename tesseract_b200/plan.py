@@ -24,6 +24,7 @@ Thresholds, with the measurement behind each:
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import List, Optional, Sequence
@@ -394,8 +395,11 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
             room = left if 2 * left >= target else target
         prefix_run = _shared_runs(tiles, blocks, room, shortest)
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
-    # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles)
-    count = int(tiles.sum()) if shared.room is None else shared.room * fold // tile + int((blocks > 0).sum())
+    # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles, as a group's last tile
+    # holds at least what both a tile and a row's heads are multiples of)
+    count = int(tiles.sum())
+    if shared.room is not None:
+        count = (shared.room * fold + int((blocks > 0).sum()) * (tile - math.gcd(fold, tile))) // tile
     return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, wide, warps)
 
 

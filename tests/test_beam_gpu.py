@@ -96,6 +96,40 @@ def test_beams_in_bfloat16_are_scored_as_the_plain_model_scores_them(model_folde
         assert np.abs(np.asarray(out.token_logprobs) - want).max() <= 2 * REL["bfloat16"] * np.abs(logits).max()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_graphs_of_many_groupings(model_folders, monkeypatch, dtype):
+    """Steps whose rows are grouped in many ways, more than there are graphs of exact sizes, against steps of twins launch by launch
+    that share nothing."""
+    from tesseract_b200 import plan
+    from tesseract_b200.engine import StepEntry
+    from tesseract_b200.engine.graph import GROUPINGS
+
+    monkeypatch.setattr(plan, "SHARED_MIN_SAVED", 0)
+    llm = engine(model_folders("b"), dtype, kv_capacity_tokens=16384, max_running=40)
+    stepper, cache = llm.stepper, llm.stepper.cache
+    prompts = {"p": random_tokens(384, 130, seed=1), "q": random_tokens(384, 200, seed=2)}
+    for twin in "ab":
+        for name, prompt in prompts.items():
+            assert cache.admit((twin, name, 0), reserve_tokens=260)
+            for k in range(0, len(prompt), 32):
+                stepper.step([StepEntry((twin, name, 0), prompt[k:k + 32], [])])
+            assert cache.fork([((twin, name, 0), (twin, name, k)) for k in range(1, 8)], reserve_tokens=260)
+    sizes = [(8, 8), (7, 8), (6, 8), (5, 8), (4, 8), (3, 8), (2, 8), (8, 5), (8, 1), (7, 7), (6, 5), (8, 4), (8, 8), (3, 6), (5, 5), (8, 2)]
+    for step, (first, second) in enumerate(sizes):
+        rows = [("p", k) for k in range(first)] + [("q", k) for k in range(second)]
+        tokens = random_tokens(384, len(rows), seed=step)
+        entries = {twin: [StepEntry((twin, *row), [token], [0]) for row, token in zip(rows, tokens)] for twin in "ab"}
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 0)
+        launch = stepper.graphs.launch(entries["a"], [0.0] * len(rows), [0.0] * len(rows))
+        got = launch.graph.logits[:launch.count].clone()
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 1 << 60)
+        want = stepper.step(entries["b"])
+        assert float((got - want).abs().max()) <= REL[dtype] * float(want.abs().max())
+    keys = list(stepper.graphs.shared_graphs)
+    assert sum(1 for key in keys if key[0] == 16 and isinstance(key[2], tuple)) == GROUPINGS
+    assert any(isinstance(key[2], int) for key in keys)
+
+
 def test_one_beam_is_greedy_generation(model_folders):
     from tesseract_b200 import SamplingParams
 

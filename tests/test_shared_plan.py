@@ -76,6 +76,11 @@ def test_a_captured_plan_has_tiles_for_every_grouping_of_as_many_groups():
         tile = kernels.attention_shared_tile(torch.bfloat16, choice.wide)
         for first in range(0, room + 1):
             assert choice.tiles >= -(-first * 4 // tile) + -(-(room - first) * 4 // tile)
+    for heads in (8, 20, 24, 40, 48, 56):
+        for groups in ([16], [3, 13], [5, 5, 6], [2] * 8, [1, 15], [7, 9]):
+            _, choice = choose([(8192, [8200] * n) for n in groups], heads=heads, room=16)
+            tile, fold = kernels.attention_shared_tile(torch.bfloat16, choice.wide), heads // 8
+            assert choice.tiles >= sum(-(-n * fold // tile) for n in groups if n > 1)
 
 
 def test_arrays_of_a_step():
