@@ -299,10 +299,15 @@ SHARED_MAX_PARTS = 64
 # every row's own keys is faster (4 rows of 32 heads of 64 at 200 keys: 4.2 us on the device, 7.0 with a launch to put parts together).
 SHARED_MIN_SAVED = 64
 # The same in bytes of keys and values from where on a decode step takes ``attention_shared`` at all: below, the kernel that rotates,
-# writes and attends in one launch is faster, as it finds the common pages in L2 (a step of the 1B sizes with and without, 8 rows
-# at 2,048 keys, 29 MB: 0.757 and 0.702 ms; 32 at 2,048, 130 MB: 0.992 and 1.068; 32 at 8,192, 520 MB: 1.136 and 1.931; of 8 layers
-# of the 8B sizes, 16 rows at 1,024, 63 MB: 1.058 and 1.050; 4 at 8,192, 101 MB: 0.975 and 1.013; 32 at 8,192: 1.179 and 2.105).
-SHARED_MIN_BYTES = 96 << 20
+# writes and attends in one launch is faster, as it finds the common pages in L2.  Behind many keys in common a third of that: that
+# kernel's runs are longer then.  A step with and without, ms: of the 1B sizes, 8 rows at 2,048 keys (29 MB) 0.756 and 0.702, 16 at 2,048
+# (63) 0.852 and 0.839, 8 at 6,144 (88) 0.801 and 0.843, 32 at 2,048 (130) 0.993 and 1.068, 32 at 8,192 1.090 and 1.922; 4 at 4,096 (25)
+# 0.744 and 0.802, 8 at 4,096 (59) 0.776 and 0.772, 2 at 16,000 (33) 0.795 and 0.798; of 8 layers of the 8B sizes, 16 at 1,024 (63)
+# 1.064 and 1.056, 8 at 3,072 (88) 0.986 and 0.990, 4 at 4,096 (50) 0.961 and 1.011, 32 at 8,192 1.135 and 2.099.
+SHARED_MIN_BYTES = 72 << 20
+SHARED_LONG = 64                # blocks of 64 keys
+
+
 # Where the form with the larger tiles is faster by more than the 3 us of host time that its launch costs.  bfloat16 (a tile of it
 # works for 128 rows whatever it holds): tiles of 16 folded rows of a group beyond the first two, or the first (at head sizes above
 # 128, where small tiles hold few keys, all of them and two more), times its blocks of common keys, kv heads and head size.  Device
@@ -331,7 +336,8 @@ def saved_blocks(sizes: Sequence[int], blocks: Sequence[int]) -> int:
 def sharing_pays(sizes: Sequence[int], blocks: Sequence[int], block_bytes: int) -> bool:
     """Whether a decode step reads common keys once a group rather than once a row, with ``block_bytes`` of keys and values in a
     block of 64 of one layer."""
-    return saved_blocks(sizes, blocks) * block_bytes >= max(1, SHARED_MIN_BYTES)
+    least = SHARED_MIN_BYTES // 3 if max(blocks, default=0) >= SHARED_LONG else SHARED_MIN_BYTES
+    return saved_blocks(sizes, blocks) * block_bytes >= max(1, least)
 
 
 def shared_attention(dtype: torch.dtype, *, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, shared,

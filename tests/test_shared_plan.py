@@ -67,6 +67,8 @@ def test_what_is_shared_and_what_not():
     assert choose([(4096, [5000])])[1].prefix_parts == 0              # alone
     block = 64 * 8 * 64 * 2 * 2
     assert not plan.sharing_pays((8,), (32,), block) and plan.sharing_pays((32,), (32,), block)
+    assert plan.sharing_pays((4,), (64,), block) and not plan.sharing_pays((4,), (63,), block)         # long ones from a third on
+    assert not plan.sharing_pays((2,), (64,), block) and not plan.sharing_pays((), (), block)
     assert not plan.sharing_pays((1, 1), (0, 0), block) and not plan.sharing_pays((4,), (100,), 0)
 
 
