@@ -27,6 +27,7 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 from functools import lru_cache
+from types import SimpleNamespace
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -318,10 +319,11 @@ SHARED_LONG = 64                # blocks of 64 keys
 # 16, 64 rows at 8,192 10.2 and 11.7, at 32,768 22.9 and 16.1.
 SHARED_WIDE_FREE = {64: 2, 128: 1, 256: -2}
 SHARED_WIDE_MIN = 49152
-# 32 bits: all tiles of 16 folded rows times blocks of common keys, by head size.  32 heads on 8 of 64, 4 rows at 2,048 keys 12.1 and
-# 13.8, 8 16.6 and 15.0, 64 93.5 and 51.2; of 128 16.7 and 18.3, 23.9 and 21.2, 172.8 and 96.3; 8 on 2 of 256, 8 rows at 8,192 keys
-# 32.7 and 34.9, 32 at 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
-SHARED_WIDE_MIN_F32 = {64: 48, 128: 48, 256: 192}
+# 32 bits: tiles of 8 folded rows beyond a group's first times its blocks of common keys, by head size.  32 heads on 8 of 64, 4 rows at
+# 2,048 keys 12.1 and 13.8, 8 16.6 and 15.0, 64 93.5 and 51.2, 16 groups of 2 at 4,096 77.2 and 74.7, of 4 129.7 and 100.9; of 128 16.7
+# and 18.3, 23.9 and 21.2, 172.8 and 96.3, 133.6 and 138.7, 225.1 and 207.2; 8 on 2 of 256, 16 rows at 4,096 keys 32.1 and 35.5, 32 at
+# 2,048 40.9 and 38.3, 32 at 8,192 154.9 and 83.3.
+SHARED_WIDE_MIN_F32 = {64: 64, 128: 64, 256: 460}
 # Blocks of threads that share a multiprocessor, by the head size that they are made for: of the form with the larger tiles, and of
 # the 32-bit one with the small.
 SHARED_WIDE_RESIDENT = {torch.bfloat16: {64: 2, 128: 2, 256: 1}, torch.float32: {64: 4, 128: 3, 256: 2}}
@@ -373,7 +375,7 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     sixteens = -(-rows // 16)
     padded = 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256            # (a kernel's head size)
     if dtype == torch.float32:
-        wide = int((sixteens * blocks).sum()) > SHARED_WIDE_MIN_F32[padded]
+        wide = int((np.maximum(-(-rows // 8) - 1, 0) * blocks).sum()) > SHARED_WIDE_MIN_F32[padded]
     else:
         beyond = np.where(sixteens > 0, np.maximum(sixteens - SHARED_WIDE_FREE[padded], 0), 0)
         wide = int((beyond * blocks).sum()) * num_kv_heads * head_dim > SHARED_WIDE_MIN
@@ -396,9 +398,10 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
         room = target
         if wide:
             room = max(1, SHARED_WIDE_RESIDENT[dtype][padded] * sms // num_kv_heads)
-        else:                                   # in one launch with the rows' own: at once with them where those leave half of the chip
+        else:                                   # in one launch with the rows' own: at once with them where those are much of the work
             left = target - int((tail_tiles * -(-tails // tail_run)).sum())
-            room = left if 2 * left >= target else target
+            few = int((tiles * blocks).sum()) > 4 * int((tail_tiles * tails).sum())
+            room = target if few or 2 * left < target else left
         prefix_run = _shared_runs(tiles, blocks, room, shortest)
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
     # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles, as a group's last tile
@@ -407,6 +410,18 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     if shared.room is not None:
         count = (shared.room * fold + int((blocks > 0).sum()) * (tile - math.gcd(fold, tile))) // tile
     return SharedAttentionPlan(count, prefix_parts, prefix_run, tail_parts, tail_run, wide, warps)
+
+
+def continuations(dtype, mixer, rows: int, context: int, page_size: int, sms: Optional[int] = None
+                  ) -> Optional[SharedAttentionPlan]:
+    """The plan of a decode step of ``rows`` continuations of one prompt of ``context`` tokens, if it reads their common keys once."""
+    common = context // 64
+    shared = SimpleNamespace(sizes=(rows,), blocks=(common,), tails=(1,) * rows, row_blocks=(common,) * rows, room=None, plans={})
+    block_bytes = 64 * 2 * mixer.num_kv_heads * mixer.head_dim * torch.empty((), dtype=dtype).element_size()
+    if not sharing_pays(shared.sizes, shared.blocks, block_bytes):
+        return None
+    return shared_attention(dtype, num_heads=mixer.num_heads, num_kv_heads=mixer.num_kv_heads, head_dim=mixer.head_dim,
+                            page_size=page_size, shared=shared, sms=sms)
 
 
 def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), context: int = 4096,
@@ -449,6 +464,9 @@ def describe(model, row_counts: Sequence[int] = (1, 8, 16, 17, 64, 512, 2048), c
                                    head_dim=mixer.head_dim, page_size=page_size, new_tokens=[1] * rows,
                                    max_context=context, prompt_kernel=mixer.prompt_kernel, sms=sms)
                 lines.append(f"    attend   decode step: {decode}")
+                together = None if mixer.window else continuations(dtype, mixer, rows, context, page_size, sms)
+                if together is not None:
+                    lines.append(f"             of one prompt's continuations: {together}")
                 if rows >= 17:
                     portion = attention(dtype, num_heads=mixer.num_heads, num_kv_heads=mixer.num_kv_heads,
                                         head_dim=mixer.head_dim, page_size=page_size, new_tokens=[rows],

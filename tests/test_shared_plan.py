@@ -2,6 +2,7 @@
 
 import os
 import re
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -70,6 +71,15 @@ def test_what_is_shared_and_what_not():
     assert plan.sharing_pays((4,), (64,), block) and not plan.sharing_pays((4,), (63,), block)         # long ones from a third on
     assert not plan.sharing_pays((2,), (64,), block) and not plan.sharing_pays((), (), block)
     assert not plan.sharing_pays((1, 1), (0, 0), block) and not plan.sharing_pays((4,), (100,), 0)
+
+
+def test_the_plan_of_a_prompts_continuations():
+    mixer = SimpleNamespace(num_heads=32, num_kv_heads=8, head_dim=128)
+    assert plan.continuations(torch.bfloat16, mixer, 1, 4096, 16, SMS) is None
+    assert plan.continuations(torch.bfloat16, mixer, 8, 1024, 16, SMS) is None
+    choice = plan.continuations(torch.bfloat16, mixer, 64, 4096, 16, SMS)
+    assert choice == choose([(4096, [4100] * 64)])[1] and choice.wide
+    assert not plan.continuations(torch.float32, SimpleNamespace(num_heads=8, num_kv_heads=8, head_dim=256), 2, 16384, 16, SMS).wide
 
 
 def test_a_captured_plan_has_tiles_for_every_grouping_of_as_many_groups():
