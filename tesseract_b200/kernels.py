@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from functools import lru_cache
 from typing import Optional
 
 import numpy as np
@@ -325,6 +326,7 @@ def attention_shared_wide(dtype: torch.dtype, head_dim: int, page_size: int) -> 
     return bool(load_library("attention_shared").tb_attention_shared_wide(_i32(_code(dtype)), _i32(head_dim), _i32(page_size)))
 
 
+@lru_cache(maxsize=None)
 def attention_shared_tile(dtype: torch.dtype, wide: bool = False) -> int:
     """Folded rows (rows of a group times query heads per kv head) that a block of ``attention_shared`` takes."""
     return load_library("attention_shared").tb_attention_shared_tile(_i32(_code(dtype)), _i32(1 if wide else 0))
@@ -353,6 +355,9 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
     _need(cache.is_contiguous() and cache.shape[1:] == (2, num_kv_heads, page_size, head_dim), "cache layout")
     _need(shared.members.numel() == rows == shared.common.numel(), "shared: a place for every row")
     _need(scale > 0.0, "the scale of the scores must be positive")
+    _need(not choice.prefix_parts or num_heads % num_kv_heads == 0
+          and choice.tiles >= shared.tiles(num_heads // num_kv_heads, attention_shared_tile(dtype, choice.wide)),
+          "choice: fewer tiles than the groups have")
     parts, at = rows * num_heads * (choice.prefix_parts + choice.tail_parts), 0
     if choice.prefix_parts or choice.tail_parts > 1:
         scratch = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)

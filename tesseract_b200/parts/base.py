@@ -309,10 +309,18 @@ class SharedRows:
     # common (None: they hold just these)
     room: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
+    counted: Dict = field(default_factory=dict)    # what ``tiles`` did
 
     def addresses(self) -> Tuple[int, ...]:
         return (self.members.data_ptr(), self.group_start.data_ptr(), self.leader.data_ptr(), self.prefix.data_ptr(),
                 self.common.data_ptr())
+
+    def tiles(self, fold: int, tile: int) -> int:
+        """Tiles of ``tile`` folded rows (``fold`` a row) of the groups that have keys in common."""
+        count = self.counted.get((fold, tile))
+        if count is None:
+            count = self.counted[fold, tile] = sum(-(-n * fold // tile) for n, b in zip(self.sizes, self.blocks) if b)
+        return count
 
     @classmethod
     def of(cls, groups: Sequence[Sequence[int]], prefixes: Sequence[int], positions: Sequence[int], device) -> "SharedRows":

@@ -283,6 +283,10 @@ def test_refusals():
                         ("shared", small.shared), ("scale", 0.0), ("scale", -1.0), ("scale", math.nan)]:
         with pytest.raises(kernels.KernelError):
             kernels.attention_shared(**{**good, name: value})
+    many = Case([(1030, [1040] * 40)], 8, 2, 64)
+    short = type(many.choice())(**{**many.choice().__dict__, "tiles": many.choice().tiles - 1})
+    with pytest.raises(kernels.KernelError, match="tiles"):
+        many.run(short)
     for dim in (8, 24, 272):
         with pytest.raises(kernels.KernelError):
             kernels.attention_shared(torch.zeros(2, 8 * dim, device="cuda"), torch.zeros(2, 8 * dim, device="cuda"),
