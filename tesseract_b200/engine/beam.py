@@ -93,8 +93,12 @@ class BeamSearch:
         self.stepper, self.cache = stepper, stepper.cache
         self.width, self.max_tokens, self.end_ids = width, max_tokens, end_ids
         self.length_penalty, self.portion = length_penalty, max(1, portion)
-        # (every beam may bring one that ends it among its first; twice the width leaves enough that go on)
-        self.top = min(2 * width, vocab)
+        # Of a beam's first tokens as many may end it as there are ids that do, and behind them `width` may have to go on.  Where
+        # that is more than one call ranks, those that go on are ranked by themselves as well.
+        ends = sorted(t for t in end_ids if 0 <= t < vocab)
+        listed = min(max(2 * width, width + len(ends)), vocab)
+        self.top = min(listed, kernels.MAX_ALTERNATIVES)
+        self._apart = ends if listed > self.top else []
         self._names = 0
 
     # ------------------------------------------------------------------ room
@@ -173,7 +177,18 @@ class BeamSearch:
         """Per row: the most probable tokens and their log probabilities, on the host."""
         none = torch.zeros(logits.shape[0], dtype=torch.int32, device=logits.device)
         _, _, values, ids = kernels.token_logprobs(logits, none, self.top)
-        return ids.tolist(), values.double().tolist()
+        ids, values = ids.tolist(), values.double().tolist()
+        if not self._apart:
+            return ids, values
+        others = logits.index_fill(1, torch.tensor(self._apart, device=logits.device), -math.inf)
+        best = kernels.token_logprobs(others, none, self.width)[3]
+        logs = [kernels.token_logprobs(logits, column.contiguous())[0].double().tolist() for column in best.unbind(1)]
+        for row, more in enumerate(best.tolist()):
+            ranked = dict(zip(ids[row], values[row]))
+            ranked.update((token, logs[k][row]) for k, token in enumerate(more))
+            ids[row] = sorted(ranked, key=lambda token: (-ranked[token], token))
+            values[row] = [ranked[token] for token in ids[row]]
+        return ids, values
 
     def _advance(self, searches: List[_Search], done: Dict[int, List[BeamOutput]]) -> List[_Search]:
         """Close what is done, then one step of all beams of the others."""

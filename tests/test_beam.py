@@ -179,3 +179,48 @@ def test_fewer_tokens_than_beams():
 def test_perplexity_of_nothing_and_of_something():
     assert TokenScores([1], [], []).perplexity == 1.0
     assert TokenScores([1, 2, 3], [math.log(0.5), math.log(0.125)], [0.0, 0.0]).perplexity == pytest.approx(4.0)
+
+
+def whole_search(prompt, width, max_tokens, ends, logits):
+    """The same with every token of every beam ranked: the best `width` that go on, and those that end among the best `width`."""
+    beams, finished = [([], 0.0)], []
+    while beams and len(finished) < width and len(beams[0][0]) < max_tokens:
+        every = []
+        for place, (tokens, total) in enumerate(beams):
+            logs = log_softmax(logits(list(prompt) + tokens))
+            order = sorted(range(VOCAB), key=lambda t: (-logs[t], t))
+            every += [(-(total + logs[t]), place, rank, t) for rank, t in enumerate(order)]
+        every.sort()
+        finished += [(beams[place][0] + [t], -negative) for negative, place, _, t in every[:width] if t in ends]
+        beams = [(beams[place][0] + [t], -negative) for negative, place, _, t in every if t not in ends][:width]
+    if beams and len(beams[0][0]) >= max_tokens:
+        finished += beams
+    return sorted(finished, key=lambda f: -f[1])[:width]
+
+
+@pytest.mark.parametrize("width, ends", [(2, (1, 4, 9)), (2, tuple(range(2, 12))), (3, (0, 5, 6, 7, 8, 20)), (4, tuple(range(6, 20))),
+                                         (5, (3, 4, 30, -1, 7, 9, 10, 11))])
+def test_many_ids_that_end_a_beam_leave_the_others_their_places(width, ends):
+    """Where most of a beam's best tokens end it, its next ones go on all the same."""
+    valid = [t for t in ends if 0 <= t < VOCAB]
+    others = [t for t in range(VOCAB) if t not in ends]
+
+    def ending(tokens):
+        row = 0.01 * logits_of(tokens)
+        if len(tokens) == 3:                                   # first: one that goes on, all that end, then the others
+            row[valid] += 4.5
+            row[others] += 4.0
+            row[others[0]] += 1.0
+        elif tokens[3] != others[0]:                           # (the others' next token is certain, the first one's is not)
+            row[others[tokens[0] % len(others)]] += 20.0
+        return row
+
+    stepper = FakeStepper(logits=ending)
+    prompts = [[k, 2 * k % VOCAB, 5] for k in range(12)]
+    shorter = 0
+    for prompt, outs in zip(prompts, HostSearch(stepper, width, 7, end_ids=frozenset(ends)).run(prompts)):
+        want = whole_search(prompt, width, 7, set(ends), ending)
+        assert [o.token_ids for o in outs] == [tokens for tokens, _ in want]
+        assert [o.score for o in outs] == pytest.approx([value for _, value in want], abs=1e-9)
+        shorter += [t for t, _ in plain_search(prompt, width, 7, set(ends), 0.0, ending)] != [t for t, _ in want]
+    assert shorter                                         # (twice the width of a beam's tokens is not enough for these)

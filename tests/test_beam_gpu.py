@@ -256,3 +256,34 @@ def test_the_command_line_scores_and_searches(model_folders):
     assert [b["beam"] for b in beams] == [0, 1, 2] and all(len(b["token_ids"]) == 4 for b in beams)
     (scored,) = run("--score")
     assert len(scored["logprobs"]) == 3 and scored["perplexity"] > 1.0
+
+
+@pytest.mark.parametrize("width, ends", [(2, range(3, 13)), (4, range(0, 380)), (4, range(0, 200)), (32, range(0, 320, 3))])
+def test_ids_that_end_a_beam_beyond_those_one_call_ranks(model_folders, width, ends):
+    """Up to more ends than a ranking holds: what goes on and what ends is what the ranking of the whole vocabulary says."""
+    folder, steps, ends = model_folders("b"), 4, set(ends)
+    config, tensors = llama.load_folder(folder)
+    prompt = random_tokens(config["vocab_size"], 20, seed=width)
+    outs = engine(folder, max_running=40).beam_search([prompt], width, steps, stop_token_ids=sorted(ends), ignore_eos=True)[0]
+    beams, finished, margin = [([], 0.0)], [], math.inf
+    while beams and len(finished) < width and len(beams[0][0]) < steps:
+        every = []
+        for tokens, total in beams:
+            logs = log_softmax(llama.forward(config, tensors, prompt + tokens)[-1].numpy())
+            every += [(-(total + logs[t]), tokens + [t]) for t in range(config["vocab_size"])]
+        every.sort()
+        going = [(tokens, -negative) for negative, tokens in every if tokens[-1] not in ends]
+        margin = min([margin, every[width][0] - every[width - 1][0]] + [a[1] - b[1] for a, b in zip(going[width - 1:], going[width:])][:1])
+        finished += [(tokens, -negative) for negative, tokens in every[:width] if tokens[-1] in ends]
+        beams = going[:width]
+    if beams and len(beams[0][0]) >= steps:
+        finished += beams
+    want = sorted(finished, key=lambda f: -f[1])
+    margin = min([margin] + [a[1] - b[1] for a, b in zip(want, want[1:width + 1])])
+    for out in outs:
+        logs = log_softmax(llama.forward(config, tensors, prompt + out.token_ids).numpy())
+        scored = [logs[len(prompt) + k - 1, token] for k, token in enumerate(out.token_ids)]
+        assert np.abs(np.asarray(out.token_logprobs) - scored).max() < 1e-4
+    assert len(outs) == min(width, len(want))
+    if margin > 1e-4:                                  # (32-bit logits of these models are off by less than a tenth of that)
+        assert [out.token_ids for out in outs] == [tokens for tokens, _ in want[:width]]
