@@ -634,10 +634,11 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + kBlock;
     auto tmem_p = [&](int j) { return tmem_o + D + (j & 1) * (kBlock / 2); };
     constexpr uint32_t kStageStep = kBlockBytes >> 4;       // a ring stage further, in the units of a descriptor's address
+    int asked_keys = 0, asked_values = 0;                         // blocks that copies were issued for (warp 5)
+    int products = 0;                                             // and products (warps 4 and 6)
 
     if (warp == 5) {
         bool ok = true;
-        int asked_keys = 0, asked_values = 0;                     // blocks that copies were issued for
         // block `it` of keys (or values) into its slot, from the pages that the lanes' keys lie in
         auto bring = [&](int it, int page, uint32_t full, uint32_t empty, uint32_t tiles, int which, int& asked) {
             const int s = it % STAGES;
@@ -676,10 +677,6 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
             abort_flag = 1;
             atomicExch(p.error, 110);
         }
-        if (!ok || abort_flag) {                                  // (no copy lands in a block that has left)
-            for (int it = max(0, asked_keys - STAGES); it < asked_keys; ++it) settle(k_full + 8 * (it % STAGES), (it / STAGES) & 1);
-            for (int it = max(0, asked_values - STAGES); it < asked_values; ++it) settle(v_full + 8 * (it % STAGES), (it / STAGES) & 1);
-        }
     } else if (warp == 4) {
         if (lane == 0) {
             constexpr uint32_t idesc_qk = idesc_bf16(kTcRows, kBlock, 0);
@@ -702,6 +699,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                             k_desc + (((kk >> 2) * kSlice + (kk & 3) * 32) >> 4), idesc_qk, kk != 0);
                 umma_commit(s_full);
                 umma_commit(k_empty + 8 * s);
+                ++products;
                 if (++s == STAGES) { s = 0; parity ^= 1; }
             }
             if (!ok) {
@@ -728,6 +726,7 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
                     umma_ts(tmem_o, tmem_p(j) + kk * 8, v_desc + ((kk * 2048) >> 4), idesc_pv, kk != 0 || j != 0);
                 umma_commit(o_full(j));
                 umma_commit(v_empty + 8 * s);
+                ++products;
                 if (++s == STAGES) { s = 0; parity ^= 1; }
             }
             if (!ok) {
@@ -852,6 +851,17 @@ __device__ void attend_tc(const SharedParams& p, const Work& w, const CUtensorMa
     }
     tc_fence_before();
     __syncthreads();
+    if (abort_flag) {
+        // A wait has run out, perhaps after the warps that issue had left their loops: what is under way is waited for here, where
+        // nothing is issued any more, so that no copy or product touches memory that this block has given back.
+        if (warp == 5) {
+            for (int it = max(0, asked_keys - STAGES); it < asked_keys; ++it) settle(k_full + 8 * (it % STAGES), (it / STAGES) & 1);
+            for (int it = max(0, asked_values - STAGES); it < asked_values; ++it) settle(v_full + 8 * (it % STAGES), (it / STAGES) & 1);
+        } else if (products > 0) {
+            settle((warp == 4 ? k_empty : v_empty) + 8 * ((products - 1) % STAGES), ((products - 1) / STAGES) & 1);
+        }
+        __syncthreads();
+    }
     if (warp == 4) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Tiles::kColumns) : "memory");

@@ -120,3 +120,20 @@ def test_tensor_memory_that_a_product_used_is_touched_behind_a_fence():
             touches += 1
             assert not waiting
     assert waits == 2 and touches >= 5                                # (o_full is waited for in product_done alone)
+
+
+def test_what_is_under_way_is_waited_for_before_a_block_that_gave_up_leaves():
+    """attend_tc: whichever warp's wait runs out, and whenever, the copies and products that others have issued are waited for once
+    nobody issues any more (behind a barrier of the whole block), and in front of the barrier behind which tensor memory goes back."""
+    with open(os.path.join(CSRC, "attention_shared.cu")) as handle:
+        code = re.sub(r"//[^\n]*", "", handle.read())
+    body = code[code.index("__device__ void attend_tc"):code.index("shared_tc_kernel")]
+    barriers = [m.start() for m in re.finditer(r"__syncthreads\(\)", body)]
+    issued = [m.start() for m in re.finditer(r"tma_load_kv\(|umma_ss\(|umma_ts\(|umma_commit\(", body)]
+    settled = [m.start() for m in re.finditer(r"settle\(", body)]
+    last, before = barriers[-1], barriers[-2]
+    assert max(issued) < before < min(settled) < max(settled) < last < body.index("tcgen05.dealloc")
+    given_up = body[before:last]
+    assert re.match(r"__syncthreads\(\);\s*if \(abort_flag\) \{", given_up)
+    for barrier in ("k_full", "v_full", "k_empty", "v_empty"):
+        assert barrier in given_up
