@@ -298,6 +298,7 @@ SHARED_MAX_PARTS = 64
 
 # Blocks of 64 keys that rows need not read themselves from where on common parts are taken by themselves: below, one launch over
 # every row's own keys is faster (4 rows of 32 heads of 64 at 200 keys: 4.2 us on the device, 7.0 with a launch to put parts together).
+# Blocks of many or large heads are worth it from fewer on: wherever a decode step would share (`sharing_pays`), its plan does.
 SHARED_MIN_SAVED = 64
 # The same in bytes of keys and values from where on a decode step takes ``attention_shared`` at all: below, the kernel that rotates,
 # writes and attends in one launch is faster, as it finds the common pages in L2.  Behind many keys in common a third of that: that
@@ -328,6 +329,11 @@ SHARED_WIDE_MIN_F32 = {64: 64, 128: 64, 256: 460}
 # the 32-bit one with the small.
 SHARED_WIDE_RESIDENT = {torch.bfloat16: {64: 2, 128: 2, 256: 1}, torch.float32: {64: 4, 128: 3, 256: 2}}
 SHARED_F32_RESIDENT = {64: 4, 128: 4, 256: 2}
+
+
+def shared_block_bytes(dtype: torch.dtype, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of the keys and values of a block of 64 tokens in one layer."""
+    return 64 * 2 * num_kv_heads * head_dim * torch.empty((), dtype=dtype).element_size()
 
 
 def saved_blocks(sizes: Sequence[int], blocks: Sequence[int]) -> int:
@@ -368,7 +374,8 @@ def _shared_runs(tiles: np.ndarray, blocks: np.ndarray, target: int, shortest: i
 def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sms) -> SharedAttentionPlan:
     sizes, blocks = np.asarray(shared.sizes), np.asarray(shared.blocks)
     tails = np.asarray(shared.tails)
-    if saved_blocks(shared.sizes, shared.blocks) < SHARED_MIN_SAVED:        # every row reads its own
+    if (saved_blocks(shared.sizes, shared.blocks) < SHARED_MIN_SAVED        # every row reads its own
+            and not sharing_pays(shared.sizes, shared.blocks, shared_block_bytes(dtype, num_kv_heads, head_dim))):
         tails = tails + np.asarray(shared.row_blocks)
         blocks = np.zeros_like(blocks)
     rows = np.where(blocks > 0, sizes * fold, 0)
@@ -417,8 +424,7 @@ def continuations(dtype, mixer, rows: int, context: int, page_size: int, sms: Op
     """The plan of a decode step of ``rows`` continuations of one prompt of ``context`` tokens, if it reads their common keys once."""
     common = context // 64
     shared = SimpleNamespace(sizes=(rows,), blocks=(common,), tails=(1,) * rows, row_blocks=(common,) * rows, room=None, plans={})
-    block_bytes = 64 * 2 * mixer.num_kv_heads * mixer.head_dim * torch.empty((), dtype=dtype).element_size()
-    if not sharing_pays(shared.sizes, shared.blocks, block_bytes):
+    if not sharing_pays(shared.sizes, shared.blocks, shared_block_bytes(dtype, mixer.num_kv_heads, mixer.head_dim)):
         return None
     return shared_attention(dtype, num_heads=mixer.num_heads, num_kv_heads=mixer.num_kv_heads, head_dim=mixer.head_dim,
                             page_size=page_size, shared=shared, sms=sms)

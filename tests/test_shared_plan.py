@@ -137,3 +137,21 @@ def test_what_is_under_way_is_waited_for_before_a_block_that_gave_up_leaves():
     assert re.match(r"__syncthreads\(\);\s*if \(abort_flag\) \{", given_up)
     for barrier in ("k_full", "v_full", "k_empty", "v_empty"):
         assert barrier in given_up
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 64), (32, 8, 128), (32, 32, 128), (32, 32, 256), (64, 16, 128), (8, 8, 256),
+                                                  (16, 1, 128), (48, 48, 80)])
+def test_a_step_that_leaves_the_ordinary_path_shares(heads, kv_heads, dim, dtype):
+    """Wherever ``sharing_pays`` sends a decode step here, its plan reads keys in common once; large blocks pay from few on."""
+    block_bytes = 64 * 2 * kv_heads * dim * (2 if dtype == torch.bfloat16 else 4)
+    assert plan.shared_block_bytes(dtype, kv_heads, dim) == block_bytes
+    paid = few = 0
+    for rows in (2, 3, 4, 8, 31, 64):
+        for blocks in (1, 2, 5, 12, 15, 33, 63, 64, 65, 200):
+            shared, choice = choose([(64 * blocks, [64 * blocks + 10] * rows)], heads, kv_heads, dim, dtype)
+            if plan.sharing_pays(shared.sizes, shared.blocks, block_bytes):
+                assert choice.prefix_parts > 0 and choice.tiles > 0
+                paid += 1
+                few += plan.saved_blocks(shared.sizes, shared.blocks) < plan.SHARED_MIN_SAVED
+    assert paid and (few > 0) == (block_bytes * (plan.SHARED_MIN_SAVED - 1) >= plan.SHARED_MIN_BYTES)
