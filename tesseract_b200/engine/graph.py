@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from .. import kernels
-from ..parts.base import GroupView, SharedRows, StepContext
+from ..parts.base import SHARED_BLOCK, GroupView, SharedRows, StepContext
 from .step import StepEntry, Stepper
 
 
@@ -109,7 +109,10 @@ class _Graph:
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=device)   # this step's token ids, chosen on the device
         groups: List[GroupView] = []
         tables = dict(zip(self.paged, self.d["tables"]))
-        shared = SharedRows(*self.d["together"], *company[1:], room=batch if any_sizes else None) if company is not None else None
+        shared = None
+        if company is not None:
+            shared = SharedRows(*self.d["together"], *company[1:], room=batch if any_sizes else None,
+                                reach=-(-columns * cache.page_size // SHARED_BLOCK))
         for index, g in enumerate(cache.groups):
             groups.append(GroupView(tables.get(index), cache.page_size if g.pool is not None else 0,
                                     shared if shared is not None and cache.shares_keys(index) else None))

@@ -308,6 +308,8 @@ class SharedRows:
     # rows that the tensors have room for, where a captured step refills them with other groupings of as many groups with keys in
     # common (None: they hold just these)
     room: Optional[int] = None
+    # and the blocks that a row of its block tables can name (None: the lengths are those above)
+    reach: Optional[int] = None
     plans: Dict = field(default_factory=dict)      # what ``plan.shared_attention`` answered for these rows
     counted: Dict = field(default_factory=dict)    # what ``tiles`` did
 

@@ -331,6 +331,19 @@ SHARED_WIDE_RESIDENT = {torch.bfloat16: {64: 2, 128: 2, 256: 1}, torch.float32: 
 SHARED_F32_RESIDENT = {64: 4, 128: 4, 256: 2}
 
 
+# A captured step keeps its plan while keys in common and rows' own grow within its tables' width.  So it is laid out for as many runs
+# as a fresh plan gives the longest that the table can name (the common parts in the proportions that they have), and shorter ones
+# are cut into as many as they have blocks for.  What it cannot know is how much of the chip the other kind takes: common parts that
+# share a launch with rows' own leave them two fifths, and rows' own in front of a launch of large tiles begin a second run only at
+# 1,024 keys.  Device time of a plan kept from right behind the fork, of a fresh one and of a captured one, us: 32 heads on 8 of 64, 4
+# rows at 4,160 keys in common and 16 of their own 9.4, 9.4 and 9.9, 4,000 27.3, 17.5 and 17.5, at 8,256 and 8,092 49.9, 25.2 and 23.4;
+# of 128, 8 rows at 4,160 and 500 16.3, 20.3 and 16.5, 4,000 49.2, 36.9 and 37.0; in 32 bits, 8 rows of 64 at 4,160 and 16 23.1, 23.1
+# and 29.4 (blocks without a run of their own), 4,000 233, 63 and 63.
+CAPTURED_ROOM = 0.6
+CAPTURED_TAIL_RUN = 4
+CAPTURED_TAIL_RUN_WIDE = 16          # bfloat16, head sizes up to 128
+
+
 def shared_block_bytes(dtype: torch.dtype, num_kv_heads: int, head_dim: int) -> int:
     """Bytes of the keys and values of a block of 64 tokens in one layer."""
     return 64 * 2 * num_kv_heads * head_dim * torch.empty((), dtype=dtype).element_size()
@@ -378,6 +391,10 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
             and not sharing_pays(shared.sizes, shared.blocks, shared_block_bytes(dtype, num_kv_heads, head_dim))):
         tails = tails + np.asarray(shared.row_blocks)
         blocks = np.zeros_like(blocks)
+    captured = shared.reach is not None
+    if captured:
+        tails = np.full_like(tails, shared.reach)
+        blocks = -(-blocks * shared.reach // max(1, int(blocks.max())))
     rows = np.where(blocks > 0, sizes * fold, 0)
     sixteens = -(-rows // 16)
     padded = 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256            # (a kernel's head size)
@@ -400,6 +417,8 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     shortest = 1 if wide and dtype == torch.float32 else SHARED_MIN_RUN[dtype]
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
+    if captured:
+        tail_run = CAPTURED_TAIL_RUN_WIDE if wide and dtype != torch.float32 and padded <= 128 else CAPTURED_TAIL_RUN
     prefix_parts, prefix_run = 0, 1
     if tiles.any():
         room = target
@@ -408,9 +427,11 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
         else:                                   # in one launch with the rows' own: at once with them where those are much of the work
             left = target - int((tail_tiles * -(-tails // tail_run)).sum())
             few = int((tiles * blocks).sum()) > 4 * int((tail_tiles * tails).sum())
-            room = target if few or 2 * left < target else left
+            room = int(target * CAPTURED_ROOM) if captured else target if few or 2 * left < target else left
         prefix_run = _shared_runs(tiles, blocks, room, shortest)
         prefix_parts = min(SHARED_MAX_PARTS, -(-int(blocks.max()) // prefix_run))
+        if captured:                            # (a table is chosen for rows of more than half its width)
+            prefix_run = _shared_runs(tiles, -(-blocks // 2), room, shortest)
     # (tensors that are refilled with other groupings of so many rows in as many groups: none has more tiles, as a group's last tile
     # holds at least what both a tile and a row's heads are multiples of)
     count = int(tiles.sum())
@@ -423,7 +444,8 @@ def continuations(dtype, mixer, rows: int, context: int, page_size: int, sms: Op
                   ) -> Optional[SharedAttentionPlan]:
     """The plan of a decode step of ``rows`` continuations of one prompt of ``context`` tokens, if it reads their common keys once."""
     common = context // 64
-    shared = SimpleNamespace(sizes=(rows,), blocks=(common,), tails=(1,) * rows, row_blocks=(common,) * rows, room=None, plans={})
+    shared = SimpleNamespace(sizes=(rows,), blocks=(common,), tails=(1,) * rows, row_blocks=(common,) * rows, room=None, reach=None,
+                             plans={})
     if not sharing_pays(shared.sizes, shared.blocks, shared_block_bytes(dtype, mixer.num_kv_heads, mixer.head_dim)):
         return None
     return shared_attention(dtype, num_heads=mixer.num_heads, num_kv_heads=mixer.num_kv_heads, head_dim=mixer.head_dim,

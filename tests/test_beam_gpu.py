@@ -287,3 +287,43 @@ def test_ids_that_end_a_beam_beyond_those_one_call_ranks(model_folders, width, e
     assert len(outs) == min(width, len(want))
     if margin > 1e-4:                                  # (32-bit logits of these models are off by less than a tenth of that)
         assert [out.token_ids for out in outs] == [tokens for tokens, _ in want[:width]]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_captured_step_whose_rows_grow(tmp_path, monkeypatch, dtype):
+    """A group captured right behind its fork whose rows' own keys grow to many blocks: the same graph, against steps of twins launch
+    by launch that share nothing."""
+    from tesseract_b200 import plan
+    from tesseract_b200.engine import StepEntry
+
+    from tesseract_b200.weights.random_init import write_random_model
+
+    monkeypatch.setattr(plan, "SHARED_MIN_SAVED", 0)
+    folder = write_random_model(str(tmp_path), dict(TINY["b"], max_position_embeddings=4096, torch_dtype="float32"), 3)
+    llm = engine(folder, dtype, kv_capacity_tokens=32768)
+    stepper, cache = llm.stepper, llm.stepper.cache
+    prompt = random_tokens(384, 1090, seed=1)
+    for twin in "ab":
+        assert cache.admit((twin, 0), reserve_tokens=2040)
+        for k in range(0, len(prompt), 64):
+            stepper.step([StepEntry((twin, 0), prompt[k:k + 64], [])])
+        assert cache.fork([((twin, 0), (twin, k)) for k in range(1, 4)], reserve_tokens=2040)
+    for own in (0, 1, 60, 130, 300, 700, 940):
+        for k in range(4):                             # (a portion a row, up to the next step that is compared; row 3 stays behind)
+            grown = own - (cache.length(("a", k)) - len(prompt)) if k < 3 else 0
+            tokens = random_tokens(384, max(1, grown), seed=own + k)
+            for twin in "ab":
+                for at in range(0, grown, 64):
+                    stepper.step([StepEntry((twin, k), tokens[at:min(at + 64, grown)], [])])
+        tokens = random_tokens(384, 4, seed=own + 9)
+        entries = {twin: [StepEntry((twin, k), [tokens[k]], [0]) for k in range(4)] for twin in "ab"}
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 0)
+        launch = stepper.graphs.launch(entries["a"], [0.0] * 4, [0.0] * 4)
+        got = launch.graph.logits[:launch.count].clone()
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 1 << 60)
+        want = stepper.step(entries["b"])
+        assert float((got - want).abs().max()) <= REL[dtype] * float(want.abs().max())
+    (graph,) = stepper.graphs.shared_graphs.values()   # (one capture serves all)
+    shared = next(view.shared for view in graph.ctx.groups if view.shared is not None)
+    (choice,) = shared.plans.values()
+    assert choice.tail_parts > 4 and choice.prefix_parts > 4

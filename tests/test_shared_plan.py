@@ -155,3 +155,50 @@ def test_a_step_that_leaves_the_ordinary_path_shares(heads, kv_heads, dim, dtype
                 paid += 1
                 few += plan.saved_blocks(shared.sizes, shared.blocks) < plan.SHARED_MIN_SAVED
     assert paid and (few > 0) == (block_bytes * (plan.SHARED_MIN_SAVED - 1) >= plan.SHARED_MIN_BYTES)
+
+
+def cut(blocks, parts, run):
+    """How the kernel cuts a row's or a common part's blocks: how many runs, and the blocks of one."""
+    if blocks == 0:
+        return 0, 0
+    n = min(parts, -(-blocks // run))
+    each = -(-blocks // n)
+    return -(-blocks // each), each
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 64), (32, 8, 128), (8, 2, 256), (20, 4, 80)])
+@pytest.mark.parametrize("rows", [2, 4, 8, 16, 32])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_a_captured_plan_is_as_good_for_later_steps(groups, rows, heads, kv_heads, dim, dtype):
+    """A step is captured right behind a fork; its rows then grow, and its groups share more, within its tables' width: a row's
+    own keys are cut into runs of 1,024 or about those of a plan made for that step, its common part into runs that leave room for rows'
+    own beside them."""
+    def made(common, own, reach=None):
+        prefixes = [64 * common * (k + 2) // (groups + 1) // 64 * 64 for k in range(groups)]
+        shared, fresh = choose([(p, [p + 64 * own - 9] * rows) for p in prefixes], heads, kv_heads, dim, dtype)
+        if reach is None:
+            return shared, fresh
+        shared.reach, shared.plans = reach, {}
+        return shared, plan.shared_attention(dtype, num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, page_size=16, shared=shared,
+                                             sms=SMS)
+
+    for reach in (64, 128, 512):
+        shared, captured = made(reach // 2 + 1, 1, reach)
+        assert captured == made(reach // 2 + 1, reach // 2 - 1, reach)[1]
+        if plan.saved_blocks(shared.sizes, shared.blocks) < plan.SHARED_MIN_SAVED:
+            continue
+        assert captured.prefix_parts > 0
+        for common in (reach // 2 + 1, 3 * reach // 4, reach - 2):
+            for own in sorted({1, 2, 5, reach // 8, reach // 3, reach - common}):
+                if common + own > reach:
+                    continue
+                shared, fresh = made(common, own)
+                if fresh.wide != captured.wide or fresh.prefix_parts == 0:
+                    continue                                            # (near the threshold; both sides' times are there)
+                mine, best = cut(own, captured.tail_parts, captured.tail_run), cut(own, fresh.tail_parts, fresh.tail_run)
+                assert mine[1] <= max(16, best[1] + 1, 1.25 * best[1]) and mine[0] <= best[0] + max(1, best[0] // 4)
+                mine = [cut(b, captured.prefix_parts, captured.prefix_run) for b in shared.blocks]
+                best = [cut(b, fresh.prefix_parts, fresh.prefix_run) for b in shared.blocks]
+                assert max(r for _, r in mine) <= 2 * max(r for _, r in best) + 1
+                assert sum(n for n, _ in mine) <= 2 * sum(n for n, _ in best) + groups
