@@ -372,6 +372,10 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, po
         choice.tiles, choice.prefix_parts, choice.prefix_run, choice.tail_parts, choice.tail_run, choice.warps, choice.wide,
         cache.shape[0], _code(dtype), scale)
     _check(_entry("attention_shared", "tb_attention_shared", _ATTENTION_SHARED)(call, _raw_stream()), "attention_shared")
+    if at:
+        global launch_count
+        # (rows' own keys, or all in small tiles; common parts in large ones; the runs put together)
+        launch_count += 2 if choice.wide and choice.tiles and choice.prefix_parts else 1
     return out
 
 

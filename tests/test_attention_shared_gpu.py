@@ -292,3 +292,28 @@ def test_refusals():
             kernels.attention_shared(torch.zeros(2, 8 * dim, device="cuda"), torch.zeros(2, 8 * dim, device="cuda"),
                                      torch.zeros(20, 2, 2, 16, dim, device="cuda"), case.positions, case.table, case.shared, 8, 2, dim,
                                      16, 1.0, case.choice())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prefix_parts, tail_parts, wide, kernels_run", [(0, 1, False, 1), (0, 1, True, 1), (0, 3, False, 2), (0, 3, True, 2),
+                                                                       (2, 1, False, 2), (2, 3, True, 3)])
+def test_every_kernel_of_a_call_is_counted(prefix_parts, tail_parts, wide, kernels_run, dtype):
+    """One kernel where results are written at once, one more where runs are put together, one more for common parts in large tiles;
+    and those are the kernels that the device saw."""
+    case = Case([(640, [700 + 9 * i for i in range(24)])], 8, 2, 64, dtype=dtype, seed=6)
+    tiles = case.shared.tiles(4, kernels.attention_shared_tile(dtype, wide))
+    choice = plan.SharedAttentionPlan(tiles, prefix_parts, 2, tail_parts, 2, wide)
+    out = torch.empty(case.q.shape, dtype=dtype, device="cuda")
+
+    def call():
+        kernels.attention_shared(case.q, out, case.cache, case.positions, case.table, case.shared, 8, 2, 64, 16, case.scale, choice)
+
+    call()
+    torch.cuda.synchronize()
+    before = kernels.launch_count
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as seen:
+        call()
+        torch.cuda.synchronize()
+    assert kernels.launch_count - before == kernels_run
+    names = [event.name for event in seen.events() if "shared_" in event.name]
+    assert len(names) == kernels_run or not names        # (nothing where the device gives no record)
