@@ -36,6 +36,7 @@ class PagePool:
         # LIFO: the last element is handed out first; start so that low ids go first.
         self._free: List[int] = list(range(first_page + num_pages - 1, first_page - 1, -1))
         self._refs = np.zeros(num_pages, dtype=np.int32)    # holders of each page (from first_page on)
+        self._ref = memoryview(self._refs)                  # the same a page at a time (a tenth of an array operation's time)
         self._quota: Dict[Hashable, int] = {}
         self._drawn: Dict[Hashable, Set[int]] = {}          # pages drawn by the owner (and not given back)
         self._borrowed: Dict[Hashable, Set[int]] = {}       # pages that it shares and others drew
@@ -99,7 +100,7 @@ class PagePool:
             raise OutOfPages(f"cache pool exhausted: {self.num_pages} pages, {len(self._free)} free, "
                              f"{self._reserved_unallocated} reserved for other requests")
         page = self._free.pop()
-        self._refs[page - self.first_page] = 1
+        self._ref[page - self.first_page] = 1
         drawn.add(page)
         return page
 
@@ -118,19 +119,21 @@ class PagePool:
 
     def give_back(self, owner: Hashable, page: int) -> None:
         """Return one page while the owner lives on (a window has passed it)."""
-        drawn, borrowed = self._drawn.get(owner, ()), self._borrowed.get(owner, ())
-        if page in borrowed:
-            borrowed.remove(page)             # (another's draw: no reservation of the owner covers it)
-        elif page not in drawn:
-            raise ValueError(f"page {page} is not held by {owner!r}")
-        elif self._refs[page - self.first_page] > 1:
-            # (the reservation would be owed a page that is not free)
-            raise ValueError(f"page {page} is shared and cannot be given back by the one who drew it before it ends")
-        else:
+        drawn, place = self._drawn.get(owner, ()), page - self.first_page
+        if page in drawn:
+            if self._ref[place] > 1:
+                # (the reservation would be owed a page that is not free)
+                raise ValueError(f"page {page} is shared and cannot be given back by the one who drew it before it ends")
             if len(drawn) <= self._quota[owner]:
                 self._reserved_unallocated += 1   # the reservation covers the peak, so it is owed again
             drawn.remove(page)
-        self._let_go([page])
+        elif page in self._borrowed.get(owner, ()):
+            self._borrowed[owner].remove(page)    # (another's draw: no reservation of the owner covers it)
+        else:
+            raise ValueError(f"page {page} is not held by {owner!r}")
+        self._ref[place] -= 1
+        if self._ref[place] == 0:
+            self._free.append(page)
 
     def _let_go(self, pages: Sequence[int]) -> None:
         """One holder less for each page; those without one are free, in the order given."""

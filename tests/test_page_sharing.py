@@ -1,6 +1,7 @@
 """Pages with several holders, continuations and compaction: nothing lost, freed early or written twice (no GPU needed)."""
 
 import random
+import time
 
 import numpy as np
 import pytest
@@ -291,3 +292,19 @@ def test_random_lives(seed, name):
         cache.release(request)
     assert cache.used_pages() == 0
     cache.check()
+
+
+def test_a_page_given_back_costs_the_host_about_what_drawing_it_did():
+    """A window that moves on gives pages back one at a time: no array operations for each (they took fifteen times a draw)."""
+    pool = PagePool(2000, 1)
+    pool.register("a")
+    ratios = []
+    for _ in range(7):
+        begin = time.perf_counter()
+        pages = [pool.allocate("a") for _ in range(2000)]
+        between = time.perf_counter()
+        for page in pages:
+            pool.give_back("a", page)
+        ratios.append((time.perf_counter() - between) / (between - begin))
+    pool.check()
+    assert pool.used_pages == 0 and min(ratios) < 5
