@@ -332,7 +332,12 @@ class CacheManager:
 
     def compact(self) -> int:
         """Move the pages in use to the lowest ids of every group (one launch); returns how many moved.  The block tables of
-        steps that are built from now on name the new places."""
+        steps that are built from now on name the new places.
+
+        No step needs it (any free page serves any request): it is for a caller of the cache that wants the pages in use together,
+        to save them or to see how small the pool could be.  Steps that were launched on the current stream before finish on the old
+        places, as the copies are behind them; a step that was built but not launched yet names places that are no longer its
+        requests', so there must be none."""
         moves: List[Tuple[List[int], List[int]]] = []
         for index, g in enumerate(self.groups):
             renamed = g.pool.compact() if g.pool is not None else {}

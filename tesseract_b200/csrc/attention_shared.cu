@@ -20,6 +20,9 @@
 //                cores, see there.  A tile of 16 would read a common part from L2 once for every 16 folded rows.
 //   attend_f32, attend_f32_wide   32-bit, tiles of 8 and of 32 folded rows, multiply-adds only, see there.
 // Which form and how many runs: plan.shared_attention, with both sides' times beside its rule.
+// What rounding the weights costs: against 64 bits a result is off by 0.0018 of its size in attend_mma and by up to 0.0023 in
+// attend_tc, whose weights are seldom taken against their own maximum (which rounds without an error); 0.0017 of both is the
+// result's own rounding.  In 32 bits it is 3e-7.
 // Keys beyond a run's end are filled with zeros on the way in and masked, so whatever lies behind a row's last key in its page
 // (numbers of an earlier owner, NaN) reaches nothing.
 #include <cstring>

@@ -11,8 +11,9 @@
 // part each); a block takes its part in chunks of sixteen logits a thread, two chunks' asynchronous copies under way while one is
 // worked on in registers.  Many rows: blocks of 256 threads, four a multiprocessor, so that one row's beginning and end run under the
 // others' loads (1,536 rows of 128,256 logits, one alternative: 133 us, 0.92 of the measured copy rate; 143 where the clocks have fallen
-// under minutes of load); few rows: blocks of 1,024, one chunk each at that vocabulary (64 rows, 20 alternatives: 14.1 us, of which
-// the 33 MB are 5.1, the rest the start, the bound, the second reading and the exchange of a cluster).  Of a chunk
+// under minutes of load); few rows: blocks of 1,024, up to eight a row (64 rows of that vocabulary, 20 alternatives, two blocks of four
+// chunks a row: 14.1 us, of which the 33 MB are 5.1, the rest the start, the bound, the second reading and the exchange of a
+// cluster).  Of a chunk
 //   * every thread adds its numbers to a maximum, S and T of its own (rescaled when its maximum rises), all in 32 bits;
 //     they meet once, at the end, in a fixed order, so a row's numbers do not depend on the timing;
 //   * every eight threads leave the largest of their 128 logits.  No block waits for anything inside the loop.
@@ -366,7 +367,7 @@ logprobs_kernel(const float* __restrict__ logits, int64_t stride, const int* __r
 
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     const int chunks = (end + kChunk - 1) / kChunk;
-    const int span = max(1, (chunks * kGroups + kMaxGroups - 1) / kMaxGroups);       // chunks that a group's largest is taken over (1 up to 1M logits)
+    const int span = max(1, (chunks * kGroups + kMaxGroups - 1) / kMaxGroups);       // chunks that a group's largest is taken over (1 up to 262,144 logits of a part)
     const int group = threadIdx.x / kGroup;
     const int groups = (chunks + span - 1) / span * kGroups;
     if ((int)threadIdx.x < ((groups + 127) & ~127) - groups) sh.group[groups + threadIdx.x] = 0;

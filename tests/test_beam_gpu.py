@@ -327,3 +327,47 @@ def test_a_captured_step_whose_rows_grow(tmp_path, monkeypatch, dtype):
     shared = next(view.shared for view in graph.ctx.groups if view.shared is not None)
     (choice,) = shared.plans.values()
     assert choice.tail_parts > 4 and choice.prefix_parts > 4
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_rule_itself_sends_a_step_to_keys_in_common(tmp_path, monkeypatch, dtype):
+    """With the thresholds as they are: 32 continuations of a long prompt take the path that reads common keys once, in a graph and launch
+    by launch, few do not; results are those of steps that share nothing."""
+    from tesseract_b200 import plan
+    from tesseract_b200.engine import StepEntry
+    from tesseract_b200.weights.random_init import write_random_model
+
+    config = dict(TINY["b"], num_key_value_heads=3, max_position_embeddings=8192, torch_dtype="float32")
+    llm = engine(write_random_model(str(tmp_path), config, 3), dtype, kv_capacity_tokens=16384, max_running=72, max_batch_tokens=512,
+                 prefill_chunk_tokens=512)
+    stepper, cache = llm.stepper, llm.stepper.cache
+    rows, prompt = 32, random_tokens(384, 64 * plan.SHARED_LONG + 70, seed=1)
+    saved = (rows - 1) * (len(prompt) // 64) * cache.shared_block_bytes
+    assert plan.SHARED_MIN_BYTES // 3 <= saved < 4 * plan.SHARED_MIN_BYTES
+    for twin in "ab":
+        assert cache.admit((twin, 0), reserve_tokens=len(prompt) + 20)
+        for k in range(0, len(prompt), 512):
+            stepper.step([StepEntry((twin, 0), prompt[k:k + 512], [])])
+        assert cache.fork([((twin, 0), (twin, k)) for k in range(1, rows)], reserve_tokens=len(prompt) + 20)
+
+    def entries(twin, count, seed):
+        return [StepEntry((twin, k), [token], [0]) for k, token in enumerate(random_tokens(384, count, seed=seed))]
+
+    def alike(got, want):
+        return float((got - want).abs().max()) <= REL[dtype] * float(want.abs().max())
+
+    least = plan.SHARED_MIN_BYTES
+    few = 1 + least // 4 // (len(prompt) // 64 * cache.shared_block_bytes)           # (saves less than a third of the threshold)
+    for step, (count, shares) in enumerate([(rows, True), (few, False), (rows, True)]):
+        assert (stepper.company(entries("a", count, step)) is not None) == shares
+        made = len(stepper.graphs.shared_graphs)
+        if step < 2:
+            launch = stepper.graphs.launch(entries("a", count, step), [0.0] * count, [0.0] * count)
+            got = launch.graph.logits[:count].clone()
+            assert (len(stepper.graphs.shared_graphs) > made) == shares
+        else:
+            got = stepper.step(entries("a", count, step)).clone()
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", 1 << 60)
+        want = stepper.step(entries("b", count, step))
+        monkeypatch.setattr(plan, "SHARED_MIN_BYTES", least)
+        assert alike(got, want)

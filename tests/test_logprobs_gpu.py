@@ -202,3 +202,40 @@ def test_refusals():
                 (logits, tokens.cpu(), 1), (logits[0], tokens, 1)]:
         with pytest.raises(kernels.KernelError):
             kernels.token_logprobs(*bad)
+
+
+@pytest.mark.parametrize("rows", [150, 300])
+@pytest.mark.parametrize("vocab", [262143, 262144, 262145, 262161])
+def test_either_side_of_the_groups_that_a_block_keeps(rows, vocab):
+    """One block a row, of 512 and of 256 threads: up to 262,144 logits of a part each group is one chunk's."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    logits = torch.randn(rows, vocab + 3, generator=gen, device="cuda")[:, :vocab]
+    logits[:, -1] = 9.0                                # (the last logit is the largest)
+    tokens = tokens_for(rows, vocab)
+    got = kernels.token_logprobs(logits, tokens, 40)
+    for r in (0, 1, 2, 3, rows - 1):
+        logs = torch.log_softmax(logits[r].double(), dim=0)
+        order = torch.sort(logits[r], descending=True, stable=True).indices[:40]
+        bound = (16 * vocab / 4096 + 60) * U * 30
+        assert torch.equal(got[3][r].long(), order) and int(order[0]) == vocab - 1
+        assert float((got[2][r].double() - logs[order]).abs().max()) <= bound
+        assert abs(float(got[0][r]) - float(logs[int(tokens[r])])) <= bound
+        assert abs(float(got[1][r]) + float((logs.exp() * logs).sum())) <= bound
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_on_another_stream_and_behind_its_inputs(rows):
+    logits = torch.randn(rows, 30011, device="cuda") * 2
+    tokens = tokens_for(rows, 30011)
+    want = kernels.token_logprobs(logits, tokens, 12)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        late, late_tokens = torch.zeros_like(logits), torch.zeros_like(tokens)
+        torch.cuda._sleep(2_000_000)
+        late.copy_(logits)
+        late_tokens.copy_(tokens)
+        got = kernels.token_logprobs(late, late_tokens, 12)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
