@@ -335,13 +335,13 @@ SHARED_F32_RESIDENT = {64: 4, 128: 4, 256: 2}
 # as a fresh plan gives the longest that the table can name (the common parts in the proportions that they have), and shorter ones
 # are cut into as many as they have blocks for.  What it cannot know is how much of the chip the other kind takes: common parts that
 # share a launch with rows' own leave them two fifths, and rows' own in front of a launch of large tiles begin a second run only at
-# 1,024 keys.  Device time of a plan kept from right behind the fork, of a fresh one and of a captured one, us: 32 heads on 8 of 64, 4
-# rows at 4,160 keys in common and 16 of their own 9.4, 9.4 and 9.9, 4,000 27.3, 17.5 and 17.5, at 8,256 and 8,092 49.9, 25.2 and 23.4;
-# of 128, 8 rows at 4,160 and 500 16.3, 20.3 and 16.5, 4,000 49.2, 36.9 and 37.0; in 32 bits, 8 rows of 64 at 4,160 and 16 23.1, 23.1
-# and 29.4 (blocks without a run of their own), 4,000 233, 63 and 63.
+# so many blocks, up to a head size.  Device time of a plan kept from right behind the fork, of a fresh one and of a captured one, us:
+# 32 heads on 8 of 64, 4 rows at 4,160 keys in common and 16 of their own 9.4, 9.4 and 9.9, 4,000 27.3, 17.5 and 17.5, at 8,256 and
+# 8,092 49.9, 25.2 and 23.4; of 128, 8 rows at 4,160 and 500 16.3, 20.3 and 16.5, 4,000 49.2, 36.9 and 37.0; in 32 bits, 8 rows of 64
+# at 4,160 and 16 23.1, 23.1 and 29.4 (blocks of threads that find no run), 4,000 231, 63 and 63.
 CAPTURED_ROOM = 0.6
-CAPTURED_TAIL_RUN = 4
-CAPTURED_TAIL_RUN_WIDE = 16          # bfloat16, head sizes up to 128
+CAPTURED_TAIL_RUN = {torch.bfloat16: 16, torch.float32: 4}
+CAPTURED_TAIL_RUN_UP_TO = {torch.bfloat16: 128, torch.float32: 256}
 
 
 def shared_block_bytes(dtype: torch.dtype, num_kv_heads: int, head_dim: int) -> int:
@@ -418,7 +418,9 @@ def _shared_attention(dtype, fold, num_kv_heads, head_dim, page_size, shared, sm
     tail_run = _shared_runs(tail_tiles, tails, target if warps == 0 else small * target, SHARED_MIN_RUN[dtype])
     tail_parts = min(SHARED_MAX_PARTS, -(-int(tails.max()) // tail_run))
     if captured:
-        tail_run = CAPTURED_TAIL_RUN_WIDE if wide and dtype != torch.float32 and padded <= 128 else CAPTURED_TAIL_RUN
+        tail_run = SHARED_MIN_RUN[dtype]
+        if wide and padded <= CAPTURED_TAIL_RUN_UP_TO[dtype]:
+            tail_run = CAPTURED_TAIL_RUN[dtype]
     prefix_parts, prefix_run = 0, 1
     if tiles.any():
         room = target
