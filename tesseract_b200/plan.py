@@ -303,9 +303,9 @@ SHARED_MIN_SAVED = 64
 # The same in bytes of keys and values from where on a decode step takes ``attention_shared`` at all: below, the kernel that rotates,
 # writes and attends in one launch is faster, as it finds the common pages in L2.  Behind many keys in common a third of that: that
 # kernel's runs are longer then.  A step with and without, ms: of the 1B sizes, 8 rows at 2,048 keys (29 MB) 0.756 and 0.702, 16 at 2,048
-# (63) 0.852 and 0.839, 8 at 6,144 (88) 0.801 and 0.843, 32 at 2,048 (130) 0.993 and 1.068, 32 at 8,192 1.090 and 1.922; 4 at 4,096 (25)
-# 0.744 and 0.802, 8 at 4,096 (59) 0.776 and 0.772, 2 at 16,000 (33) 0.795 and 0.798; of 8 layers of the 8B sizes, 16 at 1,024 (63)
-# 1.064 and 1.056, 8 at 3,072 (88) 0.986 and 0.990, 4 at 4,096 (50) 0.961 and 1.011, 32 at 8,192 1.135 and 2.099.
+# (63) 0.852 and 0.839, 8 at 6,144 (88) 0.797 and 0.847, 32 at 2,048 (130) 1.001 and 1.067, 32 at 8,192 1.091 and 1.927; 4 at 4,096 (25)
+# 0.761 and 0.807, 8 at 4,096 (59) 0.773 and 0.776, 2 at 16,000 (33) 0.792 and 0.794; of 8 layers of the 8B sizes, 16 at 1,024 (63)
+# 1.064 and 1.056, 8 at 3,072 (88) 0.986 and 0.990, 4 at 4,096 (50) 0.959 and 1.015, 32 at 8,192 1.140 and 2.098.
 SHARED_MIN_BYTES = 72 << 20
 SHARED_LONG = 64                # blocks of 64 keys
 
