@@ -37,6 +37,8 @@ INCLUDES: Dict[str, List[str]] = {
     "skinny_tcgen05": ["activation.cuh", "tma.cuh", "umma.cuh"],
     "decode_linear": ["activation.cuh"],
     "pointwise": ["activation.cuh"],
+    "token_rules": ["token_rules.cuh"],
+    "token_choice": ["token_rules.cuh"],
 }
 
 # Every source file, with the extra flags it needs.
@@ -75,6 +77,8 @@ SOURCES: Dict[str, List[str]] = {
     "copy_pages": [],
     "logprobs": [],
     "attention_shared": [],
+    "token_rules": [],
+    "token_choice": [],
 }
 
 

@@ -461,6 +461,107 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int
     return logprob, entropy, values, ids
 
 
+class _Rules(ctypes.Structure):
+    """``Rules`` of token_rules.cuh."""
+
+    _fields_ = [(name, _pointer) for name in ("slots", "table", "seen", "counts", "masks", "bias_ids", "biases")] + [
+        (name, _i32) for name in ("slot_count", "words", "stride", "room")]
+
+
+def _rules_of(what: str, rules, slots: Optional[torch.Tensor], rows: int, vocab: int, device) -> _Rules:
+    if rules is None:
+        _need(slots is None, f"{what} has slots without rules")
+        return _Rules()
+    _need(slots is not None and slots.is_cuda and slots.dtype == torch.int32 and slots.is_contiguous() and slots.numel() == rows,
+          f"{what} takes a slot a row (contiguous int32 [S])")
+    _need(rules.vocab == vocab, f"{what}: rules over {rules.vocab} tokens, logits over {vocab}")
+    _need(slots.device == device and rules.table.device == device, f"{what} takes tensors of one device")
+    return _Rules(slots.data_ptr(), rules.table.data_ptr(), rules.seen.data_ptr(), rules.counts.data_ptr(), rules.masks.data_ptr(),
+                  rules.bias_ids.data_ptr(), rules.biases.data_ptr(), rules.slots, rules.seen.stride(0), rules.counts.stride(0),
+                  rules.room)
+
+
+_NOTE_TOKENS = (_pointer, _pointer, _i32, _i32, _i32, _i32, _pointer, _pointer, _i32, _pointer, _pointer, _i32, _i32, _pointer)
+
+
+def note_tokens(rules, slots: torch.Tensor, tokens: torch.Tensor, *, starts: Optional[torch.Tensor] = None,
+                prompts: Optional[torch.Tensor] = None, restart: bool = False) -> None:
+    """Tokens into the histories of ``rules`` (:class:`~tesseract_b200.sampling.TokenRules`): row ``r`` brings ``tokens[r]``, or with
+    ``starts`` (int32 ``[R + 1]``) ``tokens[starts[r]:starts[r + 1]]``, to slot ``slots[r]`` (negative: to none).  The first
+    ``prompts[r]`` of a row's tokens (none without it) are its prompt's: had, but not counted as generated.  With ``restart`` a slot's
+    history begins anew with them (of rows that name one slot the last counts).  All int32; a token outside the vocabulary is no token."""
+    rows, count = slots.numel(), tokens.numel()
+    _cuda(slots, tokens, starts, prompts)
+    for t in (slots, tokens, starts, prompts):
+        if t is not None:
+            _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), "note_tokens takes contiguous int32 lists")
+            _need(t.device == rules.table.device, "note_tokens takes tensors of one device")
+    _need(starts.numel() == rows + 1 if starts is not None else count == rows, "note_tokens takes a token a row, or where each row's start")
+    _need(prompts is None or prompts.numel() == rows, "note_tokens takes the length of a prompt a row")
+    _check(_entry("token_rules", "tb_note_tokens", _NOTE_TOKENS)(
+        rules.seen.data_ptr(), rules.counts.data_ptr(), rules.slots, rules.seen.stride(0), rules.counts.stride(0), rules.vocab,
+        slots.data_ptr(), tokens.data_ptr(), count, starts.data_ptr() if starts is not None else None,
+        prompts.data_ptr() if prompts is not None else None, rows, int(restart), _raw_stream()), "note_tokens")
+
+
+_SHAPE_LOGITS = (_pointer, _i64, _pointer, _i64, _i32, _i32, _Rules, _pointer)
+
+
+def _logit_rows(what: str, logits: torch.Tensor) -> tuple:
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_cuda, f"{what} takes float32 logits [S, V] on a CUDA device")
+    rows, vocab = logits.shape
+    _need(vocab > 0 and (logits.stride(1) == 1 or vocab == 1), f"{what} takes logits with contiguous rows")
+    _need(rows <= 1 or logits.stride(0) >= vocab, f"{what} takes rows of logits that do not lie on each other")
+    return rows, vocab
+
+
+def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Tensor) -> torch.Tensor:
+    """Logits under the rules of the rows' slots (a row whose slot is negative: as they are): penalties, then biases, then -inf where
+    the mask does not allow a token; 64-bit arithmetic, rounded once.  Logits and out float32 ``[S, V]``, rows contiguous and any
+    distance apart; ``out`` may be the logits themselves."""
+    rows, vocab = _logit_rows("shape_logits", logits)
+    _need(_logit_rows("shape_logits", out) == (rows, vocab) and out.device == logits.device, "shape_logits out")
+    made = _rules_of("shape_logits", rules, slots, rows, vocab, logits.device)
+    if rows:
+        a, b = logits.data_ptr(), out.data_ptr()
+        ends = [p + 4 * ((rows - 1) * t.stride(0) + vocab) for p, t in ((a, logits), (b, out))]
+        _need((a == b and (rows == 1 or logits.stride(0) == out.stride(0))) or a >= ends[1] or b >= ends[0],
+              "shape_logits writes to the logits' own place or apart from them")
+    _check(_entry("token_rules", "tb_shape_logits", _SHAPE_LOGITS)(
+        logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, made, _raw_stream()), "shape_logits")
+    return out
+
+
+_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, _pointer)
+
+
+def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor, out: torch.Tensor, *,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                  rules=None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A token a row (int32 ``[S]``) from logits under the rules of the rows' slots (:func:`shape_logits`): the lowest id of the
+    largest for a temperature (float32) of 0 and below; else drawn, with the uniform draw (float64, in [0, 1)), from what ``top_k``
+    (int32; 0: all), ``min_p`` (float64, relative to the largest weight) and ``top_p`` (float64, of the mass that those two leave)
+    keep of the tokens ranked by weight, equal ones by id.  The rank is drawn from in its order (as :func:`~tesseract_b200.sampling
+    .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`).  A row with NaN or +inf among what is
+    allowed, or with nothing allowed, gets -1."""
+    rows, vocab = _logit_rows("choose_tokens", logits)
+    made = _rules_of("choose_tokens", rules, slots, rows, vocab, logits.device)
+    for t, dtype, name in ((temperature, torch.float32, "temperature"), (uniform, torch.float64, "uniform"), (top_k, torch.int32, "top_k"),
+                           (top_p, torch.float64, "top_p"), (min_p, torch.float64, "min_p"), (out, torch.int32, "out")):
+        if t is not None:
+            _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.numel() == rows,
+                  f"choose_tokens {name} must be contiguous {str(dtype)[6:]} [S]")
+            _need(t.device == logits.device, "choose_tokens takes tensors of one device")
+    if rules is not None:
+        shaped = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+        logits = shape_logits(logits, shaped, rules, slots)
+    _check(_entry("token_choice", "tb_choose_tokens", _CHOOSE_TOKENS)(
+        logits.data_ptr(), logits.stride(0), temperature.data_ptr(), uniform.data_ptr(), top_k.data_ptr() if top_k is not None else None,
+        top_p.data_ptr() if top_p is not None else None, min_p.data_ptr() if min_p is not None else None, out.data_ptr(), rows, vocab,
+        _raw_stream()), "choose_tokens")
+    return out
+
+
 _sm_counts = {}
 
 
