@@ -532,7 +532,7 @@ def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Te
     return out
 
 
-_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, _pointer)
+_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, _Rules, _pointer)
 
 
 def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor, out: torch.Tensor, *,
@@ -552,13 +552,10 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
             _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.numel() == rows,
                   f"choose_tokens {name} must be contiguous {str(dtype)[6:]} [S]")
             _need(t.device == logits.device, "choose_tokens takes tensors of one device")
-    if rules is not None:
-        shaped = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
-        logits = shape_logits(logits, shaped, rules, slots)
     _check(_entry("token_choice", "tb_choose_tokens", _CHOOSE_TOKENS)(
         logits.data_ptr(), logits.stride(0), temperature.data_ptr(), uniform.data_ptr(), top_k.data_ptr() if top_k is not None else None,
         top_p.data_ptr() if top_p is not None else None, min_p.data_ptr() if min_p is not None else None, out.data_ptr(), rows, vocab,
-        _raw_stream()), "choose_tokens")
+        made, _raw_stream()), "choose_tokens")
     return out
 
 

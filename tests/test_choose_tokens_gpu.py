@@ -85,6 +85,19 @@ def test_all_logits_equal_and_draws_at_the_ends(vocab):
         check(x, 1.0, np.array([0.0, 1e-12, 0.999, 1.0 - 2.0 ** -53]), **settings)
 
 
+@pytest.mark.parametrize("rows", [3, 32])
+@pytest.mark.parametrize("spread", [0.05, 0.8, 1.2, 30.0])
+def test_much_of_the_vocabulary_kept(rows, spread):
+    """More is kept than one block lists, call behind call."""
+    rng = np.random.RandomState(rows)
+    x = (rng.randn(rows, 128256) * spread).astype(np.float32)
+    x[1] += (np.arange(128256) == 777) * 20.0                # one far above the others
+    x[2, :64128] = -1e30                                     # half far below
+    for settings in (dict(top_p=0.95), dict(top_p=0.3), dict(top_k=30000), dict(min_p=0.05), dict(top_k=60000, top_p=0.7, min_p=0.01)):
+        for temperature in (1.5, 20.0):
+            check(x, temperature, rng.rand(rows), **settings)
+
+
 @pytest.mark.parametrize("allowed", [1, 2, 40, 0.01, 0.5])
 @pytest.mark.parametrize("vocab", [100, 50257, 128256])
 def test_masked_rows(vocab, allowed):

@@ -44,12 +44,13 @@ def choose(x, temperature, draw, top_k=0, top_p=1.0, min_p=0.0):
         best = x.max()
         k = top_k if 0 < top_k < vocab else vocab
         cut = k < vocab or top_p < 1.0 or min_p > 0.0
-        if cut:
-            scaled = x * inverse
-            d = scaled - best * inverse
-        else:
+        scaled = x * inverse
+        d = scaled - best * inverse
+        if not cut and abs(best * inverse) < 65536:
             d = (x.astype(np.float64) * np.float64(inverse) - np.float64(best * inverse)).astype(np.float32)
-    d = np.where(np.isnan(d), np.where(x == best, np.float32(0), -np.float32(np.inf)), d).astype(np.float64)
+        if not np.isfinite(best * inverse):
+            d = np.where(x == best, np.float32(0), -np.float32(np.inf))
+    d = d.astype(np.float64)
     order = np.argsort(-d, kind="stable")[:k] if cut else np.arange(vocab)
     weights = np.exp(d[order])
     order, weights = order[weights >= min(min_p, 1.0)], weights[weights >= min(min_p, 1.0)]
