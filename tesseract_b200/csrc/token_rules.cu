@@ -3,68 +3,233 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
+// ---- histories
+//
+// seen: a bit for every token of the prompt and the answer; counts: how often the answer has each.  Bound by the 4 V + V / 8 bytes that
+// a history begun anew is written with.
 
-// grid: rows.  A row's known tokens into its slot's history; `restart`: in place of what stands there (then of rows that name one
-// slot the last counts).
-__global__ void __launch_bounds__(kThreads)
-note_kernel(uint32_t* __restrict__ seen, int* __restrict__ counts, int slot_count, int words, int stride, int vocab,
-            const int* __restrict__ slots, const int* __restrict__ tokens, int total, const int* __restrict__ starts,
-            const int* __restrict__ prompts, int rows, int restart) {
-    const int row = blockIdx.x, slot = slots[row];
+constexpr int kNoteThreads = 512;
+constexpr int kNotePart = 8192;          // tokens of the vocabulary that a block begins anew
+
+// grid (parts of the vocabulary, rows): a slot's history in place of what stands there.  Every block goes through all of its row's tokens
+// (from L2, but for the first) and counts those of its part in shared memory, so that a part is written once, whole.  Of rows that name
+// one slot the last counts.
+__global__ void __launch_bounds__(kNoteThreads)
+restart_kernel(uint32_t* __restrict__ seen, int* __restrict__ counts, int slot_count, int words, int stride, int vocab,
+               const int* __restrict__ slots, const int* __restrict__ tokens, int total, const int* __restrict__ starts,
+               const int* __restrict__ prompts, int rows) {
+    __shared__ __align__(16) int times[kNotePart];
+    __shared__ __align__(16) uint32_t bits[kNotePart / 32];
+    pdl_trigger();
+    pdl_wait();
+    const int row = blockIdx.y, t = threadIdx.x, slot = slots[row];
     if (slot < 0 || slot >= slot_count) return;
-    uint32_t* bits = seen + (int64_t)slot * words;
-    int* times = counts + (int64_t)slot * stride;
-    if (restart) {
-        int later = 0;
-        for (int r = row + 1 + threadIdx.x; r < rows; r += kThreads) later |= slots[r] == slot;
-        if (__syncthreads_or(later)) return;
-        for (int i = threadIdx.x; i < words; i += kThreads) bits[i] = 0;
-        for (int i = threadIdx.x; i < stride; i += kThreads) times[i] = 0;
-        __syncthreads();
-    }
+    int later = 0;
+    for (int r = row + 1 + t; r < rows; r += kNoteThreads) later |= slots[r] == slot;
+    for (int i = t; i < kNotePart / 4; i += kNoteThreads) reinterpret_cast<int4*>(times)[i] = make_int4(0, 0, 0, 0);
+    if (t < kNotePart / 32) bits[t] = 0;
+    if (__syncthreads_or(later)) return;
+    const int first = blockIdx.x * kNotePart;
     const int begin = starts != nullptr ? max(0, starts[row]) : row;
     const int end = starts != nullptr ? min(total, starts[row + 1]) : row + 1;
     const int prompt = prompts != nullptr ? prompts[row] : 0;
-    for (int i = begin + (int)threadIdx.x; i < end; i += kThreads) {
-        const int token = tokens[i];
-        if (token < 0 || token >= vocab) continue;
-        atomicOr(bits + (token >> 5), 1u << (token & 31));
-        if (i - begin >= prompt) atomicAdd(times + token, 1);
+#pragma unroll 4
+    for (int i = begin + t; i < end; i += kNoteThreads) {
+        const unsigned at = (unsigned)tokens[i] - (unsigned)first;     // (a token below the part, or negative, is beyond it as well)
+        if (at >= (unsigned)kNotePart || (int)at + first >= vocab) continue;
+        atomicOr(bits + (at >> 5), 1u << (at & 31));
+        if (i - begin >= prompt) atomicAdd(times + at, 1);
     }
+    __syncthreads();
+    // (rows of both are multiples of 16 bytes)
+    int4* to = reinterpret_cast<int4*>(counts + (int64_t)slot * stride + first);
+    for (int i = t; i < min(kNotePart, stride - first) / 4; i += kNoteThreads) to[i] = reinterpret_cast<const int4*>(times)[i];
+    uint32_t* bits_to = seen + (int64_t)slot * words + (first >> 5);
+    if (t < min(kNotePart / 32, words - (first >> 5))) bits_to[t] = bits[t];
 }
 
-// grid: rows.
-__global__ void __launch_bounds__(kThreads)
+__device__ __forceinline__ void note(uint32_t* bits, int* times, int token, int vocab, bool counted) {
+    if (token < 0 || token >= vocab) return;
+    atomicOr(bits + (token >> 5), 1u << (token & 31));
+    if (counted) atomicAdd(times + token, 1);
+}
+
+// grid: rows.  More of a row's tokens into its slot's history.
+__global__ void __launch_bounds__(kNoteThreads)
+note_kernel(uint32_t* __restrict__ seen, int* __restrict__ counts, int slot_count, int words, int stride, int vocab,
+            const int* __restrict__ slots, const int* __restrict__ tokens, int total, const int* __restrict__ starts,
+            const int* __restrict__ prompts) {
+    pdl_trigger();
+    pdl_wait();
+    const int row = blockIdx.x, slot = slots[row];
+    if (slot < 0 || slot >= slot_count) return;
+    const int begin = max(0, starts[row]), end = min(total, starts[row + 1]);
+    const int prompt = prompts != nullptr ? prompts[row] : 0;
+    for (int i = begin + (int)threadIdx.x; i < end; i += kNoteThreads)
+        note(seen + (int64_t)slot * words, counts + (int64_t)slot * stride, tokens[i], vocab, i - begin >= prompt);
+}
+
+// A token a row: a decode step.
+__global__ void __launch_bounds__(128)
+note_one_kernel(uint32_t* __restrict__ seen, int* __restrict__ counts, int slot_count, int words, int stride, int vocab,
+                const int* __restrict__ slots, const int* __restrict__ tokens, const int* __restrict__ prompts, int rows) {
+    pdl_trigger();
+    pdl_wait();
+    const int row = blockIdx.x * 128 + threadIdx.x;
+    if (row >= rows) return;
+    const int slot = slots[row];
+    if (slot < 0 || slot >= slot_count) return;
+    note(seen + (int64_t)slot * words, counts + (int64_t)slot * stride, tokens[row], vocab, prompts == nullptr || prompts[row] <= 0);
+}
+
+// A slot's row of the table, which travels in the launch.
+__global__ void set_kernel(SlotRules* to, SlotRules row) { *to = row; }
+
+// ---- logits
+//
+// Bound by the 8 V bytes a row that are read and written (less where the mask rules out four neighbours: those are not read).  A block
+// has 4,096 tokens.  It asks for its logits first; under their latency it lists the tokens that were had (a bit each), so that every
+// thread has as many of them, and works those out in 64 bits; then everything is written, the listed ones behind the others.
+
+constexpr int kShapeThreads = 256;
+constexpr int kShapePart = 4096;
+constexpr int kEach = kShapePart / kShapeThreads;
+
+// grid (parts of the vocabulary, rows).
+__global__ void __launch_bounds__(kShapeThreads)
 shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride, int vocab, Rules rules) {
-    __shared__ float raw[kMaxBiases];
-    const int row = blockIdx.x;
-    const float* x = logits + (int64_t)row * stride;
-    float* y = out + (int64_t)row * out_stride;
+    __shared__ uint32_t mask[kShapePart / 32], had[kShapePart / 32];
+    __shared__ uint16_t some[kShapePart];
+    __shared__ float made[kShapePart];
+    __shared__ int warps[kShapeThreads / 32];
+    constexpr int kBiased = kMaxBiases / kShapeThreads;
+    pdl_trigger();
+    pdl_wait();
+    const int row = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int first = blockIdx.x * kShapePart, count = min(kShapePart, vocab - first), words = (count + 31) >> 5;
+    const float* x = logits + (int64_t)row * stride + first;
+    float* y = out + (int64_t)row * out_stride + first;
     const int slot = rules.slots[row];
     SlotRules rule = {};
     if (slot >= 0 && slot < rules.slot_count) rule = rules.table[slot];
-    const uint32_t* seen = rules.seen + (int64_t)slot * rules.words;
-    const uint32_t* mask = rules.masks + (int64_t)slot * rules.words;
-    const int* counts = rules.counts + (int64_t)slot * rules.stride;
-    const int* ids = rules.bias_ids + (int64_t)slot * rules.room;
+    const bool masked = rule.kinds & kMask, penalised = rule.kinds & kPenalties;
     const int biases = rule.kinds & kBiases ? min(rule.biases, rules.room) : 0;
-    for (int i = threadIdx.x; i < biases; i += kThreads) {
-        const int token = ids[i];
-        raw[i] = token >= 0 && token < vocab ? x[token] : 0.0f;
+    const bool wide = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
+    const bool in_place = x == y;
+    if (in_place && rule.kinds == 0) return;
+    if (t < kShapePart / 32) {
+        const int64_t at = (int64_t)slot * rules.words + (first >> 5) + t;
+        mask[t] = masked ? (t < words ? rules.masks[at] : 0u) : ~0u;
+        uint32_t bits = penalised && t < words ? rules.seen[at] : 0;
+        if (t * 32 + 32 > count && bits != 0) bits &= ~0u >> (t * 32 + 32 - count);
+        had[t] = bits;
     }
     __syncthreads();
-    auto shaped = [&](int token, float l, float bias) {
-        if (rule.kinds & kMask && !(mask[token >> 5] >> (token & 31) & 1)) return -INFINITY;
-        const bool had = rule.kinds & kPenalties && seen[token >> 5] >> (token & 31) & 1;
-        if (!had && bias == 0.0f) return l;
-        return shaped_logit(l, rule, had, had ? counts[token] : 0, bias);
-    };
-    for (int i = threadIdx.x; i < vocab; i += kThreads) y[i] = shaped(i, x[i], 0.0f);
-    __syncthreads();
-    for (int i = threadIdx.x; i < biases; i += kThreads) {
-        const int token = ids[i];
-        if (token >= 0 && token < vocab) y[token] = shaped(token, raw[i], rules.biases[(int64_t)slot * rules.room + i]);
+    // ---- the logits: four neighbours where they are aligned, else one of every 256
+    float v[kEach];
+    auto place = [&](int u) { return wide ? (u >> 2) * 4 * kShapeThreads + 4 * t + (u & 3) : u * kShapeThreads + t; };
+    auto allowed = [&](int i) { return mask[i >> 5] >> (i & 31) & 1; };
+    if (!in_place || masked) {
+        if (wide) {
+#pragma unroll
+            for (int u = 0; u < kEach; u += 4) {
+                const int i = place(u);
+                const bool any = i < count && (mask[i >> 5] >> (i & 31) & 15);
+                if (any && i + 4 <= count) {
+                    const float4 four = *reinterpret_cast<const float4*>(x + i);
+                    v[u] = four.x, v[u + 1] = four.y, v[u + 2] = four.z, v[u + 3] = four.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[u + j] = any && i + j < count ? x[i + j] : -INFINITY;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                const int i = place(u);
+                v[u] = i < count && allowed(i) ? x[i] : -INFINITY;
+            }
+        }
+    }
+    // ---- the tokens that were had and those with a bias
+    int listed = 0;
+    if (penalised) {
+        uint32_t bits = t < kShapePart / 32 ? had[t] : 0;
+        const int mine = __popc(bits);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += other;
+        }
+        if (lane == 31) warps[warp] = incl;
+        __syncthreads();
+        int at = incl - mine;
+#pragma unroll
+        for (int w = 0; w < kShapeThreads / 32; ++w) {
+            if (w < warp) at += warps[w];
+            listed += warps[w];
+        }
+        while (bits) {
+            some[at++] = (uint16_t)(t * 32 + __ffs(bits) - 1);
+            bits &= bits - 1;
+        }
+        __syncthreads();
+        const int* counts = rules.counts + (int64_t)slot * rules.stride + first;
+#pragma unroll 2
+        for (int e = t; e < listed; e += kShapeThreads) {
+            const int i = some[e];
+            made[e] = allowed(i) ? shaped_logit(x[i], rule, true, counts[i], 0.0f) : -INFINITY;
+        }
+    }
+    float biased[kBiased];
+    if (biases > 0) {
+        const int64_t at = (int64_t)slot * rules.room;
+#pragma unroll
+        for (int u = 0; u < kBiased; ++u) {
+            const int e = t + u * kShapeThreads, i = e < biases ? rules.bias_ids[at + e] - first : -1;
+            if (i < 0 || i >= count) continue;
+            const bool was = had[i >> 5] >> (i & 31) & 1;
+            biased[u] = !allowed(i) ? -INFINITY
+                                    : shaped_logit(x[i], rule, was, was ? rules.counts[(int64_t)slot * rules.stride + first + i] : 0,
+                                                   rules.biases[at + e]);
+        }
+    }
+    __syncthreads();                               // (in place: every logit that is needed has been read)
+    if (!in_place || masked) {
+        if (wide) {
+#pragma unroll
+            for (int u = 0; u < kEach; u += 4) {
+                const int i = place(u);
+                const uint32_t bits = i < count ? mask[i >> 5] >> (i & 31) : 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[u + j] = bits >> j & 1 ? v[u + j] : -INFINITY;
+                if (i + 4 <= count) {
+                    *reinterpret_cast<float4*>(y + i) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j < count) y[i + j] = v[u + j];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kEach; ++u)
+                if (place(u) < count) y[place(u)] = v[u];
+        }
+    }
+    if (penalised) {
+        __syncthreads();
+        for (int e = t; e < listed; e += kShapeThreads) y[some[e]] = made[e];
+    }
+    if (biases > 0) {
+        __syncthreads();
+        const int64_t at = (int64_t)slot * rules.room;
+#pragma unroll
+        for (int u = 0; u < kBiased; ++u) {
+            const int e = t + u * kShapeThreads, i = e < biases ? rules.bias_ids[at + e] - first : -1;
+            if (i >= 0 && i < count) y[i] = biased[u];
+        }
     }
 }
 
@@ -74,16 +239,33 @@ TB_EXPORT int tb_note_tokens(uint32_t* seen, int* counts, int slot_count, int wo
                              const int* tokens, int total, const int* starts, const int* prompts, int rows, int restart,
                              cudaStream_t stream) {
     if (rows == 0) return 0;
-    if (vocab <= 0 || rows < 0 || words < (vocab + 31) / 32 || stride < vocab) return TB_ERR_BAD_SIZE;
-    note_kernel<<<rows, kThreads, 0, stream>>>(seen, counts, slot_count, words, stride, vocab, slots, tokens, total, starts, prompts,
-                                               rows, restart);
+    if (vocab <= 0 || rows < 0 || words < (vocab + 31) / 32 || stride < vocab || stride % 4 != 0) return TB_ERR_BAD_SIZE;
+    if ((uintptr_t)counts & 15) return TB_ERR_BAD_ALIGN;
+    cudaError_t err;
+    if (restart) {
+        if (rows > 65535) return TB_ERR_BAD_SIZE;
+        err = tb_launch_pdl(restart_kernel, dim3((stride + kNotePart - 1) / kNotePart, rows), dim3(kNoteThreads), 0, stream, seen, counts,
+                            slot_count, words, stride, vocab, slots, tokens, total, starts, prompts, rows);
+    } else if (starts != nullptr) {
+        err = tb_launch_pdl(note_kernel, dim3(rows), dim3(kNoteThreads), 0, stream, seen, counts, slot_count, words, stride, vocab, slots,
+                            tokens, total, starts, prompts);
+    } else {
+        err = tb_launch_pdl(note_one_kernel, dim3((rows + 127) / 128), dim3(128), 0, stream, seen, counts, slot_count, words, stride, vocab,
+                            slots, tokens, prompts, rows);
+    }
+    return err == cudaSuccess ? tb_launch_status() : (int)err;
+}
+
+TB_EXPORT int tb_set_rules(SlotRules* to, SlotRules row, cudaStream_t stream) {
+    set_kernel<<<1, 1, 0, stream>>>(to, row);
     return tb_launch_status();
 }
 
 TB_EXPORT int tb_shape_logits(const float* logits, int64_t stride, float* out, int64_t out_stride, int rows, int vocab, Rules rules,
                               cudaStream_t stream) {
     if (rows == 0) return 0;
-    if (vocab <= 0 || rows < 0 || rules.room > kMaxBiases) return TB_ERR_BAD_SIZE;
-    shape_kernel<<<rows, kThreads, 0, stream>>>(logits, stride, out, out_stride, vocab, rules);
-    return tb_launch_status();
+    if (vocab <= 0 || rows < 0 || rows > 65535 || rules.room > kMaxBiases) return TB_ERR_BAD_SIZE;
+    const cudaError_t err = tb_launch_pdl(shape_kernel, dim3((vocab + kShapePart - 1) / kShapePart, rows), dim3(kShapeThreads), 0, stream,
+                                          logits, stride, out, out_stride, vocab, rules);
+    return err == cudaSuccess ? tb_launch_status() : (int)err;
 }

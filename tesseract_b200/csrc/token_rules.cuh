@@ -32,7 +32,7 @@ struct Rules {
     int slot_count, words, stride, room;
 };
 
-__device__ __forceinline__ float shaped_logit(float l, const SlotRules& rule, bool seen, int count, float bias) {
+__device__ __noinline__ float shaped_logit(float l, const SlotRules& rule, bool seen, int count, float bias) {
     double x = (double)l;
     if (seen) x = x > 0.0 ? __ddiv_rn(x, (double)rule.repetition) : __dmul_rn(x, (double)rule.repetition);
     if (count != 0) x = __dsub_rn(x, __dmul_rn((double)rule.frequency, (double)count));

@@ -461,24 +461,54 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, alternatives: int
     return logprob, entropy, values, ids
 
 
-class _Rules(ctypes.Structure):
-    """``Rules`` of token_rules.cuh."""
+class RulesRecord(ctypes.Structure):
+    """``Rules`` of token_rules.cuh: where a :class:`~tesseract_b200.sampling.TokenRules` lies."""
 
     _fields_ = [(name, _pointer) for name in ("slots", "table", "seen", "counts", "masks", "bias_ids", "biases")] + [
         (name, _i32) for name in ("slot_count", "words", "stride", "room")]
 
 
-def _rules_of(what: str, rules, slots: Optional[torch.Tensor], rows: int, vocab: int, device) -> _Rules:
+class RulesRow(ctypes.Structure):
+    """``SlotRules`` of token_rules.cuh: a slot's row of the table."""
+
+    _fields_ = [("numbers", _i32 * 8)]
+
+
+_NO_RULES = RulesRecord()
+_SET_RULES = (_pointer, RulesRow, _pointer)
+
+
+def set_rules(table: torch.Tensor, slot: int, row) -> None:
+    """``table[slot] = row`` (eight int32 numbers that travel in the launch: nothing has to outlive the call)."""
+    _cuda(table)
+    _need(table.dtype == torch.int32 and table.is_contiguous() and table.dim() == 2 and table.shape[1] == 8 and 0 <= slot < table.shape[0],
+          "set_rules takes a table [slots, 8] and a slot of it")
+    _check(_entry("token_rules", "tb_set_rules", _SET_RULES)(table.data_ptr() + 32 * slot, RulesRow((_i32 * 8)(*row)), _raw_stream()),
+           "set_rules")
+
+
+def _rules_of(what: str, rules, slots: Optional[torch.Tensor], rows: int, vocab: int, device: int) -> RulesRecord:
     if rules is None:
         _need(slots is None, f"{what} has slots without rules")
-        return _Rules()
-    _need(slots is not None and slots.is_cuda and slots.dtype == torch.int32 and slots.is_contiguous() and slots.numel() == rows,
-          f"{what} takes a slot a row (contiguous int32 [S])")
-    _need(rules.vocab == vocab, f"{what}: rules over {rules.vocab} tokens, logits over {vocab}")
-    _need(slots.device == device and rules.table.device == device, f"{what} takes tensors of one device")
-    return _Rules(slots.data_ptr(), rules.table.data_ptr(), rules.seen.data_ptr(), rules.counts.data_ptr(), rules.masks.data_ptr(),
-                  rules.bias_ids.data_ptr(), rules.biases.data_ptr(), rules.slots, rules.seen.stride(0), rules.counts.stride(0),
-                  rules.room)
+        return _NO_RULES
+    if slots is None or slots.dtype != torch.int32 or not slots.is_contiguous() or slots.numel() != rows:
+        raise KernelError(f"{what} takes a slot a row (contiguous int32 [S])")
+    if rules.vocab != vocab:
+        raise KernelError(f"{what}: rules over {rules.vocab} tokens, logits over {vocab}")
+    if slots.get_device() != device or rules.table.get_device() != device:
+        raise KernelError(f"{what} takes tensors of one device")
+    record = RulesRecord.from_buffer_copy(rules.record)
+    record.slots = slots.data_ptr()
+    return record
+
+
+def _list_of(what: str, t: torch.Tensor, device: int) -> int:
+    """The address of a contiguous int32 list."""
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise KernelError(f"{what} takes contiguous int32 lists")
+    if t.get_device() != device or device < 0:
+        raise KernelError(f"{what} takes tensors of one CUDA device")
+    return t.data_ptr()
 
 
 _NOTE_TOKENS = (_pointer, _pointer, _i32, _i32, _i32, _i32, _pointer, _pointer, _i32, _pointer, _pointer, _i32, _i32, _pointer)
@@ -490,49 +520,60 @@ def note_tokens(rules, slots: torch.Tensor, tokens: torch.Tensor, *, starts: Opt
     ``starts`` (int32 ``[R + 1]``) ``tokens[starts[r]:starts[r + 1]]``, to slot ``slots[r]`` (negative: to none).  The first
     ``prompts[r]`` of a row's tokens (none without it) are its prompt's: had, but not counted as generated.  With ``restart`` a slot's
     history begins anew with them (of rows that name one slot the last counts).  All int32; a token outside the vocabulary is no token."""
-    rows, count = slots.numel(), tokens.numel()
-    _cuda(slots, tokens, starts, prompts)
-    for t in (slots, tokens, starts, prompts):
-        if t is not None:
-            _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), "note_tokens takes contiguous int32 lists")
-            _need(t.device == rules.table.device, "note_tokens takes tensors of one device")
+    rows, count, device = slots.numel(), tokens.numel(), rules.table.get_device()
+    slots_at, tokens_at = _list_of("note_tokens", slots, device), _list_of("note_tokens", tokens, device)
+    starts_at = _list_of("note_tokens", starts, device) if starts is not None else None
+    prompts_at = _list_of("note_tokens", prompts, device) if prompts is not None else None
     _need(starts.numel() == rows + 1 if starts is not None else count == rows, "note_tokens takes a token a row, or where each row's start")
     _need(prompts is None or prompts.numel() == rows, "note_tokens takes the length of a prompt a row")
+    record = rules.record
     _check(_entry("token_rules", "tb_note_tokens", _NOTE_TOKENS)(
-        rules.seen.data_ptr(), rules.counts.data_ptr(), rules.slots, rules.seen.stride(0), rules.counts.stride(0), rules.vocab,
-        slots.data_ptr(), tokens.data_ptr(), count, starts.data_ptr() if starts is not None else None,
-        prompts.data_ptr() if prompts is not None else None, rows, int(restart), _raw_stream()), "note_tokens")
+        record.seen, record.counts, record.slot_count, record.words, record.stride, rules.vocab, slots_at, tokens_at, count, starts_at,
+        prompts_at, rows, int(restart), _raw_stream()), "note_tokens")
 
 
-_SHAPE_LOGITS = (_pointer, _i64, _pointer, _i64, _i32, _i32, _Rules, _pointer)
+_SHAPE_LOGITS = (_pointer, _i64, _pointer, _i64, _i32, _i32, RulesRecord, _pointer)
 
 
 def _logit_rows(what: str, logits: torch.Tensor) -> tuple:
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_cuda, f"{what} takes float32 logits [S, V] on a CUDA device")
-    rows, vocab = logits.shape
-    _need(vocab > 0 and (logits.stride(1) == 1 or vocab == 1), f"{what} takes logits with contiguous rows")
-    _need(rows <= 1 or logits.stride(0) >= vocab, f"{what} takes rows of logits that do not lie on each other")
-    return rows, vocab
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+        raise KernelError(f"{what} takes float32 logits [S, V] on a CUDA device")
+    (rows, vocab), (stride, step) = logits.shape, logits.stride()
+    if vocab == 0 or (step != 1 and vocab > 1):
+        raise KernelError(f"{what} takes logits with contiguous rows")
+    if stride < vocab and rows > 1:
+        raise KernelError(f"{what} takes rows of logits that do not lie on each other")
+    return rows, vocab, stride
 
 
 def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Tensor) -> torch.Tensor:
     """Logits under the rules of the rows' slots (a row whose slot is negative: as they are): penalties, then biases, then -inf where
     the mask does not allow a token; 64-bit arithmetic, rounded once.  Logits and out float32 ``[S, V]``, rows contiguous and any
     distance apart; ``out`` may be the logits themselves."""
-    rows, vocab = _logit_rows("shape_logits", logits)
-    _need(_logit_rows("shape_logits", out) == (rows, vocab) and out.device == logits.device, "shape_logits out")
-    made = _rules_of("shape_logits", rules, slots, rows, vocab, logits.device)
-    if rows:
-        a, b = logits.data_ptr(), out.data_ptr()
-        ends = [p + 4 * ((rows - 1) * t.stride(0) + vocab) for p, t in ((a, logits), (b, out))]
-        _need((a == b and (rows == 1 or logits.stride(0) == out.stride(0))) or a >= ends[1] or b >= ends[0],
+    rows, vocab, stride = _logit_rows("shape_logits", logits)
+    same, width, out_stride = _logit_rows("shape_logits", out)
+    device = logits.get_device()
+    _need((same, width) == (rows, vocab) and out.get_device() == device, "shape_logits out")
+    _need(rules is not None, "shape_logits takes rules")
+    record = _rules_of("shape_logits", rules, slots, rows, vocab, device)
+    a, b = logits.data_ptr(), out.data_ptr()
+    if rows and not (a == b and (rows == 1 or stride == out_stride)):
+        _need(a >= b + 4 * ((rows - 1) * out_stride + vocab) or b >= a + 4 * ((rows - 1) * stride + vocab),
               "shape_logits writes to the logits' own place or apart from them")
-    _check(_entry("token_rules", "tb_shape_logits", _SHAPE_LOGITS)(
-        logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, made, _raw_stream()), "shape_logits")
+    _check(_entry("token_rules", "tb_shape_logits", _SHAPE_LOGITS)(a, stride, b, out_stride, rows, vocab, record, _raw_stream()),
+           "shape_logits")
     return out
 
 
-_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, _Rules, _pointer)
+_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, RulesRecord, _pointer)
+
+
+def _per_row(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, device: int) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous() or t.get_device() != device:
+        raise KernelError(f"choose_tokens {name} must be contiguous {str(dtype)[6:]} [S] on the logits' device")
+    return t.data_ptr()
 
 
 def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor, out: torch.Tensor, *,
@@ -543,19 +584,17 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
     (int32; 0: all), ``min_p`` (float64, relative to the largest weight) and ``top_p`` (float64, of the mass that those two leave)
     keep of the tokens ranked by weight, equal ones by id.  The rank is drawn from in its order (as :func:`~tesseract_b200.sampling
     .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`).  A row with NaN or +inf among what is
-    allowed, or with nothing allowed, gets -1."""
-    rows, vocab = _logit_rows("choose_tokens", logits)
-    made = _rules_of("choose_tokens", rules, slots, rows, vocab, logits.device)
-    for t, dtype, name in ((temperature, torch.float32, "temperature"), (uniform, torch.float64, "uniform"), (top_k, torch.int32, "top_k"),
-                           (top_p, torch.float64, "top_p"), (min_p, torch.float64, "min_p"), (out, torch.int32, "out")):
-        if t is not None:
-            _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.numel() == rows,
-                  f"choose_tokens {name} must be contiguous {str(dtype)[6:]} [S]")
-            _need(t.device == logits.device, "choose_tokens takes tensors of one device")
+    allowed, or with nothing allowed, gets -1.  Up to 262,144 tokens and 65,535 rows."""
+    rows, vocab, stride = _logit_rows("choose_tokens", logits)
+    device = logits.get_device()
+    record = _rules_of("choose_tokens", rules, slots, rows, vocab, device)
+    if temperature is None or uniform is None or out is None:
+        raise KernelError("choose_tokens takes a temperature, a draw and a place for the token a row")
     _check(_entry("token_choice", "tb_choose_tokens", _CHOOSE_TOKENS)(
-        logits.data_ptr(), logits.stride(0), temperature.data_ptr(), uniform.data_ptr(), top_k.data_ptr() if top_k is not None else None,
-        top_p.data_ptr() if top_p is not None else None, min_p.data_ptr() if min_p is not None else None, out.data_ptr(), rows, vocab,
-        made, _raw_stream()), "choose_tokens")
+        logits.data_ptr(), stride, _per_row("temperature", temperature, torch.float32, rows, device),
+        _per_row("uniform", uniform, torch.float64, rows, device), _per_row("top_k", top_k, torch.int32, rows, device),
+        _per_row("top_p", top_p, torch.float64, rows, device), _per_row("min_p", min_p, torch.float64, rows, device),
+        _per_row("out", out, torch.int32, rows, device), rows, vocab, record, _raw_stream()), "choose_tokens")
     return out
 
 

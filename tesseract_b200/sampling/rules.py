@@ -58,6 +58,8 @@ class TokenRules:
         self.biases = torch.zeros(slots, biases, dtype=torch.float32, device=device)
         self.seen, self.counts = self._seen[:, :self.words], self._counts[:, :vocab]
         self.masks = self._masks[:, :self.words]
+        self.record = kernels.RulesRecord(None, *[t.data_ptr() for t in (self.table, self._seen, self._counts, self._masks, self.bias_ids,
+                                                                        self.biases)], slots, wide, 32 * wide, biases)
         self._host = np.zeros((slots, 8), dtype=np.int32)
         self._host[:, 2] = np.float32(1.0).view(np.int32)
 
@@ -65,8 +67,11 @@ class TokenRules:
         if not 0 <= slot < self.slots:
             raise ValueError(f"slot {slot} is outside the {self.slots} of these rules")
 
-    def _upload(self, rows) -> None:
-        self.table[rows] = torch.from_numpy(self._host[rows]).to(self.device)
+    def _upload(self, slot: Optional[int] = None) -> None:
+        if slot is None or not self.table.is_cuda:
+            self.table.copy_(torch.from_numpy(self._host))
+        else:
+            kernels.set_rules(self.table, slot, self._host[slot].tolist())
 
     def set(self, slot: int, *, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0,
             biases: Optional[Mapping[int, float]] = None, allowed: Optional[Iterable[int]] = None) -> None:
@@ -93,8 +98,9 @@ class TokenRules:
             self.biases[slot, :ids.size] = torch.from_numpy(values).to(self.device)
         if words is not None:
             self.masks[slot] = torch.from_numpy(words).to(self.device)
-        self._host[slot] = row
-        self._upload(slice(slot, slot + 1))
+        if not np.array_equal(row, self._host[slot]):
+            self._host[slot] = row
+            self._upload(slot)
 
     def _check_biases(self, ids: np.ndarray, values: np.ndarray) -> None:
         if ids.size == 0:
@@ -117,7 +123,7 @@ class TokenRules:
         self.biases[:, :n] = values
         self._host[:, 0] = self._host[:, 0] | BIASES if n else self._host[:, 0] & ~BIASES
         self._host[:, 1] = n
-        self._upload(slice(None))
+        self._upload()
 
     def set_masks(self, words: torch.Tensor) -> None:
         """The masks of all slots, int32 words ``[slots, words]`` (:func:`pack_mask`)."""
@@ -125,7 +131,7 @@ class TokenRules:
             raise ValueError(f"masks are int32 [{self.slots}, {self.words}]")
         self.masks.copy_(words)
         self._host[:, 0] |= MASK
-        self._upload(slice(None))
+        self._upload()
 
     def set_mask(self, slot: int, words: Union[np.ndarray, torch.Tensor]) -> None:
         """One slot's mask (:func:`pack_mask`)."""
@@ -136,7 +142,7 @@ class TokenRules:
         self.masks[slot].copy_(words, non_blocking=True)
         if not self._host[slot, 0] & MASK:
             self._host[slot, 0] |= MASK
-            self._upload(slice(slot, slot + 1))
+            self._upload(slot)
 
     def copy(self, sources: Sequence[int], targets: Sequence[int]) -> None:
         """Rules and histories of slots into others, in one launch; no target twice or also a source."""
