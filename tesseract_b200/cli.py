@@ -25,6 +25,14 @@ def _env(name: str, default):
     return type(default)(value) if value is not None else default
 
 
+def _ids(text: str):
+    return [int(field) for field in text.split(",") if field.strip()]
+
+
+def _biases(text: str):
+    return {int(token): float(bias) for token, bias in (field.split(":") for field in text.split(",") if field.strip())}
+
+
 def build_parser() -> argparse.ArgumentParser:
     p = argparse.ArgumentParser(prog="tesseract", description="Generate tokens with a model folder (config.json, model.safetensors) on one B200.")
     p.add_argument("--model-path", default=os.environ.get("TESSERACT_MODEL_PATH"),
@@ -53,6 +61,14 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--top-p", type=float, default=1.0)
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--ignore-eos", action="store_true")
+    p.add_argument("--top-k", type=int, default=0, help="draw from the most probable tokens only (0: all)")
+    p.add_argument("--min-p", type=float, default=0.0, help="draw from tokens at least this times as probable as the most probable")
+    p.add_argument("--repetition-penalty", type=float, default=1.0,
+                   help="divide the positive and multiply the negative logits of tokens that the request has had")
+    p.add_argument("--presence-penalty", type=float, default=0.0, help="taken off the logits of tokens that the answer has")
+    p.add_argument("--frequency-penalty", type=float, default=0.0, help="taken off for every time that the answer has a token")
+    p.add_argument("--logit-bias", type=_biases, default=None, metavar="ID:BIAS,...", help="added to the logits of tokens")
+    p.add_argument("--allowed-token-ids", type=_ids, default=None, metavar="ID,...", help="no others are generated")
     p.add_argument("--beams", type=int, default=0, metavar="WIDTH",
                    help="instead of sampling, the WIDTH most probable continuations that a beam search finds, with their log "
                         "probabilities")
@@ -88,6 +104,15 @@ def read_prompt_file(path: str):
     return prompts
 
 
+def sampling_params(args):
+    from . import SamplingParams
+
+    return SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p, seed=args.seed,
+                          ignore_eos=args.ignore_eos, top_k=args.top_k, min_p=args.min_p, repetition_penalty=args.repetition_penalty,
+                          presence_penalty=args.presence_penalty, frequency_penalty=args.frequency_penalty,
+                          logit_bias=args.logit_bias, allowed_token_ids=args.allowed_token_ids)
+
+
 def run_scored(llm, prompts, args, scratch) -> int:
     """``--score`` and ``--beams``."""
     if args.score:
@@ -99,7 +124,7 @@ def run_scored(llm, prompts, args, scratch) -> int:
                 print(f"[{index}] perplexity {out.perplexity:.4f}: " + " ".join(f"{v:.4f}" for v in out.logprobs))
     else:
         found = llm.beam_search(prompts, args.beams, args.max_tokens, length_penalty=args.length_penalty,
-                                ignore_eos=args.ignore_eos)
+                                ignore_eos=args.ignore_eos, rules=sampling_params(args))
         for index, outs in enumerate(found):
             for rank, out in enumerate(outs):
                 if args.json:
@@ -114,7 +139,7 @@ def run_scored(llm, prompts, args, scratch) -> int:
 
 def main(argv=None) -> int:
     args = build_parser().parse_args(argv)
-    from . import LLM, SamplingParams
+    from . import LLM
     from .config import load_plugins
 
     load_plugins(args.plugin)
@@ -161,8 +186,7 @@ def main(argv=None) -> int:
         return 2
     if args.score or args.beams:
         return run_scored(llm, prompts, args, scratch)
-    params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
-                            seed=args.seed, ignore_eos=args.ignore_eos)
+    params = sampling_params(args)
     started = time.time()
     outputs = llm.generate(prompts, params)
     elapsed = time.time() - started

@@ -5,6 +5,9 @@ hold its full pages together, and a decode step reads those once for all beams o
 Every step asks each beam's logits for its most probable tokens and their log probabilities (``kernels.token_logprobs``); the best
 ``width`` of all beams' go on: a beam chosen more than once is forked, one chosen no more is let go, all copies of a step in one
 launch.  Not in the reference, whose server takes one sequence a request (src/engine/types.rs:14-37).
+
+Under rules (penalties, biases, allowed tokens) the logits are changed in front of that (``kernels.shape_logits``), and a beam that is
+forked has its parent's history of tokens.
 """
 
 from __future__ import annotations
@@ -16,6 +19,7 @@ from typing import Dict, FrozenSet, Hashable, List, Optional, Sequence, Tuple
 import torch
 
 from .. import kernels
+from ..sampling.params import SamplingParams, TokenChoice
 from ..sampling.sampler import InvalidLogits
 from .scheduler import FINISH_LENGTH, FINISH_STOP, RequestRejected
 from .step import StepEntry, StepError, Stepper
@@ -79,11 +83,20 @@ def _rank(total: float, length: int, penalty: float) -> float:
 class BeamSearch:
     """``width`` beams a prompt, up to ``max_tokens`` tokens each.  A sequence's score is the sum of its tokens' log probabilities,
     divided by their number to the power of ``length_penalty``.  A beam that would go on with one of ``end_ids`` is finished there;
-    a prompt is done when ``width`` of its continuations are finished or the beams have ``max_tokens`` tokens."""
+    a prompt is done when ``width`` of its continuations are finished or the beams have ``max_tokens`` tokens.  ``rules``: penalties,
+    biases and allowed tokens for every beam (no grammar; its temperature and cuts say nothing here)."""
 
     def __init__(self, stepper: Stepper, width: int, max_tokens: int, *, end_ids: FrozenSet[int] = frozenset(),
-                 length_penalty: float = 0.0, portion: int = 512):
+                 length_penalty: float = 0.0, portion: int = 512, rules: Optional[SamplingParams] = None):
         vocab = stepper.vocab_size
+        if rules is not None:
+            rules.validate()
+            rules.check_vocabulary(vocab)
+            if rules.grammar is not None:
+                raise ValueError("a beam search takes no grammar")
+            if rules.ruled and vocab > kernels.MAX_CHOICE_VOCAB:
+                raise ValueError(f"rules on tokens take vocabularies of up to {kernels.MAX_CHOICE_VOCAB} tokens")
+        self.rules = rules if rules is not None and rules.ruled else None
         if width < 1 or max_tokens < 1:
             raise ValueError("beam search needs a width and a number of tokens of at least one")
         if min(2 * width, vocab) > kernels.MAX_ALTERNATIVES:
@@ -165,13 +178,23 @@ class BeamSearch:
             for begin in range(0, len(prompt), self.portion):
                 part = prompt[begin:begin + self.portion]
                 last = begin + len(part) == len(prompt)
-                logits = self.stepper.step([StepEntry(request, part, [len(part) - 1] if last else [])])
+                logits = self.stepper.step([StepEntry(request, part, [len(part) - 1] if last else [], self._choice(prompt))])
         except BaseException:
             cache.release(request)
             raise
         search = _Search(index, prompt, [_Beam(request, [], [], 0.0)])
         searches.append(search)                          # (whose beams go back to the cache whatever happens from here on)
-        self._choose([search], self._alternatives(logits))
+        self._choose([search], self._alternatives(self._shaped(logits, search.beams)))
+
+    def _choice(self, prompt: Sequence[int]) -> Optional[TokenChoice]:
+        return TokenChoice(self.rules, len(prompt)) if self.rules is not None else None
+
+    def _shaped(self, logits: torch.Tensor, beams: Sequence[_Beam]) -> torch.Tensor:
+        """The beams' logits under the rules."""
+        if self.rules is None:
+            return logits
+        slots = torch.tensor([self.cache.slot(beam.request) for beam in beams], dtype=torch.int32, device=logits.device)
+        return kernels.shape_logits(logits, torch.empty_like(logits), self.stepper.rules, slots)
 
     def _alternatives(self, logits: torch.Tensor):
         """Per row: the most probable tokens and their log probabilities, on the host."""
@@ -206,8 +229,9 @@ class BeamSearch:
             done[search.index] = search.finished[:self.width]
         if going:
             beams = [beam for search in going for beam in search.beams]
-            logits = self._step([StepEntry(beam.request, [beam.tokens[-1]], [0]) for beam in beams])
-            self._choose(going, self._alternatives(logits))
+            logits = self._step([StepEntry(beam.request, [beam.tokens[-1]], [0], self._choice(search.prompt))
+                                 for search in going for beam in search.beams])
+            self._choose(going, self._alternatives(self._shaped(logits, beams)))
         return going
 
     def _step(self, entries: List[StepEntry]) -> torch.Tensor:
@@ -263,6 +287,9 @@ class BeamSearch:
         if not self.cache.fork([(parent, child) for _, parent, child in forks],
                                [len(search.prompt) + self.max_tokens for search, _, _ in forks]):
             raise RequestRejected("the cache has no room for the beams: other requests hold it")
+        if self.rules is not None and forks:
+            slot = self.cache.slot
+            self.stepper.rules.copy([slot(parent) for _, parent, _ in forks], [slot(child) for _, _, child in forks])
 
 
 def score(stepper: Stepper, sequence: Sequence[int], alternatives: int = 0, portion: int = 512) -> TokenScores:

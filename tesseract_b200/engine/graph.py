@@ -50,6 +50,8 @@ def graph_safe(model) -> bool:
     return all(getattr(part, "graph_safe", False) for part in parts)
 
 
+SAMPLED, CUT, RULED = 0, 1, 2     # how a step's tokens are chosen: as ever; some from a part of the distribution; some under rules
+
 HOST_RING = 3          # pinned copies of a graph's metadata: a launch may be prepared while two are still in flight
 
 
@@ -59,15 +61,18 @@ class _Graph:
     grouping into groups of the same sizes, or (``any_sizes``) into as many groups of any size, whose launches are laid out for more
     tiles than most have."""
 
-    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None, any_sizes: bool = False):
+    def __init__(self, stepper: Stepper, batch: int, columns: int, sampled: torch.Tensor, company=None, any_sizes: bool = False,
+                 choosing: int = SAMPLED):
         cache, device = stepper.cache, stepper.runtime.device
-        self.batch, self.columns = batch, columns
+        self.batch, self.columns, self.choosing = batch, columns, choosing
+        self.rules = stepper.rules if choosing == RULED else None
         self.paged = [i for i, g in enumerate(cache.groups) if g.pool is not None]
         # members, group starts, leaders, keys in common of each group and each row (parts.base.SharedRows)
         together = [batch, batch + 1, batch, batch, batch] if company is not None else []
-        ints = 4 * batch + len(self.paged) * batch * columns + sum(together)
+        chosen = 3 * batch if choosing else 0                       # rule slots, prompt tokens, top-k
+        ints = 4 * batch + len(self.paged) * batch * columns + sum(together) + chosen
         ints = (ints + 1) // 2 * 2                                  # keep the float64 block 8-byte aligned
-        self.nbytes = ints * 4 + batch * 4 + (batch % 2) * 4 + batch * 8
+        self.nbytes = ints * 4 + batch * 4 + (batch % 2) * 4 + batch * 8 * (3 if choosing else 1)
         self.hosts = [torch.zeros(self.nbytes, dtype=torch.uint8, pin_memory=True) for _ in range(HOST_RING)]
         self.host_events: List[Optional[torch.cuda.Event]] = [None] * HOST_RING
         self.next_host = 0
@@ -87,10 +92,15 @@ class _Graph:
             for size in together:
                 out["together"].append(buffer[at:at + size * 4].view(torch.int32))
                 at += size * 4
+            for name in ("rule_slots", "prompts", "top_k") if choosing else ():
+                out[name] = buffer[at:at + batch * 4].view(torch.int32)
+                at += batch * 4
             at = ints * 4
             out["temps"] = buffer[at:at + batch * 4].view(torch.float32)
             at += batch * 4 + (batch % 2) * 4
-            out["uniform"] = buffer[at:at + batch * 8].view(torch.float64)
+            for name in ("uniform", "top_p", "min_p") if choosing else ("uniform",):
+                out[name] = buffer[at:at + batch * 8].view(torch.float64)
+                at += batch * 8
             return out
 
         self.d = carve(self.dev)
@@ -100,6 +110,9 @@ class _Graph:
             arrays = {k: (v.numpy() if not isinstance(v, list) else [t.numpy() for t in v]) for k, v in views.items()}
             arrays["slots"][:] = cache.scratch_slot
             arrays["feed"][:] = -1
+            if choosing:
+                arrays["rule_slots"][:] = -1
+                arrays["top_p"][:] = 1.0
             if company is not None:
                 self.put_together(arrays, company[0])
             self.h_np.append(arrays)
@@ -148,7 +161,14 @@ class _Graph:
         # a row's token comes from the host or, for a sequence that decoded in the step before, from that step's
         # sampler output, which never leaves the device
         kernels.select_tokens(self.d["tokens"], self.d["feed"], self.sampled, self.tokens, stepper.vocab_size)
+        if self.choosing == RULED:
+            kernels.note_tokens(self.rules, self.d["rule_slots"], self.tokens, prompts=self.d["prompts"])
         logits = stepper.model.forward(self.ctx, stepper.cache.bindings, self.want_rows, want_every_row=True)
+        if self.choosing:
+            kernels.choose_tokens(logits, self.d["temps"], self.d["uniform"], self.sampled[:self.batch], top_k=self.d["top_k"],
+                                  top_p=self.d["top_p"], min_p=self.d["min_p"], rules=self.rules,
+                                  slots=self.d["rule_slots"] if self.rules is not None else None)
+            return logits
         # the head may have left each of its CTAs' best token per row: the sampler's second stage of the argmax
         partials = getattr(stepper.model.head, "argmax_partials", lambda: None)()
         kernels.sample(logits, self.d["temps"], self.d["uniform"], self.sampled[:self.batch], partials=partials)
@@ -211,6 +231,8 @@ class DecodeGraphs:
         self.graphs: Dict[Tuple[int, int], _Graph] = {}
         # of steps whose rows have keys in common (Stepper.company): by those groups' sizes, or (`_grouping`) their number
         self.shared_graphs: Dict[Tuple[int, int, object], _Graph] = {}
+        # (both kinds again for steps whose tokens are chosen in another way)
+        self.choosing_graphs = {CUT: ({}, {}), RULED: ({}, {})}
         self.replays = 0
         self.captures = 0
         self.kernels_replayed = 0
@@ -225,24 +247,36 @@ class DecodeGraphs:
         return (self.safe and len(entries) <= self.max_batch
                 and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries))
 
-    def _grouping(self, batch: int, columns: int, company) -> Tuple[int, int, object]:
+    def _grouping(self, batch: int, columns: int, company, graphs) -> Tuple[int, int, object]:
         """The key of a step with company: the sizes of the groups that have keys in common, which a captured launch is laid out for
         (beams keep theirs), or, where a batch has met many, their number, which bounds them."""
         sizes = tuple(sorted(n for n, blocks in zip(company[1], company[2]) if blocks))
         key = (batch, columns, sizes)
-        if key not in self.shared_graphs:
-            met = sum(1 for other in self.shared_graphs if other[:2] == key[:2] and not isinstance(other[2], int))
+        if key not in graphs:
+            met = sum(1 for other in graphs if other[:2] == key[:2] and not isinstance(other[2], int))
             if met >= GROUPINGS:
                 return (batch, columns, len(sizes))
         return key
 
     def launch(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float],
-               previous: Optional[DecodeLaunch] = None, fed: Optional[Sequence[bool]] = None) -> DecodeLaunch:
+               previous: Optional[DecodeLaunch] = None, fed: Optional[Sequence[bool]] = None,
+               top_ps: Optional[Sequence[float]] = None) -> DecodeLaunch:
         """Enqueue one pure-decode step and return at once.  ``fed[i]`` says that entry i's token is whatever
         ``previous`` sampled for the same request (the entry's own token is then ignored): the step can be
-        launched before the host has seen that token."""
+        launched before the host has seen that token.  Top-p comes with the entries' choices, or as ``top_ps``."""
         stepper, cache = self.stepper, self.stepper.cache
         stepper._validate(entries)
+        choosing = SAMPLED
+        params = [e.choice.params if e.choice is not None else None for e in entries]
+        if top_ps is None:
+            top_ps = [p.top_p if p is not None else 1.0 for p in params]
+        if any(p is not None and p.ruled for p in params):
+            choosing = RULED
+            stepper.begin_rules(entries)
+        elif any(p is not None and p.cut for p in params) or any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps)):
+            choosing = CUT
+        if stepper.vocab_size > kernels.MAX_CHOICE_VOCAB:
+            choosing = SAMPLED
         for entry in entries:
             cache.extend(entry.request, 1)
         count = len(entries)
@@ -250,10 +284,11 @@ class DecodeGraphs:
         pages = -(-(max(lengths) + 1) // cache.page_size)
         batch, columns = min(_next_pow2(count), max(self.max_batch, count)), max(8, _next_pow2(pages))
         company = stepper.company(entries, batch - count)
-        graphs, key = (self.graphs, (batch, columns)) if company is None else (self.shared_graphs, self._grouping(batch, columns, company))
+        alone, shared = self.choosing_graphs.get(choosing, (self.graphs, self.shared_graphs))
+        graphs, key = (alone, (batch, columns)) if company is None else (shared, self._grouping(batch, columns, company, shared))
         graph = graphs.get(key)
         if graph is None:
-            graph = _Graph(stepper, batch, columns, self.sampled, company, company is not None and isinstance(key[2], int))
+            graph = _Graph(stepper, batch, columns, self.sampled, company, company is not None and isinstance(key[2], int), choosing)
             graphs[key] = graph
             self.captures += 1
         slot_index, h = graph.host_arrays()
@@ -271,6 +306,13 @@ class DecodeGraphs:
         h["slots"][:count] = slots
         h["temps"][:count] = temperatures
         h["uniform"][:count] = draws
+        if choosing:
+            h["rule_slots"][:] = -1
+            h["rule_slots"][:count] = stepper.rule_slots(entries)
+            h["prompts"][:count] = [1 if e.choice is not None and n < e.choice.prompt_tokens else 0 for e, n in zip(entries, lengths)]
+            h["top_k"][:count] = [p.top_k if p is not None else 0 for p in params]
+            h["top_p"][:count] = top_ps
+            h["min_p"][:count] = [p.min_p if p is not None else 0.0 for p in params]
         if count < graph.batch:
             h["tokens"][count:] = 0
             h["feed"][count:] = -1
@@ -302,10 +344,10 @@ class DecodeGraphs:
         self.kernels_replayed += graph.kernels_per_replay
         return DecodeLaunch({e.request: i for i, e in enumerate(entries)}, count, self._token_ring[ring], done, graph)
 
-    def step(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float]
-             ) -> Tuple[List[int], torch.Tensor]:
+    def step(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float],
+             top_ps: Optional[Sequence[float]] = None) -> Tuple[List[int], torch.Tensor]:
         """Run one pure-decode step and wait for it; returns (tokens, logits [B, vocab] on the device)."""
-        launch = self.launch(entries, temperatures, draws)
+        launch = self.launch(entries, temperatures, draws, top_ps=top_ps)
         return launch.tokens(), launch.graph.logits[:launch.count]
 
 

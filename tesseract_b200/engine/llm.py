@@ -64,7 +64,8 @@ class LLM:
                                    capacity_tokens=self.stepper.cache.num_pages * page_size,
                                    run_and_sample=self.stepper.step_and_sample,
                                    launch_decode=self.stepper.launch_decode if cuda_graphs else None,
-                                   can_launch_decode=self.stepper.can_launch_decode if cuda_graphs else None)
+                                   can_launch_decode=self.stepper.can_launch_decode if cuda_graphs else None,
+                                   vocab_size=self.model.spec.vocab_size)
         self.tokenizer = self._load_tokenizer(model_path)
 
     @staticmethod
@@ -112,15 +113,15 @@ class LLM:
         return out
 
     def beam_search(self, prompts: Sequence[Union[str, Sequence[int]]], width: int = 4, max_tokens: int = 128, *,
-                    length_penalty: float = 0.0, stop_token_ids: Sequence[int] = (), ignore_eos: bool = False
-                    ) -> List[List[BeamOutput]]:
+                    length_penalty: float = 0.0, stop_token_ids: Sequence[int] = (), ignore_eos: bool = False,
+                    rules: Optional[SamplingParams] = None) -> List[List[BeamOutput]]:
         """The ``width`` most probable continuations of every prompt that a beam search finds, best first (:class:`BeamSearch`: a
-        prompt's beams hold its cache pages together).  It drives this engine's own step function and cache; use it while no
+        prompt's beams hold its cache pages together), under the penalties, biases and allowed tokens of ``rules``.  It drives this engine's own step function and cache; use it while no
         generation is in flight."""
         self._need_idle("beam search")
         ends = frozenset(stop_token_ids) | (frozenset() if ignore_eos else frozenset(self.model.spec.eos_token_ids))
         search = BeamSearch(self.stepper, width, max_tokens, end_ids=ends, length_penalty=length_penalty,
-                            portion=self.config.prefill_chunk_tokens)
+                            portion=self.config.prefill_chunk_tokens, rules=rules)
         outputs = search.run([self._encode(p) for p in prompts])
         self._check_device_waits()
         return outputs

@@ -33,18 +33,21 @@ from __future__ import annotations
 
 import itertools
 from collections import deque
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Callable, Deque, Dict, Hashable, List, Optional, Sequence, Tuple
 
 from ..config.engine_config import EngineConfig
-from ..sampling.params import SamplingParams
+from ..sampling.params import SamplingParams, TokenChoice
 from ..sampling.rng import SplitMix64
+from ..sampling.rules import pack_mask
 from .step import StepEntry
 
 FINISH_STOP = "stop"
 FINISH_LENGTH = "length"
 FINISH_CANCELLED = "cancelled"
 FINISH_ERROR = "error"
+
+NO_TOKEN = "no token could be chosen: its rules allow none, or its logits are not finite"
 
 
 class EngineOverloaded(RuntimeError):
@@ -65,6 +68,7 @@ class Request:
     computed_tokens: int = 0
     finish_reason: Optional[str] = None
     error: Optional[str] = None
+    choice: Optional[TokenChoice] = None        # (set where its options need more than a temperature and a draw)
 
     @property
     def target_tokens(self) -> int:
@@ -126,7 +130,7 @@ class Scheduler:
     def __init__(self, config: EngineConfig, cache, run_step: Callable, sample: Callable, *, eos_token_ids=(),
                  max_positions: Optional[int] = None, capacity_tokens: Optional[int] = None,
                  run_and_sample: Optional[Callable] = None, launch_decode: Optional[Callable] = None,
-                 can_launch_decode: Optional[Callable] = None):
+                 can_launch_decode: Optional[Callable] = None, vocab_size: Optional[int] = None):
         config.validate()
         self.config = config
         self.cache = cache
@@ -140,6 +144,7 @@ class Scheduler:
         self._inflight: Optional[Tuple[List[ScheduledSequence], object]] = None   # launched, tokens not read yet
         self.eos_token_ids = frozenset(int(t) for t in eos_token_ids)
         self.max_positions = max_positions
+        self.vocab_size = vocab_size
         self.capacity_tokens = capacity_tokens if capacity_tokens is not None else config.kv_capacity_tokens
         self.requests: Dict[Hashable, Request] = {}
         self.waiting: Deque[Hashable] = deque()
@@ -152,6 +157,8 @@ class Scheduler:
         if len(self.requests) >= self.config.max_pending + self.config.max_running:
             raise EngineOverloaded("the inference engine is overloaded")
         params.validate()
+        if self.vocab_size is not None:
+            params.check_vocabulary(self.vocab_size)
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise RequestRejected("the prompt is empty")
@@ -166,7 +173,7 @@ class Scheduler:
         if request_id in self.requests:
             raise RequestRejected(f"request id {request_id!r} is already in use")
         seed = params.seed if params.seed is not None else hash(request_id) & ((1 << 64) - 1)
-        self.requests[request_id] = Request(request_id, prompt, params, SplitMix64(seed))
+        self.requests[request_id] = Request(request_id, prompt, params, SplitMix64(seed), choice=TokenChoice.of(params, len(prompt)))
         self.waiting.append(request_id)
         return request_id
 
@@ -234,10 +241,16 @@ class Scheduler:
             return self._step_launched_ahead()
         drained = self._drain()
         batch = self.build_batch()
+        batch, allowed, refused = self._ask_grammars(batch)
+        if refused is not None:
+            if drained is not None:
+                refused.absorb_earlier(drained)
+            drained = refused
         if not batch:
             return drained or StepResult([], {}, [])
         self.steps += 1
-        entries = [StepEntry(s.request.id, s.tokens, [len(s.tokens) - 1] if s.samples else []) for s in batch]
+        entries = [StepEntry(s.request.id, s.tokens, [len(s.tokens) - 1] if s.samples else [], allowed.get(s.request.id, s.request.choice))
+                   for s in batch]
         sampled = [s for s in batch if s.samples]
         try:
             temperatures = [s.request.params.temperature for s in sampled]
@@ -258,6 +271,29 @@ class Scheduler:
             result.absorb_earlier(drained)
         return result
 
+    def _ask_grammars(self, batch):
+        """What the grammars of the requests that get a token allow; one that raises, or names what is no token, fails its request
+        alone.  Returns the batch without those, the choices with masks, and what failed."""
+        allowed: Dict[Hashable, TokenChoice] = {}
+        failed: List[Request] = []
+        for s in batch:
+            request, choice = s.request, s.request.choice
+            if not s.samples or choice is None or choice.params.grammar is None:
+                continue
+            try:
+                words = pack_mask(choice.params.grammar(tuple(request.generated)), self.vocab_size)
+                if choice.params.allowed_token_ids is not None:
+                    words = words & pack_mask(choice.params.allowed_token_ids, self.vocab_size)
+                allowed[request.id] = replace(choice, allowed=words)
+            except Exception as exc:  # noqa: BLE001 - the request's own code
+                request.error = f"{type(exc).__name__}: {exc}"
+                done = self._finish(request.id, FINISH_ERROR)
+                if done is not None:
+                    failed.append(done)
+        if not failed:
+            return batch, allowed, None
+        return [s for s in batch if s.request.finish_reason is None], allowed, StepResult([], {}, failed)
+
     def _fail(self, batch, exc) -> StepResult:
         finished = []
         for s in batch:
@@ -273,6 +309,8 @@ class Scheduler:
         requests = [self.requests[i] for i in self.running]
         if any(r.computed_tokens < len(r.prompt) for r in requests):
             return False                                  # prompt portions: those steps run the ordinary way
+        if any(r.params.grammar is not None for r in requests):
+            return False                                  # a grammar is asked with the tokens so far
         return bool(self.can_launch_decode(len(requests), [r.params.top_p for r in requests]))
 
     def _step_launched_ahead(self) -> StepResult:
@@ -282,7 +320,7 @@ class Scheduler:
             return self._drain() or StepResult([], {}, [])
         self.steps += 1
         fed = [s.tokens[0] is None for s in batch]        # the token is still on the device: feed it from there
-        entries = [StepEntry(s.request.id, [0 if f else s.tokens[0]], [0]) for s, f in zip(batch, fed)]
+        entries = [StepEntry(s.request.id, [0 if f else s.tokens[0]], [0], s.request.choice) for s, f in zip(batch, fed)]
         try:
             launch = self.launch_decode(entries, [s.request.params.temperature for s in batch],
                                         [s.draw for s in batch], previous[1] if previous else None, fed)
@@ -324,6 +362,9 @@ class Scheduler:
             if request.finish_reason is not None:
                 continue                                  # ended meanwhile: this row was computed in vain
             token = int(token)
+            if token < 0:
+                finished += self._without_token(request, s.slot)
+                continue
             request.generated[s.slot] = token
             new_tokens.setdefault(request.id, []).append(token)
             reason = self._stop_reason(request, token, s.slot + 1)
@@ -352,6 +393,9 @@ class Scheduler:
         for s, token in zip(sampled, tokens):
             request = s.request
             token = int(token)
+            if token < 0:
+                finished += self._without_token(request, len(request.generated))
+                continue
             request.generated.append(token)
             new_tokens.setdefault(request.id, []).append(token)
             reason = self._stop_reason(request, token, len(request.generated))
@@ -360,6 +404,14 @@ class Scheduler:
                 if done is not None:
                     finished.append(done)
         return StepResult(batch, new_tokens, finished)
+
+    def _without_token(self, request: Request, generated: int) -> List[Request]:
+        """A request of which no token could be chosen ends with those that it has."""
+        request.error = NO_TOKEN
+        del request.generated[generated:]
+        request.computed_tokens = min(request.computed_tokens, len(request.prompt) + generated)
+        done = self._finish(request.id, FINISH_ERROR)
+        return [] if done is None else [done]
 
     def _finish(self, request_id: Hashable, reason: str) -> Optional[Request]:
         request = self.requests.pop(request_id, None)

@@ -18,8 +18,9 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
-from .. import plan
+from .. import kernels, plan
 from ..parts.base import GroupView, Runtime, SharedRows, StepContext, shared_arrays
+from ..sampling.params import MAX_BIASES, TokenChoice
 
 
 @dataclass
@@ -29,6 +30,7 @@ class StepEntry:
     request: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = ()
+    choice: Optional[TokenChoice] = None        # how its token is chosen, beyond a temperature and a draw
 
 
 class StepError(ValueError):
@@ -85,6 +87,49 @@ class Stepper:
         self.graphs = None          # set by enable_graphs()
         self.chunk_graphs = None    # set by enable_graphs(chunk_rows=...)
         self._sampler = None
+        self._rules = None          # made when a request first has rules
+
+    # ------------------------------------------------------------------ rules on next tokens
+    @property
+    def rules(self):
+        """The :class:`TokenRules` of the running requests, by their state slots."""
+        if self._rules is None:
+            from ..sampling.rules import TokenRules
+
+            self._rules = TokenRules(self.cache.max_requests, self.vocab_size, self.runtime.device, biases=MAX_BIASES)
+        return self._rules
+
+    def rule_slots(self, entries: Sequence[StepEntry]) -> List[int]:
+        """The entries' slots in :attr:`rules`; -1 for those without rules."""
+        return [self.cache.slot(e.request) if e.choice is not None and e.choice.params.ruled else -1 for e in entries]
+
+    def begin_rules(self, entries: Sequence[StepEntry]) -> None:
+        """In front of a step: the rules of requests that begin with it, and what grammars allow in it."""
+        for entry in entries:
+            choice = entry.choice
+            if choice is None or not choice.params.ruled:
+                continue
+            params, slot = choice.params, self.cache.slot(entry.request)
+            if self.cache.length(entry.request) == 0:
+                self.rules.set(slot, repetition=params.repetition_penalty, presence=params.presence_penalty,
+                               frequency=params.frequency_penalty, biases=params.logit_bias, allowed=params.allowed_token_ids)
+                self.rules.clear(slot)
+            if choice.allowed is not None:
+                self.rules.set_mask(slot, choice.allowed)
+
+    def note_entries(self, entries: Sequence[StepEntry]) -> None:
+        """The tokens that a step brings go into the histories of the requests with penalties."""
+        noted = [e for e in entries if e.choice is not None and e.choice.params.penalised]
+        if not noted:
+            return
+        counts = [len(e.tokens) for e in noted]
+        starts = np.zeros(len(noted) + 1, dtype=np.int32)
+        np.cumsum(counts, out=starts[1:])
+        tokens = np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in noted])
+        slots = np.asarray([self.cache.slot(e.request) for e in noted], dtype=np.int32)
+        prompts = np.asarray([e.choice.prompt_tokens - self.cache.length(e.request) for e in noted], dtype=np.int32)
+        slots, tokens, starts, prompts = self._staging.upload([slots, tokens, starts, prompts])
+        kernels.note_tokens(self.rules, slots, tokens, starts=starts, prompts=prompts)
 
     # ------------------------------------------------------------------ validation
     def _validate(self, entries: Sequence[StepEntry]) -> List[Sequence[int]]:
@@ -183,6 +228,10 @@ class Stepper:
     def step(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
         """Run one batch; return float32 logits ``[wanted, vocab]`` on the device, or ``None``.  (A replayed
         prompt portion returns a buffer that the next such step overwrites: read it before that.)"""
+        if any(e.choice is not None for e in entries):
+            self._validate(entries)
+            self.begin_rules(entries)
+            self.note_entries(entries)
         if self.chunk_graphs is not None and self.chunk_graphs.eligible(entries):
             return self.chunk_graphs.step(entries)
         tokens = self._validate(entries)
@@ -216,10 +265,12 @@ class Stepper:
                         draws: Sequence[float]) -> List[int]:
         """One step, then one token per wanted row (entries want at most their last place).
 
-        ``temperatures``, ``top_ps`` and ``draws`` hold one value per wanted row, in order.
+        ``temperatures``, ``top_ps`` and ``draws`` hold one value per wanted row, in order.  A row whose request has rules (or a cut)
+        and that no token may follow gets -1.
         """
         from ..sampling.sampler import Sampler, sample_top_p_host
 
+        self._check_choices(entries)
         if self._sampler is None:
             self._sampler = Sampler(self.runtime.device)
         wanted = sum(len(e.want) for e in entries)
@@ -227,22 +278,36 @@ class Stepper:
             self.step(entries)
             return []
         if self.graphs is not None and wanted == len(entries) and self.graphs.eligible(entries):
-            out, logits = self.graphs.step(entries, temperatures, draws)
-            for i, (t, p) in enumerate(zip(temperatures, top_ps)):
-                if t > 0.0 and p < 1.0:
-                    out[i] = sample_top_p_host(logits[i].cpu().numpy(), t, p, draws[i])
+            out, logits = self.graphs.step(entries, temperatures, draws, top_ps)
+            if self.vocab_size > kernels.MAX_CHOICE_VOCAB:
+                for i, (t, p) in enumerate(zip(temperatures, top_ps)):
+                    if t > 0.0 and p < 1.0:
+                        out[i] = sample_top_p_host(logits[i].cpu().numpy(), t, p, draws[i])
             return out
         logits = self.step(entries)
-        return self._sampler.sample(logits, temperatures, top_ps, draws)
+        chosen = [e for e in entries if e.want]
+        if all(e.choice is None for e in chosen):
+            return self._sampler.sample(logits, temperatures, top_ps, draws)
+        slots = self.rule_slots(chosen)
+        ruled = max(slots) >= 0
+        return self._sampler.choose(logits, temperatures, draws, top_ks=[e.choice.params.top_k if e.choice else 0 for e in chosen],
+                                    top_ps=top_ps, min_ps=[e.choice.params.min_p if e.choice else 0.0 for e in chosen],
+                                    rules=self.rules if ruled else None, slots=slots if ruled else None)
+
+    def _check_choices(self, entries: Sequence[StepEntry]) -> None:
+        if self.vocab_size > kernels.MAX_CHOICE_VOCAB and any(e.choice is not None and (
+                e.choice.params.ruled or e.choice.params.top_k > 0 or e.choice.params.min_p > 0.0) for e in entries):
+            raise StepError(f"rules on tokens, top-k and min-p take vocabularies of up to {kernels.MAX_CHOICE_VOCAB} tokens")
 
     def can_launch_decode(self, rows: int, top_ps: Sequence[float]) -> bool:
         """Whether :meth:`launch_decode` takes a batch of ``rows`` single-token rows with these top-p values: a
         graph-replayed decode step, sampled on the device."""
         return (self.graphs is not None and self.graphs.safe and 0 < rows <= self.graphs.max_batch
-                and all(p >= 1.0 for p in top_ps))
+                and (self.vocab_size <= kernels.MAX_CHOICE_VOCAB or all(p >= 1.0 for p in top_ps)))
 
     def launch_decode(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float],
                       previous=None, fed: Optional[Sequence[bool]] = None):
         """Enqueue a decode step without waiting for it; ``launch.tokens()`` waits and returns its tokens.  Entries
         marked in ``fed`` take their token from ``previous`` (the launch before) on the device."""
+        self._check_choices(entries)
         return self.graphs.launch(entries, temperatures, draws, previous, fed)

@@ -565,6 +565,7 @@ def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Te
     return out
 
 
+MAX_CHOICE_VOCAB = 262144
 _CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, RulesRecord, _pointer)
 
 

@@ -16,9 +16,9 @@ import numpy as np
 import torch
 
 from .. import kernels
+from .params import MAX_BIASES
 
 PENALTIES, BIASES, MASK = 1, 2, 4
-MAX_BIASES = 1024
 
 
 def mask_words(vocab: int) -> int:
@@ -143,6 +143,12 @@ class TokenRules:
         if not self._host[slot, 0] & MASK:
             self._host[slot, 0] |= MASK
             self._upload(slot)
+
+    def clear(self, slot: int) -> None:
+        """A slot's history begins anew."""
+        self._check(slot)
+        self._seen[slot].zero_()
+        self._counts[slot].zero_()
 
     def copy(self, sources: Sequence[int], targets: Sequence[int]) -> None:
         """Rules and histories of slots into others, in one launch; no target twice or also a source."""

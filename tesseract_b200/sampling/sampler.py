@@ -2,15 +2,16 @@
 
 Greedy and temperature rows are chosen on the device by the package's sampling kernel
 (argmax with ties to the lowest id, src/cuda/kernels.rs:803-873; inverse-CDF sampling
-with the step's uniform draw).  Rows with ``top_p < 1`` are read back and chosen on the
-host by a restatement of the reference's host sampler (src/engine/sampling.rs:38-75):
+with the step's uniform draw).  Rows with ``top_p < 1``, the reference's host sampler (src/engine/sampling.rs:38-75:
 weights ``exp(l/T - max)`` in 64-bit, sorted by weight, the shortest prefix holding
-``top_p`` of the mass, then the draw scaled by the retained mass.
+``top_p`` of the mass, then the draw scaled by the retained mass), are chosen on the device too, by the kernel that also takes top-k,
+min-p and a request's rules on its logits (``kernels.choose_tokens``); ``sample_top_p_host`` is the same on the host, for
+vocabularies beyond that kernel's.
 """
 
 from __future__ import annotations
 
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -54,6 +55,11 @@ class Sampler:
             return []
         if not (len(temperatures) == len(top_ps) == len(draws) == rows):
             raise ValueError("one temperature, top_p and draw per logits row")
+        if any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps)) and logits.shape[1] <= kernels.MAX_CHOICE_VOCAB:
+            tokens = self.choose(logits, temperatures, draws, top_ps=top_ps)
+            if min(tokens) < 0:
+                raise InvalidLogits("sampler received empty or non-finite logits")
+            return tokens
         out = torch.empty(rows, dtype=torch.int32, device=self.device)
         if all(t == 0.0 for t in temperatures):
             kernels.argmax(logits, out)
@@ -69,3 +75,21 @@ class Sampler:
             for k, i in enumerate(nucleus):
                 tokens[i] = sample_top_p_host(host[k], temperatures[i], top_ps[i], draws[i])
         return tokens
+
+    def choose(self, logits: torch.Tensor, temperatures: Sequence[float], draws: Sequence[float], *,
+               top_ks: Optional[Sequence[int]] = None, top_ps: Optional[Sequence[float]] = None,
+               min_ps: Optional[Sequence[float]] = None, rules=None, slots: Optional[Sequence[int]] = None) -> List[int]:
+        """One token per logits row by ``kernels.choose_tokens``; -1 for a row that has none."""
+        rows = logits.shape[0]
+        # (one copy for all that a row brings: its 64-bit numbers, then those of 32)
+        wide, narrow = np.empty((3, rows), dtype=np.float64), np.zeros((3, rows + rows % 2), dtype=np.int32)
+        wide[0], wide[1], wide[2] = draws, 1.0 if top_ps is None else top_ps, 0.0 if min_ps is None else min_ps
+        narrow[0, :rows] = np.asarray(temperatures, dtype=np.float32).view(np.int32)
+        narrow[1, :rows] = 0 if top_ks is None else top_ks
+        narrow[2, :rows] = -1 if slots is None else slots
+        sent = torch.from_numpy(np.concatenate([wide.reshape(-1), narrow.reshape(-1).view(np.float64)])).to(self.device)
+        wide, narrow = sent[:3 * rows].view(3, rows), sent[3 * rows:].view(torch.int32).view(3, -1)[:, :rows]
+        out = torch.empty(rows, dtype=torch.int32, device=self.device)
+        kernels.choose_tokens(logits, narrow[0].view(torch.float32), wide[0], out, top_k=narrow[1], top_p=wide[1], min_p=wide[2],
+                              rules=rules, slots=narrow[2] if rules is not None else None)
+        return out.cpu().tolist()
