@@ -88,11 +88,12 @@ __global__ void set_kernel(SlotRules* to, SlotRules row) { *to = row; }
 // ---- logits
 //
 // Bound by the 8 V bytes a row that are read and written (less where the mask rules out four neighbours: those are not read).  A block
-// has 4,096 tokens.  It asks for its logits first; under their latency it lists the tokens that were had (a bit each), so that every
+// has 4,096 tokens, every so many-th run of 128 (low ids are had more often than high ones).  It asks for its logits first; under their latency it lists the tokens that were had (a bit each), so that every
 // thread has as many of them, and works those out in 64 bits; then everything is written, the listed ones behind the others.
 
 constexpr int kShapeThreads = 256;
 constexpr int kShapePart = 4096;
+constexpr int kRun = 128;
 constexpr int kEach = kShapePart / kShapeThreads;
 
 // grid (parts of the vocabulary, rows).
@@ -105,10 +106,11 @@ shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride
     constexpr int kBiased = kMaxBiases / kShapeThreads;
     pdl_trigger();
     pdl_wait();
-    const int row = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int first = blockIdx.x * kShapePart, count = min(kShapePart, vocab - first), words = (count + 31) >> 5;
-    const float* x = logits + (int64_t)row * stride + first;
-    float* y = out + (int64_t)row * out_stride + first;
+    const int row = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, part = blockIdx.x, parts = gridDim.x;
+    // the block's tokens are numbered 0 ... 4,095; which one of the vocabulary a number stands for
+    auto token_of = [&](int i) { return ((i / kRun) * parts + part) * kRun + i % kRun; };
+    const float* x = logits + (int64_t)row * stride;
+    float* y = out + (int64_t)row * out_stride;
     const int slot = rules.slots[row];
     SlotRules rule = {};
     if (slot >= 0 && slot < rules.slot_count) rule = rules.table[slot];
@@ -118,11 +120,11 @@ shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride
     const bool in_place = x == y;
     if (in_place && rule.kinds == 0) return;
     if (t < kShapePart / 32) {
-        const int64_t at = (int64_t)slot * rules.words + (first >> 5) + t;
-        mask[t] = masked ? (t < words ? rules.masks[at] : 0u) : ~0u;
-        uint32_t bits = penalised && t < words ? rules.seen[at] : 0;
-        if (t * 32 + 32 > count && bits != 0) bits &= ~0u >> (t * 32 + 32 - count);
-        had[t] = bits;
+        const int token = token_of(32 * t), left = vocab - token;     // (of a word; what is behind the vocabulary is not allowed)
+        const int64_t at = (int64_t)slot * rules.words + (token >> 5);
+        const uint32_t there = left >= 32 ? ~0u : left > 0 ? ~0u >> (32 - left) : 0u;
+        mask[t] = masked && left > 0 ? rules.masks[at] & there : there;
+        had[t] = penalised && left > 0 ? rules.seen[at] & there : 0u;
     }
     __syncthreads();
     // ---- the logits: four neighbours where they are aligned, else one of every 256
@@ -133,21 +135,21 @@ shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride
         if (wide) {
 #pragma unroll
             for (int u = 0; u < kEach; u += 4) {
-                const int i = place(u);
-                const bool any = i < count && (mask[i >> 5] >> (i & 31) & 15);
-                if (any && i + 4 <= count) {
-                    const float4 four = *reinterpret_cast<const float4*>(x + i);
+                const int i = place(u), token = token_of(i);
+                const bool any = mask[i >> 5] >> (i & 31) & 15;
+                if (any && token + 4 <= vocab) {
+                    const float4 four = *reinterpret_cast<const float4*>(x + token);
                     v[u] = four.x, v[u + 1] = four.y, v[u + 2] = four.z, v[u + 3] = four.w;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[u + j] = any && i + j < count ? x[i + j] : -INFINITY;
+                    for (int j = 0; j < 4; ++j) v[u + j] = any && token + j < vocab ? x[token + j] : -INFINITY;
                 }
             }
         } else {
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
                 const int i = place(u);
-                v[u] = i < count && allowed(i) ? x[i] : -INFINITY;
+                v[u] = allowed(i) ? x[token_of(i)] : -INFINITY;
             }
         }
     }
@@ -175,23 +177,25 @@ shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride
             bits &= bits - 1;
         }
         __syncthreads();
-        const int* counts = rules.counts + (int64_t)slot * rules.stride + first;
+        const int* counts = rules.counts + (int64_t)slot * rules.stride;
 #pragma unroll 2
         for (int e = t; e < listed; e += kShapeThreads) {
             const int i = some[e];
-            made[e] = allowed(i) ? shaped_logit(x[i], rule, true, counts[i], 0.0f) : -INFINITY;
+            made[e] = allowed(i) ? shaped_logit(x[token_of(i)], rule, true, counts[token_of(i)], 0.0f) : -INFINITY;
         }
     }
     float biased[kBiased];
+    auto mine = [&](int token) { return token >= 0 && token < vocab && token / kRun % parts == part; };
     if (biases > 0) {
         const int64_t at = (int64_t)slot * rules.room;
 #pragma unroll
         for (int u = 0; u < kBiased; ++u) {
-            const int e = t + u * kShapeThreads, i = e < biases ? rules.bias_ids[at + e] - first : -1;
-            if (i < 0 || i >= count) continue;
+            const int e = t + u * kShapeThreads, token = e < biases ? rules.bias_ids[at + e] : -1;
+            if (!mine(token)) continue;
+            const int i = token / kRun / parts * kRun + token % kRun;
             const bool was = had[i >> 5] >> (i & 31) & 1;
             biased[u] = !allowed(i) ? -INFINITY
-                                    : shaped_logit(x[i], rule, was, was ? rules.counts[(int64_t)slot * rules.stride + first + i] : 0,
+                                    : shaped_logit(x[token], rule, was, was ? rules.counts[(int64_t)slot * rules.stride + token] : 0,
                                                    rules.biases[at + e]);
         }
     }
@@ -200,35 +204,37 @@ shape_kernel(const float* logits, int64_t stride, float* out, int64_t out_stride
         if (wide) {
 #pragma unroll
             for (int u = 0; u < kEach; u += 4) {
-                const int i = place(u);
-                const uint32_t bits = i < count ? mask[i >> 5] >> (i & 31) : 0;
+                const int i = place(u), token = token_of(i);
+                const uint32_t bits = mask[i >> 5] >> (i & 31);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[u + j] = bits >> j & 1 ? v[u + j] : -INFINITY;
-                if (i + 4 <= count) {
-                    *reinterpret_cast<float4*>(y + i) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
+                if (token + 4 <= vocab) {
+                    *reinterpret_cast<float4*>(y + token) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (i + j < count) y[i + j] = v[u + j];
+                        if (token + j < vocab) y[token + j] = v[u + j];
                 }
             }
         } else {
 #pragma unroll
-            for (int u = 0; u < kEach; ++u)
-                if (place(u) < count) y[place(u)] = v[u];
+            for (int u = 0; u < kEach; ++u) {
+                const int token = token_of(place(u));
+                if (token < vocab) y[token] = v[u];
+            }
         }
     }
     if (penalised) {
         __syncthreads();
-        for (int e = t; e < listed; e += kShapeThreads) y[some[e]] = made[e];
+        for (int e = t; e < listed; e += kShapeThreads) y[token_of(some[e])] = made[e];
     }
     if (biases > 0) {
         __syncthreads();
         const int64_t at = (int64_t)slot * rules.room;
 #pragma unroll
         for (int u = 0; u < kBiased; ++u) {
-            const int e = t + u * kShapeThreads, i = e < biases ? rules.bias_ids[at + e] - first : -1;
-            if (i >= 0 && i < count) y[i] = biased[u];
+            const int e = t + u * kShapeThreads, token = e < biases ? rules.bias_ids[at + e] : -1;
+            if (mine(token)) y[token] = biased[u];
         }
     }
 }
