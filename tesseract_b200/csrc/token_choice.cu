@@ -373,44 +373,44 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         const int* ids = rules.bias_ids + (int64_t)slot * rules.room;
         constexpr int kMine = kMaxBiases / kThreads;
         float raw[kMine];
+        auto biased = [&](int e) {                 // the token of a thread's bias, -1 for none of this block's
+            const int at = t + e * kThreads, i = at < biases ? ids[at] - first : -1;
+            return i < count ? i : -1;
+        };
+        // the tokens that were had are listed, so that every thread has as many: under the logits' latency
+        static_assert(kMaxChunk / 32 <= kThreads && kMaxChunk <= kListed * 4, "a word a thread, and room for all tokens of a block");
+        uint16_t* some = reinterpret_cast<uint16_t*>(list);
+        int listed = 0, mine = 0, times = 0;
+        if (rule.kinds & kPenalties) {
+            uint32_t bits = t < words ? seen[t] : 0;
+            if (bits != 0 && t * 32 + 32 > count) bits &= ~0u >> (t * 32 + 32 - count);
+            const Sums<int> of = sum_before(__popc(bits), sh.counts[0]);
+            listed = of.all;
+            int at = of.before;
+#pragma unroll 1
+            while (bits) {
+                some[at++] = (uint16_t)(t * 32 + __ffs(bits) - 1);
+                bits &= bits - 1;
+            }
+            __syncthreads();
+            mine = t < listed ? some[t] : 0;
+            times = t < listed ? had[mine] : 0;
+        }
         copies_done();
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < kMine; ++e) {
-            const int at = t + e * kThreads, i = at < biases ? ids[at] - first : -1;
-            raw[e] = i >= 0 && i < count ? s[i] : 0.0f;
-        }
-        if (rule.kinds & kPenalties) {
-            // the tokens that were had are listed, so that every thread has as many
-            constexpr int kRound = kListed * 4 / 32;                   // words whose tokens the list's place holds
-            uint16_t* some = reinterpret_cast<uint16_t*>(list);
-            for (int w0 = 0; w0 < words; w0 += kRound) {
-                const int w = w0 + t;
-                uint32_t bits = t < kRound && w < words ? seen[w] : 0;
-                if (bits != 0 && w * 32 + 32 > count) bits &= ~0u >> (w * 32 + 32 - count);
-                const Sums<int> of = sum_before(__popc(bits), sh.counts[0]);
-                int n = of.all, at = of.before;
+        for (int e = 0; e < kMine; ++e) raw[e] = biased(e) >= 0 ? s[biased(e)] : 0.0f;
+        __syncthreads();
+        if (t < listed) s[mine] = shaped_logit(s[mine], rule, true, times, 0.0f);
 #pragma unroll 1
-                while (bits) {
-                    some[at++] = (uint16_t)(w * 32 + __ffs(bits) - 1);
-                    bits &= bits - 1;
-                }
-                __syncthreads();
-#pragma unroll 1
-                for (int e = t; e < n; e += kThreads) {
-                    const int i = some[e];
-                    s[i] = shaped_logit(s[i], rule, true, had[i], 0.0f);
-                }
-                __syncthreads();
-            }
-        }
+        for (int e = t + kThreads; e < listed; e += kThreads) s[some[e]] = shaped_logit(s[some[e]], rule, true, had[some[e]], 0.0f);
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < kMine; ++e) {
-            const int at = t + e * kThreads, i = at < biases ? ids[at] - first : -1;
-            if (i < 0 || i >= count) continue;
+            const int i = biased(e);
+            if (i < 0) continue;
             const bool was = rule.kinds & kPenalties && seen[i >> 5] >> (i & 31) & 1;
-            s[i] = shaped_logit(raw[e], rule, was, was ? had[i] : 0, rules.biases[(int64_t)slot * rules.room + at]);
+            s[i] = shaped_logit(raw[e], rule, was, was ? had[i] : 0, rules.biases[(int64_t)slot * rules.room + t + e * kThreads]);
         }
     }
     copies_done();
@@ -660,6 +660,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             lo = p * lo;
             hi = fmin(hi, p * hi + one_weight(of.cut_from > 0 ? (float)of.cut_from / row.scale : 0.0f, sh.table));
         }
+        if (whole) of.end = of.cut_to;             // (what is behind top_p's cut is in the mass already)
         of.draw_from = min(first_bin(most, u * lo, false), of.end);
         of.draw_to = min(first_bin(least, u * hi, true), of.end);
         if (lane == 0) {
@@ -703,7 +704,6 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     }
     if (sh.windows.expected <= kListed) {
         // ---- list the windows' tokens, sum what lies in front of and between them
-        // Tokens of a thread, a bit each: those in windows, and those kept that lie in front of, between or behind them.
         const float stop = end < kBins - 1 ? (float)(end + 1) : INFINITY;
         float begins[kWindows], ends[kWindows];
 #pragma unroll
@@ -711,53 +711,48 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             begins[v] = v < windows ? (float)from[v] : INFINITY;
             ends[v] = v < windows && to[v] < kBins - 1 ? (float)(to[v] + 1) : INFINITY;
         }
-        uint32_t inside = 0, rest[kWindows + 1] = {0, 0, 0, 0};
-#pragma unroll 2
+        uint32_t mine = 0;                         // a bit a token of the thread's that is kept, or may be
+#pragma unroll 4
         for (int i = t, e = 0; i < count; i += kThreads, ++e) {
+            const float d = row.distance(s[i]);
+            mine |= row.at(d) < stop && d <= edge ? 1u << e : 0u;
+        }
+        double gap[kWindows + 1] = {0.0, 0.0, 0.0, 0.0};
+        uint32_t gaps_low = 0, gaps_high = 0;      // counts of 16 bits each
+#pragma unroll 1
+        while (mine) {
+            const int i = t + (__ffs(mine) - 1) * kThreads;
+            mine &= mine - 1;
             const float d = row.distance(s[i]), at = row.at(d);
-            const uint32_t bit = at < stop && d <= edge && d < INFINITY ? 1u << e : 0u;
-            if (bit == 0) continue;
-            if (at < begins[0]) {
-                rest[0] |= bit;
-            } else if (at < ends[0]) {
-                inside |= bit;
-            } else if (at < begins[1]) {
-                rest[1] |= bit;
-            } else if (at < ends[1]) {
-                inside |= bit;
-            } else if (at < begins[2]) {
-                rest[2] |= bit;
-            } else if (at < ends[2]) {
-                inside |= bit;
+            const int w = (at < ends[0] ? 0 : 1) + (at < ends[1] ? 0 : 1) + (at < ends[2] ? 0 : 1);
+            if (at >= (w == 0 ? begins[0] : w == 1 ? begins[1] : w == 2 ? begins[2] : INFINITY)) {
+                list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                       // (any order: it is sorted)
+                atomicAdd(&sh.inside[w], 1);
             } else {
-                rest[3] |= bit;
+                const double weight = weight_of(d, sh.table);
+#pragma unroll
+                for (int v = 0; v <= kWindows; ++v) gap[v] += v == w ? weight : 0.0;
+                const uint32_t one = 1u << (w & 1) * 16;
+                gaps_low += w < 2 ? one : 0u;
+                gaps_high += w < 2 ? 0u : one;
             }
         }
-#pragma unroll 1
-        while (inside) {
-            const int i = t + (__ffs(inside) - 1) * kThreads;
-            inside &= inside - 1;
-            const float d = row.distance(s[i]), at = row.at(d);
-            const int w = (at < ends[0] ? 0 : 1) + (at < ends[1] ? 0 : 1);
-            list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                           // (any order: it is sorted)
-            atomicAdd(&sh.inside[w], 1);
-        }
-#pragma unroll 1
-        for (int v = 0; v <= windows; ++v) {
-            uint32_t mine = v == 0 ? rest[0] : v == 1 ? rest[1] : v == 2 ? rest[2] : rest[3];
-            const int n = __reduce_add_sync(0xffffffffu, __popc(mine));
-            double gap = 0.0;
-#pragma unroll 1
-            while (mine) {
-                const int i = t + (__ffs(mine) - 1) * kThreads;
-                mine &= mine - 1;
-                gap += weight_of(row.distance(s[i]), sh.table);
-            }
-            __syncwarp();
-            gap = row.across(gap);
-            if (lane == 0) {
-                sh.sums[v][warp] = gap;
-                sh.counts[v][warp] = n;
+        __syncwarp();
+        // four sums over a warp at once: each exchange with a lane half as far away leaves half as many to a lane
+        {
+            const bool upper = lane & 16, odd = lane & 8;
+            const double a = upper ? gap[2] : gap[0], b = upper ? gap[3] : gap[1];
+            const double c = a + __shfl_xor_sync(0xffffffffu, upper ? gap[0] : gap[2], 16);
+            const double d = b + __shfl_xor_sync(0xffffffffu, upper ? gap[1] : gap[3], 16);
+            double sum = (odd ? d : c) + __shfl_xor_sync(0xffffffffu, odd ? c : d, 8);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int v = (upper ? 2 : 0) + (odd ? 1 : 0);
+            gaps_low = __reduce_add_sync(0xffffffffu, gaps_low);
+            gaps_high = __reduce_add_sync(0xffffffffu, gaps_high);
+            if ((lane & 7) == 0) {
+                sh.sums[v][warp] = sum;
+                sh.counts[v][warp] = (int)((v < 2 ? gaps_low : gaps_high) >> (v & 1) * 16 & 0xffff);
             }
         }
         __syncthreads();
