@@ -50,6 +50,7 @@ struct Shared {
     // each bin; in the end the entries of the list a cell
     alignas(16) uint32_t cells[kCells];
     double table[kTable];                // 2^(i / 256)
+    uint16_t some[kWarps][64];           // tokens of a warp that wait for 32 to be together
     double sums[kWindows + 1][32];
     int counts[kWindows + 1][32];
     int listed;
@@ -711,33 +712,51 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             begins[v] = v < windows ? (float)from[v] : INFINITY;
             ends[v] = v < windows && to[v] < kBins - 1 ? (float)(to[v] + 1) : INFINITY;
         }
+        double gap[kWindows + 1] = {0.0, 0.0, 0.0, 0.0};
+        uint32_t gaps_low = 0, gaps_high = 0;      // counts of 16 bits each
         uint32_t mine = 0;                         // a bit a token of the thread's that is kept, or may be
 #pragma unroll 4
         for (int i = t, e = 0; i < count; i += kThreads, ++e) {
             const float d = row.distance(s[i]);
             mine |= row.at(d) < stop && d <= edge ? 1u << e : 0u;
         }
-        double gap[kWindows + 1] = {0.0, 0.0, 0.0, 0.0};
-        uint32_t gaps_low = 0, gaps_high = 0;      // counts of 16 bits each
-#pragma unroll 1
-        while (mine) {
-            const int i = t + (__ffs(mine) - 1) * kThreads;
-            mine &= mine - 1;
-            const float d = row.distance(s[i]), at = row.at(d);
-            const int w = (at < ends[0] ? 0 : 1) + (at < ends[1] ? 0 : 1) + (at < ends[2] ? 0 : 1);
-            if (at >= (w == 0 ? begins[0] : w == 1 ? begins[1] : w == 2 ? begins[2] : INFINITY)) {
-                list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                       // (any order: it is sorted)
-                atomicAdd(&sh.inside[w], 1);
-            } else {
-                const double weight = weight_of(d, sh.table);
+        // few of a warp's are, and some lanes have more than others: they are worked on side by side, up to 64 together
+        uint16_t* some = sh.some[warp];
+        int place = __popc(mine);
 #pragma unroll
-                for (int v = 0; v <= kWindows; ++v) gap[v] += v == w ? weight : 0.0;
-                const uint32_t one = 1u << (w & 1) * 16;
-                gaps_low += w < 2 ? one : 0u;
-                gaps_high += w < 2 ? 0u : one;
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, place, o);
+            if (lane >= o) place += other;
         }
-        __syncwarp();
+        const int total = __shfl_sync(0xffffffffu, place, 31);
+        place -= __popc(mine);
+#pragma unroll 1
+        for (int base = 0; base < total; base += 64) {
+#pragma unroll 1
+            while (mine && place < base + 64) {
+                some[place++ - base] = (uint16_t)(t + (__ffs(mine) - 1) * kThreads);
+                mine &= mine - 1;
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int e = lane; e < min(64, total - base); e += 32) {
+                const int i = some[e];
+                const float d = row.distance(s[i]), at = row.at(d);
+                const int w = (at < ends[0] ? 0 : 1) + (at < ends[1] ? 0 : 1) + (at < ends[2] ? 0 : 1);
+                if (at >= (w == 0 ? begins[0] : w == 1 ? begins[1] : w == 2 ? begins[2] : INFINITY)) {
+                    list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                   // (any order: it is sorted)
+                    atomicAdd(&sh.inside[w], 1);
+                } else {
+                    const double weight = weight_of(d, sh.table);
+#pragma unroll
+                    for (int v = 0; v <= kWindows; ++v) gap[v] += v == w ? weight : 0.0;
+                    const uint32_t one = 1u << (w & 1) * 16;
+                    gaps_low += w < 2 ? one : 0u;
+                    gaps_high += w < 2 ? 0u : one;
+                }
+            }
+            __syncwarp();
+        }
         // four sums over a warp at once: each exchange with a lane half as far away leaves half as many to a lane
         {
             const bool upper = lane & 16, odd = lane & 8;
