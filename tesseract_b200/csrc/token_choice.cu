@@ -27,6 +27,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 16;
 constexpr int kMaxChunk = 16384;         // tokens of a block (a bin's count and sum of eighths share 32 bits)
 constexpr int kBins = 1024;
+constexpr int kNear = 384;               // bins that are counted first: most cuts lie in them, and few tokens
 constexpr int kListed = 4096;
 constexpr int kCells = 2 * kBins;        // of the list's sort
 constexpr int kCell = 16;                // entries of a cell that one thread sorts
@@ -570,37 +571,43 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     for (int b = t; b < kBins; b += kThreads) sh.cells[b] = 0;
     __syncthreads();
     const bool whole = !by_k && !by_floor;         // top_p goes by the mass of all tokens
+    const float edge = by_floor ? fmaxf(__double2float_rd(-log(floor)), 0.0f) : INFINITY;      // d of min_p
+    double* least = reinterpret_cast<double*>(list);                   // (the list's place: 2 * kBins numbers)
+    double* most = least + kBins;
+    int* upto = reinterpret_cast<int*>(sh.cells + kBins);
     double mass = 0.0;
-    int far = 0;
-    {
+#pragma unroll 1
+    for (int begin = 0, stop = kNear; begin < kBins; begin = stop, stop = kBins) {
+        int far = 0;
+        const float high = stop < kBins ? (float)stop : (float)(kBins - 1);
         auto tally = [&](int i) {
             const float d = i < count ? row.distance(s[i]) : INFINITY, at = row.at(d);
-            const bool last = !(at < (float)(kBins - 1));
-            // (the last bin may have most of the tokens)
-            const unsigned there = __ballot_sync(0xffffffffu, last);
-            if (there) far += __popc(__ballot_sync(0xffffffffu, last && d < INFINITY));
-            if (!last) {
+            if (at < high && at >= (float)begin) {
                 const int eighths = (int)(at * 8.0f);
                 atomicAdd(&sh.cells[eighths >> 3], 1u << 17 | (eighths & 7));
             }
             return d;
         };
-        if (whole) {
+        if (begin > 0) {
+            // (the last bin, which is whatever lies behind the others, may have most of the tokens)
+#pragma unroll 2
+            for (int i0 = 0; i0 < count; i0 += kThreads) {
+                const float d = tally(i0 + t);
+                far += __popc(__ballot_sync(0xffffffffu, d < INFINITY && !(row.at(d) < high)));
+            }
+            if (lane == 0 && far > 0) atomicAdd(&sh.cells[kBins - 1], (uint32_t)far << 17);
+            row.meet();
+        } else if (whole) {
 #pragma unroll 4
             for (int i0 = 0; i0 < count; i0 += kThreads) mass += weight_of(tally(i0 + t), sh.table);
+            mass = row.row_sum(mass);
+            if (blocks == 1) row.meet();
         } else {
 #pragma unroll 4
             for (int i0 = 0; i0 < count; i0 += kThreads) tally(i0 + t);
+            row.meet();
         }
-    }
-    if (lane == 0 && far > 0) atomicAdd(&sh.cells[kBins - 1], (uint32_t)far << 17);
-    if (whole) mass = row.row_sum(mass);
-    if (!whole || blocks == 1) row.meet();
-    // ---- tokens, and what the mass is at least and at most, up to and with each bin
-    double* least = reinterpret_cast<double*>(list);                   // (the list's place: 2 * kBins numbers)
-    double* most = least + kBins;
-    int* upto = reinterpret_cast<int*>(sh.cells + kBins);
-    {
+        // tokens, and what the mass is at least and at most, up to and with each bin
         constexpr int kEach = kBins / kThreads;
         const double unit = row.scale > 0.0f ? 1.0 / (double)row.scale : 0.0;
         int n[kEach], tokens = 0;
@@ -608,8 +615,10 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int bin = kEach * t + e;
-            int eighths = 0;
             n[e] = 0;
+            a[e] = b[e] = 0.0;
+            if (bin >= stop) continue;
+            int eighths = 0;
             uint32_t of[kMaxBlocks];
 #pragma unroll
             for (int c = 0; c < kMaxBlocks; ++c)                       // (all under way at once)
@@ -620,9 +629,9 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 eighths += (int)(of[c] & 0x1ffff);
             }
             // the tokens' places in the bin: between `eighths` / 8 and that and n / 8 together;  1 - x <= e^-x <= 1 - x + x^2 / 2
-            const double edge = one_weight((float)((double)bin * unit), sh.table), m = n[e];
-            a[e] = bin < kBins - 1 ? edge * (m - unit * 0.125 * (eighths + m)) : 0.0;
-            b[e] = bin < kBins - 1 ? edge * (m - unit * 0.125 * eighths + 0.5 * unit * unit * m) : edge * m;
+            const double top = one_weight((float)((double)bin * unit), sh.table), m = n[e];
+            a[e] = bin < kBins - 1 ? top * (m - unit * 0.125 * (eighths + m)) : 0.0;
+            b[e] = bin < kBins - 1 ? top * (m - unit * 0.125 * eighths + 0.5 * unit * unit * m) : top * m;
             tokens += n[e];
             lower += a[e];
             upper += b[e];
@@ -637,9 +646,11 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             most[kEach * t + e] = (over += b[e]) * (1.0 + kSpare);
         }
         __syncthreads();
+        // does a cut lie in what was counted?
+        if (whole ? least[stop - 1] >= p * mass : (by_k && upto[stop - 1] >= k) || (by_floor && row.at(edge) < (float)stop)) break;
+        if (stop < kBins) row.meet();              // (everyone has read the counts)
     }
     // ---- the bins that the cuts and the draw may lie in
-    const float edge = by_floor ? fmaxf(__double2float_rd(-log(floor)), 0.0f) : INFINITY;      // d of min_p
     if (warp == 0) {
         Windows of = {};
         of.end = kBins - 1;
