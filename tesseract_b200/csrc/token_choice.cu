@@ -18,6 +18,8 @@
 //   3. the tokens of those bins are listed, what weighs in front of and between them is summed in 64 bits;
 //   4. one block sorts the list, and the sums in the order of the rank give every cut and the token.
 // Where those bins have more tokens than a list holds (great numbers of equal logits), the place in the rank is halved instead.
+#include <mutex>
+
 #include "token_rules.cuh"
 
 namespace {
@@ -298,7 +300,7 @@ struct Row {
         }
         // (a thousandth of a bin to spare)
         const float near = scale > 0.0f ? fmaxf(0.0f, (float)from - 1e-3f) / scale : 0.0f;
-        const float far = scale > 0.0f && to < kBins - 1 ? ((float)to + 1.001f) / scale : INFINITY;
+        const float far = scale == 0.0f ? 0.0f : to < kBins - 1 ? ((float)to + 1.001f) / scale : INFINITY;
         uint64_t low = key_of(near, 0), high = min((unsigned long long)key_of(far, (1 << kIds) - 1), (unsigned long long)bound);
 #pragma unroll 1
         while (low < high) {
@@ -959,24 +961,6 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
 int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const float* logits, int64_t stride, const float* temperature,
                 const double* uniform, const int* top_k, const double* top_p, const double* min_p, int* out, const Rules& rules) {
     const int chunk = ((vocab + blocks - 1) / blocks + 127) / 128 * 128;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(blocks, rows, 1);
-    config.blockDim = dim3(kThreads);
-    // the list; behind it the logits, in whose place the first block later has the row's list and its sums
-    const size_t logits_at = kListed * 8, space = (size_t)(chunk + 4) * 4, later = 2 * kListed * 8;
-    config.dynamicSmemBytes = logits_at + (space > later ? space : later);
-    config.stream = stream;
-    static bool told[64];
-    int device = 0;
-    if (const cudaError_t err = cudaGetDevice(&device)) return (int)err;
-    if (device < 0 || device >= 64 || !told[device]) {
-        if (const cudaError_t err = cudaFuncSetAttribute(choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                         (int)(logits_at + 2 * kListed * 8 + 16)))
-            return (int)err;
-        if (const cudaError_t err = cudaFuncSetAttribute(choose_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1))
-            return (int)err;
-        if (device >= 0 && device < 64) told[device] = true;
-    }
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
     attribute[0].val.clusterDim.x = blocks;
@@ -984,8 +968,38 @@ int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const floa
     attribute[0].val.clusterDim.z = 1;
     attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // may start under the end of the head
     attribute[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(blocks, rows, 1);
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
     config.attrs = attribute;
     config.numAttrs = 2;
+    // the list; behind it the logits, in whose place the first block later has the row's list and its sums
+    const size_t logits_at = kListed * 8, space = (size_t)(chunk + 4) * 4, later = 2 * kListed * 8;
+    // Once a device: what the kernel may have, and how many rows of so many blocks find a multiprocessor a block at the same time.  Those
+    // are kept apart, by shared memory that they do not use (12 rows of 128,256 logits 22.6 us, 28.8 with two blocks a multiprocessor).
+    constexpr size_t kAlone = 120 * 1024;
+    static std::mutex lock;
+    static int rows_apart[64][kMaxBlocks + 1];
+    int device = 0, apart = 0;
+    if (const cudaError_t err = cudaGetDevice(&device)) return (int)err;
+    if (device < 0 || device >= 64) return TB_ERR_BAD_SIZE;
+    {
+        std::lock_guard<std::mutex> guard(lock);
+        if (rows_apart[device][blocks] == 0) {
+            if (const cudaError_t err = cudaFuncSetAttribute(choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAlone))
+                return (int)err;
+            if (const cudaError_t err = cudaFuncSetAttribute(choose_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1))
+                return (int)err;
+            config.dynamicSmemBytes = kAlone;
+            int clusters = 0;
+            if (const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, choose_kernel, &config)) return (int)err;
+            rows_apart[device][blocks] = 1 + clusters;                 // (0: not asked yet)
+        }
+        apart = rows_apart[device][blocks] - 1;
+    }
+    config.dynamicSmemBytes = logits_at + (space > later ? space : later);
+    if (blocks > 1 && rows <= apart) config.dynamicSmemBytes = kAlone;
     const cudaError_t err = cudaLaunchKernelEx(&config, choose_kernel, logits, stride, temperature, uniform, top_k, top_p, min_p,
                                                out, vocab, chunk, rules);
     return err == cudaSuccess ? tb_launch_status() : (int)err;
@@ -1008,11 +1022,12 @@ TB_EXPORT int tb_choose_tokens(const float* logits, int64_t stride, const float*
                                cudaStream_t stream) {
     if (rows == 0) return 0;
     if (vocab <= 0 || rows < 0 || rows > 65535 || vocab > kMaxBlocks * kMaxChunk || rules.room > kMaxBiases) return TB_ERR_BAD_SIZE;
-    // As few blocks a row as hold it, and up to eight while each has a multiprocessor of its own.  (Device time, 8 / 4 blocks a row:
-    // 8 rows of 50,257 logits 20.7 / 22.5 us, 64 rows 56 / 31; 16 blocks of 128,256 logits: 1 row 27.6 us, 28.7 with 8, 8 rows 39, 30
-    // with 8, as few clusters of 16 fit the chip.  Blocks of 1,024 threads: 16 rows 56 us, 40 with 512, two blocks a multiprocessor.)
-    int blocks = 1;
-    while (vocab > blocks * kMaxChunk) blocks <<= 1;
-    while (blocks < 8 && rows * blocks * 2 <= sm_count() && vocab > blocks * 2048) blocks <<= 1;
+    // As few blocks a row as hold it, and up to eight while each has a multiprocessor of its own and 2,048 tokens.  (Device time, 8 / 4
+    // blocks a row: 8 rows of 50,257 logits 20.7 / 22.5 us, 64 rows 56 / 31; 16 blocks of 128,256 logits: 1 row 27.6 us, 28.7 with 8, 8
+    // rows 39, 30 with 8, as few clusters of 16 fit the chip.  Blocks of 1,024 threads: 16 rows 56 us, 40 with 512, two blocks a
+    // multiprocessor.)
+    int blocks = (vocab + kMaxChunk - 1) / kMaxChunk;
+    const int more = min(min(8, sm_count() / rows), vocab / 2048);
+    if (blocks < more) blocks = more;
     return launch_rows(rows, vocab, blocks, stream, logits, stride, temperature, uniform, top_k, top_p, min_p, out, rules);
 }
