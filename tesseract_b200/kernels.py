@@ -497,6 +497,7 @@ def _rules_of(what: str, rules, slots: Optional[torch.Tensor], rows: int, vocab:
         raise KernelError(f"{what}: rules over {rules.vocab} tokens, logits over {vocab}")
     if slots.get_device() != device or rules.table.get_device() != device:
         raise KernelError(f"{what} takes tensors of one device")
+    _need(rules.table.is_cuda, f"{what} takes rules on a CUDA device")
     record = RulesRecord.from_buffer_copy(rules.record)
     record.slots = slots.data_ptr()
     return record
@@ -521,6 +522,7 @@ def note_tokens(rules, slots: torch.Tensor, tokens: torch.Tensor, *, starts: Opt
     ``prompts[r]`` of a row's tokens (none without it) are its prompt's: had, but not counted as generated.  With ``restart`` a slot's
     history begins anew with them (of rows that name one slot the last counts).  All int32; a token outside the vocabulary is no token."""
     rows, count, device = slots.numel(), tokens.numel(), rules.table.get_device()
+    _need(device >= 0 and device == torch.cuda.current_device(), "note_tokens runs on the current device, where the rules are")
     slots_at, tokens_at = _list_of("note_tokens", slots, device), _list_of("note_tokens", tokens, device)
     starts_at = _list_of("note_tokens", starts, device) if starts is not None else None
     prompts_at = _list_of("note_tokens", prompts, device) if prompts is not None else None
@@ -543,6 +545,8 @@ def _logit_rows(what: str, logits: torch.Tensor) -> tuple:
         raise KernelError(f"{what} takes logits with contiguous rows")
     if stride < vocab and rows > 1:
         raise KernelError(f"{what} takes rows of logits that do not lie on each other")
+    if logits.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{what} runs on the current device, where the logits are")
     return rows, vocab, stride
 
 

@@ -10,8 +10,8 @@ Not in the reference either: what a request may say about its next tokens.  Its 
 ``repetition_penalty`` (divides the positive and multiplies the negative logits of tokens of the prompt and the answer),
 ``frequency_penalty`` (taken off for every time that the answer has a token), ``presence_penalty`` (taken off once),
 ``logit_bias`` ({token: bias}, up to 1,024), and then only ``allowed_token_ids`` and what ``grammar`` returns may follow (a callable
-that is given the tokens generated so far and returns the ids of those that may come next; it is asked on the host in front of every
-token).  With a temperature above 0 the token is drawn from the ``top_k`` most probable (0: all), of those the ones at least ``min_p``
+that is given the tokens generated so far and returns the ids of those that may come next, or a numpy array of truth values, one a
+token of the vocabulary; it is asked on the host in front of every token).  With a temperature above 0 the token is drawn from the ``top_k`` most probable (0: all), of those the ones at least ``min_p``
 times as probable as the most probable, of those the fewest that hold ``top_p``.
 """
 

@@ -27,7 +27,13 @@ def mask_words(vocab: int) -> int:
 
 
 def pack_mask(allowed: Iterable[int], vocab: int) -> np.ndarray:
-    """The mask words of the given token ids; ids outside the vocabulary raise."""
+    """The mask words of the given token ids, or of truth values, one a token (an array ``[vocab]``); ids outside the vocabulary raise."""
+    if isinstance(allowed, np.ndarray) and allowed.dtype == np.bool_:
+        if allowed.shape != (vocab,):
+            raise ValueError(f"a mask of truth values has one for each of the vocabulary's {vocab}")
+        bits = np.zeros(mask_words(vocab) * 32, dtype=np.bool_)
+        bits[:vocab] = allowed
+        return np.packbits(bits, bitorder="little").view(np.int32)
     ids = np.asarray(allowed if isinstance(allowed, np.ndarray) else list(allowed))
     bits = np.zeros(mask_words(vocab) * 32, dtype=np.uint8)
     if ids.size:

@@ -3,6 +3,7 @@ hands on, grammars, and requests that no token can follow."""
 
 import math
 
+import numpy as np
 import pytest
 
 from tesseract_b200.config.engine_config import EngineConfig
@@ -123,6 +124,15 @@ def test_a_grammar_is_asked_with_the_tokens_so_far_in_front_of_every_token():
     masks = [choice.allowed for request, choice in fake.choices if request == a]
     for words in masks:
         assert [t for t in range(2000) if int(words[t // 32]) >> t % 32 & 1] == [1000, 1001, 1002, 1003]
+
+
+def test_a_grammar_may_return_truth_values():
+    s, fake = make()
+    allowed = np.zeros(2000, dtype=bool)
+    allowed[1000:1003] = True
+    a = s.add_request([1, 2], SamplingParams(max_tokens=9, temperature=0.0, grammar=lambda tokens: allowed, ignore_eos=True))
+    done = {r.id: r for r in run_all(s)}
+    assert done[a].generated == [1000, 1001, 1002] and done[a].finish_reason == FINISH_ERROR
 
 
 def test_a_grammar_that_fails_ends_its_request_alone():

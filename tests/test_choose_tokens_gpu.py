@@ -44,7 +44,7 @@ SETTINGS = [dict(), dict(top_k=1), dict(top_k=5), dict(top_k=50, top_p=0.9), dic
             dict(top_k=20000), dict(top_k=20000, top_p=0.8)]
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 32, 33, 257, 1000, 2049, 8192, 16385, 50257, 128256, 262144])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 32, 33, 257, 1000, 2049, 8192, 16385, 50257, 128256, 151936, 262144])
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
 def test_sizes_and_cuts(vocab, settings):
     rng = np.random.RandomState(vocab + len(str(settings)))
@@ -237,7 +237,10 @@ def test_refusals():
             ((x, t[:1], u, out), {}), ((x[0], t, u, out), {}), ((x.t().contiguous().t(), t, u, out), {}), ((x[:, :0], t, u, out), {}),
             ((x, t, u, out), {"top_k": u}), ((x, t, u, out), {"top_p": t}), ((x, t, u, out), {"min_p": t}),
             ((x, t, u, out), {"top_p": u[:1]}), ((x, t, u, out), {"slots": out}), ((x, t, u, out), {"rules": rules}),
-            ((x, t, u, out), {"rules": TokenRules(2, 11, "cuda"), "slots": out}), ((x, t, u, out.cpu()), {})):
+            ((x, t, u, out), {"rules": TokenRules(2, 11, "cuda"), "slots": out}), ((x, t, u, out.cpu()), {}),
+            ((x, None, u, out), {}), ((torch.zeros(2, 262145, device="cuda"), t, u, out), {}),
+            ((x, t, u, out), {"rules": TokenRules(2, 10, "cpu"), "slots": out}), ((x.cpu(), t, u, out), {}),
+            ((torch.zeros(2, 19, device="cuda").as_strided((2, 10), (9, 1)), t, u, out), {})):
         with pytest.raises(kernels.KernelError):
             kernels.choose_tokens(*arguments, **keywords)
     none = torch.empty(0, 10, device="cuda")

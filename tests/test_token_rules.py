@@ -16,10 +16,13 @@ def test_masks_are_bits_in_order(vocab):
     assert words.dtype == np.int32 and words.shape == (mask_words(vocab),)
     assert [t for t in range(mask_words(vocab) * 32) if int(words[t // 32]) >> t % 32 & 1] == allowed
     assert not pack_mask([], vocab).any()
+    truth = np.zeros(vocab, dtype=bool)
+    truth[allowed] = True
+    assert np.array_equal(pack_mask(truth, vocab), words)
 
 
 def test_masks_refuse_what_is_no_token():
-    for allowed in ([-1], [100], [0.5], np.array([3, 100])):
+    for allowed in ([-1], [100], [0.5], np.array([3, 100]), np.zeros(99, dtype=bool)):
         with pytest.raises(ValueError):
             pack_mask(allowed, 100)
 
