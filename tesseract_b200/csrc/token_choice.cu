@@ -34,6 +34,7 @@ constexpr int kListed = 4096;
 constexpr int kCells = 2 * kBins;        // of the list's sort
 constexpr int kCell = 16;                // entries of a cell that one thread sorts
 constexpr int kTable = 256;
+constexpr int kInside = 4;
 constexpr int kWindows = 3;              // where the draw, top_p's cut and top_k's cut may lie
 constexpr int kIds = 18;                 // bits of an id: kMaxBlocks * kMaxChunk tokens
 constexpr float kReach = 32.0f;          // the bins cover d down to -32 at most; what is below is in the last
@@ -46,6 +47,7 @@ struct Windows {
     int from[kWindows], to[kWindows];
     int draw_from, draw_to, cut_from, cut_to, cut_bin;
     int end;                             // the last bin with anything kept
+    int tail[kWindows], in_front;        // tokens up to the end of each window that are in windows; in front of the last, in none
 };
 
 struct Shared {
@@ -62,13 +64,12 @@ struct Shared {
     float best, low;
     int first;
     double mass[2];
-    // what the first block is told by each: entries of its list, and in which windows; the mass and the number of what is kept in no
-    // window but in front of each, or behind the last
-    int listed_of[kMaxBlocks], inside_of[kMaxBlocks][kWindows], gaps_of[kMaxBlocks][kWindows + 1];
+    // what the first block is told by each: the entries of its list; the mass of what is kept in front of each window and behind the
+    // one before, and behind the last
+    int listed_of[kMaxBlocks];
     double gap_of[kMaxBlocks][kWindows + 1];
-    int inside[kWindows];
     double base[kWindows + 1];
-    int behind[kWindows + 1], tail[kWindows];
+    uint8_t region[kBins];               // a bin's: the window (kInside and more) or the gap that it is in
 };
 
 __device__ __forceinline__ uint32_t peer_address(const void* local, uint32_t rank) {
@@ -693,8 +694,12 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 }
             }
 #pragma unroll 1
-            for (int v = 0; v < of.count; ++v)
-                of.expected += upto[sh.windows.to[v]] - (sh.windows.from[v] > 0 ? upto[sh.windows.from[v] - 1] : 0);
+            for (int v = 0; v < of.count; ++v) {
+                const int ahead = sh.windows.from[v] > 0 ? upto[sh.windows.from[v] - 1] : 0;
+                sh.windows.in_front = ahead - of.expected;
+                of.expected += upto[sh.windows.to[v]] - ahead;
+                sh.windows.tail[v] = of.expected;
+            }
             sh.windows.count = of.count;
             sh.windows.expected = of.expected;
             sh.windows.draw_from = of.draw_from;
@@ -706,9 +711,8 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             sh.listed = 0;
         }
     }
-    if (t >= 32 && t < 32 + kWindows) sh.inside[t - 32] = 0;
     __syncthreads();                               // (from here on the list's place is free)
-    const int windows = sh.windows.count, end = sh.windows.end;
+    const int windows = sh.windows.count, end = sh.windows.end, upto_end = upto[end];
     by_k = sh.windows.cut_bin >= 0;
     int from[kWindows], to[kWindows];
 #pragma unroll
@@ -718,58 +722,67 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     }
     if (sh.windows.expected <= kListed) {
         // ---- list the windows' tokens, sum what lies in front of and between them
-        const float stop = end < kBins - 1 ? (float)(end + 1) : INFINITY;
-        float begins[kWindows], ends[kWindows];
 #pragma unroll
-        for (int v = 0; v < kWindows; ++v) {
-            begins[v] = v < windows ? (float)from[v] : INFINITY;
-            ends[v] = v < windows && to[v] < kBins - 1 ? (float)(to[v] + 1) : INFINITY;
+        for (int e = 0; e < kBins / kThreads; ++e) {
+            const int bin = t + e * kThreads;
+            int region = windows;
+#pragma unroll
+            for (int v = kWindows - 1; v >= 0; --v) region = bin < from[v] ? min(region, v) : bin <= to[v] ? kInside : region;
+            sh.region[bin] = (uint8_t)region;
         }
+        __syncthreads();
         double gap[kWindows + 1] = {0.0, 0.0, 0.0, 0.0};
-        uint32_t gaps_low = 0, gaps_high = 0;      // counts of 16 bits each
-        uint32_t mine = 0;                         // a bit a token of the thread's that is kept, or may be
+        auto take = [&](int i, float d) {
+            const float at = row.at(d);
+            const int region = sh.region[at < (float)(kBins - 1) ? (int)at : kBins - 1];
+            if (region == kInside) {
+                list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                       // (any order: it is sorted)
+            } else {
+                const double weight = weight_of(d, sh.table);
+                if (region == 0) gap[0] += weight;
+                if (region == 1) gap[1] += weight;
+                if (region == 2) gap[2] += weight;
+                if (region == 3) gap[3] += weight;
+            }
+        };
+        const float stop = end < kBins - 1 ? (float)(end + 1) : INFINITY, limit = fminf(edge, 3.402823466e38f);
+        if (upto_end > vocab / 4) {
+#pragma unroll 2
+            for (int i = t; i < count; i += kThreads) {
+                const float d = row.distance(s[i]);
+                if (row.at(d) < stop && d <= limit) take(i, d);
+            }
+        } else {
+            uint32_t mine = 0;                     // a bit a token of the thread's that is kept, or may be
 #pragma unroll 4
-        for (int i = t, e = 0; i < count; i += kThreads, ++e) {
-            const float d = row.distance(s[i]);
-            mine |= row.at(d) < stop && d <= edge ? 1u << e : 0u;
-        }
-        // few of a warp's are, and some lanes have more than others: they are worked on side by side, up to 64 together
-        uint16_t* some = sh.some[warp];
-        int place = __popc(mine);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int other = __shfl_up_sync(0xffffffffu, place, o);
-            if (lane >= o) place += other;
-        }
-        const int total = __shfl_sync(0xffffffffu, place, 31);
-        place -= __popc(mine);
-#pragma unroll 1
-        for (int base = 0; base < total; base += 64) {
-#pragma unroll 1
-            while (mine && place < base + 64) {
-                some[place++ - base] = (uint16_t)(t + (__ffs(mine) - 1) * kThreads);
-                mine &= mine - 1;
+            for (int i = t, e = 0; i < count; i += kThreads, ++e) {
+                const float d = row.distance(s[i]);
+                mine |= row.at(d) < stop && d <= limit ? 1u << e : 0u;
             }
-            __syncwarp();
-#pragma unroll 1
-            for (int e = lane; e < min(64, total - base); e += 32) {
-                const int i = some[e];
-                const float d = row.distance(s[i]), at = row.at(d);
-                const int w = (at < ends[0] ? 0 : 1) + (at < ends[1] ? 0 : 1) + (at < ends[2] ? 0 : 1);
-                if (at >= (w == 0 ? begins[0] : w == 1 ? begins[1] : w == 2 ? begins[2] : INFINITY)) {
-                    list[atomicAdd(&sh.listed, 1)] = key_of(d, first + i);                   // (any order: it is sorted)
-                    atomicAdd(&sh.inside[w], 1);
-                } else {
-                    const double weight = weight_of(d, sh.table);
+            // few of a warp's are, and some lanes have more than others: they are worked on side by side, up to 64 together
+            uint16_t* some = sh.some[warp];
+            int place = __popc(mine);
 #pragma unroll
-                    for (int v = 0; v <= kWindows; ++v) gap[v] += v == w ? weight : 0.0;
-                    const uint32_t one = 1u << (w & 1) * 16;
-                    gaps_low += w < 2 ? one : 0u;
-                    gaps_high += w < 2 ? 0u : one;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, place, o);
+                if (lane >= o) place += other;
+            }
+            const int total = __shfl_sync(0xffffffffu, place, 31);
+            place -= __popc(mine);
+#pragma unroll 1
+            for (int base = 0; base < total; base += 64) {
+#pragma unroll 1
+                while (mine && place < base + 64) {
+                    some[place++ - base] = (uint16_t)(t + (__ffs(mine) - 1) * kThreads);
+                    mine &= mine - 1;
                 }
+                __syncwarp();
+#pragma unroll 1
+                for (int e = lane; e < min(64, total - base); e += 32) take(some[e], row.distance(s[some[e]]));
+                __syncwarp();
             }
-            __syncwarp();
         }
+        __syncwarp();
         // four sums over a warp at once: each exchange with a lane half as far away leaves half as many to a lane
         {
             const bool upper = lane & 16, odd = lane & 8;
@@ -779,28 +792,15 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             double sum = (odd ? d : c) + __shfl_xor_sync(0xffffffffu, odd ? c : d, 8);
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const int v = (upper ? 2 : 0) + (odd ? 1 : 0);
-            gaps_low = __reduce_add_sync(0xffffffffu, gaps_low);
-            gaps_high = __reduce_add_sync(0xffffffffu, gaps_high);
-            if ((lane & 7) == 0) {
-                sh.sums[v][warp] = sum;
-                sh.counts[v][warp] = (int)((v < 2 ? gaps_low : gaps_high) >> (v & 1) * 16 & 0xffff);
-            }
+            if ((lane & 7) == 0) sh.sums[(upper ? 2 : 0) + (odd ? 1 : 0)][warp] = sum;
         }
         __syncthreads();
         // (each block tells the first; what another one reads in its turn stays where it is until the end)
         if (t <= windows) {
             double sum = 0.0;
-            int n = 0;
 #pragma unroll 8
-            for (int w = 0; w < kWarps; ++w) {
-                sum += sh.sums[t][w];
-                n += sh.counts[t][w];
-            }
+            for (int w = 0; w < kWarps; ++w) sum += sh.sums[t][w];
             tell(&sh.gap_of[block][t], 0, sum);
-            tell(&sh.gaps_of[block][t], 0, n);
-        } else if (t >= 32 && t < 32 + kWindows) {
-            tell(&sh.inside_of[block][t - 32], 0, sh.inside[t - 32]);
         } else if (t == 64) {
             tell(&sh.listed_of[block], 0, sh.listed);
         }
@@ -811,18 +811,11 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             uint64_t* sorted = keys + kListed;
             if (t == 0) {
                 double base = 0.0;
-                int behind = 0, tail = 0;
 #pragma unroll 1
                 for (int v = 0; v <= windows; ++v) {
 #pragma unroll 4
-                    for (int b = 0; b < blocks; ++b) {
-                        base += sh.gap_of[b][v];
-                        behind += sh.gaps_of[b][v];
-                        tail += v < windows ? sh.inside_of[b][v] : 0;
-                    }
+                    for (int b = 0; b < blocks; ++b) base += sh.gap_of[b][v];
                     sh.base[v] = base;
-                    sh.behind[v] = behind;
-                    if (v < windows) sh.tail[v] = tail;
                 }
             }
             int before = lane < blocks ? sh.listed_of[lane] : 0;       // a lane a block: the entries up to and with it
@@ -920,15 +913,15 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
 #pragma unroll 1
             for (int e = first_of; e < last_of; ++e) {
                 run += sums[e];
-                const int v = (e >= sh.tail[0] ? 1 : 0) + (windows > 1 && e >= sh.tail[1] ? 1 : 0);
+                const int v = (e >= sh.windows.tail[0] ? 1 : 0) + (windows > 1 && e >= sh.windows.tail[1] ? 1 : 0);
                 sums[e] = sh.base[min(v, windows - 1)] + run;
             }
             __syncthreads();
             if (t == 0) {
                 int kept = n;
                 double total = of.all + sh.base[windows];
-                if (by_k && k - sh.behind[windows - 1] < n) {
-                    kept = max(1, k - sh.behind[windows - 1]);
+                if (by_k && k - sh.windows.in_front < n) {
+                    kept = max(1, k - sh.windows.in_front);
                     total = sums[kept - 1];
                 }
                 if (whole) total = mass;
