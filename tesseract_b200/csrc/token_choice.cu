@@ -12,12 +12,21 @@
 // A row is shared by a thread-block cluster; each block reads its part of the vocabulary once, into shared memory, and all that follows
 // runs there:
 //   1. rules and mask are applied, the row's largest and smallest logit found;
-//   2. the tokens are counted in 1,024 bins of d, each with its place in the bin to an eighth, and (where top_p goes by it) the mass of
-//      all is summed.  Of a bin of width h whose tokens lie F eighths into it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the
+//   2. the tokens are counted in 1,024 bins of d, each with its place in the bin to an eighth (the nearest 384 first: that is where most
+//      cuts lie, and few tokens, of 14 cycles an atomic instruction), and where top_p goes by it the mass of all is summed.  Of a bin of width h whose tokens lie F eighths into it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the
 //      cumulative mass is known bin by bin to some 0.4 %, and with it the few bins in which each cut and the draw can lie;
 //   3. the tokens of those bins are listed, what weighs in front of and between them is summed in 64 bits;
 //   4. one block sorts the list, and the sums in the order of the rank give every cut and the token.
-// Where those bins have more tokens than a list holds (great numbers of equal logits), the place in the rank is halved instead.
+// Where those bins have more tokens than a list holds (great numbers of equal logits), the place in the rank is halved instead.  No sum
+// depends on the order of atomics: those count, or fill a list that is sorted.
+//
+// What bounds it: of the 4 V bytes a row, read once, a call of few rows takes a small part (one row of 128,256 logits: 0.1 us of 21).
+// It is a chain of some twenty dependent phases and four cluster barriers: 3 us until the logits are there, 1.5 for the largest, 4.5 for
+// weights and counts (32 tokens a thread), 4 to put the blocks' counts together, 1.7 to find the bins, 3 to list, 5 for the first
+// block's sort, sums and searches.  Up to 15 rows of that vocabulary take no longer (22.8 us; one block a multiprocessor), 32 take 31
+// (two), and beyond that rows queue, as a row's logits fill half of eight multiprocessors' shared memory: 64 rows 60 us, 256 rows 224,
+// at 1.7 instructions a cycle and a third of all warps' time at barriers.  Reading the logits again from L2 in place of shared memory, for
+// more blocks a multiprocessor, was slower (64 rows 98 us against 83 then).
 #include <mutex>
 
 #include "token_rules.cuh"

@@ -5,8 +5,9 @@ namespace {
 
 // ---- histories
 //
-// seen: a bit for every token of the prompt and the answer; counts: how often the answer has each.  Bound by the 4 V + V / 8 bytes that
-// a history begun anew is written with.
+// seen: a bit for every token of the prompt and the answer; counts: how often the answer has each.  A history begun anew writes 4 V + V / 8
+// bytes: 32 requests of up to 8,192 tokens over 128,256 take 8.3 us on the device, of which 4.8 remain when no block goes through the
+// tokens (17 MB are 2.7 us at the copy rate); one request 2.7 us, a launch and three dependent loads.
 
 constexpr int kNoteThreads = 512;
 constexpr int kNotePart = 8192;          // tokens of the vocabulary that a block begins anew
@@ -87,7 +88,10 @@ __global__ void set_kernel(SlotRules* to, SlotRules row) { *to = row; }
 
 // ---- logits
 //
-// Bound by the 8 V bytes a row that are read and written (less where the mask rules out four neighbours: those are not read).  A block
+// 8 V bytes a row are read and written (less where the mask rules out four neighbours: those are not read): 64 rows of 128,256 without
+// rules take 13.5 us (4.9 TB/s), with a mask 15.7, with penalties, biases and a mask 23.8.  What bounds those is the blocks' own chain
+// (rules, bits, counts, 64-bit arithmetic between barriers: a third of all warps' time) with four blocks a multiprocessor; more blocks with
+// fewer registers were no faster.  A block
 // has 4,096 tokens, every so many-th run of 128 (low ids are had more often than high ones).  It asks for its logits first; under their latency it lists the tokens that were had (a bit each), so that every
 // thread has as many of them, and works those out in 64 bits; then everything is written, the listed ones behind the others.
 

@@ -491,25 +491,30 @@ def _rules_of(what: str, rules, slots: Optional[torch.Tensor], rows: int, vocab:
     if rules is None:
         _need(slots is None, f"{what} has slots without rules")
         return _NO_RULES
-    if slots is None or slots.dtype != torch.int32 or not slots.is_contiguous() or slots.numel() != rows:
+    if slots is None or slots.dtype is not _int32 or not slots.is_contiguous() or slots.numel() != rows:
         raise KernelError(f"{what} takes a slot a row (contiguous int32 [S])")
     if rules.vocab != vocab:
         raise KernelError(f"{what}: rules over {rules.vocab} tokens, logits over {vocab}")
-    if slots.get_device() != device or rules.table.get_device() != device:
-        raise KernelError(f"{what} takes tensors of one device")
-    _need(rules.table.is_cuda, f"{what} takes rules on a CUDA device")
+    if slots.get_device() != device or rules.index != device:
+        raise KernelError(f"{what} takes tensors of one CUDA device")
     record = RulesRecord.from_buffer_copy(rules.record)
     record.slots = slots.data_ptr()
     return record
 
 
-def _list_of(what: str, t: torch.Tensor, device: int) -> int:
+def _list_of(t: Optional[torch.Tensor], device: int) -> Optional[int]:
     """The address of a contiguous int32 list."""
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-        raise KernelError(f"{what} takes contiguous int32 lists")
-    if t.get_device() != device or device < 0:
-        raise KernelError(f"{what} takes tensors of one CUDA device")
+    if t is None:
+        return None
+    if t.dtype is not _int32 or t.dim() != 1 or not t.is_contiguous():
+        raise KernelError("note_tokens takes contiguous int32 lists")
+    if t.get_device() != device:
+        raise KernelError("note_tokens takes tensors of one CUDA device")
     return t.data_ptr()
+
+
+_int32 = torch.int32
+_current_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 _NOTE_TOKENS = (_pointer, _pointer, _i32, _i32, _i32, _i32, _pointer, _pointer, _i32, _pointer, _pointer, _i32, _i32, _pointer)
@@ -521,17 +526,17 @@ def note_tokens(rules, slots: torch.Tensor, tokens: torch.Tensor, *, starts: Opt
     ``starts`` (int32 ``[R + 1]``) ``tokens[starts[r]:starts[r + 1]]``, to slot ``slots[r]`` (negative: to none).  The first
     ``prompts[r]`` of a row's tokens (none without it) are its prompt's: had, but not counted as generated.  With ``restart`` a slot's
     history begins anew with them (of rows that name one slot the last counts).  All int32; a token outside the vocabulary is no token."""
-    rows, count, device = slots.numel(), tokens.numel(), rules.table.get_device()
-    _need(device >= 0 and device == torch.cuda.current_device(), "note_tokens runs on the current device, where the rules are")
-    slots_at, tokens_at = _list_of("note_tokens", slots, device), _list_of("note_tokens", tokens, device)
-    starts_at = _list_of("note_tokens", starts, device) if starts is not None else None
-    prompts_at = _list_of("note_tokens", prompts, device) if prompts is not None else None
-    _need(starts.numel() == rows + 1 if starts is not None else count == rows, "note_tokens takes a token a row, or where each row's start")
-    _need(prompts is None or prompts.numel() == rows, "note_tokens takes the length of a prompt a row")
-    record = rules.record
+    rows, count, device = slots.numel(), tokens.numel(), rules.index
+    if device < 0 or device != _current_device():
+        raise KernelError("note_tokens runs on the current CUDA device, where the rules are")
+    if (count != rows if starts is None else starts.numel() != rows + 1):
+        raise KernelError("note_tokens takes a token a row, or where each row's start")
+    if prompts is not None and prompts.numel() != rows:
+        raise KernelError("note_tokens takes the length of a prompt a row")
+    seen, counts, slot_count, words, stride = rules.history
     _check(_entry("token_rules", "tb_note_tokens", _NOTE_TOKENS)(
-        record.seen, record.counts, record.slot_count, record.words, record.stride, rules.vocab, slots_at, tokens_at, count, starts_at,
-        prompts_at, rows, int(restart), _raw_stream()), "note_tokens")
+        seen, counts, slot_count, words, stride, rules.vocab, _list_of(slots, device), _list_of(tokens, device), count,
+        _list_of(starts, device), _list_of(prompts, device), rows, 1 if restart else 0, _stream_of(device)), "note_tokens")
 
 
 _SHAPE_LOGITS = (_pointer, _i64, _pointer, _i64, _i32, _i32, RulesRecord, _pointer)
@@ -545,7 +550,7 @@ def _logit_rows(what: str, logits: torch.Tensor) -> tuple:
         raise KernelError(f"{what} takes logits with contiguous rows")
     if stride < vocab and rows > 1:
         raise KernelError(f"{what} takes rows of logits that do not lie on each other")
-    if logits.get_device() != torch.cuda.current_device():
+    if logits.get_device() != _current_device():
         raise KernelError(f"{what} runs on the current device, where the logits are")
     return rows, vocab, stride
 
@@ -564,7 +569,7 @@ def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Te
     if rows and not (a == b and (rows == 1 or stride == out_stride)):
         _need(a >= b + 4 * ((rows - 1) * out_stride + vocab) or b >= a + 4 * ((rows - 1) * stride + vocab),
               "shape_logits writes to the logits' own place or apart from them")
-    _check(_entry("token_rules", "tb_shape_logits", _SHAPE_LOGITS)(a, stride, b, out_stride, rows, vocab, record, _raw_stream()),
+    _check(_entry("token_rules", "tb_shape_logits", _SHAPE_LOGITS)(a, stride, b, out_stride, rows, vocab, record, _stream_of(device)),
            "shape_logits")
     return out
 
@@ -599,7 +604,7 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
         logits.data_ptr(), stride, _per_row("temperature", temperature, torch.float32, rows, device),
         _per_row("uniform", uniform, torch.float64, rows, device), _per_row("top_k", top_k, torch.int32, rows, device),
         _per_row("top_p", top_p, torch.float64, rows, device), _per_row("min_p", min_p, torch.float64, rows, device),
-        _per_row("out", out, torch.int32, rows, device), rows, vocab, record, _raw_stream()), "choose_tokens")
+        _per_row("out", out, torch.int32, rows, device), rows, vocab, record, _stream_of(device)), "choose_tokens")
     return out
 
 

@@ -66,6 +66,8 @@ class TokenRules:
         self.masks = self._masks[:, :self.words]
         self.record = kernels.RulesRecord(None, *[t.data_ptr() for t in (self.table, self._seen, self._counts, self._masks, self.bias_ids,
                                                                         self.biases)], slots, wide, 32 * wide, biases)
+        self.index = self.table.get_device()                 # (-1 on the host)
+        self.history = (self._seen.data_ptr(), self._counts.data_ptr(), slots, wide, 32 * wide)
         self._host = np.zeros((slots, 8), dtype=np.int32)
         self._host[:, 2] = np.float32(1.0).view(np.int32)
 
