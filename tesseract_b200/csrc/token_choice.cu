@@ -17,7 +17,8 @@
 //      cumulative mass is known bin by bin to some 0.4 %, and with it the few bins in which each cut and the draw can lie;
 //   3. the tokens of those bins are listed, what weighs in front of and between them is summed in 64 bits;
 //   4. one block sorts the list, and the sums in the order of the rank give every cut and the token.
-// Where those bins have more tokens than a list holds (great numbers of equal logits), the place in the rank is halved instead.  No sum
+// Where those bins have more tokens than a list holds (great numbers of equal logits), the distance is found by halving its interval, and
+// the place among those equal to it by counting them.  No sum
 // depends on the order of atomics: those count, or fill a list that is sorted.
 //
 // What bounds it: of the 4 V bytes a row, read once, a call of few rows takes a small part (one row of 128,256 logits: 0.1 us of 21).
@@ -73,6 +74,8 @@ struct Shared {
     float best, low;
     int first;
     double mass[2];
+    int equal;
+    uint64_t place;
     // what the first block is told by each: the entries of its list; the mass of what is kept in front of each window and behind the
     // one before, and behind the last
     int listed_of[kMaxBlocks];
@@ -308,22 +311,52 @@ struct Row {
             from = 0;
             to = kBins - 1;
         }
-        // (a thousandth of a bin to spare)
+        // the distance (a thousandth of a bin to spare)
         const float near = scale > 0.0f ? fmaxf(0.0f, (float)from - 1e-3f) / scale : 0.0f;
         const float far = scale == 0.0f ? 0.0f : to < kBins - 1 ? ((float)to + 1.001f) / scale : INFINITY;
-        uint64_t low = key_of(near, 0), high = min((unsigned long long)key_of(far, (1 << kIds) - 1), (unsigned long long)bound);
+        constexpr uint64_t kAll = (1u << kIds) - 1;
+        uint64_t low = key_of(near, 0) >> kIds, high = min((unsigned long long)key_of(far, 0), (unsigned long long)bound) >> kIds;
 #pragma unroll 1
         while (low < high) {
             const uint64_t middle = low + (high - low) / 2;
-            const double v = through(mass, middle);
-            if (reach(v)) {
-                high = middle;
-                sum = v;
-            } else {
-                low = middle + 1;
-            }
+            if (reach(through(mass, min((unsigned long long)bound, (unsigned long long)(middle << kIds | kAll))))) high = middle; else low = middle + 1;
         }
-        return high;
+        // of the tokens at that distance, by id, the fewest that reach it
+        const float d = distance_of(high << kIds);
+        const double in_front = high > 0 ? through(mass, (high << kIds) - 1) : 0.0, each = mass ? one_weight(d, sh.table) : 1.0;
+        const int part = (count + kThreads - 1) / kThreads, begin = min(count, (int)threadIdx.x * part), end = min(count, begin + part);
+        auto equal = [&](int i) { return distance(s[i]) == d && key_of(d, first + i) <= bound; };
+        int mine = 0;
+#pragma unroll 1
+        for (int i = begin; i < end; ++i) mine += equal(i);
+        const Sums<int> here = sum_before(mine, sh.counts[0]);
+        if (threadIdx.x == 0) sh.equal = here.all;
+        meet();
+        int upto = lane() < blocks ? (blocks > 1 ? peer(&sh.equal, lane()) : here.all) : 0;          // a lane a block
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane() >= o) upto += other;
+        }
+        const int all = __shfl_sync(0xffffffffu, upto, 31), before = block > 0 ? __shfl_sync(0xffffffffu, upto, max(0, block - 1)) : 0;
+        int least = 1, most = max(1, all);
+#pragma unroll 1
+        while (least < most) {
+            const int middle = (least + most) >> 1;
+            if (reach(in_front + (double)middle * each)) most = middle; else least = middle + 1;
+        }
+        sum = in_front + (double)most * each;
+        const int owner = max(0, __ffs(__ballot_sync(0xffffffffu, upto >= most)) - 1);
+        int left = most - before - here.before;                        // (it is the thread's left-th)
+        if (block == owner && left > 0 && left <= mine) {
+#pragma unroll 1
+            for (int i = begin; i < end; ++i)
+                if (equal(i) && --left == 0) sh.place = key_of(d, first + i);
+        }
+        meet();
+        const uint64_t found = blocks > 1 ? peer_u64(&sh.place, owner) : sh.place;
+        meet();                                                        // (the next one may be written)
+        return found;
     }
 };
 

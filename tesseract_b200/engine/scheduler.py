@@ -159,6 +159,8 @@ class Scheduler:
         params.validate()
         if self.vocab_size is not None:
             params.check_vocabulary(self.vocab_size)
+        if (params.ruled or params.top_k > 0 or params.min_p > 0.0) and (self.run_and_sample is None or self.vocab_size is None):
+            raise RequestRejected("this scheduler's sampler takes a temperature and top-p")
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise RequestRejected("the prompt is empty")

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from tesseract_b200.config.engine_config import EngineConfig
-from tesseract_b200.engine.scheduler import FINISH_ERROR, FINISH_LENGTH, Scheduler
+from tesseract_b200.engine.scheduler import FINISH_ERROR, FINISH_LENGTH, RequestRejected, Scheduler
 from tesseract_b200.sampling import SamplingParams
 from tesseract_b200.sampling.params import TokenChoice
 from tests.test_scheduler import FakeAheadEngine, run_all
@@ -86,6 +86,17 @@ def test_a_token_outside_the_vocabulary_is_refused_when_the_request_arrives():
         with pytest.raises(ValueError):
             s.add_request([1, 2], SamplingParams(**given))
     assert not s.has_work()
+
+
+def test_a_scheduler_whose_sampler_takes_no_rules_refuses_them():
+    config = EngineConfig(max_queue=8, max_running=4, max_batch_tokens=32, prefill_chunk_tokens=8,
+                          kv_capacity_tokens=512, max_sequence_length=512)
+    fake = Choosing(config)
+    plain = Scheduler(config, fake.cache, fake.run_step, fake.sample, max_positions=400)
+    for given in (dict(top_k=4), dict(min_p=0.1), dict(logit_bias={3: 1.0}), dict(grammar=lambda tokens: [1])):
+        with pytest.raises(RequestRejected):
+            plain.add_request([1, 2], SamplingParams(**given))
+    plain.add_request([1, 2], SamplingParams(max_tokens=2, top_p=0.5))
 
 
 @pytest.mark.parametrize("ahead", [False, True])
