@@ -47,6 +47,7 @@ constexpr int kTable = 256;
 constexpr int kInside = 4;
 constexpr int kWindows = 3;              // where the draw, top_p's cut and top_k's cut may lie
 constexpr int kIds = 18;                 // bits of an id: kMaxBlocks * kMaxChunk tokens
+constexpr float kWeightless = 700.0f;
 constexpr float kReach = 32.0f;          // the bins cover d down to -32 at most; what is below is in the last
 // To spare in a mass that the bins bound: the bins' width and the weights of their edges are rounded to 32 bits, 2^-24 * 32 in d.
 constexpr double kSpare = 1e-5;
@@ -127,11 +128,11 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 // e^-d for d from -2^-8 on in 64 bits, by a table of 2^(i / 256) and the series of what is left (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point arithmetic", 1989): -d = (256 m + i) ln 2 / 256 + r, |r| <= ln 2 / 512,
 // e^r by its series up to r^3: what is left is below 1.4e-13, and of one sign, so that most of it is common to a row's weights.
-// Beyond 700 (+inf among it) it is e^-700, 10^-304, which is nothing beside the largest weight, 1.
+// Beyond kWeightless (+inf among it) it is e^-700, 10^-304, which is nothing beside the largest weight, 1.
 __device__ __forceinline__ double weight_of(float d, const double* table) {
     constexpr double kSteps = -256.0 / 0.693147180559945309417232121458, kStep = 0.693147180559945309417232121458 / 256.0;
     constexpr double kRound = 6755399441055744.0;                              // 1.5 * 2^52: adding it rounds to a whole number
-    const double x = (double)fminf(d, 700.0f), whole = fma(x, kSteps, kRound);
+    const double x = (double)fminf(d, kWeightless), whole = fma(x, kSteps, kRound);
     const int n = __double2loint(whole);
     const double r = fma(whole - kRound, -kStep, -x), two = table[n & (kTable - 1)];
     const double step = __hiloint2double(__double2hiint(two) + (n >> 8 << 20), __double2loint(two));
@@ -554,9 +555,15 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         // ---- in the order of ids: a warp has a run of tokens
         const int part = ((count + kWarps - 1) / kWarps + 31) & ~31;
         const int begin = min(count, warp * part), end = min(count, begin + part);
+        // (a draw of 0 takes the first token that weighs anything)
+        auto weight = [&](float l) {
+            const float d = fmaf(-l, row.inverse, row.top);
+            const double w = weight_of(d, sh.table);
+            return d <= kWeightless ? w : 0.0;
+        };
         double mine = 0.0;
 #pragma unroll 4
-        for (int i = begin + lane; i < end; i += 32) mine += weight_of(fmaf(-s[i], row.inverse, row.top), sh.table);
+        for (int i = begin + lane; i < end; i += 32) mine += weight(s[i]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane == 0) sh.sums[1][warp] = mine;
@@ -566,7 +573,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         row.meet();
         // a lane a block: the masses up to and with it
         double upto = blocks > 1 ? (lane < blocks ? peer(&sh.mass[0], lane) : 0.0) : lane == 0 ? here : 0.0;
-        const bool some = upto > 1e-300;
+        const bool some = upto > 0.0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double other = __shfl_up_sync(0xffffffffu, upto, o);
@@ -579,7 +586,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         const double before = owner > 0 ? __shfl_sync(0xffffffffu, upto, max(0, owner - 1)) : 0.0;
         if (block == owner) {
             double run = lane < kWarps ? sh.sums[1][lane] : 0.0;
-            const bool any_here = run > 1e-300;
+            const bool any_here = run > 0.0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double other = __shfl_up_sync(0xffffffffu, run, o);
@@ -593,16 +600,15 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 int token = -1, spare = -1;
                 for (int i0 = begin; i0 < end && token < 0; i0 += 32) {
                     const int i = i0 + lane;
-                    const float l = i < end ? s[i] : -INFINITY;
-                    const double w = one_weight(fmaf(-l, row.inverse, row.top), sh.table);
+                    const double w = i < end ? weight(s[i]) : 0.0;
                     double incl = w;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const double other = __shfl_up_sync(0xffffffffu, incl, o);
                         if (lane >= o) incl += other;
                     }
-                    const unsigned passed = __ballot_sync(0xffffffffu, l > -INFINITY && in_front + incl > target);
-                    const unsigned any = __ballot_sync(0xffffffffu, l > -INFINITY);
+                    const unsigned passed = __ballot_sync(0xffffffffu, w > 0.0 && in_front + incl > target);
+                    const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
                     if (any) spare = first + i0 + 31 - __clz(any);
                     if (passed) token = first + i0 + __ffs(passed) - 1;
                     in_front += __shfl_sync(0xffffffffu, incl, 31);

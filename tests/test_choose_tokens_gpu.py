@@ -128,6 +128,16 @@ def test_rows_without_a_token():
             assert got[1:5] == [-1] * 4 and got[5] == 0 and got[7] == 5 and min(got[0], got[6]) >= 0
 
 
+@pytest.mark.parametrize("vocab", [3, 100, 20000, 128256])
+def test_a_draw_of_nothing_takes_the_first_token_that_weighs_anything(vocab):
+    x = np.zeros((4, vocab), dtype=np.float32)
+    for row, low in enumerate((-np.inf, -3.4028235e38, -1e4, -1500.0)):
+        x[row, :vocab - 2] = low
+    for settings in (dict(), dict(top_k=vocab - 1), dict(top_p=0.9)):
+        check(x, 1.0, 0.0, **settings)
+        assert run(torch.from_numpy(x).cuda(), 1.0, 0.0, **settings) == [vocab - 2] * 4
+
+
 @pytest.mark.parametrize("temperature", [1e-40, 1e-38, 1e-30, 1e-6, 1e-3, 30.0, 1e6, 1e30, 3e38])
 def test_temperatures_far_from_one(temperature):
     rng = np.random.RandomState(7)
