@@ -258,6 +258,17 @@ class DecodeGraphs:
                 return (batch, columns, len(sizes))
         return key
 
+    def _choosing(self, entries: Sequence[StepEntry], temperatures: Sequence[float], top_ps: Optional[Sequence[float]]) -> int:
+        """How a step's tokens are chosen."""
+        if self.stepper.vocab_size > kernels.MAX_CHOICE_VOCAB:
+            return SAMPLED
+        params = [e.choice.params for e in entries if e.choice is not None]
+        if any(p.ruled for p in params):
+            return RULED
+        if any(p.cut for p in params) or (top_ps is not None and any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps))):
+            return CUT
+        return SAMPLED
+
     def launch(self, entries: Sequence[StepEntry], temperatures: Sequence[float], draws: Sequence[float],
                previous: Optional[DecodeLaunch] = None, fed: Optional[Sequence[bool]] = None,
                top_ps: Optional[Sequence[float]] = None) -> DecodeLaunch:
@@ -266,17 +277,9 @@ class DecodeGraphs:
         launched before the host has seen that token.  Top-p comes with the entries' choices, or as ``top_ps``."""
         stepper, cache = self.stepper, self.stepper.cache
         stepper._validate(entries)
-        choosing = SAMPLED
-        params = [e.choice.params if e.choice is not None else None for e in entries]
-        if top_ps is None:
-            top_ps = [p.top_p if p is not None else 1.0 for p in params]
-        if any(p is not None and p.ruled for p in params):
-            choosing = RULED
+        choosing = self._choosing(entries, temperatures, top_ps)
+        if choosing == RULED:
             stepper.begin_rules(entries)
-        elif any(p is not None and p.cut for p in params) or any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps)):
-            choosing = CUT
-        if stepper.vocab_size > kernels.MAX_CHOICE_VOCAB:
-            choosing = SAMPLED
         for entry in entries:
             cache.extend(entry.request, 1)
         count = len(entries)
@@ -307,12 +310,15 @@ class DecodeGraphs:
         h["temps"][:count] = temperatures
         h["uniform"][:count] = draws
         if choosing:
+            choices = [e.choice for e in entries]
+            if top_ps is None:
+                top_ps = [c.params.top_p if c is not None else 1.0 for c in choices]
             h["rule_slots"][:] = -1
             h["rule_slots"][:count] = stepper.rule_slots(entries)
-            h["prompts"][:count] = [1 if e.choice is not None and n < e.choice.prompt_tokens else 0 for e, n in zip(entries, lengths)]
-            h["top_k"][:count] = [p.top_k if p is not None else 0 for p in params]
+            h["prompts"][:count] = [1 if c is not None and n < c.prompt_tokens else 0 for c, n in zip(choices, lengths)]
+            h["top_k"][:count] = [c.params.top_k if c is not None else 0 for c in choices]
             h["top_p"][:count] = top_ps
-            h["min_p"][:count] = [p.min_p if p is not None else 0.0 for p in params]
+            h["min_p"][:count] = [c.params.min_p if c is not None else 0.0 for c in choices]
         if count < graph.batch:
             h["tokens"][count:] = 0
             h["feed"][count:] = -1
