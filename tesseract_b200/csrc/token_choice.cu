@@ -47,8 +47,8 @@ constexpr int kTable = 256;
 constexpr int kInside = 4;
 constexpr int kWindows = 3;              // where the draw, top_p's cut and top_k's cut may lie
 constexpr int kIds = 18;                 // bits of an id: kMaxBlocks * kMaxChunk tokens
-constexpr float kWeightless = 700.0f;
-constexpr float kReach = 32.0f;          // the bins cover d down to -32 at most; what is below is in the last
+constexpr float kWeightless = 700.0f;    // a token beyond weighs nothing
+constexpr float kReach = 32.0f;          // the bins cover d up to 32 at most; what is beyond is in the last
 // To spare in a mass that the bins bound: the bins' width and the weights of their edges are rounded to 32 bits, 2^-24 * 32 in d.
 constexpr double kSpare = 1e-5;
 
@@ -66,7 +66,7 @@ struct Shared {
     // each bin; in the end the entries of the list a cell
     alignas(16) uint32_t cells[kCells];
     double table[kTable];                // 2^(i / 256)
-    uint16_t some[kWarps][64];           // tokens of a warp that wait for 32 to be together
+    uint16_t some[kWarps][64];           // tokens of a warp that are worked on together
     double sums[kWindows + 1][32];
     int counts[kWindows + 1][32];
     int listed;
@@ -82,7 +82,7 @@ struct Shared {
     int listed_of[kMaxBlocks];
     double gap_of[kMaxBlocks][kWindows + 1];
     double base[kWindows + 1];
-    uint8_t region[kBins];               // a bin's: the window (kInside and more) or the gap that it is in
+    uint8_t region[kBins];               // a bin's: kInside, or the gap between windows that it is in
 };
 
 __device__ __forceinline__ uint32_t peer_address(const void* local, uint32_t rank) {
@@ -427,8 +427,8 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         constexpr int kMine = kMaxBiases / kThreads;
         float raw[kMine];
         auto biased = [&](int e) {                 // the token of a thread's bias, -1 for none of this block's
-            const int at = t + e * kThreads, i = at < biases ? ids[at] - first : -1;
-            return i < count ? i : -1;
+            const int at = t + e * kThreads, id = at < biases ? ids[at] : -1;
+            return id >= first && id < first + count ? id - first : -1;
         };
         // the tokens that were had are listed, so that every thread has as many: under the logits' latency
         static_assert(kMaxChunk / 32 <= kThreads && kMaxChunk <= kListed * 4, "a word a thread, and room for all tokens of a block");
