@@ -12,20 +12,21 @@
 // A row is shared by a thread-block cluster; each block reads its part of the vocabulary once, into shared memory, and all that follows
 // runs there:
 //   1. rules and mask are applied, the row's largest and smallest logit found;
-//   2. the tokens are counted in 1,024 bins of d, each with its place in the bin to an eighth (the nearest 384 first, as most cuts lie
-//      in those: 64 rows 59.5 us, 63.3 with all at once, but 46 in place of 55 where a flat distribution needs all), and where top_p goes by it the mass of all is summed.  Of a bin of width h whose tokens lie F eighths into it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the
-//      cumulative mass is known bin by bin to some 0.4 %, and with it the few bins in which each cut and the draw can lie;
+//   2. the tokens are counted in 1,024 bins of d, each with its place in the bin to an eighth, and where top_p goes by it the mass of
+//      all is summed.  The blocks' counts are put together, of the nearest 384 bins first, as most cuts lie in those (64 rows 58.7 us,
+//      63.2 with all at once; where a flat distribution needs all, 47.8 and 45.7).  Of a bin of width h whose tokens lie F eighths into
+//      it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the cumulative mass is known bin by bin to some 0.4 %, and with it the
+//      few bins in which each cut and the draw can lie;
 //   3. the tokens of those bins are listed, what weighs in front of and between them is summed in 64 bits;
 //   4. one block sorts the list, and the sums in the order of the rank give every cut and the token.
 // Where those bins have more tokens than a list holds (great numbers of equal logits), the distance is found by halving its interval, and
-// the place among those equal to it by counting them.  No sum
-// depends on the order of atomics: those count, or fill a list that is sorted.
+// the place among those equal to it by counting them.  No sum depends on the order of atomics: those count, or fill a list that is sorted.
 //
-// What bounds it: of the 4 V bytes a row, read once, a call of few rows takes a small part (one row of 128,256 logits: 0.1 us of 21).
+// What bounds it: of the 4 V bytes a row, read once, a call of few rows takes a small part (one row of 128,256 logits: 0.1 us of 20).
 // It is a chain of some twenty dependent phases and four cluster barriers: 3 us until the logits are there, 1.5 for the largest, 4.5 for
 // weights and counts (32 tokens a thread), 4 to put the blocks' counts together, 1.7 to find the bins, 3 to list, 5 for the first
-// block's sort, sums and searches.  Up to 15 rows of that vocabulary take no longer (22.8 us; one block a multiprocessor), 32 take 31
-// (two), and beyond that rows queue, as a row's logits fill half of eight multiprocessors' shared memory: 64 rows 60 us, 256 rows 224,
+// block's sort, sums and searches.  Up to 15 rows of that vocabulary take no longer (21.7 us; one block a multiprocessor), 32 take 30
+// (two), and beyond that rows queue, as a row's logits fill half of eight multiprocessors' shared memory: 64 rows 59 us, 256 rows 217,
 // at 1.7 instructions a cycle and a third of all warps' time at barriers.  Reading the logits again from L2 in place of shared memory, for
 // more blocks a multiprocessor, was slower (64 rows 98 us against 83 then).
 #include <mutex>
@@ -39,7 +40,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 16;
 constexpr int kMaxChunk = 16384;         // tokens of a block (a bin's count and sum of eighths share 32 bits)
 constexpr int kBins = 1024;
-constexpr int kNear = 384;               // bins that are counted first
+constexpr int kNear = 384;               // bins that are put together first
 constexpr int kListed = 4096;
 constexpr int kCells = 2 * kBins;        // of the list's sort
 constexpr int kCell = 16;                // entries of a cell that one thread sorts
@@ -624,7 +625,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         const float reach = fminf(row.distance(low), kReach);
         row.scale = reach > 0.0f ? fminf((float)kBins / reach, 1e30f) : 0.0f;
     }
-    for (int b = t; b < kBins; b += kThreads) sh.cells[b] = 0;
+    for (int b = t; b < kBins + 32; b += kThreads) sh.cells[b] = 0;
     __syncthreads();
     const bool whole = !by_k && !by_floor;         // top_p goes by the mass of all tokens
     const float edge = by_floor ? fmaxf(__double2float_rd(-log(floor)), 0.0f) : INFINITY;      // d of min_p
@@ -632,27 +633,15 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     double* most = least + kBins;
     int* upto = reinterpret_cast<int*>(sh.cells + kBins);
     double mass = 0.0;
-#pragma unroll 1
-    for (int begin = 0, stop = kNear; begin < kBins; begin = stop, stop = kBins) {
-        int far = 0;
-        const int low = row.behind(begin), high = row.behind(min(stop, kBins - 1));
+    {
+        // (without a branch: what lies beyond the bins, which may be most, goes to a cell a lane behind them; what is ruled out, d = +inf,
+        // whose place is +inf or NaN, adds 0)
+        const int beyond = row.behind(kBins - 1);
         auto tally = [&](float d) {
-            // (tokens that are not counted add to cells behind the bins: no branch around the atomic)
             const int at = row.eighth(d);
-            atomicAdd(&sh.cells[at >= low && at < high ? at >> 3 & (kBins - 1) : kBins + lane], 1u << 17 | (at & 7));
+            atomicAdd(&sh.cells[at < beyond ? at >> 3 & (kBins - 1) : kBins + lane], at < 0x7f800000 ? 1u << 17 | (at & 7) : 0u);
         };
-        auto distance_at = [&](int i) { return i < count ? row.distance(s[i]) : INFINITY; };
-        if (begin > 0) {
-            // (the last bin, which is whatever lies behind the others, may have most of the tokens)
-#pragma unroll 2
-            for (int i0 = 0; i0 < count; i0 += kThreads) {
-                const float d = distance_at(i0 + t);
-                tally(d);
-                far += __popc(__ballot_sync(0xffffffffu, d < INFINITY && row.eighth(d) >= high));
-            }
-            if (lane == 0 && far > 0) atomicAdd(&sh.cells[kBins - 1], (uint32_t)far << 17);
-            row.meet();
-        } else if (whole) {
+        if (whole) {
             auto weigh = [&](float d) {
                 tally(d);
                 mass += weight_of(d, sh.table);
@@ -665,13 +654,21 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             }
 #pragma unroll 1
             for (; i < count; i += kThreads) weigh(row.distance(s[i]));
-            mass = row.row_sum(mass);
-            if (blocks == 1) row.meet();
         } else {
 #pragma unroll 4
             for (int i = t; i < count; i += kThreads) tally(row.distance(s[i]));
-            row.meet();
         }
+        __syncthreads();
+        if (warp == 1) {                           // the last bin is whatever lies beyond the others
+            const unsigned far = __reduce_add_sync(0xffffffffu, sh.cells[kBins + lane] >> 17);
+            if (lane == 0) sh.cells[kBins - 1] = far << 17;
+        }
+        if (whole) mass = row.row_sum(mass);
+        if (!whole || blocks == 1) row.meet();
+    }
+    // The blocks' counts together: of the near bins first.
+#pragma unroll 1
+    for (int stop = kNear;; stop = kBins) {
         // tokens, and what the mass is at least and at most, up to and with each bin
         constexpr int kEach = kBins / kThreads;
         const double unit = row.scale > 0.0f ? 1.0 / (double)row.scale : 0.0;
@@ -712,8 +709,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         }
         __syncthreads();
         // does a cut lie in what was counted?
-        if (whole ? least[stop - 1] >= p * mass : (by_k && upto[stop - 1] >= k) || (by_floor && row.bin(edge) < stop)) break;
-        if (stop < kBins) row.meet();              // (everyone has read the counts)
+        if (stop == kBins || (whole ? least[stop - 1] >= p * mass : (by_k && upto[stop - 1] >= k) || (by_floor && row.bin(edge) < stop))) break;
     }
     // ---- the bins that the cuts and the draw may lie in
     if (warp == 0) {
