@@ -57,8 +57,13 @@ class Sampler:
             raise ValueError("one temperature, top_p and draw per logits row")
         if any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps)) and logits.shape[1] <= kernels.MAX_CHOICE_VOCAB:
             tokens = self.choose(logits, temperatures, draws, top_ps=top_ps)
-            if min(tokens) < 0:
+            without = [i for i, token in enumerate(tokens) if token < 0]
+            if any(temperatures[i] > 0.0 and top_ps[i] < 1.0 for i in without):
                 raise InvalidLogits("sampler received empty or non-finite logits")
+            if without:                              # (rows that top-p says nothing of have the token that they have without it)
+                rest = self.sample(logits[without], [temperatures[i] for i in without], [1.0] * len(without), [draws[i] for i in without])
+                for i, token in zip(without, rest):
+                    tokens[i] = token
             return tokens
         out = torch.empty(rows, dtype=torch.int32, device=self.device)
         if all(t == 0.0 for t in temperatures):

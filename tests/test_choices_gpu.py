@@ -42,6 +42,28 @@ def ruled_logits(logits, params, prompt, generated, allowed=None):
     return plain.shaped(logits, rule, seen, counts, params.logit_bias, mask)
 
 
+def test_a_sampler_keeps_the_tokens_of_rows_beside_top_p():
+    """Rows that top-p says nothing of have, beside one that it cuts, the token that they have without it, with NaN and +inf too; a row
+    that it cuts with such logits is refused."""
+    import torch
+
+    from tesseract_b200.sampling.sampler import InvalidLogits, Sampler
+
+    logits = np.random.RandomState(3).randn(6, 500).astype(np.float32)
+    logits[1, 40] = np.inf
+    logits[2, 3:9] = np.nan
+    logits[3] = np.nan
+    logits[4, 7] = np.inf
+    sampler, on_device = Sampler("cuda"), torch.from_numpy(logits).cuda()
+    temperatures, draws = [0.7, 0.0, 0.0, 0.0, 0.7, 0.7], [0.1, 0.2, 0.3, 0.4, 0.5, 0.6]
+    alone = sampler.sample(on_device, temperatures, [1.0] * 6, draws)
+    beside = sampler.sample(on_device, temperatures, [0.5] + [1.0] * 5, draws)
+    assert beside[1:] == alone[1:]
+    assert beside[0] == plain.choose(logits[0], 0.7, 0.1, 0, 0.5, 0.0)
+    with pytest.raises(InvalidLogits):
+        sampler.sample(on_device, temperatures, [1.0] * 4 + [0.5] * 2, draws)
+
+
 def check_answer(config, tensors, prompt, params, out):
     """Every token is the plain model's under the rules; 32-bit logits may be off by 1e-5 of the largest, so a greedy token may be that
     much below the best, and a drawn one that of a draw (or of a temperature) a little beside it."""
