@@ -37,6 +37,7 @@ from dataclasses import dataclass, field, replace
 from typing import Callable, Deque, Dict, Hashable, List, Optional, Sequence, Tuple
 
 from ..config.engine_config import EngineConfig
+from ..kernels import MAX_CHOICE_VOCAB
 from ..sampling.params import SamplingParams, TokenChoice
 from ..sampling.rng import SplitMix64
 from ..sampling.rules import pack_mask
@@ -159,8 +160,11 @@ class Scheduler:
         params.validate()
         if self.vocab_size is not None:
             params.check_vocabulary(self.vocab_size)
-        if (params.ruled or params.top_k > 0 or params.min_p > 0.0) and (self.run_and_sample is None or self.vocab_size is None):
-            raise RequestRejected("this scheduler's sampler takes a temperature and top-p")
+        if params.ruled or params.top_k > 0 or params.min_p > 0.0:
+            if self.run_and_sample is None or self.vocab_size is None:
+                raise RequestRejected("this scheduler's sampler takes a temperature and top-p")
+            if self.vocab_size > MAX_CHOICE_VOCAB:
+                raise RequestRejected(f"rules on tokens, top-k and min-p take vocabularies of up to {MAX_CHOICE_VOCAB} tokens")
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise RequestRejected("the prompt is empty")

@@ -26,6 +26,12 @@ import numpy as np
 MAX_BIASES = 1024
 
 
+def single(value: float) -> float:
+    """A number as the kernels have it, in 32 bits; what lies beyond their range is an infinity."""
+    with np.errstate(over="ignore", under="ignore"):
+        return float(np.float32(value))
+
+
 @dataclass(frozen=True)
 class SamplingParams:
     max_tokens: int = 128
@@ -52,6 +58,10 @@ class SamplingParams:
         if self.allowed_token_ids is not None:
             object.__setattr__(self, "allowed_token_ids", tuple(self.allowed_token_ids))
         self.validate()
+        if self.logit_bias is not None:
+            object.__setattr__(self, "logit_bias", {int(token): float(bias) for token, bias in self.logit_bias.items()})
+        if self.allowed_token_ids is not None:
+            object.__setattr__(self, "allowed_token_ids", tuple(int(token) for token in self.allowed_token_ids))
 
     def validate(self) -> None:
         if self.max_tokens <= 0:
@@ -66,18 +76,18 @@ class SamplingParams:
             raise ValueError("top_k must be a number of tokens (0 for all)")
         if not 0.0 <= self.min_p <= 1.0:
             raise ValueError("min_p must be in [0, 1]")
-        if not math.isfinite(self.repetition_penalty) or self.repetition_penalty <= 0.0:
-            raise ValueError("repetition_penalty must be finite and positive")
-        if not math.isfinite(self.presence_penalty) or not math.isfinite(self.frequency_penalty):
-            raise ValueError("presence_penalty and frequency_penalty must be finite")
+        if not math.isfinite(single(self.repetition_penalty)) or single(self.repetition_penalty) <= 0.0:
+            raise ValueError("repetition_penalty must be finite and positive (in 32 bits)")
+        if not math.isfinite(single(self.presence_penalty)) or not math.isfinite(single(self.frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite (in 32 bits)")
         if self.logit_bias is not None:
             if len(self.logit_bias) > MAX_BIASES:
                 raise ValueError(f"logit_bias takes up to {MAX_BIASES} tokens")
             for token, bias in self.logit_bias.items():
                 if not isinstance(token, (int, np.integer)) or token < 0:
                     raise ValueError("logit_bias names tokens by their ids")
-                if math.isnan(bias) or bias == math.inf:
-                    raise ValueError("biases must be finite (or -inf, which rules a token out)")
+                if math.isnan(bias) or single(bias) == math.inf:
+                    raise ValueError("biases must be finite in 32 bits (or -inf, which rules a token out)")
         if self.allowed_token_ids is not None:
             if not self.allowed_token_ids:
                 raise ValueError("allowed_token_ids must not be empty")

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from .. import kernels
-from .params import MAX_BIASES
+from .params import MAX_BIASES, single
 
 PENALTIES, BIASES, MASK = 1, 2, 4
 
@@ -85,6 +85,7 @@ class TokenRules:
             biases: Optional[Mapping[int, float]] = None, allowed: Optional[Iterable[int]] = None) -> None:
         """A slot's rules from now on, in place of those it had; its history stays (``kernels.note_tokens(..., restart=True)``)."""
         self._check(slot)
+        repetition, presence, frequency = single(repetition), single(presence), single(frequency)
         if not (math.isfinite(repetition) and repetition > 0.0 and math.isfinite(presence) and math.isfinite(frequency)):
             raise ValueError("penalties must be finite, and the one for repetition positive")
         row = np.zeros(8, dtype=np.int32)
@@ -96,7 +97,7 @@ class TokenRules:
             words = pack_mask(allowed, self.vocab)
             row[0] |= MASK
         if biases:
-            ids, values = np.asarray(list(biases.keys())), np.asarray(list(biases.values()), dtype=np.float32)
+            ids, values = np.asarray(list(biases.keys())), np.asarray([single(bias) for bias in biases.values()], dtype=np.float32)
             if ids.size > self.room:
                 raise ValueError(f"{ids.size} biases, and room for {self.room}")
             self._check_biases(ids[None], values[None])

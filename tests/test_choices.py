@@ -18,10 +18,20 @@ from tests.test_scheduler import FakeAheadEngine, run_all
     dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=math.inf), dict(presence_penalty=math.nan),
     dict(frequency_penalty=math.inf), dict(logit_bias={-1: 1.0}), dict(logit_bias={"a": 1.0}), dict(logit_bias={1: math.nan}),
     dict(logit_bias={1: math.inf}), dict(logit_bias={t: 1.0 for t in range(1025)}), dict(allowed_token_ids=[]),
-    dict(allowed_token_ids=[-1]), dict(allowed_token_ids=[0.5]), dict(grammar=7)], ids=str)
+    dict(allowed_token_ids=[-1]), dict(allowed_token_ids=[0.5]), dict(grammar=7),
+    # (what the kernels' 32 bits do not hold)
+    dict(logit_bias={1: 1e39}), dict(repetition_penalty=1e39), dict(repetition_penalty=1e-60), dict(presence_penalty=-1e39),
+    dict(frequency_penalty=1e39)], ids=str)
 def test_options_that_are_refused(given):
     with pytest.raises(ValueError):
         SamplingParams(**given)
+
+
+def test_options_are_kept_as_numbers():
+    params = SamplingParams(logit_bias={True: 2, np.int64(7): np.float32(0.5), 9: -1e39}, allowed_token_ids=np.asarray([True, False]).tolist())
+    assert params.logit_bias == {1: 2.0, 7: 0.5, 9: -1e39} and params.allowed_token_ids == (1, 0)
+    assert [type(token) for token in (*params.logit_bias, *params.allowed_token_ids)] == [int] * 5
+    assert [type(bias) for bias in params.logit_bias.values()] == [float] * 3
 
 
 def test_which_options_are_rules_and_which_are_cuts():
@@ -97,6 +107,22 @@ def test_a_scheduler_whose_sampler_takes_no_rules_refuses_them():
         with pytest.raises(RequestRejected):
             plain.add_request([1, 2], SamplingParams(**given))
     plain.add_request([1, 2], SamplingParams(max_tokens=2, top_p=0.5))
+
+
+def test_a_vocabulary_beyond_the_kernels_takes_no_rules():
+    """A request that a step could only fail with all that stand beside it is refused at once."""
+    config = EngineConfig(max_queue=8, max_running=4, max_batch_tokens=32, prefill_chunk_tokens=8,
+                          kv_capacity_tokens=512, max_sequence_length=512)
+    fake = Choosing(config)
+    for vocab, taken in ((262144, True), (262145, False)):
+        s = Scheduler(config, fake.cache, fake.run_step, fake.sample, max_positions=400, run_and_sample=fake.run_and_sample, vocab_size=vocab)
+        for given in (dict(top_k=4), dict(min_p=0.1), dict(logit_bias={3: 1.0}), dict(grammar=lambda tokens: [1])):
+            if taken:
+                s.add_request([1, 2], SamplingParams(**given))
+            else:
+                with pytest.raises(RequestRejected):
+                    s.add_request([1, 2], SamplingParams(**given))
+        s.add_request([1, 2], SamplingParams(max_tokens=2, top_p=0.5))
 
 
 @pytest.mark.parametrize("ahead", [False, True])

@@ -50,7 +50,7 @@ def test_refusals():
     for slot, given in ((2, {}), (-1, {}), (0, {"repetition": 0.0}), (0, {"repetition": -1.0}), (0, {"presence": math.inf}),
                         (0, {"frequency": math.nan}), (0, {"biases": {10: 1.0}}), (0, {"biases": {-1: 1.0}}),
                         (0, {"biases": {0: math.nan}}), (0, {"biases": {0: math.inf}}), (0, {"biases": {0: 1.0, 1: 1.0, 2: 1.0}}),
-                        (0, {"allowed": [10]})):
+                        (0, {"allowed": [10]}), (0, {"biases": {0: 1e39}}), (0, {"presence": 1e39}), (0, {"repetition": 1e-60})):
         with pytest.raises(ValueError):
             rules.set(slot, **given)
         assert not rules.table.any()                         # (a refused call leaves the rules as they were)
