@@ -14,11 +14,11 @@
 //   1. rules and mask are applied, the row's largest and smallest logit found;
 //   2. the tokens are counted in 1,024 bins of d, each with its place in the bin to an eighth, and where top_p goes by it the mass of
 //      all is summed.  The blocks' counts are put together, of the nearest 384 bins first, as most cuts lie in those (64 rows 58.7 us,
-//      63.2 with all at once; where a flat distribution needs all, 47.8 and 45.7).  Of a bin of width h whose tokens lie F eighths into
-//      it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the cumulative mass is known bin by bin to some 0.4 %, and with it the
-//      few bins in which each cut and the draw can lie;
+//      with all at once 63.2; where a flat distribution needs all, 47.8 and 45.7; both before blocks left early).  Of a bin of width h
+//      whose tokens lie F eighths into it the mass is e^(-b h) (n - h F / 8) but for h / 8, so the cumulative mass is known bin by bin
+//      to some 0.4 %, and with it the few bins in which each cut and the draw can lie;
 //   3. the tokens of those bins are listed, what weighs in front of and between them is summed in 64 bits;
-//   4. one block sorts the list, and the sums in the order of the rank give every cut and the token.
+//   4. one block sorts the list, and the sums in the order of the rank give every cut and the token; the others have left by then.
 // Where those bins have more tokens than a list holds (great numbers of equal logits), the distance is found by halving its interval, and
 // the place among those equal to it by counting them.  No sum depends on the order of atomics: those count, or fill a list that is sorted.
 //
@@ -26,7 +26,7 @@
 // It is a chain of some twenty dependent phases and four cluster barriers: 3 us until the logits are there, 1.5 for the largest, 4.5 for
 // weights and counts (32 tokens a thread), 4 to put the blocks' counts together, 1.7 to find the bins, 3 to list, 5 for the first
 // block's sort, sums and searches.  Up to 15 rows of that vocabulary take no longer (21.7 us; one block a multiprocessor), 32 take 30
-// (two), and beyond that rows queue, as a row's logits fill half of eight multiprocessors' shared memory: 64 rows 59 us, 256 rows 217,
+// (two), and beyond that rows queue, as a row's logits fill half of eight multiprocessors' shared memory: 64 rows 57 us, 256 rows 200,
 // at 1.7 instructions a cycle and a third of all warps' time at barriers.  Reading the logits again from L2 in place of shared memory, for
 // more blocks a multiprocessor, was slower (64 rows 98 us against 83 then).
 #include <mutex>
@@ -269,6 +269,13 @@ struct Row {
         else
             __syncthreads();
     }
+    // The cluster's last meeting in two halves: a block has read what it needs of others' shared memory, and all have.
+    __device__ __forceinline__ void done() const {
+        if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    }
+    __device__ __forceinline__ void leave() const {
+        if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    }
     __device__ __forceinline__ float distance(float l) const { return __fsub_rn(top, __fmul_rn(l, inverse)); }
     // Where a distance lies, in eighths of a bin: what stands above 2^23 in a number that is rounded down there, so that neither a
     // conversion nor a second rounding is needed (distances beyond the bins, +inf and NaN are above all of them).
@@ -386,7 +393,6 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
               int vocab, int chunk, Rules rules) {
     __shared__ Shared sh;
     extern __shared__ uint4 dynamic[];
-    pdl_trigger();
     pdl_wait();                                    // the logits, and the histories, come from kernels in front
     const int r = blockIdx.y, blocks = gridDim.x, block = blockIdx.x, t = threadIdx.x;
     const int first = min(vocab, block * chunk), count = min(vocab, first + chunk) - first;
@@ -580,6 +586,8 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
             const double other = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += other;
         }
+        __syncwarp();
+        row.done();                                // (only one block goes on: the others' places are free for another row)
         const double target = u * __shfl_sync(0xffffffffu, upto, 31);
         // the block, and in it the warp, that passes the target; should rounding leave none, the last with any weight
         const unsigned past = __ballot_sync(0xffffffffu, lane < blocks && some && upto > target), any_of = __ballot_sync(0xffffffffu, some);
@@ -617,7 +625,8 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 if (lane == 0) out[r] = token >= 0 ? token : spare;
             }
         }
-        row.meet();
+        __syncwarp();
+        row.leave();
         return;
     }
     // ---- counts by bins, and the mass of all
@@ -896,6 +905,9 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 }
                 if (e < n) keys[e] = blocks > 1 ? peer_u64(list + e - begin, b) : list[e];
             }
+            __syncwarp();
+            // (the other blocks leave while this one sorts, their places are the next rows': 256 rows 200 us, 216 with all until the end)
+            row.done();
             // ---- sorted by cells: a bin of a window is so many of them that there are some 2,048
             int bins = 0, offset[kWindows];
 #pragma unroll
@@ -974,6 +986,9 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 sums[e] = sh.base[min(v, windows - 1)] + run;
             }
             __syncthreads();
+            // A launch behind is let in only now (by the other blocks' leaving, and here): one that may place its rows while most blocks
+            // have left and the first ones not, finds worse places for them (32 rows of top-p in launches like this 35.6 us, 29.6 so).
+            pdl_trigger();
             if (t == 0) {
                 int kept = n;
                 double total = of.all + sh.base[windows];
@@ -988,7 +1003,12 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
                 }
                 out[r] = id_of(sorted[max(0, min(first_to(sums, kept, u * total, true), kept - 1))]);
             }
+        } else {
+            row.done();
         }
+        __syncwarp();
+        row.leave();
+        return;
     } else {
         // ---- more than a list holds: cut by cut  (on a copy, so that the row itself stays in registers)
         Row again = row;
