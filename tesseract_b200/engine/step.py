@@ -286,7 +286,8 @@ class Stepper:
             return out
         logits = self.step(entries)
         chosen = [e for e in entries if e.want]
-        if all(e.choice is None for e in chosen):
+        # (beyond the kernel's vocabularies top-p is all that a choice may say: the sampler asks the host)
+        if self.vocab_size > kernels.MAX_CHOICE_VOCAB or all(e.choice is None for e in chosen):
             return self._sampler.sample(logits, temperatures, top_ps, draws)
         slots = self.rule_slots(chosen)
         ruled = max(slots) >= 0

@@ -1,0 +1,54 @@
+"""How a step chooses the tokens of its rows, up to the kernels (no device): a step function whose sampler is a stand-in."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import tesseract_b200.parts  # noqa: F401
+from tesseract_b200 import kernels
+from tesseract_b200.cache import CacheManager
+from tesseract_b200.engine.step import StepEntry, Stepper
+from tesseract_b200.parts import PagedKVNeed
+from tesseract_b200.sampling import SamplingParams
+from tesseract_b200.sampling.params import TokenChoice
+
+
+def make_stepper(requests, vocab=100, model=None):
+    cache = CacheManager([PagedKVNeed(2, 16)], [None], num_pages=64, page_size=16, max_requests=len(requests), dtype=torch.float32,
+                         device="cpu", max_step_tokens=64, allocate_storage=False)
+    for request in requests:
+        assert cache.admit(request)
+    made = SimpleNamespace(runtime=SimpleNamespace(device=torch.device("cpu")), spec=SimpleNamespace(vocab_size=vocab, max_positions=256))
+    if model is not None:
+        made.forward = model
+    return Stepper(made, cache)
+
+
+class Told:
+    """A sampler that keeps what it is asked."""
+
+    def __init__(self):
+        self.sampled, self.chosen = [], []
+
+    def sample(self, logits, temperatures, top_ps, draws):
+        self.sampled.append(dict(rows=logits.shape[0], temperatures=list(temperatures), top_ps=list(top_ps), draws=list(draws)))
+        return [5] * logits.shape[0]
+
+    def choose(self, logits, temperatures, draws, **given):
+        self.chosen.append(dict(rows=logits.shape[0], temperatures=list(temperatures), draws=list(draws), **given))
+        return [6] * logits.shape[0]
+
+
+@pytest.mark.parametrize("vocab", [kernels.MAX_CHOICE_VOCAB, kernels.MAX_CHOICE_VOCAB + 1])
+def test_top_p_beyond_the_kernels_vocabulary_goes_to_the_hosts_sampler(vocab):
+    """A step that is not captured: the one in which a prompt ends, whose row stands beside others."""
+    stepper = make_stepper("abc", vocab)
+    stepper._sampler = told = Told()
+    stepper.step = lambda entries: torch.zeros(3, 8)
+    cut, plain = SamplingParams(top_p=0.5), SamplingParams(temperature=0.0)
+    entries = [StepEntry("a", [1, 2], [1], TokenChoice.of(cut, 2)), StepEntry("b", [3], [0], TokenChoice.of(plain, 1)), StepEntry("c", [4], [0])]
+    tokens = stepper.step_and_sample(entries, [1.0, 0.0, 0.7], [0.5, 1.0, 1.0], [0.1, 0.2, 0.3])
+    given = (told.chosen if vocab <= kernels.MAX_CHOICE_VOCAB else told.sampled)
+    assert len(told.chosen) + len(told.sampled) == 1 and len(given) == 1 and len(tokens) == 3
+    assert given[0]["rows"] == 3 and given[0]["top_ps"] == [0.5, 1.0, 1.0] and given[0]["draws"] == [0.1, 0.2, 0.3]
