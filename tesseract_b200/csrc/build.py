@@ -38,7 +38,8 @@ INCLUDES: Dict[str, List[str]] = {
     "decode_linear": ["activation.cuh"],
     "pointwise": ["activation.cuh"],
     "token_rules": ["token_rules.cuh"],
-    "token_choice": ["token_rules.cuh"],
+    "token_choice": ["sample_rows.cuh", "token_rules.cuh"],
+    "sampling": ["sample_rows.cuh"],
 }
 
 # Every source file, with the extra flags it needs.

@@ -14,11 +14,11 @@
 // of the chunk, scanned 32 tokens at a time, so prefix sums are taken in token order with coalesced reads.  The
 // blocks exchange their maxima and their sums through distributed shared memory; every block applies the same
 // rule to the same numbers, so they agree on the block that holds the sampled token without a leader.
-#include "common.cuh"
+#include "sample_rows.cuh"
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = kSampleThreads;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPartStride = 16;     // rows per CTA in the partial results that a product leaves (at most 16 rows)
 
@@ -278,23 +278,9 @@ sample_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     if (blocks > 1) cluster_sync();   // no block leaves while a peer may still read its shared memory
 }
 
-// Blocks per row: as many (a power of two up to the portable cluster size) as keep the grid within one wave.
-int blocks_per_row(int rows, int vocab) {
-    static int sms = 0;
-    if (sms == 0) {
-        int device = 0;
-        cudaGetDevice(&device);
-        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 1;
-    }
-    int blocks = 8;
-    while (blocks > 1 && (rows * blocks > sms || vocab < blocks * kThreads)) blocks >>= 1;
-    return blocks;
-}
-
 template <typename Kernel, typename... Args>
 int launch_rows(Kernel kernel, int rows, int vocab, cudaStream_t stream, Args... args) {
-    const int blocks = blocks_per_row(rows, vocab);
-    const int chunk = ((vocab + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads;
+    const int blocks = sample_blocks(rows, vocab), chunk = sample_chunk(blocks, vocab);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(blocks, rows, 1);
     config.blockDim = dim3(kThreads);

@@ -6,8 +6,8 @@
 //     token = the first of the rank whose cumulative weight is above u * (mass of what is kept)
 //   A row without any cut is drawn from in the order of ids with d = fma(-x, 1 / T, max z), as tb_sample does (where max z is 65,536 and
 //   more, at temperatures of a thousandth and below, that would leave the largest logit itself away from 0: there d as above).
-//   A row with NaN or +inf, or with nothing above -inf, has no token: -1.  Where max z leaves the 32 bits' range, the largest logits have
-//   d = 0 and the others weigh nothing.
+//   A row with NaN or +inf, or with nothing above -inf, has no token: -1 (`as_sampled`: the one that tb_sample gives it).  Where max z
+//   leaves the 32 bits' range, the largest logits have d = 0 and the others weigh nothing.
 //
 // A row is shared by a thread-block cluster; each block reads its part of the vocabulary once, into shared memory, and all that follows
 // runs there:
@@ -31,6 +31,7 @@
 // more blocks a multiprocessor, was slower (64 rows 98 us against 83 then).
 #include <mutex>
 
+#include "sample_rows.cuh"
 #include "token_rules.cuh"
 
 namespace {
@@ -303,6 +304,62 @@ struct Row {
         turn ^= 1;
         return v;
     }
+    // What all threads of the cluster bring, the largest or (`most` false) all bits.
+    __device__ __noinline__ uint64_t row_all(uint64_t v, bool most) {
+        uint64_t* scratch = reinterpret_cast<uint64_t*>(sh.sums[0]);
+        auto across = [&]() {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const uint64_t other = __shfl_xor_sync(0xffffffffu, v, o);
+                v = most ? (other > v ? other : v) : v | other;
+            }
+        };
+        across();
+        __syncthreads();
+        if (lane() == 0) scratch[warp()] = v;
+        __syncthreads();
+        v = lane() < kWarps ? scratch[lane()] : 0;
+        across();
+        if (blocks == 1) return v;
+        if (threadIdx.x == 0) sh.place = v;
+        meet();
+        v = lane() < blocks ? peer_u64(&sh.place, lane()) : 0;
+        across();
+        meet();                                                        // (the next one may be written)
+        return v;
+    }
+    // The token that tb_sample gives a row with NaN or +inf, or with nothing above -inf (the whole cluster calls it): NaN is never the
+    // largest, and without another token 0 is.  Drawn, such a row's mass is NaN and no block passes the draw: it has the last token that
+    // weighs anything in the blocks of tb_sample (`apart` tokens each, 8 at most) whose weights are all numbers, else the largest.
+    __device__ __noinline__ int sampled_token(float temp, int apart) {
+        uint64_t mine = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < count; i += kThreads) {
+            const float l = s[i] + 0.0f;                               // (-0 and 0 are equal)
+            if (!(l > -INFINITY)) continue;
+            const uint32_t bits = __float_as_uint(l), order = bits >> 31 ? ~bits : bits | 0x80000000u;
+            const uint64_t key = (uint64_t)order << 32 | ~(uint32_t)(first + i);
+            mine = key > mine ? key : mine;
+        }
+        const uint64_t key = row_all(mine, true);
+        const uint32_t order = (uint32_t)(key >> 32);
+        const float largest = key == 0 ? -INFINITY : __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order);
+        const int lowest = key == 0 ? 0 : (int)~(uint32_t)key;
+        if (!(temp > 0.0f)) return lowest;
+        const float by = 1.0f / temp, largest_by = largest * by;
+        auto weight = [&](int i) { return exp((double)fmaf(s[i], by, -largest_by)); };
+        uint64_t none = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < count; i += kThreads)
+            if (isnan(weight(i))) none |= 1ull << (first + i) / apart;
+        none = row_all(none, false);
+        mine = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < count; i += kThreads)
+            if (!(none >> (first + i) / apart & 1) && weight(i) > 0.0) mine = first + i + 1;
+        mine = row_all(mine, true);
+        return mine > 0 ? (int)mine - 1 : lowest;
+    }
     // The mass, or the number, of the tokens of the rank up to `place`.
     __device__ __noinline__ double through(bool mass, uint64_t place) {
         double mine = 0.0;
@@ -389,8 +446,8 @@ __device__ __noinline__ int first_bin(const T* of, T target, bool above) {
 // grid (blocks a row, rows); the blocks of a row are one cluster.
 __global__ void __launch_bounds__(kThreads, 2)
 choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __restrict__ temperature, const double* __restrict__ uniform,
-              const int* __restrict__ top_k, const double* __restrict__ top_p, const double* __restrict__ min_p, int* __restrict__ out,
-              int vocab, int chunk, Rules rules) {
+              const int* __restrict__ top_k, const double* __restrict__ top_p, const double* __restrict__ min_p,
+              const int* __restrict__ as_sampled, int* __restrict__ out, int vocab, int chunk, int apart, Rules rules) {
     __shared__ Shared sh;
     extern __shared__ uint4 dynamic[];
     pdl_wait();                                    // the logits, and the histories, come from kernels in front
@@ -537,7 +594,12 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         }
     }
     if (!(best < INFINITY) || best == -INFINITY || greedy) {
-        if (block == 0 && t == 0) out[r] = best < INFINITY && best > -INFINITY ? lowest : -1;
+        int token = best < INFINITY && best > -INFINITY ? lowest : -1;
+        if (token < 0 && as_sampled != nullptr && as_sampled[r] != 0) {
+            Row again = row;                       // (a copy, so that the row itself stays in registers)
+            token = again.sampled_token(temp, apart);
+        }
+        if (block == 0 && t == 0) out[r] = token;
         row.meet();                                // no block leaves while a peer may still read its shared memory
         return;
     }
@@ -1029,7 +1091,8 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
 }
 
 int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const float* logits, int64_t stride, const float* temperature,
-                const double* uniform, const int* top_k, const double* top_p, const double* min_p, int* out, const Rules& rules) {
+                const double* uniform, const int* top_k, const double* top_p, const double* min_p, const int* as_sampled, int* out,
+                const Rules& rules) {
     const int chunk = ((vocab + blocks - 1) / blocks + 127) / 128 * 128;
     cudaLaunchAttribute attribute[2];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -1071,7 +1134,7 @@ int launch_rows(int rows, int vocab, int blocks, cudaStream_t stream, const floa
     config.dynamicSmemBytes = logits_at + (space > later ? space : later);
     if (blocks > 1 && rows <= apart) config.dynamicSmemBytes = kAlone;
     const cudaError_t err = cudaLaunchKernelEx(&config, choose_kernel, logits, stride, temperature, uniform, top_k, top_p, min_p,
-                                               out, vocab, chunk, rules);
+                                               as_sampled, out, vocab, chunk, sample_chunk(sample_blocks(rows, vocab), vocab), rules);
     return err == cudaSuccess ? tb_launch_status() : (int)err;
 }
 
@@ -1088,8 +1151,8 @@ int sm_count() {
 }  // namespace
 
 TB_EXPORT int tb_choose_tokens(const float* logits, int64_t stride, const float* temperature, const double* uniform, const int* top_k,
-                               const double* top_p, const double* min_p, int* out, int rows, int vocab, Rules rules,
-                               cudaStream_t stream) {
+                               const double* top_p, const double* min_p, const int* as_sampled, int* out, int rows, int vocab,
+                               Rules rules, cudaStream_t stream) {
     if (rows == 0) return 0;
     if (vocab <= 0 || rows < 0 || rows > 65535 || vocab > kMaxBlocks * kMaxChunk || rules.room > kMaxBiases) return TB_ERR_BAD_SIZE;
     // As few blocks a row as hold it, and up to eight while each has a multiprocessor of its own and 2,048 tokens.  (Device time, 8 / 4
@@ -1099,5 +1162,5 @@ TB_EXPORT int tb_choose_tokens(const float* logits, int64_t stride, const float*
     int blocks = (vocab + kMaxChunk - 1) / kMaxChunk;
     const int more = min(min(8, sm_count() / rows), vocab / 2048);
     if (blocks < more) blocks = more;
-    return launch_rows(rows, vocab, blocks, stream, logits, stride, temperature, uniform, top_k, top_p, min_p, out, rules);
+    return launch_rows(rows, vocab, blocks, stream, logits, stride, temperature, uniform, top_k, top_p, min_p, as_sampled, out, rules);
 }

@@ -23,6 +23,7 @@ import torch
 
 from .. import kernels
 from ..parts.base import SHARED_BLOCK, GroupView, SharedRows, StepContext
+from ..sampling.params import TokenChoice
 from .step import StepEntry, Stepper
 
 
@@ -69,7 +70,7 @@ class _Graph:
         self.paged = [i for i, g in enumerate(cache.groups) if g.pool is not None]
         # members, group starts, leaders, keys in common of each group and each row (parts.base.SharedRows)
         together = [batch, batch + 1, batch, batch, batch] if company is not None else []
-        chosen = 3 * batch if choosing else 0                       # rule slots, prompt tokens, top-k
+        chosen = 4 * batch if choosing else 0                       # rule slots, prompt tokens, top-k, rows without rules and cuts
         ints = 4 * batch + len(self.paged) * batch * columns + sum(together) + chosen
         ints = (ints + 1) // 2 * 2                                  # keep the float64 block 8-byte aligned
         self.nbytes = ints * 4 + batch * 4 + (batch % 2) * 4 + batch * 8 * (3 if choosing else 1)
@@ -92,7 +93,7 @@ class _Graph:
             for size in together:
                 out["together"].append(buffer[at:at + size * 4].view(torch.int32))
                 at += size * 4
-            for name in ("rule_slots", "prompts", "top_k") if choosing else ():
+            for name in ("rule_slots", "prompts", "top_k", "plain") if choosing else ():
                 out[name] = buffer[at:at + batch * 4].view(torch.int32)
                 at += batch * 4
             at = ints * 4
@@ -167,7 +168,7 @@ class _Graph:
         if self.choosing:
             kernels.choose_tokens(logits, self.d["temps"], self.d["uniform"], self.sampled[:self.batch], top_k=self.d["top_k"],
                                   top_p=self.d["top_p"], min_p=self.d["min_p"], rules=self.rules,
-                                  slots=self.d["rule_slots"] if self.rules is not None else None)
+                                  slots=self.d["rule_slots"] if self.rules is not None else None, as_sampled=self.d["plain"])
             return logits
         # the head may have left each of its CTAs' best token per row: the sampler's second stage of the argmax
         partials = getattr(stepper.model.head, "argmax_partials", lambda: None)()
@@ -319,6 +320,7 @@ class DecodeGraphs:
             h["top_k"][:count] = [c.params.top_k if c is not None else 0 for c in choices]
             h["top_p"][:count] = top_ps
             h["min_p"][:count] = [c.params.min_p if c is not None else 0.0 for c in choices]
+            h["plain"][:count] = [TokenChoice.plain(c, t, p) for c, t, p in zip(choices, temperatures, top_ps)]
         if count < graph.batch:
             h["tokens"][count:] = 0
             h["feed"][count:] = -1

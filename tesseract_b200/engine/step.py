@@ -265,8 +265,8 @@ class Stepper:
                         draws: Sequence[float]) -> List[int]:
         """One step, then one token per wanted row (entries want at most their last place).
 
-        ``temperatures``, ``top_ps`` and ``draws`` hold one value per wanted row, in order.  A row whose request has rules (or a cut)
-        and that no token may follow gets -1.
+        ``temperatures``, ``top_ps`` and ``draws`` hold one value per wanted row, in order.  A row whose request has rules or a cut, and
+        that no token may follow, gets -1; others always get a token, whatever stands beside them.
         """
         from ..sampling.sampler import Sampler, sample_top_p_host
 
@@ -293,7 +293,8 @@ class Stepper:
         ruled = max(slots) >= 0
         return self._sampler.choose(logits, temperatures, draws, top_ks=[e.choice.params.top_k if e.choice else 0 for e in chosen],
                                     top_ps=top_ps, min_ps=[e.choice.params.min_p if e.choice else 0.0 for e in chosen],
-                                    rules=self.rules if ruled else None, slots=slots if ruled else None)
+                                    rules=self.rules if ruled else None, slots=slots if ruled else None,
+                                    as_sampled=[TokenChoice.plain(e.choice, t, p) for e, t, p in zip(chosen, temperatures, top_ps)])
 
     def _check_choices(self, entries: Sequence[StepEntry]) -> None:
         if self.vocab_size > kernels.MAX_CHOICE_VOCAB and any(e.choice is not None and (

@@ -575,7 +575,7 @@ def shape_logits(logits: torch.Tensor, out: torch.Tensor, rules, slots: torch.Te
 
 
 MAX_CHOICE_VOCAB = 262144
-_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 6, _i32, _i32, RulesRecord, _pointer)
+_CHOOSE_TOKENS = (_pointer, _i64, *[_pointer] * 7, _i32, _i32, RulesRecord, _pointer)
 
 
 def _per_row(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, device: int) -> Optional[int]:
@@ -588,14 +588,16 @@ def _per_row(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int
 
 def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor, out: torch.Tensor, *,
                   top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
-                  rules=None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  rules=None, slots: Optional[torch.Tensor] = None, as_sampled: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A token a row (int32 ``[S]``) from logits under the rules of the rows' slots (:func:`shape_logits`): the lowest id of the
     largest for a temperature (float32) of 0 and below; else drawn, with the uniform draw (float64, in [0, 1)), from what ``top_k``
     (int32; 0: all), ``min_p`` (float64, relative to the largest weight) and ``top_p`` (float64, of the mass that those two leave)
     keep of the tokens ranked by weight, equal ones by id.  The rank is drawn from in its order (as :func:`~tesseract_b200.sampling
     .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`); a token
     that weighs less than e^-700 of the largest is not drawn.  A row with NaN or +inf among what is
-    allowed, or with nothing allowed, gets -1.  Up to 262,144 tokens and 65,535 rows."""
+    allowed, or with nothing allowed, gets -1, or where ``as_sampled`` (int32) is not 0 the token that :func:`sample` gives such a row
+    in a call of as many (which makes a row without rules and cuts independent of those beside it).  Up to 262,144 tokens and 65,535
+    rows."""
     rows, vocab, stride = _logit_rows("choose_tokens", logits)
     device = logits.get_device()
     record = _rules_of("choose_tokens", rules, slots, rows, vocab, device)
@@ -605,7 +607,8 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
         logits.data_ptr(), stride, _per_row("temperature", temperature, torch.float32, rows, device),
         _per_row("uniform", uniform, torch.float64, rows, device), _per_row("top_k", top_k, torch.int32, rows, device),
         _per_row("top_p", top_p, torch.float64, rows, device), _per_row("min_p", min_p, torch.float64, rows, device),
-        _per_row("out", out, torch.int32, rows, device), rows, vocab, record, _stream_of(device)), "choose_tokens")
+        _per_row("as_sampled", as_sampled, torch.int32, rows, device), _per_row("out", out, torch.int32, rows, device), rows, vocab,
+        record, _stream_of(device)), "choose_tokens")
     return out
 
 

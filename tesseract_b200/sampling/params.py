@@ -130,6 +130,15 @@ class TokenChoice:
     prompt_tokens: int
     allowed: Optional[np.ndarray] = None
 
+    @staticmethod
+    def plain(choice: Optional["TokenChoice"], temperature: float, top_p: float) -> bool:
+        """Whether neither rules nor a cut say anything about a row's token: whatever its logits are, it has the token that it has
+        beside rows of its kind."""
+        params = choice.params if choice is not None else None
+        if params is not None and params.ruled:
+            return False
+        return not (temperature > 0.0 and (top_p < 1.0 or (params is not None and (params.top_k > 0 or params.min_p > 0.0))))
+
     @classmethod
     def of(cls, params: SamplingParams, prompt_tokens: int) -> Optional["TokenChoice"]:
         return cls(params, prompt_tokens) if params.ruled or params.cut else None

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from .. import kernels
+from .params import TokenChoice
 
 
 class InvalidLogits(ValueError):
@@ -56,14 +57,10 @@ class Sampler:
         if not (len(temperatures) == len(top_ps) == len(draws) == rows):
             raise ValueError("one temperature, top_p and draw per logits row")
         if any(t > 0.0 and p < 1.0 for t, p in zip(temperatures, top_ps)) and logits.shape[1] <= kernels.MAX_CHOICE_VOCAB:
-            tokens = self.choose(logits, temperatures, draws, top_ps=top_ps)
-            without = [i for i, token in enumerate(tokens) if token < 0]
-            if any(temperatures[i] > 0.0 and top_ps[i] < 1.0 for i in without):
+            tokens = self.choose(logits, temperatures, draws, top_ps=top_ps,
+                                 as_sampled=[TokenChoice.plain(None, t, p) for t, p in zip(temperatures, top_ps)])
+            if min(tokens) < 0:
                 raise InvalidLogits("sampler received empty or non-finite logits")
-            if without:                              # (rows that top-p says nothing of have the token that they have without it)
-                rest = self.sample(logits[without], [temperatures[i] for i in without], [1.0] * len(without), [draws[i] for i in without])
-                for i, token in zip(without, rest):
-                    tokens[i] = token
             return tokens
         out = torch.empty(rows, dtype=torch.int32, device=self.device)
         if all(t == 0.0 for t in temperatures):
@@ -83,18 +80,21 @@ class Sampler:
 
     def choose(self, logits: torch.Tensor, temperatures: Sequence[float], draws: Sequence[float], *,
                top_ks: Optional[Sequence[int]] = None, top_ps: Optional[Sequence[float]] = None,
-               min_ps: Optional[Sequence[float]] = None, rules=None, slots: Optional[Sequence[int]] = None) -> List[int]:
+               min_ps: Optional[Sequence[float]] = None, rules=None, slots: Optional[Sequence[int]] = None,
+               as_sampled: Optional[Sequence[bool]] = None) -> List[int]:
         """One token per logits row by ``kernels.choose_tokens``; -1 for a row that has none."""
         rows = logits.shape[0]
         # (one copy for all that a row brings: its 64-bit numbers, then those of 32)
-        wide, narrow = np.empty((3, rows), dtype=np.float64), np.zeros((3, rows + rows % 2), dtype=np.int32)
+        wide, narrow = np.empty((3, rows), dtype=np.float64), np.zeros((4, rows + rows % 2), dtype=np.int32)
         wide[0], wide[1], wide[2] = draws, 1.0 if top_ps is None else top_ps, 0.0 if min_ps is None else min_ps
         narrow[0, :rows] = np.asarray(temperatures, dtype=np.float32).view(np.int32)
         narrow[1, :rows] = 0 if top_ks is None else top_ks
         narrow[2, :rows] = -1 if slots is None else slots
+        narrow[3, :rows] = 0 if as_sampled is None else as_sampled
         sent = torch.from_numpy(np.concatenate([wide.reshape(-1), narrow.reshape(-1).view(np.float64)])).to(self.device)
-        wide, narrow = sent[:3 * rows].view(3, rows), sent[3 * rows:].view(torch.int32).view(3, -1)[:, :rows]
+        wide, narrow = sent[:3 * rows].view(3, rows), sent[3 * rows:].view(torch.int32).view(4, -1)[:, :rows]
         out = torch.empty(rows, dtype=torch.int32, device=self.device)
         kernels.choose_tokens(logits, narrow[0].view(torch.float32), wide[0], out, top_k=narrow[1], top_p=wide[1], min_p=wide[2],
-                              rules=rules, slots=narrow[2] if rules is not None else None)
+                              rules=rules, slots=narrow[2] if rules is not None else None,
+                              as_sampled=narrow[3] if as_sampled is not None else None)
         return out.cpu().tolist()

@@ -52,3 +52,19 @@ def test_top_p_beyond_the_kernels_vocabulary_goes_to_the_hosts_sampler(vocab):
     given = (told.chosen if vocab <= kernels.MAX_CHOICE_VOCAB else told.sampled)
     assert len(told.chosen) + len(told.sampled) == 1 and len(given) == 1 and len(tokens) == 3
     assert given[0]["rows"] == 3 and given[0]["top_ps"] == [0.5, 1.0, 1.0] and given[0]["draws"] == [0.1, 0.2, 0.3]
+
+
+def test_rows_that_nothing_is_said_of_are_marked():
+    """Beside rows with rules and cuts they keep the sampler's token whatever their logits are."""
+    kinds = [SamplingParams(), SamplingParams(temperature=0.0, top_p=0.5, top_k=3, min_p=0.1), SamplingParams(top_p=0.5),
+             SamplingParams(top_k=4), SamplingParams(min_p=0.2), SamplingParams(temperature=0.0, presence_penalty=1.0)]
+    stepper = make_stepper(range(len(kinds)))
+    stepper._sampler = told = Told()
+    stepper._rules = object()
+    stepper.step = lambda entries: torch.zeros(len(kinds), 8)
+    entries = [StepEntry(i, [1], [0], TokenChoice.of(params, 1)) for i, params in enumerate(kinds)]
+    stepper.step_and_sample(entries, [p.temperature for p in kinds], [p.top_p for p in kinds], [0.5] * len(kinds))
+    assert told.chosen[0]["as_sampled"] == [True, True, False, False, False, False]
+    assert [TokenChoice.plain(e.choice, p.temperature, p.top_p) for e, p in zip(entries, kinds)] == [True, True, False, False, False, False]
+    # (top-p may come without a choice)
+    assert not TokenChoice.plain(None, 1.0, 0.5) and TokenChoice.plain(None, 0.0, 0.5) and TokenChoice.plain(None, 1.0, 1.0)

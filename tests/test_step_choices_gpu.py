@@ -1,7 +1,10 @@
 """How the engine's steps choose their rows' tokens, captured and launched one by one, against the plain model."""
 
+import numpy as np
 import pytest
+import torch
 
+from tesseract_b200 import kernels
 from tests.helpers import TINY, make_model_folder, random_tokens
 from tests.plain import llama
 from tests.test_choices_gpu import check_answer, engine
@@ -27,3 +30,66 @@ def test_top_p_on_either_side_of_the_kernels_largest_vocabulary(tmp_path, vocab,
     for prompt, params, out in zip(prompts, kinds, outs):
         assert out.finish_reason == "length" and len(out.token_ids) == 4, out.error
         check_answer(config, tensors, prompt, params, out.token_ids)
+
+
+@pytest.mark.parametrize("rows", [6, 30, 200])
+@pytest.mark.parametrize("vocab", [1, 3, 1000, 5000, 20000, 128256, 200000])
+def test_logits_that_are_not_finite_give_a_marked_row_the_samplers_token(rows, vocab):
+    """Equal tokens, with no tolerance: the row of ``sample`` in a call of as many rows.  Others have none."""
+    rng = np.random.RandomState(rows + vocab)
+    x = (rng.randn(rows, vocab) * 2).astype(np.float32)
+    for row in range(rows):
+        kind, some = row % 6, rng.permutation(vocab)[:1 + row % 3]
+        if kind == 1:
+            x[row, some] = np.nan
+        elif kind == 2:
+            x[row, some] = np.inf
+        elif kind == 3:
+            x[row] = np.nan if row % 4 < 2 else -np.inf
+        elif kind == 4:
+            x[row, vocab // 2:] = np.nan if row % 4 < 2 else -np.inf
+            x[row, some] = np.nan
+        elif kind == 5:
+            x[row, some[0]], x[row, some[-1]] = np.inf, np.nan
+    logits = torch.from_numpy(x).cuda()
+    draws = torch.from_numpy(rng.rand(rows)).cuda()
+    marked = torch.from_numpy((rng.rand(rows) < 0.7).astype(np.int32)).cuda()
+    invalid = ~(x < np.inf).all(axis=1) | (x.max(axis=1) == -np.inf)
+    for temperature in (0.0, 0.7, 1e-38, None):
+        of_rows = np.full(rows, temperature) if temperature is not None else rng.choice([0.0, 0.4, 1.0, 2.0], rows)
+        of_rows = torch.from_numpy(of_rows.astype(np.float32)).cuda()
+        want, got = (torch.full((rows,), -9, dtype=torch.int32, device="cuda") for _ in range(2))
+        kernels.sample(logits, of_rows, draws, want)
+        kernels.choose_tokens(logits, of_rows, draws, got, as_sampled=marked)
+        keep = marked.cpu().numpy() != 0
+        want, got = want.cpu().numpy(), got.cpu().numpy()
+        assert np.array_equal(got[invalid & keep], want[invalid & keep])
+        assert (got[invalid & ~keep] == -1).all()
+        if temperature != 1e-38:                 # (there the largest logit's own distance is rounded otherwise)
+            assert np.array_equal(got[~invalid], want[~invalid])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("spoiled", ["nan", "inf", "all"])
+def test_a_request_that_says_nothing_does_not_fail_for_its_neighbours_rules(model_folders, spoiled, graphs, dtype):
+    """A model some of whose logits are not finite: a greedy request and one that is drawn from everything have the tokens beside
+    requests with rules and cuts that they have beside each other."""
+    from tesseract_b200 import SamplingParams
+
+    llm = engine(model_folders("b"), dtype=dtype, cuda_graphs=graphs)
+    weight = llm.model.head.proj.weight
+    if spoiled == "all":
+        weight.fill_(float("nan"))
+    else:
+        weight[7, 5] = float(spoiled)
+    same = dict(max_tokens=8, ignore_eos=True)
+    plain = [SamplingParams(temperature=0.0, **same), SamplingParams(temperature=0.8, seed=3, **same)]
+    prompts = [random_tokens(384, n, seed=n) for n in (9, 20, 3)]
+    alone = llm.generate(prompts, plain + [plain[1]])
+    assert [o.finish_reason for o in alone] == ["length"] * 3
+    for other in (SamplingParams(temperature=0.8, top_p=0.5, **same), SamplingParams(temperature=0.0, presence_penalty=0.5, **same),
+                  SamplingParams(temperature=0.9, top_k=5, logit_bias={7: -1.0}, **same)):
+        beside = llm.generate(prompts, plain + [other])
+        assert [o.finish_reason for o in beside[:2]] == ["length"] * 2, [o.error for o in beside]
+        assert [o.token_ids for o in beside[:2]] == [o.token_ids for o in alone[:2]]
