@@ -622,6 +622,7 @@ class ChunkGraphs:
         copied.record()
         graph.host_events[index] = copied
         graph.graph.replay()
+        stepper.note_entries(entries)
         for entry in entries:
             cache.commit(entry.request, len(entry.tokens))
         stepper.steps_run += 1

@@ -118,7 +118,8 @@ class Stepper:
                 self.rules.set_mask(slot, choice.allowed)
 
     def note_entries(self, entries: Sequence[StepEntry]) -> None:
-        """The tokens that a step brings go into the histories of the requests with penalties."""
+        """The tokens that a step brings go into the histories of the requests with penalties: when its launches are under way and
+        before the cache counts them, so that a step that fails and is tried again brings them once."""
         noted = [e for e in entries if e.choice is not None and e.choice.params.penalised]
         if not noted:
             return
@@ -231,7 +232,6 @@ class Stepper:
         if any(e.choice is not None for e in entries):
             self._validate(entries)
             self.begin_rules(entries)
-            self.note_entries(entries)
         if self.chunk_graphs is not None and self.chunk_graphs.eligible(entries):
             return self.chunk_graphs.step(entries)
         tokens = self._validate(entries)
@@ -242,6 +242,7 @@ class Stepper:
         # the same path as a replayed decode step, bit for bit
         every_row = all(list(e.want) == list(range(len(e.tokens))) for e in entries)
         logits = self.model.forward(ctx, self.cache.bindings, want_rows, want_every_row=every_row)
+        self.note_entries(entries)
         for entry in entries:
             self.cache.commit(entry.request, len(entry.tokens))
         self.steps_run += 1

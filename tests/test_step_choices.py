@@ -2,6 +2,7 @@
 
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
@@ -12,6 +13,7 @@ from tesseract_b200.engine.step import StepEntry, Stepper
 from tesseract_b200.parts import PagedKVNeed
 from tesseract_b200.sampling import SamplingParams
 from tesseract_b200.sampling.params import TokenChoice
+from tests import token_choice_plain as plain
 
 
 def make_stepper(requests, vocab=100, model=None):
@@ -46,8 +48,8 @@ def test_top_p_beyond_the_kernels_vocabulary_goes_to_the_hosts_sampler(vocab):
     stepper = make_stepper("abc", vocab)
     stepper._sampler = told = Told()
     stepper.step = lambda entries: torch.zeros(3, 8)
-    cut, plain = SamplingParams(top_p=0.5), SamplingParams(temperature=0.0)
-    entries = [StepEntry("a", [1, 2], [1], TokenChoice.of(cut, 2)), StepEntry("b", [3], [0], TokenChoice.of(plain, 1)), StepEntry("c", [4], [0])]
+    cut, greedy = SamplingParams(top_p=0.5), SamplingParams(temperature=0.0)
+    entries = [StepEntry("a", [1, 2], [1], TokenChoice.of(cut, 2)), StepEntry("b", [3], [0], TokenChoice.of(greedy, 1)), StepEntry("c", [4], [0])]
     tokens = stepper.step_and_sample(entries, [1.0, 0.0, 0.7], [0.5, 1.0, 1.0], [0.1, 0.2, 0.3])
     given = (told.chosen if vocab <= kernels.MAX_CHOICE_VOCAB else told.sampled)
     assert len(told.chosen) + len(told.sampled) == 1 and len(given) == 1 and len(tokens) == 3
@@ -68,3 +70,61 @@ def test_rows_that_nothing_is_said_of_are_marked():
     assert [TokenChoice.plain(e.choice, p.temperature, p.top_p) for e, p in zip(entries, kinds)] == [True, True, False, False, False, False]
     # (top-p may come without a choice)
     assert not TokenChoice.plain(None, 1.0, 0.5) and TokenChoice.plain(None, 0.0, 0.5) and TokenChoice.plain(None, 1.0, 1.0)
+
+
+class Noted:
+    """Histories on the host in place of the kernel's, and what was asked for them."""
+
+    def __init__(self, monkeypatch, slots, vocab=100):
+        self.seen, self.counts, self.calls = np.zeros((slots, vocab), dtype=bool), np.zeros((slots, vocab), dtype=np.int64), []
+        monkeypatch.setattr(kernels, "note_tokens", self.note)
+
+    def note(self, rules, slots, tokens, *, starts=None, prompts=None, restart=False):
+        slots, tokens, starts = slots.tolist(), tokens.tolist(), starts.tolist()
+        prompts = [0] * len(slots) if prompts is None else prompts.tolist()
+        self.calls.append((slots, [tokens[a:b] for a, b in zip(starts, starts[1:])], prompts, restart))
+        for slot, part, prompt in zip(*self.calls[-1][:3]):
+            plain.note(self.seen, self.counts, slot, part, prompt, restart)
+
+
+class OnHost:
+    """The staging of arrays without a device."""
+
+    @staticmethod
+    def upload(arrays):
+        return [torch.from_numpy(np.ascontiguousarray(a).copy()) for a in arrays]
+
+
+def noting_stepper(monkeypatch, requests, forward):
+    stepper = make_stepper(requests, model=forward)
+    stepper._staging = OnHost
+    return stepper, Noted(monkeypatch, stepper.cache.max_requests)
+
+
+def test_a_step_that_fails_leaves_histories_as_they_were(monkeypatch):
+    """Tried again it brings its tokens once."""
+    failing = []
+
+    def forward(*args, **kwargs):
+        if failing:
+            raise RuntimeError(failing.pop())
+        return torch.zeros(1, 100)
+
+    stepper, noted = noting_stepper(monkeypatch, "ab", forward)
+    slot = stepper.cache.slot("a")
+    choice = TokenChoice.of(SamplingParams(frequency_penalty=0.5), 3)
+    for tokens in ([5, 6], [7], [8], [8], [9]):                        # (a prompt of three, then its answer)
+        before = noted.seen.copy(), noted.counts.copy()
+        failing.append("injected")
+        with pytest.raises(RuntimeError, match="injected"):
+            stepper.step([StepEntry("a", tokens, [], choice)])
+        assert np.array_equal(noted.seen, before[0]) and np.array_equal(noted.counts, before[1])
+        stepper.step([StepEntry("a", tokens, [], choice)])
+    assert np.flatnonzero(noted.seen[slot]).tolist() == [5, 6, 7, 8, 9]
+    assert noted.counts[slot, [5, 6, 7, 8, 9]].tolist() == [0, 0, 0, 2, 1] and noted.counts.sum() == 3
+    # pages that run out in the middle of a step
+    stepper.cache.extend("b", 49 * 16)
+    before = noted.counts.copy()
+    with pytest.raises(Exception, match="(?i)pages"):
+        stepper.step([StepEntry("a", [3] * 241, [], choice)])
+    assert np.array_equal(noted.counts, before) and not noted.seen[slot, 3]

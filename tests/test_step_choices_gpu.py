@@ -93,3 +93,45 @@ def test_a_request_that_says_nothing_does_not_fail_for_its_neighbours_rules(mode
         beside = llm.generate(prompts, plain + [other])
         assert [o.finish_reason for o in beside[:2]] == ["length"] * 2, [o.error for o in beside]
         assert [o.token_ids for o in beside[:2]] == [o.token_ids for o in alone[:2]]
+
+
+def test_a_replayed_portion_that_fails_leaves_histories_as_they_were(model_folders):
+    """Steps with a prompt's portion and its end, captured: tried again after a failure in front of the launch, their tokens are in
+    the history once."""
+    from tesseract_b200 import SamplingParams
+    from tesseract_b200.engine.step import StepEntry
+    from tesseract_b200.sampling.params import TokenChoice
+
+    stepper = engine(model_folders("b")).stepper
+    prompt = random_tokens(384, 50, seed=1)
+    choice = TokenChoice.of(SamplingParams(temperature=0.0, frequency_penalty=0.5), 45)      # (the last five count as an answer's)
+
+    def feed(request):
+        slot = stepper.cache.slot(request)
+        for part, want in ((prompt[:32], []), (prompt[32:], [17])):
+            stepper.step([StepEntry(request, part, want, choice)])
+        return stepper.rules.counts[slot].cpu().numpy(), stepper.rules.seen[slot].cpu().numpy()
+
+    assert stepper.cache.admit("first") and stepper.cache.admit("second")
+    counts, seen = feed("first")
+    assert np.array_equal(counts, np.bincount(prompt[45:], minlength=384)) and stepper.chunk_graphs.replays == 2
+
+    class Failing:
+        def __init__(self, graph):
+            self.graph, self.failed = graph, False
+
+        def replay(self):
+            if not self.failed:
+                self.failed = True
+                raise RuntimeError("injected")
+            self.graph.replay()
+
+    for graph in stepper.chunk_graphs.graphs.values():
+        graph.graph = Failing(graph.graph)
+    slot = stepper.cache.slot("second")
+    for part, want in ((prompt[:32], []), (prompt[32:], [17])):
+        with pytest.raises(RuntimeError, match="injected"):
+            stepper.step([StepEntry("second", part, want, choice)])
+        stepper.step([StepEntry("second", part, want, choice)])
+    assert np.array_equal(stepper.rules.counts[slot].cpu().numpy(), counts)
+    assert np.array_equal(stepper.rules.seen[slot].cpu().numpy(), seen)
