@@ -281,6 +281,7 @@ class DecodeGraphs:
         choosing = self._choosing(entries, temperatures, top_ps)
         if choosing == RULED:
             stepper.begin_rules(entries)
+            stepper.begin_histories(entries)
         for entry in entries:
             cache.extend(entry.request, 1)
         count = len(entries)

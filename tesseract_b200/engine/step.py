@@ -113,24 +113,32 @@ class Stepper:
             if self.cache.length(entry.request) == 0:
                 self.rules.set(slot, repetition=params.repetition_penalty, presence=params.presence_penalty,
                                frequency=params.frequency_penalty, biases=params.logit_bias, allowed=params.allowed_token_ids)
-                self.rules.clear(slot)
             if choice.allowed is not None:
                 self.rules.set_mask(slot, choice.allowed)
 
     def note_entries(self, entries: Sequence[StepEntry]) -> None:
-        """The tokens that a step brings go into the histories of the requests with penalties: when its launches are under way and
-        before the cache counts them, so that a step that fails and is tried again brings them once."""
+        """The tokens that a step brings go into the histories of the requests with penalties, those of requests that begin with it in
+        place of what their slots had: when its launches are under way and before the cache counts them, so that a step that fails and is
+        tried again brings them once."""
         noted = [e for e in entries if e.choice is not None and e.choice.params.penalised]
-        if not noted:
+        for begins in (True, False) if noted else ():
+            self._note([e for e in noted if (self.cache.length(e.request) == 0) == begins], restart=begins)
+
+    def begin_histories(self, entries: Sequence[StepEntry]) -> None:
+        """In front of a captured step, which notes its own tokens: requests that begin with it have had none."""
+        self._note([e for e in entries if e.choice is not None and e.choice.params.penalised and self.cache.length(e.request) == 0],
+                   restart=True, tokens=False)
+
+    def _note(self, entries: Sequence[StepEntry], restart: bool, tokens: bool = True) -> None:
+        if not entries:
             return
-        counts = [len(e.tokens) for e in noted]
-        starts = np.zeros(len(noted) + 1, dtype=np.int32)
-        np.cumsum(counts, out=starts[1:])
-        tokens = np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in noted])
-        slots = np.asarray([self.cache.slot(e.request) for e in noted], dtype=np.int32)
-        prompts = np.asarray([e.choice.prompt_tokens - self.cache.length(e.request) for e in noted], dtype=np.int32)
-        slots, tokens, starts, prompts = self._staging.upload([slots, tokens, starts, prompts])
-        kernels.note_tokens(self.rules, slots, tokens, starts=starts, prompts=prompts)
+        parts = [np.asarray(e.tokens if tokens else (), dtype=np.int32) for e in entries]
+        starts = np.zeros(len(entries) + 1, dtype=np.int32)
+        np.cumsum([part.size for part in parts], out=starts[1:])
+        slots = np.asarray([self.cache.slot(e.request) for e in entries], dtype=np.int32)
+        prompts = np.asarray([e.choice.prompt_tokens - self.cache.length(e.request) for e in entries], dtype=np.int32)
+        slots, brought, starts, prompts = self._staging.upload([slots, np.concatenate(parts), starts, prompts])
+        kernels.note_tokens(self.rules, slots, brought, starts=starts, prompts=prompts, restart=restart)
 
     # ------------------------------------------------------------------ validation
     def _validate(self, entries: Sequence[StepEntry]) -> List[Sequence[int]]:

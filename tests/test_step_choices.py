@@ -128,3 +128,25 @@ def test_a_step_that_fails_leaves_histories_as_they_were(monkeypatch):
     with pytest.raises(Exception, match="(?i)pages"):
         stepper.step([StepEntry("a", [3] * 241, [], choice)])
     assert np.array_equal(noted.counts, before) and not noted.seen[slot, 3]
+
+
+def test_a_request_that_begins_has_its_tokens_in_place_of_what_its_slot_had(monkeypatch):
+    """One call for the requests that begin with a step and one for the others, and none for those without penalties."""
+    stepper, noted = noting_stepper(monkeypatch, "abc", lambda *args, **kwargs: torch.zeros(3, 100))
+    slot = {request: stepper.cache.slot(request) for request in "abc"}
+    noted.seen[:], noted.counts[:] = True, 7                           # (slots that others had)
+    penalised, biased = SamplingParams(presence_penalty=0.5), SamplingParams(logit_bias={3: 1.0})
+    choice = {"a": TokenChoice.of(penalised, 3), "b": TokenChoice.of(biased, 2), "c": TokenChoice.of(penalised, 1)}
+    stepper.step([StepEntry("a", [5, 6], [], choice["a"]), StepEntry("b", [9, 9], [], choice["b"])])
+    assert noted.calls == [([slot["a"]], [[5, 6]], [3], True)]
+    stepper.step([StepEntry("a", [7, 8], [], choice["a"]), StepEntry("c", [4, 4, 4], [], choice["c"])])
+    assert noted.calls[1:] == [([slot["c"]], [[4, 4, 4]], [1], True), ([slot["a"]], [[7, 8]], [1], False)]
+    stepper.step([StepEntry("c", [4], [], choice["c"]), StepEntry("a", [8], [], choice["a"]), StepEntry("b", [1], [], choice["b"])])
+    assert noted.calls[3:] == [([slot["c"], slot["a"]], [[4], [8]], [-2, -1], False)]
+    assert np.flatnonzero(noted.seen[slot["a"]]).tolist() == [5, 6, 7, 8] and noted.counts[slot["a"], 8] == 2
+    assert noted.counts[slot["a"]].sum() == 2 and noted.counts[slot["c"], 4] == 3 and noted.counts[slot["c"]].sum() == 3
+    # in front of a captured step, which notes what it is fed
+    stepper.cache.release("a")
+    assert stepper.cache.admit("d")
+    stepper.begin_histories([StepEntry("d", [5], [0], choice["a"]), StepEntry("c", [5], [0], choice["c"]), StepEntry("b", [1], [0], choice["b"])])
+    assert noted.calls[4:] == [([stepper.cache.slot("d")], [[]], [3], True)] and not noted.seen[stepper.cache.slot("d")].any()

@@ -62,3 +62,14 @@ def test_refusals():
         rules.set_masks(torch.zeros(2, 3, dtype=torch.int32))
     with pytest.raises(ValueError):
         rules.set_mask(0, np.zeros(2, dtype=np.int32))
+
+
+def test_a_slots_history_may_be_cleared():
+    rules = TokenRules(3, 100, "cpu")
+    rules.seen.fill_(-1)
+    rules.counts.fill_(4)
+    rules.clear(1)
+    assert not rules.seen[1].any() and not rules.counts[1].any()
+    assert (rules.counts[[0, 2]] == 4).all() and (rules.seen[[0, 2]] == -1).all()
+    with pytest.raises(ValueError):
+        rules.clear(3)
