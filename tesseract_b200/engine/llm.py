@@ -65,7 +65,7 @@ class LLM:
                                    run_and_sample=self.stepper.step_and_sample,
                                    launch_decode=self.stepper.launch_decode if cuda_graphs else None,
                                    can_launch_decode=self.stepper.can_launch_decode if cuda_graphs else None,
-                                   vocab_size=self.model.spec.vocab_size)
+                                   vocab_size=self.model.spec.vocab_size, prepare_rules=self.stepper.prepare_rules)
         self.tokenizer = self._load_tokenizer(model_path)
 
     @staticmethod

@@ -131,7 +131,8 @@ class Scheduler:
     def __init__(self, config: EngineConfig, cache, run_step: Callable, sample: Callable, *, eos_token_ids=(),
                  max_positions: Optional[int] = None, capacity_tokens: Optional[int] = None,
                  run_and_sample: Optional[Callable] = None, launch_decode: Optional[Callable] = None,
-                 can_launch_decode: Optional[Callable] = None, vocab_size: Optional[int] = None):
+                 can_launch_decode: Optional[Callable] = None, vocab_size: Optional[int] = None,
+                 prepare_rules: Optional[Callable] = None):
         config.validate()
         self.config = config
         self.cache = cache
@@ -146,6 +147,8 @@ class Scheduler:
         self.eos_token_ids = frozenset(int(t) for t in eos_token_ids)
         self.max_positions = max_positions
         self.vocab_size = vocab_size
+        # makes what requests with rules need on the device, once (a step that had to would fail with all its rows)
+        self.prepare_rules = prepare_rules
         self.capacity_tokens = capacity_tokens if capacity_tokens is not None else config.kv_capacity_tokens
         self.requests: Dict[Hashable, Request] = {}
         self.waiting: Deque[Hashable] = deque()
@@ -178,6 +181,11 @@ class Scheduler:
             request_id = next(self._ids)
         if request_id in self.requests:
             raise RequestRejected(f"request id {request_id!r} is already in use")
+        if params.ruled and self.prepare_rules is not None:
+            try:
+                self.prepare_rules()
+            except Exception as exc:  # noqa: BLE001 - whatever keeps them from being made
+                raise RequestRejected(f"rules on tokens cannot be taken: {type(exc).__name__}: {exc}") from exc
         seed = params.seed if params.seed is not None else hash(request_id) & ((1 << 64) - 1)
         self.requests[request_id] = Request(request_id, prompt, params, SplitMix64(seed), choice=TokenChoice.of(params, len(prompt)))
         self.waiting.append(request_id)

@@ -87,17 +87,21 @@ class Stepper:
         self.graphs = None          # set by enable_graphs()
         self.chunk_graphs = None    # set by enable_graphs(chunk_rows=...)
         self._sampler = None
-        self._rules = None          # made when a request first has rules
+        self._rules = None          # made when a request with rules first arrives (prepare_rules)
 
     # ------------------------------------------------------------------ rules on next tokens
-    @property
-    def rules(self):
-        """The :class:`TokenRules` of the running requests, by their state slots."""
+    def prepare_rules(self):
+        """Make :attr:`rules`, if no request has had any yet."""
         if self._rules is None:
             from ..sampling.rules import TokenRules
 
             self._rules = TokenRules(self.cache.max_requests, self.vocab_size, self.runtime.device, biases=MAX_BIASES)
         return self._rules
+
+    @property
+    def rules(self):
+        """The :class:`TokenRules` of the running requests, by their state slots."""
+        return self.prepare_rules()
 
     def rule_slots(self, entries: Sequence[StepEntry]) -> List[int]:
         """The entries' slots in :attr:`rules`; -1 for those without rules."""

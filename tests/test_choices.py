@@ -213,3 +213,27 @@ def test_command_line_options(monkeypatch):
     assert (params.presence_penalty, params.frequency_penalty) == (0.5, 0.25)
     assert params.logit_bias == {5: -2.5, 7: 1.0} and params.allowed_token_ids == (5, 7, 9)
     assert not cli.sampling_params(cli.build_parser().parse_args([])).ruled
+
+
+def test_a_request_whose_rules_have_no_room_is_refused_alone():
+    """The table of rules is made when a request that needs it arrives: no step fails for want of it."""
+    s, _ = make()
+    asked = []
+
+    def no_room():
+        asked.append(len(s.requests))
+        raise MemoryError("nothing left on the device")
+
+    s.prepare_rules = no_room
+    a = s.add_request([1, 2], SamplingParams(max_tokens=3, temperature=0.0, ignore_eos=True))
+    b = s.add_request([3], SamplingParams(max_tokens=3, top_p=0.5, top_k=4, ignore_eos=True))          # (a cut needs none)
+    assert asked == []
+    with pytest.raises(RequestRejected, match="nothing left on the device"):
+        s.add_request([1, 2], SamplingParams(max_tokens=3, presence_penalty=1.0))
+    with pytest.raises(RequestRejected, match="capacity"):                                             # (nor one that is refused anyway)
+        s.add_request([1, 2], SamplingParams(max_tokens=3000, presence_penalty=1.0))
+    assert asked == [2] and len(s.requests) == 2
+    s.prepare_rules = lambda: asked.append("made")
+    c = s.add_request([1, 2], SamplingParams(max_tokens=3, temperature=0.0, presence_penalty=1.0, ignore_eos=True))
+    assert asked == [2, "made"]
+    assert {r.id: len(r.generated) for r in run_all(s)} == {a: 3, b: 3, c: 3}

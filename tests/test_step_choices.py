@@ -150,3 +150,13 @@ def test_a_request_that_begins_has_its_tokens_in_place_of_what_its_slot_had(monk
     assert stepper.cache.admit("d")
     stepper.begin_histories([StepEntry("d", [5], [0], choice["a"]), StepEntry("c", [5], [0], choice["c"]), StepEntry("b", [1], [0], choice["b"])])
     assert noted.calls[4:] == [([stepper.cache.slot("d")], [[]], [3], True)] and not noted.seen[stepper.cache.slot("d")].any()
+
+
+def test_the_table_of_rules_is_made_on_demand_and_once():
+    stepper = make_stepper("ab")
+    assert stepper._rules is None
+    stepper.prepare_rules()
+    rules = stepper._rules
+    assert rules.slots == stepper.cache.max_requests and rules.vocab == 100
+    stepper.prepare_rules()
+    assert stepper._rules is rules and stepper.rules is rules

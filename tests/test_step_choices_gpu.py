@@ -135,3 +135,26 @@ def test_a_replayed_portion_that_fails_leaves_histories_as_they_were(model_folde
         stepper.step([StepEntry("second", part, want, choice)])
     assert np.array_equal(stepper.rules.counts[slot].cpu().numpy(), counts)
     assert np.array_equal(stepper.rules.seen[slot].cpu().numpy(), seen)
+
+
+def test_rules_without_room_on_the_device_fail_no_step(model_folders, monkeypatch):
+    from tesseract_b200 import SamplingParams
+    from tesseract_b200.engine.scheduler import RequestRejected
+    from tesseract_b200.sampling import rules
+
+    def no_room(*args, **kwargs):
+        raise torch.OutOfMemoryError("CUDA out of memory")
+
+    llm = engine(model_folders("a"))
+    same = dict(max_tokens=6, temperature=0.0, ignore_eos=True)
+    want = llm.generate([[1, 2, 3]], SamplingParams(**same))[0].token_ids
+    first = llm.scheduler.add_request([1, 2, 3], SamplingParams(**same))
+    with monkeypatch.context() as patch:
+        patch.setattr(rules, "TokenRules", no_room)
+        with pytest.raises(RequestRejected, match="out of memory"):
+            llm.scheduler.add_request([4], SamplingParams(presence_penalty=1.0, **same))
+    second = llm.scheduler.add_request([4], SamplingParams(presence_penalty=1e4, **same))
+    done = {}
+    while llm.scheduler.has_work():
+        done.update({r.id: r for r in llm.scheduler.step().finished})
+    assert done[first].generated == want and len(set(done[second].generated)) == 6
