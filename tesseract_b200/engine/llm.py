@@ -149,6 +149,8 @@ class LLM:
         if len(sampling_params) != len(prompts):
             raise ValueError("one SamplingParams per prompt (or one for all)")
         encoded = [self._encode(p) for p in prompts]
+        for tokens, params in zip(encoded, sampling_params):             # (before any of them is taken)
+            self.scheduler.check_request(tokens, params)
         pending = list(zip(range(len(prompts)), encoded, sampling_params))
         room = self.config.max_pending + self.config.max_running
         done: Dict[int, Request] = {}

@@ -157,9 +157,8 @@ class Scheduler:
         self.steps = 0
 
     # ------------------------------------------------------------------ requests
-    def add_request(self, prompt: Sequence[int], params: SamplingParams, request_id: Hashable = None) -> Hashable:
-        if len(self.requests) >= self.config.max_pending + self.config.max_running:
-            raise EngineOverloaded("the inference engine is overloaded")
+    def check_request(self, prompt: Sequence[int], params: SamplingParams) -> List[int]:
+        """Raise what :meth:`add_request` raises for a request that this engine never takes; returns its prompt."""
         params.validate()
         if self.vocab_size is not None:
             params.check_vocabulary(self.vocab_size)
@@ -177,15 +176,21 @@ class Scheduler:
             limit = min(limit, self.max_positions)
         if total > limit:
             raise RequestRejected(f"prompt plus max_tokens ({total}) exceeds the configured capacity ({limit})")
-        if request_id is None:
-            request_id = next(self._ids)
-        if request_id in self.requests:
-            raise RequestRejected(f"request id {request_id!r} is already in use")
         if params.ruled and self.prepare_rules is not None:
             try:
                 self.prepare_rules()
             except Exception as exc:  # noqa: BLE001 - whatever keeps them from being made
                 raise RequestRejected(f"rules on tokens cannot be taken: {type(exc).__name__}: {exc}") from exc
+        return prompt
+
+    def add_request(self, prompt: Sequence[int], params: SamplingParams, request_id: Hashable = None) -> Hashable:
+        if len(self.requests) >= self.config.max_pending + self.config.max_running:
+            raise EngineOverloaded("the inference engine is overloaded")
+        prompt = self.check_request(prompt, params)
+        if request_id is None:
+            request_id = next(self._ids)
+        if request_id in self.requests:
+            raise RequestRejected(f"request id {request_id!r} is already in use")
         seed = params.seed if params.seed is not None else hash(request_id) & ((1 << 64) - 1)
         self.requests[request_id] = Request(request_id, prompt, params, SplitMix64(seed), choice=TokenChoice.of(params, len(prompt)))
         self.waiting.append(request_id)

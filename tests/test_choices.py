@@ -237,3 +237,38 @@ def test_a_request_whose_rules_have_no_room_is_refused_alone():
     c = s.add_request([1, 2], SamplingParams(max_tokens=3, temperature=0.0, presence_penalty=1.0, ignore_eos=True))
     assert asked == [2, "made"]
     assert {r.id: len(r.generated) for r in run_all(s)} == {a: 3, b: 3, c: 3}
+
+
+def bare_llm(scheduler):
+    """``LLM.generate`` over a scheduler without a device."""
+    from tesseract_b200 import LLM
+
+    llm = LLM.__new__(LLM)
+    llm.scheduler, llm.config, llm.tokenizer = scheduler, scheduler.config, None
+    llm._check_device_waits = lambda: None
+    return llm
+
+
+@pytest.mark.parametrize("refused, error", [
+    (dict(allowed_token_ids=[2000]), ValueError), (dict(logit_bias={2001: 1.0}), ValueError), (dict(max_tokens=5000), RequestRejected),
+    (dict(presence_penalty=1.0), RequestRejected)], ids=str)
+def test_a_request_that_is_refused_leaves_nothing_of_its_call_behind(refused, error):
+    """The call raises before any of its requests is taken, however many wait, and the next one runs."""
+    s, fake = make()
+
+    def no_room():
+        raise MemoryError("nothing left on the device")
+
+    s.prepare_rules = no_room
+    llm = bare_llm(s)
+    same = dict(max_tokens=3, temperature=0.0, ignore_eos=True)
+    plain, prompts = SamplingParams(**same), [[k + 1] for k in range(20)]       # (more than fit at once)
+    for place in (1, 19):
+        with pytest.raises(error):
+            llm.generate(prompts, [SamplingParams(**{**same, **refused}) if k == place else plain for k in range(20)])
+        assert not s.has_work() and not s.requests and fake.batches == []
+    with pytest.raises(RequestRejected):
+        llm.generate([[1], []], plain)
+    assert not s.has_work()
+    assert [o.token_ids for o in llm.generate(prompts, plain)] == [[1000, 1001, 1002]] * 20
+    fake.cache.check()
