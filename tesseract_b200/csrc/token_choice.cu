@@ -129,7 +129,7 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 
 // e^-d for d from -2^-8 on in 64 bits, by a table of 2^(i / 256) and the series of what is left (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point arithmetic", 1989): -d = (256 m + i) ln 2 / 256 + r, |r| <= ln 2 / 512,
-// e^r by its series up to r^3: what is left is below 1.4e-13, and of one sign, so that most of it is common to a row's weights.
+// e^r by its series up to r^4: what is left is below 2^-54, so that a weight is as exact as 64 bits are.
 // Beyond kWeightless (+inf among it) it is e^-700, 10^-304, which is nothing beside the largest weight, 1.
 __device__ __forceinline__ double weight_of(float d, const double* table) {
     constexpr double kSteps = -256.0 / 0.693147180559945309417232121458, kStep = 0.693147180559945309417232121458 / 256.0;
@@ -138,7 +138,7 @@ __device__ __forceinline__ double weight_of(float d, const double* table) {
     const int n = __double2loint(whole);
     const double r = fma(whole - kRound, -kStep, -x), two = table[n & (kTable - 1)];
     const double step = __hiloint2double(__double2hiint(two) + (n >> 8 << 20), __double2loint(two));
-    return fma(step * r, fma(r, fma(r, 1.0 / 6, 0.5), 1.0), step);
+    return fma(step * r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), step);
 }
 __device__ __noinline__ double one_weight(float d, const double* table) { return weight_of(d, table); }
 

@@ -1,5 +1,7 @@
 """How the engine's steps choose their rows' tokens, captured and launched one by one, against the plain model."""
 
+import decimal
+
 import numpy as np
 import pytest
 import torch
@@ -158,3 +160,28 @@ def test_rules_without_room_on_the_device_fail_no_step(model_folders, monkeypatc
     while llm.scheduler.has_work():
         done.update({r.id: r for r in llm.scheduler.step().finished})
     assert done[first].generated == want and len(set(done[second].generated)) == 6
+
+
+def test_weights_are_those_of_64_bits():
+    """Two tokens, draws and top-p on either side of the border between them.  A weight e^-d is off by: its series behind r^4, r^5 / 120
+    with |r| <= ln 2 / 512, below 2^-54; the table's power of two, 2^-52; r's two roundings, d 2^-53 and less; four roundings on the way,
+    2^-53 each: 2^-50 (1 + d / 2) holds them all.  The border w0 / (w0 + w1) moves by no more, and the sums, products and the draw itself
+    are rounded by 2^-53 each, 2^-51 together."""
+    rng = np.random.RandomState(5)
+    d = rng.uniform(0.01, 4.0, 4000).astype(np.float32)
+    x = np.full((d.size, 3), -1e30, dtype=np.float32)
+    x[:, 0], x[:, 1] = 0.0, -d
+    logits = torch.from_numpy(x).cuda()
+    ones, out = torch.ones(d.size, device="cuda"), torch.empty(d.size, dtype=torch.int32, device="cuda")
+    with decimal.localcontext(prec=40):
+        border = [1 / (1 + (-decimal.Decimal(float(v))).exp()) for v in d]
+        off = [decimal.Decimal(2.0 ** -50 * (1.0 + 0.5 * float(v)) + 2.0 ** -51) for v in d]
+        sides = [np.array([float(b * (1 + sign * o)) for b, o in zip(border, off)]) for sign in (-1, 1)]
+    for token, side in enumerate(sides):
+        draws = torch.from_numpy(side).cuda()
+        for cut in (None, torch.full((d.size,), 2, dtype=torch.int32, device="cuda")):       # (in the order of ids, and of the rank)
+            kernels.choose_tokens(logits, ones, draws, out, top_k=cut)
+            assert (out == token).all()
+        late = torch.full((d.size,), 1.0 - 2.0 ** -20, dtype=torch.float64, device="cuda")
+        kernels.choose_tokens(logits, ones, late, out, top_p=draws)                          # (the first alone is kept, or both)
+        assert (out == token).all()
