@@ -49,7 +49,7 @@ constexpr int kTable = 256;
 constexpr int kInside = 4;
 constexpr int kWindows = 3;              // where the draw, top_p's cut and top_k's cut may lie
 constexpr int kIds = 18;                 // bits of an id: kMaxBlocks * kMaxChunk tokens
-constexpr float kWeightless = 700.0f;    // a token beyond weighs nothing
+constexpr float kWeightless = 700.0f;    // weights of tokens beyond are taken as e^-700: nothing beside the largest, 1
 constexpr float kReach = 32.0f;          // the bins cover d up to 32 at most; what is beyond is in the last
 // To spare in a mass that the bins bound: the bins' width and the weights of their edges are rounded to 32 bits, 2^-24 * 32 in d.
 constexpr double kSpare = 1e-5;
@@ -130,7 +130,7 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 // e^-d for d from -2^-8 on in 64 bits, by a table of 2^(i / 256) and the series of what is left (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point arithmetic", 1989): -d = (256 m + i) ln 2 / 256 + r, |r| <= ln 2 / 512,
 // e^r by its series up to r^4: what is left is below 2^-54, so that a weight is as exact as 64 bits are.
-// Beyond kWeightless (+inf among it) it is e^-700, 10^-304, which is nothing beside the largest weight, 1.
+// Beyond kWeightless (+inf among it) it is e^-700, 10^-304.
 __device__ __forceinline__ double weight_of(float d, const double* table) {
     constexpr double kSteps = -256.0 / 0.693147180559945309417232121458, kStep = 0.693147180559945309417232121458 / 256.0;
     constexpr double kRound = 6755399441055744.0;                              // 1.5 * 2^52: adding it rounds to a whole number
@@ -141,6 +141,15 @@ __device__ __forceinline__ double weight_of(float d, const double* table) {
     return fma(step * r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), step);
 }
 __device__ __noinline__ double one_weight(float d, const double* table) { return weight_of(d, table); }
+// The last distance that weighs anything where tb_sample works weights out: exp, a unit off at most, may round the last one to 0.  (From
+// kWeightless on in units of 32-bit numbers, 2^-14 there: 20 steps reach up to 763.)
+__device__ __noinline__ float last_weight() {
+    int last = __float_as_int(kWeightless);
+#pragma unroll 1
+    for (int step = 1 << 19; step > 0; step >>= 1)
+        if (exp(-(double)__int_as_float(last + step)) > 0.0) last += step;
+    return __int_as_float(last);
+}
 
 // A token's place in the rank: ascending keys.
 __device__ __forceinline__ uint64_t key_of(float d, int id) { return (uint64_t)__float_as_uint(d) << kIds | (uint32_t)id; }
@@ -624,11 +633,12 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         // ---- in the order of ids: a warp has a run of tokens
         const int part = ((count + kWarps - 1) / kWarps + 31) & ~31;
         const int begin = min(count, warp * part), end = min(count, begin + part);
-        // (a draw of 0 takes the first token that weighs anything)
+        // (a draw of 0 takes the first token that weighs anything; no other gets to those beyond kWeightless)
+        const float last = u > 0.0 ? kWeightless : last_weight();
         auto weight = [&](float l) {
             const float d = fmaf(-l, row.inverse, row.top);
             const double w = weight_of(d, sh.table);
-            return d <= kWeightless ? w : 0.0;
+            return d <= last ? w : 0.0;
         };
         double mine = 0.0;
 #pragma unroll 4

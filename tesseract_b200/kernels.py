@@ -593,9 +593,8 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
     largest for a temperature (float32) of 0 and below; else drawn, with the uniform draw (float64, in [0, 1)), from what ``top_k``
     (int32; 0: all), ``min_p`` (float64, relative to the largest weight) and ``top_p`` (float64, of the mass that those two leave)
     keep of the tokens ranked by weight, equal ones by id.  The rank is drawn from in its order (as :func:`~tesseract_b200.sampling
-    .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`); a token
-    that weighs less than e^-700 of the largest is not drawn.  A row with NaN or +inf among what is
-    allowed, or with nothing allowed, gets -1, or where ``as_sampled`` (int32) is not 0 the token that :func:`sample` gives such a row
+    .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`); a token whose weight is nothing in 64 bits
+    (below e^-745 of the largest) is not drawn.  A row with NaN or +inf among what is allowed, or with nothing allowed, gets -1, or where ``as_sampled`` (int32) is not 0 the token that :func:`sample` gives such a row
     in a call of as many (which makes a row without rules and cuts independent of those beside it).  Up to 262,144 tokens and 65,535
     rows."""
     rows, vocab, stride = _logit_rows("choose_tokens", logits)

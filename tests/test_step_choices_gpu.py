@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tesseract_b200 import kernels
+from tests import token_choice_plain as choices
 from tests.helpers import TINY, make_model_folder, random_tokens
 from tests.plain import llama
 from tests.test_choices_gpu import check_answer, engine
@@ -185,3 +186,21 @@ def test_weights_are_those_of_64_bits():
         late = torch.full((d.size,), 1.0 - 2.0 ** -20, dtype=torch.float64, device="cuda")
         kernels.choose_tokens(logits, ones, late, out, top_p=draws)                          # (the first alone is kept, or both)
         assert (out == token).all()
+
+
+@pytest.mark.parametrize("vocab", [3, 100, 20000, 128256])
+@pytest.mark.parametrize("below", [699.0, 701.0, 712.5, 730.0, 744.0, 745.0, 746.0, 800.0])
+def test_a_draw_of_nothing_takes_the_samplers_first_token(vocab, below):
+    """A row without a cut: the first token whose weight is a number of 64 bits above 0, down to e^-745.  (That is 5.0e-324, and the
+    least number above 0 is 4.9e-324: a library's exp that is a unit off may give 0.  e^-744, 1.36e-323, is further from it.)"""
+    x = np.full((3, vocab), -1e4, dtype=np.float32)
+    x[:, -1] = 3.0
+    x[1, vocab // 2] = x[2, 0] = 3.0 - below
+    logits = torch.from_numpy(x).cuda()
+    ones, draws = torch.ones(3, device="cuda"), torch.zeros(3, dtype=torch.float64, device="cuda")
+    want, got = (torch.full((3,), -9, dtype=torch.int32, device="cuda") for _ in range(2))
+    kernels.sample(logits, ones, draws, want)
+    kernels.choose_tokens(logits, ones, draws, got)
+    first = [vocab - 1, vocab // 2, 0] if below < 745.5 else [vocab - 1] * 3
+    assert got.tolist() == want.tolist()
+    assert first == [choices.choose(row, 1.0, 0.0) for row in x] and (got.tolist() == first or below == 745.0)
