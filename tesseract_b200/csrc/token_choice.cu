@@ -5,7 +5,8 @@
 //     kept = the first top_k of the rank; of those w >= min_p; of those the shortest beginning with mass >= top_p * their mass
 //     token = the first of the rank whose cumulative weight is above u * (mass of what is kept)
 //   A row without any cut is drawn from in the order of ids with d = fma(-x, 1 / T, max z), as tb_sample does (where max z is 65,536 and
-//   more, at temperatures of a thousandth and below, that would leave the largest logit itself away from 0: there d as above).
+//   more, at temperatures of a thousandth and below, that would leave the largest logit itself away from 0: there d as above, unless
+//   the row is marked by `as_sampled` and max z is below 2^32).
 //   A row with NaN or +inf, or with nothing above -inf, has no token: -1 (`as_sampled`: the one that tb_sample gives it).  Where max z
 //   leaves the 32 bits' range, the largest logits have d = 0 and the others weigh nothing.
 //
@@ -127,7 +128,7 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
 
-// e^-d for d from -2^-8 on in 64 bits, by a table of 2^(i / 256) and the series of what is left (P. T. P. Tang, "Table-driven
+// e^-d for d from -700 on in 64 bits, by a table of 2^(i / 256) and the series of what is left (P. T. P. Tang, "Table-driven
 // implementation of the exponential function in IEEE floating-point arithmetic", 1989): -d = (256 m + i) ln 2 / 256 + r, |r| <= ln 2 / 512,
 // e^r by its series up to r^4: what is left is below 2^-54, so that a weight is as exact as 64 bits are.
 // Beyond kWeightless (+inf among it) it is e^-700, 10^-304.
@@ -614,9 +615,14 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
     }
     const int k = top_k != nullptr ? top_k[r] : 0;
     const double p = top_p != nullptr ? top_p[r] : 1.0, floor = min_p != nullptr ? min_p[r] : 0.0, u = uniform[r];
+    bool by_k = k > 0 && k < vocab, by_floor = floor > 0.0;
+    const bool uncut = !(by_k || by_floor || p < 1.0);
     row.inverse = 1.0f / temp;
     row.top = best * row.inverse;
-    if (!(fabsf(row.top) < 65536.0f) || row.inverse == 0.0f) {
+    bool far = !(fabsf(row.top) < 65536.0f) || row.inverse == 0.0f;
+    // (a row that is to have tb_sample's token has its distances, up to where the largest one's own, half a unit of max z, is 128)
+    if (far && uncut && fabsf(row.top) < 4294967296.0f && row.inverse > 0.0f && as_sampled != nullptr && as_sampled[r] != 0) far = false;
+    if (far) {
         // (temperatures far from 1: the distances themselves take the logits' place, negative as those are)
         const bool finite = fabsf(row.top) < INFINITY;
         for (int i = t; i < count; i += kThreads) {
@@ -628,8 +634,7 @@ choose_kernel(const float* __restrict__ logits, int64_t stride, const float* __r
         row.top = 0.0f;
         __syncthreads();
     }
-    bool by_k = k > 0 && k < vocab, by_floor = floor > 0.0;
-    if (!(by_k || by_floor || p < 1.0)) {
+    if (uncut) {
         // ---- in the order of ids: a warp has a run of tokens
         const int part = ((count + kWarps - 1) / kWarps + 31) & ~31;
         const int begin = min(count, warp * part), end = min(count, begin + part);

@@ -595,8 +595,8 @@ def choose_tokens(logits: torch.Tensor, temperature: torch.Tensor, uniform: torc
     keep of the tokens ranked by weight, equal ones by id.  The rank is drawn from in its order (as :func:`~tesseract_b200.sampling
     .sample_top_p_host`), a row without any cut in the order of ids (as :func:`sample`); a token whose weight is nothing in 64 bits
     (below e^-745 of the largest) is not drawn.  A row with NaN or +inf among what is allowed, or with nothing allowed, gets -1, or where ``as_sampled`` (int32) is not 0 the token that :func:`sample` gives such a row
-    in a call of as many (which makes a row without rules and cuts independent of those beside it).  Up to 262,144 tokens and 65,535
-    rows."""
+    in a call of as many; a row without cuts that it marks is rounded as there at the lowest temperatures too (which makes rows
+    without rules and cuts independent of those beside them).  Up to 262,144 tokens and 65,535 rows."""
     rows, vocab, stride = _logit_rows("choose_tokens", logits)
     device = logits.get_device()
     record = _rules_of("choose_tokens", rules, slots, rows, vocab, device)

@@ -204,3 +204,25 @@ def test_a_draw_of_nothing_takes_the_samplers_first_token(vocab, below):
     first = [vocab - 1, vocab // 2, 0] if below < 745.5 else [vocab - 1] * 3
     assert got.tolist() == want.tolist()
     assert first == [choices.choose(row, 1.0, 0.0) for row in x] and (got.tolist() == first or below == 745.0)
+
+
+@pytest.mark.parametrize("temperature", [2e-3, 2e-4, 1e-4, 1e-5, 1e-6, 1e-8])
+def test_a_marked_row_has_the_samplers_token_at_low_temperatures(temperature):
+    """Logits a few units of their last place apart, whose distances from the largest are rounded in one way by ``sample`` and in another
+    for cuts: a row without a cut has ``sample``'s tokens.  Each side sums in 64 bits, 2,000 weights, in its own order: 2^-42 of the whole
+    at most, within which a draw falls once in 10^8 rows."""
+    rng = np.random.RandomState(3)
+    rows, vocab = 400, 2000
+    steps = rng.randint(0, 40, (rows, vocab)).astype(np.float32)
+    x = (np.float32(15.7) + steps * np.float32(2.0 ** -20)) * rng.choice([1.0, -1.0, 0.25], (rows, 1)).astype(np.float32)
+    x = x.astype(np.float32)
+    logits = torch.from_numpy(x).cuda()
+    of_rows, draws = torch.full((rows,), temperature, device="cuda"), torch.from_numpy(rng.rand(rows)).cuda()
+    want, got = (torch.full((rows,), -9, dtype=torch.int32, device="cuda") for _ in range(2))
+    kernels.sample(logits, of_rows, draws, want)
+    kernels.choose_tokens(logits, of_rows, draws, got, as_sampled=torch.ones(rows, dtype=torch.int32, device="cuda"))
+    assert got.tolist() == want.tolist()
+    # (a mark says nothing about a row with a cut)
+    cut = torch.full((rows,), 0.9, dtype=torch.float64, device="cuda")
+    without = kernels.choose_tokens(logits, of_rows, draws, want, top_p=cut).tolist()
+    assert kernels.choose_tokens(logits, of_rows, draws, got, top_p=cut, as_sampled=torch.ones(rows, dtype=torch.int32, device="cuda")).tolist() == without
