@@ -226,3 +226,58 @@ def test_a_marked_row_has_the_samplers_token_at_low_temperatures(temperature):
     cut = torch.full((rows,), 0.9, dtype=torch.float64, device="cuda")
     without = kernels.choose_tokens(logits, of_rows, draws, want, top_p=cut).tolist()
     assert kernels.choose_tokens(logits, of_rows, draws, got, top_p=cut, as_sampled=torch.ones(rows, dtype=torch.int32, device="cuda")).tolist() == without
+
+
+@pytest.mark.parametrize("rows, vocab", [(70, 131073), (30, 200001), (150, 262144)])
+def test_more_rows_than_fit_at_once_of_more_than_eight_blocks(rows, vocab):
+    rng = np.random.RandomState(rows)
+    x = (rng.randn(rows, vocab) * 2.5).astype(np.float32)
+    temperature, draws = rng.choice([0.0, 0.6, 1.0, 1.5], rows).astype(np.float32), rng.rand(rows)
+    top_k, top_p = rng.choice([0, 0, 5, 3000], rows).astype(np.int32), rng.choice([1.0, 1.0, 0.9, 0.4], rows)
+    out = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+    kernels.choose_tokens(*(torch.from_numpy(a).cuda() for a in (x, temperature, draws)), out, top_k=torch.from_numpy(top_k).cuda(),
+                          top_p=torch.from_numpy(top_p).cuda())
+    assert out.tolist() == [choices.choose(x[r], temperature[r], draws[r], top_k[r], top_p[r]) for r in range(rows)]
+
+
+def test_top_p_of_a_sampler_draws_from_what_is_not_ruled_out():
+    """Logits of -inf weigh nothing; a row that top-p cuts of which NaN, +inf or nothing is left is refused."""
+    from tesseract_b200.sampling.sampler import InvalidLogits, Sampler
+
+    rng = np.random.RandomState(8)
+    x = (rng.randn(4, 700) * 2).astype(np.float32)
+    x[0, rng.permutation(700)[:600]] = -np.inf
+    x[1, 1:] = -np.inf
+    sampler, draws = Sampler("cuda"), [0.2, 0.9, 0.5, 0.7]
+    got = sampler.sample(torch.from_numpy(x).cuda(), [0.9] * 4, [0.8, 0.5, 0.9, 1.0], draws)
+    assert got == [choices.choose(x[r], 0.9, draws[r], 0, p) for r, p in enumerate((0.8, 0.5, 0.9, 1.0))]
+    for spoiled in (np.full(700, -np.inf), np.where(np.arange(700) == 3, np.nan, x[2]), np.where(np.arange(700) == 3, np.inf, x[2])):
+        x[2] = spoiled
+        with pytest.raises(InvalidLogits):
+            sampler.sample(torch.from_numpy(x).cuda(), [0.9] * 4, [0.8, 0.5, 0.9, 1.0], draws)
+
+
+def test_kinds_of_captured_steps_follow_one_another(model_folders):
+    """Requests with rules, cuts and neither that begin and end at different steps, so that a batch goes from one kind of captured step
+    to another while rows are in flight: each has the answer that it has alone."""
+    from tesseract_b200 import SamplingParams
+
+    folder = model_folders("b")
+
+    def kind(k, tokens):
+        same = dict(max_tokens=tokens, ignore_eos=True, seed=k)
+        return [SamplingParams(temperature=0.0, **same), SamplingParams(temperature=0.9, **same), SamplingParams(temperature=0.9, top_p=0.7, **same),
+                SamplingParams(temperature=0.8, top_k=7, frequency_penalty=0.4, **same), SamplingParams(temperature=0.0, repetition_penalty=1.4, **same),
+                SamplingParams(temperature=0.7, min_p=0.1, **same)][k % 6]
+
+    # (and ten that say nothing at the end)
+    kinds = [kind(k, 2 + (7 * k) % 23) for k in range(30)] + [kind(k % 2, 4 + k) for k in range(10)]
+    prompts = [random_tokens(384, 1 + (5 * k) % 9, seed=400 + k) for k in range(40)]
+    alone = engine(folder, max_running=1)
+    want = [alone.generate([prompt], params)[0].token_ids for prompt, params in zip(prompts, kinds)]
+    for running in (3, 5, 8):
+        llm = engine(folder, max_running=running)
+        assert [o.token_ids for o in llm.generate(prompts, kinds)] == want
+        graphs = llm.stepper.graphs
+        assert graphs.graphs and all(graphs.choosing_graphs[choosing][0] for choosing in (1, 2))
+        assert llm.stepper.cache.used_pages() == 0
