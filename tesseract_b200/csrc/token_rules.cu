@@ -5,9 +5,11 @@ namespace {
 
 // ---- histories
 //
-// seen: a bit for every token of the prompt and the answer; counts: how often the answer has each.  A history begun anew writes 4 V + V / 8
-// bytes: 32 requests of up to 8,192 tokens over 128,256 take 8.3 us on the device, of which 4.8 remain when no block goes through the
-// tokens (17 MB are 2.7 us at the copy rate); one request 2.7 us, a launch and three dependent loads.
+// seen: a bit for every token of the prompt and the answer; counts: how often the answer has each.  A history begun anew (the requests
+// whose first tokens a step brings) writes 4 V + V / 8 bytes: 32 requests of 512 tokens over 128,256 take 6.4 us on the device, of up to
+// 8,192 tokens 8.3, of which 4.8 remain when no block goes through the tokens (17 MB are 2.7 us at the copy rate); one request 2.8 us, a
+// launch and three dependent loads.  Tokens added to histories that are there (later portions, decode steps) touch two sectors each: 32
+// portions of 512 tokens 2.0 us, a token a row 1.4 for 1 to 32 rows, a launch and what the loads and atomics take to come back.
 
 constexpr int kNoteThreads = 512;
 constexpr int kNotePart = 8192;          // tokens of the vocabulary that a block begins anew
@@ -89,11 +91,12 @@ __global__ void set_kernel(SlotRules* to, SlotRules row) { *to = row; }
 // ---- logits
 //
 // 8 V bytes a row are read and written (less where the mask rules out four neighbours: those are not read): 64 rows of 128,256 without
-// rules take 13.5 us (4.9 TB/s), with a mask 15.7, with penalties, biases and a mask 23.8.  What bounds those is the blocks' own chain
-// (rules, bits, counts, 64-bit arithmetic between barriers: a third of all warps' time) with four blocks a multiprocessor; more blocks with
-// fewer registers were no faster.  A block
-// has 4,096 tokens, every so many-th run of 128 (low ids are had more often than high ones).  It asks for its logits first; under their latency it lists the tokens that were had (a bit each), so that every
-// thread has as many of them, and works those out in 64 bits; then everything is written, the listed ones behind the others.
+// rules take 13.5 us (4.9 TB/s), with a mask 15.7, with penalties, biases and a mask 23.6.  What bounds those is the blocks' own chain
+// (slot, the slot's rules and its bits, behind which the logits are asked for; counts, 64-bit arithmetic between barriers: a third of all
+// warps' time) with four blocks a multiprocessor; more blocks with fewer registers were no faster.  A block has 4,096 tokens, every so
+// many-th run of 128 (low ids are had more often than high ones).  While its logits are on their way it lists the tokens that were had (a
+// bit each), so that every thread has as many of them, and works those out in 64 bits; then everything is written, the listed ones
+// behind the others.
 
 constexpr int kShapeThreads = 256;
 constexpr int kShapePart = 4096;
